@@ -1,4 +1,5 @@
-"""ctypes binding of liblightdelta_hip.so (the C ABI declared in include/lightdelta_hip.h).
+"""ctypes binding of liblightdelta_hip.so (the C ABI declared in include/lightdelta_hip.h and
+include/lightdelta_linear_hip.h).
 
 torch is imported first on purpose: torch ships its own libamdhip64.so.7, and loading it
 before the library makes the library's `libamdhip64.so.7` dependency resolve to that same
@@ -116,6 +117,88 @@ class PrefillArgs(ctypes.Structure):
     ]
 
 
+class LinearDecodeArgs(ctypes.Structure):
+    """Mirror of ld_linear_decode_args (include/lightdelta_linear_hip.h)."""
+
+    _fields_ = [
+        ("qkv", _vp),
+        ("qkv_row_stride", _c_i64),
+        ("log_decay", _vp),
+        ("log_decay_row_stride", _c_i64),
+        ("indices", _vp),
+        ("cu", _vp),
+        ("accepted", _vp),
+        ("state", _vp),
+        ("state_slot_stride", _c_i64),
+        ("gate", _vp),
+        ("gate_row_stride", _c_i64),
+        ("norm_weight", _vp),
+        ("out", _vp),
+        ("num_tokens", _c_i64),
+        ("num_slots", _c_i32),
+        ("num_requests", _c_i32),
+        ("width", _c_i32),
+        ("num_k_heads", _c_i32),
+        ("num_v_heads", _c_i32),
+        ("norm_weight_dtype", _c_i32),
+        ("scale", ctypes.c_float),
+        ("eps", ctypes.c_float),
+        ("cache_policy", _c_i32),
+    ]
+
+
+class LinearPrefillArgs(ctypes.Structure):
+    """Mirror of ld_linear_prefill_args (include/lightdelta_linear_hip.h)."""
+
+    _fields_ = [
+        ("qkv", _vp),
+        ("qkv_row_stride", _c_i64),
+        ("log_decay", _vp),
+        ("log_decay_row_stride", _c_i64),
+        ("slots", _vp),
+        ("has_initial", _vp),
+        ("cu_seqlens", _vp),
+        ("state", _vp),
+        ("state_slot_stride", _c_i64),
+        ("gate", _vp),
+        ("gate_row_stride", _c_i64),
+        ("norm_weight", _vp),
+        ("out", _vp),
+        ("num_tokens", _c_i64),
+        ("num_slots", _c_i32),
+        ("num_sequences", _c_i32),
+        ("num_k_heads", _c_i32),
+        ("num_v_heads", _c_i32),
+        ("norm_weight_dtype", _c_i32),
+        ("scale", ctypes.c_float),
+        ("eps", ctypes.c_float),
+        ("workspace", _vp),
+        ("workspace_bytes", _c_i64),
+    ]
+
+
+class NormRopeArgs(ctypes.Structure):
+    """Mirror of ld_norm_rope_args (include/lightdelta_linear_hip.h)."""
+
+    _fields_ = [
+        ("qkv", _vp),
+        ("qkv_row_stride", _c_i64),
+        ("q_weight", _vp),
+        ("k_weight", _vp),
+        ("q_weight_dtype", _c_i32),
+        ("k_weight_dtype", _c_i32),
+        ("positions", _vp),
+        ("positions_int64", _c_i32),
+        ("rotary", _c_i32),
+        ("inv_freq", _vp),
+        ("num_tokens", _c_i64),
+        ("q_heads", _c_i32),
+        ("k_heads", _c_i32),
+        ("interleaved", _c_i32),
+        ("eps", ctypes.c_float),
+    ]
+
+
 PREFILL_AUTO, PREFILL_TOKEN_SERIAL, PREFILL_CHUNKED, PREFILL_CHUNKED_32 = 0, 1, 2, 3
 PREFILL_STATIC_SCRATCH_BYTES = 64 << 20
 
@@ -147,6 +230,14 @@ SIGNATURES = {
     "ld_abi_version": ([], ctypes.c_int),
 }
 
+# include/lightdelta_linear_hip.h's.
+LINEAR_SIGNATURES = {
+    "ld_linear_decode": ([ctypes.POINTER(LinearDecodeArgs), _vp], ctypes.c_int),
+    "ld_linear_prefill": ([ctypes.POINTER(LinearPrefillArgs), _vp], ctypes.c_int),
+    "ld_linear_prefill_workspace_bytes": ([_c_i64, _c_i32, _c_i32], _c_i64),
+    "ld_norm_rope": ([ctypes.POINTER(NormRopeArgs), _vp], ctypes.c_int),
+}
+
 _lock = threading.Lock()
 _lib = None
 
@@ -164,7 +255,7 @@ def load() -> ctypes.CDLL:
                     "(hipcc, gfx950) before using the lightdelta ops"
                 )
             lib = ctypes.CDLL(str(LIBRARY_PATH))
-            for name, (argtypes, restype) in SIGNATURES.items():
+            for name, (argtypes, restype) in {**SIGNATURES, **LINEAR_SIGNATURES}.items():
                 fn = getattr(lib, name)
                 fn.argtypes = argtypes
                 fn.restype = restype

@@ -21,7 +21,8 @@ LIBRARY = PACKAGE / "liblightdelta_hip.so"
 # torch.ops.lightdelta dispatcher kernels (host C++ over the C ABI; see csrc/torch_ops.cpp)
 TORCH_LIBRARY = PACKAGE / "liblightdelta_torch.so"
 SOURCES = ("abi.hip", "gdn_decode.hip", "prefill_serial.hip", "prefill_chunked.hip",
-           "prefill_heads.hip", "state_io.hip")
+           "prefill_heads.hip", "state_io.hip", "linear_decode.hip", "linear_prefill.hip",
+           "norm_rope.hip")
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [
@@ -43,10 +44,11 @@ HIPCC_FLAGS = [
 ]
 
 
-# Per-source additions.  gdn_decode.hip: its decode kernel takes the request-metadata pointers
-# and the head count as its first 7 argument dwords, which the hardware then preloads into
-# SGPRs at launch (kernels without such leading scalar arguments preload nothing).
-EXTRA_FLAGS = {"gdn_decode.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=7"]}
+# Per-source additions.  The decode kernels take the request-metadata pointers and the head
+# count as their first 7 argument dwords, which the hardware then preloads into SGPRs at launch
+# (kernels without such leading scalar arguments preload nothing).
+EXTRA_FLAGS = {name: ["-mllvm", "-amdgpu-kernarg-preload-count=7"]
+               for name in ("gdn_decode.hip", "linear_decode.hip")}
 
 
 def _rocm() -> Path:

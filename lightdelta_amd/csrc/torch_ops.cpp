@@ -2,20 +2,24 @@
 // PyTorch-ROCm): decode and decode_conv with the argument checks of the reference's launcher
 // (csrc/gdn_decode.cu:366-403), generalised to any H, HV with HV % H == 0, with its
 // messages; the state-pool ops with the checks of the reference's state_io
-// (csrc/state_io.cu:29-49) and of the additive ones; then the C ABI of liblightdelta_hip.so
-// on the current HIP stream of the tensors' device.  The schemas are defined by
+// (csrc/state_io.cu:29-49) and of the additive ones; the linear-attention ops (linear_decode,
+// linear_prefill, norm_rope); then the C ABI of liblightdelta_hip.so on the current HIP stream
+// of the tensors' device.  The schemas are defined by
 // lightdelta_amd/ops.py, which loads this library (prefill keeps a Python kernel).
 // Host-only C++ (no device code): one eager call costs a few microseconds of host time, as
 // the reference's C++ launcher does, where a Python kernel costs about twelve.
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
 #include <atomic>
+#include <cmath>
 #include <optional>
 
 #include "lightdelta_hip.h"
+#include "lightdelta_linear_hip.h"
 
 namespace {
 
@@ -375,6 +379,197 @@ void packed_plan(const at::Tensor& slots, const at::Tensor& cu, const at::Tensor
   TORCH_CHECK(rc == LD_OK, ld_last_error());
 }
 
+// ---- linear attention with a decay for each head -------------------------------------------
+
+// The checks that linear_decode and linear_prefill share (ops.py _linear_layout restates them);
+// returns H, HV.
+std::pair<int64_t, int64_t> check_linear(const at::Tensor& qkv, const at::Tensor& log_decay,
+                                         const at::Tensor& state,
+                                         const std::optional<at::Tensor>& gate,
+                                         const std::optional<at::Tensor>& weight,
+                                         const at::Tensor& out, double scale, double eps) {
+  TORCH_CHECK(qkv.is_cuda() && qkv.scalar_type() == at::kBFloat16, "qkv must be CUDA BF16");
+  const c10::Device device = qkv.device();
+  TORCH_CHECK(state.device() == device && state.scalar_type() == at::kFloat && state.dim() == 4 &&
+                  state.size(2) == kDim && state.size(3) == kDim && state.stride(3) == 1 &&
+                  state.stride(2) == kDim && state.stride(1) == kDim * kDim,
+              "state must be CUDA FP32 [slots,HV,128,128] with dense heads");
+  const int64_t hv = state.size(1);
+  const int64_t cols = qkv.dim() == 2 ? qkv.size(1) : 0;
+  const int64_t h2 = cols / kDim - hv;
+  const int64_t h = h2 / 2;
+  TORCH_CHECK(qkv.dim() == 2 && hv > 0 && cols % kDim == 0 && h2 > 0 && h2 % 2 == 0 &&
+                  hv % h == 0 && qkv.stride(1) == 1,
+              "qkv must be [tokens,(2*H+HV)*128] with HV a multiple of H");
+  const int64_t n = qkv.size(0);
+  const int64_t ld = log_decay.dim();
+  TORCH_CHECK(log_decay.device() == device && log_decay.scalar_type() == at::kFloat &&
+                  ((ld == 1 && log_decay.size(0) == hv) ||
+                   (ld == 2 && log_decay.size(0) == n && log_decay.size(1) == hv)) &&
+                  log_decay.stride(-1) == 1,
+              "log_decay must be CUDA FP32 [HV] or [tokens,HV] with dense rows");
+  TORCH_CHECK(out.device() == device && out.scalar_type() == at::kBFloat16 && out.dim() == 3 &&
+                  out.size(0) == n && out.size(1) == hv && out.size(2) == kDim &&
+                  out.is_contiguous(),
+              "out must be contiguous CUDA BF16 [tokens,HV,128]");
+  TORCH_CHECK(gate.has_value() == weight.has_value(), "gate and weight must be given together");
+  if (gate.has_value()) {
+    TORCH_CHECK(gate->device() == device && gate->scalar_type() == at::kBFloat16 &&
+                    gate->dim() == 3 && gate->size(0) == n && gate->size(1) == hv &&
+                    gate->size(2) == kDim && gate->stride(2) == 1 && gate->stride(1) == kDim,
+                "gate must be CUDA BF16 [tokens,HV,128] with dense rows");
+    TORCH_CHECK(weight->device() == device && weight->is_contiguous() && floats(*weight) &&
+                    weight->numel() == kDim,
+                "weight must be contiguous CUDA FP32/BF16 [128]");
+  }
+  TORCH_CHECK(std::isfinite(scale), "scale must be finite");
+  TORCH_CHECK(eps > 0, "norm epsilon must be positive");
+  TORCH_CHECK(state.size(0) <= INT32_MAX && hv <= INT32_MAX / kDim, "state pool too large");
+  return {h, hv};
+}
+
+// The arguments that both entry points' structs have.
+template <typename Args>
+Args linear_args(const at::Tensor& qkv, const at::Tensor& log_decay, const at::Tensor& state,
+                 const std::optional<at::Tensor>& gate, const std::optional<at::Tensor>& weight,
+                 const at::Tensor& out, double scale, double eps,
+                 std::pair<int64_t, int64_t> heads) {
+  Args args{};
+  args.qkv = qkv.data_ptr();
+  args.qkv_row_stride = qkv.stride(0);
+  args.log_decay = static_cast<const float*>(log_decay.data_ptr());
+  args.log_decay_row_stride = log_decay.dim() == 2 ? log_decay.stride(0) : 0;
+  args.state = static_cast<float*>(state.data_ptr());
+  args.state_slot_stride = state.stride(0);
+  if (gate.has_value()) {
+    args.gate = gate->data_ptr();
+    args.gate_row_stride = gate->stride(0);
+    args.norm_weight = weight->data_ptr();
+    args.norm_weight_dtype = dtype_code(*weight);
+  }
+  args.out = out.data_ptr();
+  args.num_tokens = qkv.size(0);
+  args.num_slots = static_cast<int32_t>(state.size(0));
+  args.num_k_heads = static_cast<int32_t>(heads.first);
+  args.num_v_heads = static_cast<int32_t>(heads.second);
+  args.scale = static_cast<float>(scale);
+  args.eps = static_cast<float>(eps);
+  return args;
+}
+
+void linear_decode(const at::Tensor& qkv, const at::Tensor& log_decay, const at::Tensor& indices,
+                   const at::Tensor& cu, const at::Tensor& accepted, at::Tensor state,
+                   const std::optional<at::Tensor>& gate, const std::optional<at::Tensor>& weight,
+                   at::Tensor out, double scale, double eps) {
+  const auto heads = check_linear(qkv, log_decay, state, gate, weight, out, scale, eps);
+  for (const at::Tensor* t : {&indices, &cu, &accepted})
+    TORCH_CHECK(t->device() == qkv.device() && t->scalar_type() == at::kInt && t->is_contiguous(),
+                "metadata must be contiguous CUDA int32");
+  TORCH_CHECK(indices.dim() == 2 && indices.size(1) >= 1 && indices.size(1) <= LD_MAX_TOKENS,
+              "decode/MTP supports 1 through 4 tokens per request");
+  const int64_t requests = indices.size(0);
+  TORCH_CHECK(cu.dim() == 1 && cu.numel() == requests + 1 && accepted.dim() == 1 &&
+                  accepted.numel() == requests && requests <= INT32_MAX,
+              "invalid request metadata shapes");
+  if (requests == 0 || qkv.size(0) == 0) return;
+  auto args = linear_args<ld_linear_decode_args>(qkv, log_decay, state, gate, weight, out, scale,
+                                                 eps, heads);
+  args.indices = static_cast<const int32_t*>(indices.data_ptr());
+  args.cu = static_cast<const int32_t*>(cu.data_ptr());
+  args.accepted = static_cast<const int32_t*>(accepted.data_ptr());
+  args.num_requests = static_cast<int32_t>(requests);
+  args.width = static_cast<int32_t>(indices.size(1));
+  args.cache_policy = g_cache_policy.load(std::memory_order_relaxed);
+  const c10::DeviceGuard guard(qkv.device());
+  const int rc = ld_linear_decode(&args, stream_of(qkv));
+  TORCH_CHECK(rc == LD_OK, ld_last_error());
+}
+
+void linear_prefill(const at::Tensor& qkv, const at::Tensor& log_decay, const at::Tensor& slots,
+                    const at::Tensor& has_initial, const at::Tensor& cu_seqlens, at::Tensor state,
+                    const std::optional<at::Tensor>& gate, const std::optional<at::Tensor>& weight,
+                    at::Tensor out, double scale, double eps) {
+  const auto heads = check_linear(qkv, log_decay, state, gate, weight, out, scale, eps);
+  for (const at::Tensor* t : {&slots, &cu_seqlens})
+    TORCH_CHECK(t->device() == qkv.device() && t->scalar_type() == at::kInt && t->dim() == 1 &&
+                    t->is_contiguous(),
+                "metadata must be contiguous CUDA int32");
+  TORCH_CHECK(has_initial.device() == qkv.device() && has_initial.scalar_type() == at::kBool &&
+                  has_initial.dim() == 1 && has_initial.is_contiguous(),
+              "has_initial must be a contiguous CUDA bool vector");
+  const int64_t sequences = slots.numel();
+  TORCH_CHECK(cu_seqlens.numel() == sequences + 1 && has_initial.numel() == sequences &&
+                  sequences <= INT32_MAX,
+              "invalid sequence metadata shapes");
+  if (sequences == 0) return;
+  auto args = linear_args<ld_linear_prefill_args>(qkv, log_decay, state, gate, weight, out, scale,
+                                                  eps, heads);
+  args.slots = static_cast<const int32_t*>(slots.data_ptr());
+  args.has_initial = static_cast<const uint8_t*>(has_initial.data_ptr());
+  args.cu_seqlens = static_cast<const int32_t*>(cu_seqlens.data_ptr());
+  args.num_sequences = static_cast<int32_t>(sequences);
+  const c10::DeviceGuard guard(qkv.device());
+  // From torch's caching allocator for this call alone: on one stream the next call may take the
+  // same memory, in order; under capture it is the graph's own.
+  at::Tensor workspace;
+  const int64_t bytes = ld_linear_prefill_workspace_bytes(args.num_tokens, args.num_sequences,
+                                                          args.num_v_heads);
+  if (bytes > 0) {
+    workspace = at::empty({bytes}, qkv.options().dtype(at::kByte));
+    args.workspace = workspace.data_ptr();
+    args.workspace_bytes = bytes;
+  }
+  const int rc = ld_linear_prefill(&args, stream_of(qkv));
+  TORCH_CHECK(rc == LD_OK, ld_last_error());
+}
+
+void norm_rope(at::Tensor qkv, const at::Tensor& q_weight, const at::Tensor& k_weight,
+               const at::Tensor& positions, const at::Tensor& inv_freq, int64_t q_heads,
+               int64_t k_heads, double eps, bool interleaved) {
+  TORCH_CHECK(qkv.is_cuda() && qkv.scalar_type() == at::kBFloat16, "qkv must be CUDA BF16");
+  TORCH_CHECK(q_heads >= 0 && k_heads >= 0 && q_heads <= INT32_MAX / kDim &&
+                  k_heads <= INT32_MAX / kDim && qkv.dim() == 2 &&
+                  qkv.size(1) >= (q_heads + k_heads) * kDim && qkv.stride(1) == 1,
+              "qkv must be [tokens,>=(q_heads+k_heads)*128] with dense rows");
+  const int64_t n = qkv.size(0);
+  TORCH_CHECK(n <= 1 || qkv.stride(0) >= (q_heads + k_heads) * kDim, "qkv rows must not overlap");
+  for (const at::Tensor* t : {&q_weight, &k_weight})
+    TORCH_CHECK(t->device() == qkv.device() && t->is_contiguous() && floats(*t) &&
+                    t->numel() == kDim,
+                "weights must be contiguous CUDA FP32/BF16 [128]");
+  TORCH_CHECK(positions.device() == qkv.device() &&
+                  (positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong) &&
+                  positions.dim() == 1 && positions.size(0) == n && positions.is_contiguous(),
+              "positions must be contiguous CUDA int32/int64 [tokens]");
+  const int64_t rotary = 2 * inv_freq.numel();
+  TORCH_CHECK(inv_freq.device() == qkv.device() && inv_freq.scalar_type() == at::kFloat &&
+                  inv_freq.dim() == 1 && inv_freq.is_contiguous() && rotary <= kDim &&
+                  (interleaved || rotary % 16 == 0),
+              "inv_freq must be contiguous CUDA FP32 [rotary/2], rotary at most 128 and a multiple "
+              "of 16 unless interleaved");
+  TORCH_CHECK(eps > 0, "norm epsilon must be positive");
+  if (n == 0 || q_heads + k_heads == 0) return;
+  ld_norm_rope_args args{};
+  args.qkv = qkv.data_ptr();
+  args.qkv_row_stride = qkv.stride(0);
+  args.q_weight = q_weight.data_ptr();
+  args.k_weight = k_weight.data_ptr();
+  args.q_weight_dtype = dtype_code(q_weight);
+  args.k_weight_dtype = dtype_code(k_weight);
+  args.positions = positions.data_ptr();
+  args.positions_int64 = positions.scalar_type() == at::kLong;
+  args.rotary = static_cast<int32_t>(rotary);
+  args.inv_freq = static_cast<const float*>(inv_freq.data_ptr());
+  args.num_tokens = n;
+  args.q_heads = static_cast<int32_t>(q_heads);
+  args.k_heads = static_cast<int32_t>(k_heads);
+  args.interleaved = interleaved;
+  args.eps = static_cast<float>(eps);
+  const c10::DeviceGuard guard(qkv.device());
+  const int rc = ld_norm_rope(&args, stream_of(qkv));
+  TORCH_CHECK(rc == LD_OK, ld_last_error());
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(lightdelta, CUDA, m) {
@@ -388,6 +583,9 @@ TORCH_LIBRARY_IMPL(lightdelta, CUDA, m) {
   m.impl("copy_state_checked", &copy_state_checked);
   m.impl("zero_slots", &zero_slots);
   m.impl("packed_plan", &packed_plan);
+  m.impl("linear_decode", &linear_decode);
+  m.impl("linear_prefill", &linear_prefill);
+  m.impl("norm_rope", &norm_rope);
 }
 
 // The state cache policy these kernels pass (LD_CACHE_KEEP / LD_CACHE_STREAM), set from

@@ -40,11 +40,25 @@ Additive ops (no reference counterpart):
                                         state_io = "packed") in one launch: each request's
                                         source slot and validity, its scratch rows, and the
                                         slots its per-token states go back to
+  linear_decode(qkv, log_decay, indices, cu, accepted, state, gate, weight, out, scale, eps)
+                                        linear attention with a decay for each head, S <-
+                                        exp(g) S + v k^T, o = scale S q, on the same pool and
+                                        request metadata as decode (1 to 4 tokens a request);
+                                        log_decay fp32 [HV] or [tokens, HV]; with gate and
+                                        weight the gated RMSNorm of o, with both None o itself
+  linear_prefill(qkv, log_decay, slots, has_initial, cu_seqlens, state, gate, weight, out,
+                 scale, eps)            the same for prompts, metadata as prefill's
+  norm_rope(qkv, q_weight, k_weight, positions, inv_freq, q_heads, k_heads, eps, interleaved)
+                                        RMSNorm of every q and k head with its weight and the
+                                        rotation of its first 2 * len(inv_freq) elements by
+                                        positions * inv_freq, in place on qkv's first
+                                        (q_heads + k_heads) * 128 columns
 
 Every kernel launches on the caller's current stream and reads no device memory on the host,
 so it can be captured in a HIP graph.  None allocates, except prefill's chunked form, which
 keeps one workspace per device and stream for later eager calls (release_prefill_workspaces
-frees them) and gives a call under graph capture a workspace the graph keeps.  The kernels of every op but prefill are C++ (csrc/torch_ops.cpp,
+frees them) and gives a call under graph capture a workspace the graph keeps, and
+linear_prefill, which takes a long prompt's workspace from torch's allocator for the call.  The kernels of every op but prefill are C++ (csrc/torch_ops.cpp,
 liblightdelta_torch.so); the check_* functions below restate their argument checks so they
 can run without a GPU.
 """
@@ -52,6 +66,7 @@ can run without a GPU.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 from pathlib import Path
 
@@ -89,6 +104,20 @@ SCHEMAS = {
         "Tensor(v!) valid, Tensor(i!) indices, Tensor(d!) destinations) -> ()"
     ),
     "scatter_slots": "scatter_slots(Tensor packed, Tensor slots, Tensor(p!) pool) -> ()",
+    "linear_decode": (
+        "linear_decode(Tensor qkv, Tensor log_decay, Tensor indices, Tensor cu, Tensor accepted, "
+        "Tensor(s!) state, Tensor? gate, Tensor? weight, Tensor(o!) out, float scale, float eps) "
+        "-> ()"
+    ),
+    "linear_prefill": (
+        "linear_prefill(Tensor qkv, Tensor log_decay, Tensor slots, Tensor has_initial, "
+        "Tensor cu_seqlens, Tensor(s!) state, Tensor? gate, Tensor? weight, Tensor(o!) out, "
+        "float scale, float eps) -> ()"
+    ),
+    "norm_rope": (
+        "norm_rope(Tensor(q!) qkv, Tensor q_weight, Tensor k_weight, Tensor positions, "
+        "Tensor inv_freq, int q_heads, int k_heads, float eps, bool interleaved) -> ()"
+    ),
 }
 
 HEAD_DIM = _lib.HEAD_DIM
@@ -515,6 +544,107 @@ def check_zero(pool, slots):
 
 
 # ---------------------------------------------------------------------------------------
+# linear attention: the checks of the C++ kernels (csrc/torch_ops.cpp), restated
+# ---------------------------------------------------------------------------------------
+
+
+def _linear_layout(qkv, log_decay, state, gate, weight, out, scale, eps):
+    """What linear_decode and linear_prefill share; returns (H, HV)."""
+    _require(_is_gpu(qkv) and qkv.dtype == torch.bfloat16, "qkv must be CUDA BF16")
+    _require(
+        state.device == qkv.device and state.dtype == torch.float32 and state.dim() == 4
+        and tuple(state.shape[2:]) == (HEAD_DIM, HEAD_DIM)
+        and tuple(state.stride()[1:]) == (HEAD_DIM * HEAD_DIM, HEAD_DIM, 1),
+        "state must be CUDA FP32 [slots,HV,128,128] with dense heads",
+    )
+    h, hv = decode_geometry(qkv, state)
+    _require(qkv.dim() == 2 and h > 0 and qkv.stride(1) == 1,
+             "qkv must be [tokens,(2*H+HV)*128] with HV a multiple of H")
+    n = qkv.shape[0]
+    _require(
+        log_decay.device == qkv.device and log_decay.dtype == torch.float32
+        and tuple(log_decay.shape) in ((hv,), (n, hv)) and log_decay.stride(-1) == 1,
+        "log_decay must be CUDA FP32 [HV] or [tokens,HV] with dense rows",
+    )
+    _require(
+        out.device == qkv.device and out.dtype == torch.bfloat16
+        and tuple(out.shape) == (n, hv, HEAD_DIM) and out.is_contiguous(),
+        "out must be contiguous CUDA BF16 [tokens,HV,128]",
+    )
+    _require((gate is None) == (weight is None), "gate and weight must be given together")
+    if gate is not None:
+        _require(
+            gate.device == qkv.device and gate.dtype == torch.bfloat16
+            and tuple(gate.shape) == (n, hv, HEAD_DIM)
+            and tuple(gate.stride()[1:]) == (HEAD_DIM, 1),
+            "gate must be CUDA BF16 [tokens,HV,128] with dense rows",
+        )
+        _require(
+            weight.device == qkv.device and weight.is_contiguous() and weight.dtype in _FLOATS
+            and weight.numel() == HEAD_DIM,
+            "weight must be contiguous CUDA FP32/BF16 [128]",
+        )
+    _require(math.isfinite(scale), "scale must be finite")
+    _require(eps > 0, "norm epsilon must be positive")
+    return h, hv
+
+
+def check_linear_decode(qkv, log_decay, indices, cu, accepted, state, gate, weight, out, scale,
+                        eps):
+    """Validation of linear_decode; returns (H, HV)."""
+    heads = _linear_layout(qkv, log_decay, state, gate, weight, out, scale, eps)
+    for t in (indices, cu, accepted):
+        _require(t.device == qkv.device and t.dtype == torch.int32 and t.is_contiguous(),
+                 "metadata must be contiguous CUDA int32")
+    _require(indices.dim() == 2 and 1 <= indices.shape[1] <= _lib.MAX_TOKENS,
+             "decode/MTP supports 1 through 4 tokens per request")
+    requests = indices.shape[0]
+    _require(tuple(cu.shape) == (requests + 1,) and tuple(accepted.shape) == (requests,),
+             "invalid request metadata shapes")
+    return heads
+
+
+def check_linear_prefill(qkv, log_decay, slots, has_initial, cu_seqlens, state, gate, weight, out,
+                         scale, eps):
+    """Validation of linear_prefill; returns (H, HV)."""
+    heads = _linear_layout(qkv, log_decay, state, gate, weight, out, scale, eps)
+    for t in (slots, cu_seqlens):
+        _require(t.device == qkv.device and t.dtype == torch.int32 and t.dim() == 1
+                 and t.is_contiguous(), "metadata must be contiguous CUDA int32")
+    _require(has_initial.device == qkv.device and has_initial.dtype == torch.bool
+             and has_initial.dim() == 1 and has_initial.is_contiguous(),
+             "has_initial must be a contiguous CUDA bool vector")
+    _require(cu_seqlens.numel() == slots.numel() + 1 and has_initial.numel() == slots.numel(),
+             "invalid sequence metadata shapes")
+    return heads
+
+
+def check_norm_rope(qkv, q_weight, k_weight, positions, inv_freq, q_heads, k_heads, eps,
+                    interleaved):
+    """Validation of norm_rope."""
+    _require(_is_gpu(qkv) and qkv.dtype == torch.bfloat16, "qkv must be CUDA BF16")
+    columns = (q_heads + k_heads) * HEAD_DIM
+    _require(q_heads >= 0 and k_heads >= 0 and qkv.dim() == 2 and qkv.shape[1] >= columns
+             and qkv.stride(1) == 1,
+             "qkv must be [tokens,>=(q_heads+k_heads)*128] with dense rows")
+    n = qkv.shape[0]
+    _require(n <= 1 or qkv.stride(0) >= columns, "qkv rows must not overlap")
+    for t in (q_weight, k_weight):
+        _require(t.device == qkv.device and t.is_contiguous() and t.dtype in _FLOATS
+                 and t.numel() == HEAD_DIM, "weights must be contiguous CUDA FP32/BF16 [128]")
+    _require(positions.device == qkv.device and positions.dtype in (torch.int32, torch.int64)
+             and tuple(positions.shape) == (n,) and positions.is_contiguous(),
+             "positions must be contiguous CUDA int32/int64 [tokens]")
+    rotary = 2 * inv_freq.numel()
+    _require(inv_freq.device == qkv.device and inv_freq.dtype == torch.float32
+             and inv_freq.dim() == 1 and inv_freq.is_contiguous() and rotary <= HEAD_DIM
+             and (interleaved or rotary % 16 == 0),
+             "inv_freq must be contiguous CUDA FP32 [rotary/2], rotary at most 128 and a "
+             "multiple of 16 unless interleaved")
+    _require(eps > 0, "norm epsilon must be positive")
+
+
+# ---------------------------------------------------------------------------------------
 # registration
 # ---------------------------------------------------------------------------------------
 
@@ -522,7 +652,8 @@ def check_zero(pool, slots):
 # path is on every decode step.  prefill's kernel is the Python function below (it keeps the
 # chunked form's workspace cache and the algorithm choice).
 _CXX_KERNELS = ("decode", "decode_conv", "gather_state", "scatter_state", "gather_slots",
-                "scatter_slots", "copy_state", "copy_state_checked", "zero_slots", "packed_plan")
+                "scatter_slots", "copy_state", "copy_state_checked", "zero_slots", "packed_plan",
+                "linear_decode", "linear_prefill", "norm_rope")
 _IMPLS = {
     "prefill": _prefill_impl,
 }
