@@ -4,16 +4,21 @@
 //   o_t = scale (e^(c_t) S q_t + sum over s <= t of e^(c_t - c_s) (k_s . q_t) v_s)
 //   S'  = e^(c_63) S + sum over s of k_s (e^(c_63 - c_s) v_s)^T
 //
-// A workgroup of four waves walks the chunks of one (sequence, v-head).  Wave w owns state rows
-// v = 32 w .. 32 w + 31 as S^T in the accumulator layout of v_mfma_f32_32x32x16_bf16, with the
-// summation index assigned as in prefill_heads.hip: for lane l, lj = l % 32 and hi = l / 32, an
-// accumulator holds rows i(r) = 8 (r / 4) + 4 hi + r % 4, r < 16, of column lj, so its registers
-// 8 u .. 8 u + 7, split into bf16 planes, are directly the operand of step u of the next product.
+// A workgroup of eight waves walks the chunks of one (sequence, v-head).  Wave w owns state rows
+// v = 16 w .. 16 w + 15 as S^T in the accumulators of v_mfma_f32_16x16x32_bf16: for lane l,
+// li = l % 16 and lg = l / 16, an accumulator holds rows 4 lg + r, r < 4, of column li, an operand
+// A[i = li][k = 8 lg + e] or B[k = 8 lg + e][j = li], e < 8.  The summation index may be assigned
+// to (step, lg, e) freely as long as both operands agree, so two accumulators, split into bf16
+// planes, are directly the operand of a step of the next product:
+//   keys     row 4 lg + r of accumulators (n, a) is k = 32 n + 8 lg + 4 a + r, so that step n takes
+//            16 consecutive bytes of a q row
+//   tokens   step i takes token 32 i + 16 (e / 4) + 4 lg + e % 4
 //   O = Q S^T          S as two planes
-//   P = (K Q^T) . D    a strip of 16 tokens t a wave, two planes, exchanged through LDS
+//   P = (K Q^T) . D    16 x 16 blocks over the waves, two planes, exchanged through LDS
 //   O = diag(e^c) O + P V
 //   S' = e^(c_63) S + K^T (e^(c_63 - c) V)    e V as three planes
-// and O crosses LDS in fp32 to whole rows, for the norm and 16-byte stores.
+// and O crosses LDS in fp32 to whole rows, for the norm and 16-byte stores.  The transposed
+// operands come by ds_read_b64_tr_b16.
 //
 // Decays come from differences of 64-bit prefix sums: their error over thousands of tokens would
 // be the state's.  Roundings to fewer than 32 bits, each of operands of the bf16 matrix cores
@@ -31,13 +36,15 @@
 namespace ld {
 namespace {
 
+constexpr int kBlockWaves = 8;
+constexpr int kBlock = 64 * kBlockWaves;
 constexpr int kTokens = 64;                     // tokens per chunk
 constexpr int kRowsBytes = kTokens * kTileRow;  // q, k or v of a chunk
 constexpr int64_t kTileFloats = kDim * kDim;
 
 // Per-token scalars of a chunk: c in units of log 2 as a sum of two floats, scale * e^c and
 // e^(c_63 - c); and e^(c_63).
-struct ChunkScalars {
+struct alignas(16) ChunkScalars {
   float hi[kTokens], lo[kTokens], eq[kTokens], ek[kTokens];
   float gamma;
 };
@@ -48,11 +55,11 @@ struct SegmentLds {
   alignas(16) uint8_t q[kRowsBytes];
   alignas(16) uint8_t v[kRowsBytes];
   alignas(16) uint8_t p[2][kTokens * kTokens * 2];
-  alignas(16) ChunkScalars scalars[2];
+  ChunkScalars scalars[2];
   alignas(16) float weight[kDim];
 };
 struct SearchLds {
-  int wave_sums[kWaves];
+  int wave_sums[kBlockWaves];
   int found[3];
 };
 static_assert(2 * (sizeof(SegmentLds) + sizeof(SearchLds)) <= 160 * 1024, "two workgroups a CU");
@@ -130,16 +137,14 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lj = lane & 31;
-  const int hi = lane >> 5;
   const int li = lane & 15;
   const int lg = lane >> 4;
   const int key_head = head / p.group;
   const int chunks = (rows + kTokens - 1) / kTokens;
 
-  // ---- a chunk's rows, in registers on their way to LDS: row 16 i + srow, 16 bytes ----
+  // ---- a chunk's rows, in registers on their way to LDS: row 32 i + srow, 16 bytes ----
   struct Staged {
-    u32x4 q[4], k[4], v[4];
+    u32x4 q[2], k[2], v[2];
   } staged;
   const int srow = tid >> 4;
   const int spiece = tid & 15;
@@ -150,26 +155,25 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
     const int live = min(kTokens, rows - c * kTokens);
     const int64_t first = bos + static_cast<int64_t>(c) * kTokens;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = srow + 16 * i;
-      const uint16_t* const row = columns + (first + min(r, live - 1)) * p.qkv_row;
+    for (int i = 0; i < 2; ++i) {
+      const uint16_t* const row = columns + (first + min(srow + 32 * i, live - 1)) * p.qkv_row;
       __builtin_memcpy(&staged.k[i], row + k_col, 16);
       __builtin_memcpy(&staged.v[i], row + v_col, 16);
       if constexpr (Out) __builtin_memcpy(&staged.q[i], row, 16);
     }
     if (live < kTokens) {   // rows past the end are zeros
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (srow + 16 * i >= live) {
+      for (int i = 0; i < 2; ++i)
+        if (srow + 32 * i >= live) {
           staged.k[i] = staged.v[i] = u32x4{0u, 0u, 0u, 0u};
           if constexpr (Out) staged.q[i] = u32x4{0u, 0u, 0u, 0u};
         }
     }
   };
   const uint32_t dst = srow * kTileRow + ((spiece ^ swizzle(srow)) << 4);
-  auto put = [&](uint8_t* tile, const u32x4 (&x)[4]) __attribute__((always_inline)) {
+  auto put = [&](uint8_t* tile, const u32x4 (&x)[2]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(tile + dst + 16 * i * kTileRow) = x[i];
+    for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4*>(tile + dst + 32 * i * kTileRow) = x[i];
   };
   auto load_decay = [&](int c) __attribute__((always_inline)) {
     const int t = c * kTokens + lane;
@@ -182,39 +186,36 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
     if (w == 0) total += chunk_scalars(lds.scalars[0], load_decay(0), p.scale, lane);
   }
 
-  // st[T][8 u + 4 h + r] = S[32 w + lj][32 T + 16 u + 8 hi + 4 h + r]
-  f32x16 st[4];
-  const int tile_at = (32 * w + lj) * kDim + 8 * hi;
+  // st[n][a][r] = S[16 w + li][32 n + 8 lg + 4 a + r]
+  f32x4 st[4][2];
+  const int tile_at = (16 * w + li) * kDim + 8 * lg;
 #pragma unroll
-  for (int T = 0; T < 4; ++T)
+  for (int n = 0; n < 4; ++n)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int a = 0; a < 2; ++a) {
+      st[n][a] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       if (start != nullptr)
-        x = *reinterpret_cast<const f32x4*>(start + tile_at + 32 * T + 16 * (q >> 1) + 4 * (q & 1));
-#pragma unroll
-      for (int r = 0; r < 4; ++r) st[T][4 * q + r] = x[r];
+        st[n][a] = *reinterpret_cast<const f32x4*>(start + tile_at + 32 * n + 4 * a);
     }
 
   // lane addresses of the operands (the parts of the swizzle that depend on the step are XORed in)
-  const uint32_t a_at = lj * kTileRow + ((hi ^ swizzle(lj)) << 4);       // ^ ((4 T + 2 u) << 4)
-  const uint32_t strip_at = li * kTileRow + ((lg ^ swizzle(li)) << 4);   // ^ (step << 6)
-  const int m = lane & 15;
-  const int c16 = (lane >> 4) & 1;
-  const uint32_t tr_row = (4 * hi + (m >> 2)) * kTileRow;
-  // transposed k: rows 16 u + 8 h + .., columns in the accumulator's order   ^ (T << 6) ^ (h << 5)
-  const uint32_t kt_at =
-      tr_row + (((2 * c16 + (m & 1)) ^ ((m >> 2) << 2) ^ hi) << 4) + ((m >> 1) & 1) * 8;
-  // transposed v: rows 8 q + .., the wave's columns   ^ ((q & 1) << 5)
-  const uint32_t vt_at =
-      tr_row + (((4 * w + 2 * c16 + ((m & 3) >> 1)) ^ ((m >> 2) << 2) ^ hi) << 4) + (m & 1) * 8;
-  // P[t][s] of a plane: the quad of s at 16 u + 8 a + 4 hi is half a of row t's 16-byte piece
-  // 2 u + hi, the pieces of a row XORed with t % 8
-  const uint32_t p_at = lj * (2 * kTokens) + ((hi ^ (lj & 7)) << 4);     // ^ (u << 5)
-  // O in fp32: row t's 16-byte pieces XORed with the parity of t and 8 (t / 4 % 2)
-  const int row = tid >> 2;
-  const int part = tid & 3;
-  const int o_swizzle = (row & 1) | (((row >> 2) & 1) << 3);
+  uint32_t a_at = li * kTileRow + ((lg ^ swizzle(li)) << 4);       // ^ (step << 6)
+  const int quad = li >> 2;
+  const uint32_t tr_row = (4 * lg + quad) * kTileRow;
+  // transposed k: rows 32 s + 16 h + .., columns 32 n + 8 (i / 4) + 4 a + i % 4   ^ (n << 6)
+  uint32_t kt_at = tr_row + (((li & 3) ^ (quad << 2) ^ lg) << 4);
+  // transposed v: rows 32 s + 16 h + .., the wave's columns
+  const uint32_t vt_at = tr_row + (((2 * w + ((li & 3) >> 1)) ^ (quad << 2) ^ lg) << 4) + (li & 1) * 8;
+  // P[t][s] of a plane: the quad of s at 32 i + 16 a + 4 lg is half a of row t's 16-byte piece
+  // 4 i + lg, the pieces of a row XORed with t % 8
+  uint32_t p_at = li * (2 * kTokens) + ((lg ^ (li & 7)) << 4);     // ^ (i << 6)
+  // the wave's part of P: rows of strip w / 2; columns 16 w % 2 of the first two, 32 (w % 2) and
+  // 16 more of the others
+  const int strip = w >> 1;
+  // O in fp32: row t's 16-byte pieces XORed with 4 (t / 4 % 4)
+  const int row = tid >> 3;
+  const int part = tid & 7;
+  const int o_at = row * kDim + (((2 * part) ^ (((row >> 2) & 3) << 2)) << 2);
 
   if (chunks > 0) {
     put(lds.k, staged.k);
@@ -225,39 +226,45 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
     const ChunkScalars& s = lds.scalars[c & 1];
     const bool more = c + 1 < chunks;
     float next_g = 0.0f;
+    // (opaque here, so that their XORed forms are made where they are used, not held in registers
+    // over the loop)
+    pin(a_at);
+    pin(kt_at);
+    pin(p_at);
     lds_barrier();   // the chunk's rows and scalars are in LDS
     if (more) fetch(c + 1);
     if (more && w == 0) next_g = load_decay(c + 1);
-    f32x16 o[2];
+    f32x4 o[4];
     const float gamma = s.gamma;
     if constexpr (Out) {
-      // ---- P: tokens t = 16 w .. of the chunk against s <= t ----
+      // ---- P ----
       bf16x8 qf[4];
 #pragma unroll
       for (int step = 0; step < 4; ++step)
-        qf[step] = *reinterpret_cast<const bf16x8*>(lds.q + 16 * w * kTileRow +
-                                                    (strip_at ^ (step << 6)));
-      const float thi = s.hi[16 * w + li], tlo = s.lo[16 * w + li];
+        qf[step] = *reinterpret_cast<const bf16x8*>(lds.q + 16 * strip * kTileRow +
+                                                    (a_at ^ (step << 6)));
+      const float thi = s.hi[16 * strip + li], tlo = s.lo[16 * strip + li];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (j > (w | 1)) break;   // 32 x 32 blocks above the diagonal are not read
+      for (int i = 0; i < 2; ++i) {
+        if (i == 1 && strip < 2) break;
+        const int j = strip < 2 ? w & 1 : 2 * (w & 1) + i;
         f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (j <= w) {
+        if (j <= strip) {
 #pragma unroll
           for (int step = 0; step < 4; ++step)
             x = mfma16(*reinterpret_cast<const bf16x8*>(lds.k + 16 * j * kTileRow +
-                                                        (strip_at ^ (step << 6))),
+                                                        (a_at ^ (step << 6))),
                        qf[step], x);
           const f32x4 shi = *reinterpret_cast<const f32x4*>(&s.hi[16 * j + 4 * lg]);
           const f32x4 slo = *reinterpret_cast<const f32x4*>(&s.lo[16 * j + 4 * lg]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float d = __builtin_amdgcn_exp2f((thi - shi[r]) + (tlo - slo[r])) * p.scale;
-            x[r] = j < w || 4 * lg + r <= li ? x[r] * d : 0.0f;
+            x[r] = j < strip || 4 * lg + r <= li ? x[r] * d : 0.0f;
           }
         }
-        uint8_t* const at = lds.p[0] + (16 * w + li) * (2 * kTokens) +
-                            (((2 * j + (lg & 1)) ^ (li & 7)) << 4) + (lg >> 1) * 8;
+        uint8_t* const at = lds.p[0] + (16 * strip + li) * (2 * kTokens) +
+                            (((4 * (j >> 1) + lg) ^ (li & 7)) << 4) + (j & 1) * 8;
 #pragma unroll
         for (int plane = 0; plane < 2; ++plane) {
           const uint2 bits = {bf16_pair(f32x2{x[0], x[1]}), bf16_pair(f32x2{x[2], x[3]})};
@@ -268,128 +275,128 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
           x[3] -= __builtin_bit_cast(float, bits.y & 0xffff0000u);
         }
       }
-      // ---- O = Q S^T, and S scaled once it is split ----
-      o[0] = o[1] = f32x16{};
+      // ---- O = Q S^T ----
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const int T = n >> 1, u = n & 1;
+      for (int tt = 0; tt < 4; ++tt) o[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = st[T][8 * u + e];
+        for (int e = 0; e < 8; ++e) x[e] = st[n][e >> 2][e & 3];
         const Planes<2> split(x);
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-          const bf16x8 a = *reinterpret_cast<const bf16x8*>(lds.q + 32 * tt * kTileRow +
-                                                            (a_at ^ (n << 5)));
-          o[tt] = mfma32(a, split[1], o[tt]);
-          o[tt] = mfma32(a, split[0], o[tt]);
+        for (int tt = 0; tt < 4; ++tt) {
+          const bf16x8 a = *reinterpret_cast<const bf16x8*>(lds.q + 16 * tt * kTileRow +
+                                                            (a_at ^ (n << 6)));
+          o[tt] = mfma16(a, split[1], o[tt]);
+          o[tt] = mfma16(a, split[0], o[tt]);
         }
       }
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 eq = *reinterpret_cast<const f32x4*>(&s.eq[32 * tt + 8 * q + 4 * hi]);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[tt][4 * q + r] *= eq[r];
-        }
+      for (int tt = 0; tt < 4; ++tt) {
+        const f32x4 eq = *reinterpret_cast<const f32x4*>(&s.eq[16 * tt + 4 * lg]);
+        o[tt] *= eq;
+      }
     }
 #pragma unroll
-    for (int T = 0; T < 4; ++T) st[T] *= gamma;
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int a = 0; a < 2; ++a) st[n][a] *= gamma;
     if constexpr (Out) lds_barrier();   // P is in LDS
     if (more && w == 0)
       total += chunk_scalars(lds.scalars[(c + 1) & 1], next_g, p.scale, lane);
 
-    // ---- O += P V and S += K^T (e V), 16 tokens a step ----
-    u32x4 gate[4];
+    // ---- O += P V and S += K^T (e V), 32 tokens a step ----
+    u32x4 gate[2];
     const int64_t token = bos + static_cast<int64_t>(c) * kTokens + row;
     const bool stored = c * kTokens + row < rows;
     if constexpr (Out) {
       if (p.gate != nullptr && stored) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          __builtin_memcpy(&gate[i], p.gate + token * p.gate_row + head * kDim + 8 * part + 32 * i, 16);
+        for (int i = 0; i < 2; ++i)
+          __builtin_memcpy(&gate[i], p.gate + token * p.gate_row + head * kDim + 8 * part + 64 * i, 16);
       }
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const bf16x8 v = join(read_tr(lds.v + vt_at + 16 * u * kTileRow),
-                            read_tr(lds.v + (vt_at ^ (1 << 5)) + (16 * u + 8) * kTileRow));
+    for (int i = 0; i < 2; ++i) {
+      const bf16x8 v = join(read_tr(lds.v + vt_at + 32 * i * kTileRow),
+                            read_tr(lds.v + vt_at + (32 * i + 16) * kTileRow));
       if constexpr (Out) {
 #pragma unroll
-        for (int tt = u < 2 ? 0 : 1; tt < 2; ++tt)
+        for (int tt = 2 * i; tt < 4; ++tt)
 #pragma unroll
           for (int plane = 1; plane >= 0; --plane)
-            o[tt] = mfma32(*reinterpret_cast<const bf16x8*>(
-                               lds.p[plane] + 32 * tt * (2 * kTokens) + (p_at ^ (u << 5))),
+            o[tt] = mfma16(*reinterpret_cast<const bf16x8*>(
+                               lds.p[plane] + 16 * tt * (2 * kTokens) + (p_at ^ (i << 6))),
                            v, o[tt]);
       }
       float x[8];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const f32x4 ek = *reinterpret_cast<const f32x4*>(&s.ek[16 * u + 8 * h + 4 * hi]);
+        const f32x4 ek = *reinterpret_cast<const f32x4*>(&s.ek[32 * i + 16 * h + 4 * lg]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[4 * h + r] = static_cast<float>(v[4 * h + r]) * ek[r];
       }
       const Planes<3> split(x);
 #pragma unroll
-      for (int T = 0; T < 4; ++T) {
-        const bf16x8 k = join(read_tr(lds.k + (kt_at ^ (T << 6)) + 16 * u * kTileRow),
-                              read_tr(lds.k + (kt_at ^ (T << 6) ^ (1 << 5)) + (16 * u + 8) * kTileRow));
+      for (int n = 0; n < 4; ++n)
 #pragma unroll
-        for (int plane = 2; plane >= 0; --plane) st[T] = mfma32(k, split[plane], st[T]);
-      }
+        for (int a = 0; a < 2; ++a) {
+          const uint8_t* const at = lds.k + (kt_at ^ (n << 6)) + 8 * a;
+          const bf16x8 k = join(read_tr(at + 32 * i * kTileRow), read_tr(at + (32 * i + 16) * kTileRow));
+#pragma unroll
+          for (int plane = 2; plane >= 0; --plane) st[n][a] = mfma16(k, split[plane], st[n][a]);
+        }
     }
     lds_barrier();   // every read of the chunk's rows and P is done
     if constexpr (Out) {
       float* const o_rows = reinterpret_cast<float*>(lds.k);
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
+      for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int t = 32 * tt + 8 * (r >> 2) + 4 * hi + (r & 3);
-          const int piece = (8 * w + (lj >> 2)) ^ ((r & 1) | (hi << 3));
-          o_rows[t * kDim + piece * 4 + (lj & 3)] = o[tt][r];
-        }
+        for (int r = 0; r < 4; ++r)
+          o_rows[(16 * tt + 4 * lg + r) * kDim + (((4 * w + (li >> 2)) ^ (lg << 2)) << 2) + (li & 3)] =
+              o[tt][r];
       if (more) put(lds.v, staged.v);
       lds_barrier();   // O is in LDS
-      // ---- a quarter of one row a thread: columns 8 part + 32 i .. + 7 ----
-      float y[4][8];
+      // ---- an eighth of one row a thread: columns 8 part + 64 i .. + 7 ----
+      float y[2][8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const f32x4 x = *reinterpret_cast<const f32x4*>(
-              o_rows + row * kDim + (((2 * part + 8 * i + h) ^ o_swizzle) << 2));
+              o_rows + o_at + 64 * i + 4 * h);
 #pragma unroll
           for (int e = 0; e < 4; ++e) y[i][4 * h + e] = x[e];
         }
       if (p.gate != nullptr) {
         float ss = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 8; ++e) ss = fmaf(y[i][e], y[i][e], ss);
         ss += dpp<kDppQuadXor1>(ss);
         ss += dpp<kDppQuadXor2>(ss);
+        ss += dpp<kDppRowHalfMirror>(ss);
         const float rstd = fast_rsqrt(ss * (1.0f / kDim) + p.eps);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const uint32_t pair = gate[i][e >> 1];
             const float g = __builtin_bit_cast(float, e & 1 ? pair & 0xffff0000u : pair << 16);
-            y[i][e] = ((y[i][e] * rstd) * lds.weight[8 * part + 32 * i + e]) * silu(g);
+            y[i][e] = ((y[i][e] * rstd) * lds.weight[8 * part + 64 * i + e]) * silu(g);
           }
       }
       if (stored) {
         uint16_t* const to = p.out + (token * p.num_v_heads + head) * kDim + 8 * part;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
           u32x4 bits;
 #pragma unroll
           for (int e = 0; e < 4; ++e) bits[e] = bf16_pair(f32x2{y[i][2 * e], y[i][2 * e + 1]});
-          __builtin_memcpy(to + 32 * i, &bits, 16);
+          __builtin_memcpy(to + 64 * i, &bits, 16);
         }
       }
       lds_barrier();   // O is read
@@ -405,11 +412,10 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
 
   if (end != nullptr) {
 #pragma unroll
-    for (int T = 0; T < 4; ++T)
+    for (int n = 0; n < 4; ++n)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<f32x4*>(end + tile_at + 32 * T + 16 * (q >> 1) + 4 * (q & 1)) =
-            f32x4{st[T][4 * q], st[T][4 * q + 1], st[T][4 * q + 2], st[T][4 * q + 3]};
+      for (int a = 0; a < 2; ++a)
+        *reinterpret_cast<f32x4*>(end + tile_at + 32 * n + 4 * a) = st[n][a];
   }
   return total;
 }
@@ -428,7 +434,7 @@ __device__ bool find_segment(const LinearParams& p, SearchLds& lds, int num_sequ
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   int base = 0;
-  for (int first = 0; first < num_sequences; first += kThreads) {
+  for (int first = 0; first < num_sequences; first += kBlock) {
     const int n = first + tid;
     int mine = 0;
     if (n < num_sequences) {
@@ -447,7 +453,7 @@ __device__ bool find_segment(const LinearParams& p, SearchLds& lds, int num_sequ
     __syncthreads();
     int all = 0;
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) {
+    for (int v = 0; v < kBlockWaves; ++v) {
       if (v < tid >> 6) sum += lds.wave_sums[v];
       all += lds.wave_sums[v];
     }
@@ -498,7 +504,7 @@ __device__ __forceinline__ void load_weight(const LinearParams& p, SegmentLds& l
 // The first launch.  Item j < later is later segment j's predecessor: the sequence's first
 // segment, walked from its state, or a middle one, reduced to its update; item later + n is
 // sequence n if it is a single segment.
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(4, 4)))
 void linear_first_kernel(const LinearParams p, const Segments g) {
   __shared__ SegmentLds lds;
   __shared__ SearchLds search;
@@ -528,12 +534,13 @@ void linear_first_kernel(const LinearParams p, const Segments g) {
              live && p.has_initial[seq] != 0 ? home : nullptr, whole ? (live ? home : nullptr) : tile);
 }
 
-// The second: the state at every later segment's start, along each sequence; a sixteenth of a
-// tile a workgroup.
-__global__ __launch_bounds__(kThreads) void linear_join_kernel(const LinearParams p, const Segments g) {
+// The second: the state at every later segment's start, along each sequence; an eighth of a tile
+// a workgroup.
+constexpr int kJoinParts = kTileFloats / 4 / kBlock;
+__global__ __launch_bounds__(kBlock) void linear_join_kernel(const LinearParams p, const Segments g) {
   __shared__ SearchLds search;
-  const int part = blockIdx.x & 15;
-  const int pair = blockIdx.x >> 4;
+  const int part = blockIdx.x % kJoinParts;
+  const int pair = blockIdx.x / kJoinParts;
   const int j = pair / p.num_v_heads;
   const int head = pair - j * p.num_v_heads;
   int seq, index, count;
@@ -541,7 +548,7 @@ __global__ __launch_bounds__(kThreads) void linear_join_kernel(const LinearParam
   count = min(count, g.later - j);
   const int64_t step = p.num_v_heads * kTileFloats;
   float* at = g.tiles + (static_cast<int64_t>(j) * p.num_v_heads + head) * kTileFloats +
-              (part * kThreads + threadIdx.x) * 4;
+              (part * kBlock + threadIdx.x) * 4;
   const float* decay = g.decays + static_cast<int64_t>(j) * p.num_v_heads + head;
   f32x4 s = *reinterpret_cast<const f32x4*>(at);
   for (int i = 1; i < count; ++i) {
@@ -553,7 +560,7 @@ __global__ __launch_bounds__(kThreads) void linear_join_kernel(const LinearParam
 }
 
 // The third: the later segments, each from its state.
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(4, 4)))
 void linear_later_kernel(const LinearParams p, const Segments g) {
   __shared__ SegmentLds lds;
   __shared__ SearchLds search;
@@ -619,7 +626,7 @@ extern "C" int ld_linear_prefill(const ld_linear_prefill_args* args, void* strea
   auto blocks_of = [&](int64_t items) {
     return (items * a.num_k_heads + 7) / 8 * 8 * p.group;
   };
-  if (blocks_of(later + a.num_sequences) > 0xffffff || later * a.num_v_heads * 16 > 0xffffff)
+  if (blocks_of(later + a.num_sequences) > 0x7fffff || later * a.num_v_heads * kJoinParts > 0x7fffff)
     return fail(LD_ERR_INVALID_ARGUMENT, "too many (sequence, head) tiles");
   Segments g{};
   g.num_sequences = a.num_sequences;
@@ -629,12 +636,12 @@ extern "C" int ld_linear_prefill(const ld_linear_prefill_args* args, void* strea
   g.decays = g.tiles + later * a.num_v_heads * kTileFloats;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(linear_first_kernel, dim3(static_cast<uint32_t>(blocks_of(later + a.num_sequences))),
-                     dim3(kThreads), 0, s, p, g);
+                     dim3(kBlock), 0, s, p, g);
   if (later > 1)   // (a lone later segment starts from what the first launch left)
-    hipLaunchKernelGGL(linear_join_kernel, dim3(static_cast<uint32_t>(later * a.num_v_heads * 16)),
-                       dim3(kThreads), 0, s, p, g);
+    hipLaunchKernelGGL(linear_join_kernel, dim3(static_cast<uint32_t>(later * a.num_v_heads * kJoinParts)),
+                       dim3(kBlock), 0, s, p, g);
   if (later > 0)
     hipLaunchKernelGGL(linear_later_kernel, dim3(static_cast<uint32_t>(blocks_of(later))),
-                       dim3(kThreads), 0, s, p, g);
+                       dim3(kBlock), 0, s, p, g);
   return check_launch("ld_linear_prefill");
 }
