@@ -13,12 +13,12 @@
 //   keys     row 4 lg + r of accumulators (n, a) is k = 32 n + 8 lg + 4 a + r, so that step n takes
 //            16 consecutive bytes of a q row
 //   tokens   step i takes token 32 i + 16 (e / 4) + 4 lg + e % 4
-//   O = Q S^T          S as two planes
 //   P = (K Q^T) . D    16 x 16 blocks over the waves, two planes, exchanged through LDS
-//   O = diag(e^c) O + P V
+//   O^T = S Q^T        S as two planes
+//   O^T = O^T diag(e^c) + V^T P^T
 //   S' = e^(c_63) S + K^T (e^(c_63 - c) V)    e V as three planes
-// and O crosses LDS in fp32 to whole rows, for the norm and 16-byte stores.  The transposed
-// operands come by ds_read_b64_tr_b16.
+// O crosses LDS in fp32, in the place of v, to whole rows, whose norm and 16-byte stores run
+// beside the next chunk's first products.  The transposed operands come by ds_read_b64_tr_b16.
 //
 // Decays come from differences of 64-bit prefix sums: their error over thousands of tokens would
 // be the state's.  Roundings to fewer than 32 bits, each of operands of the bf16 matrix cores
@@ -40,7 +40,10 @@ constexpr int kBlockWaves = 8;
 constexpr int kBlock = 64 * kBlockWaves;
 constexpr int kTokens = 64;                     // tokens per chunk
 constexpr int kRowsBytes = kTokens * kTileRow;  // q, k or v of a chunk
+constexpr int kPlaneUpper = 32 * 32 * 2;
+constexpr int kPlaneBytes = kPlaneUpper + 32 * 64 * 2;
 constexpr int64_t kTileFloats = kDim * kDim;
+constexpr int64_t kMaxRow = 1 << 23;            // a chunk's rows within 32-bit byte offsets
 
 // Per-token scalars of a chunk: c in units of log 2 as a sum of two floats, scale * e^c and
 // e^(c_63 - c); and e^(c_63).
@@ -50,11 +53,12 @@ struct alignas(16) ChunkScalars {
 };
 
 struct SegmentLds {
-  // k, then q (behind them, in their place, the chunk's O in fp32); v; the two planes of P
   alignas(16) uint8_t k[kRowsBytes];
   alignas(16) uint8_t q[kRowsBytes];
-  alignas(16) uint8_t v[kRowsBytes];
-  alignas(16) uint8_t p[2][kTokens * kTokens * 2];
+  // v; behind it, in its place and another 16 KiB, the chunk's O in fp32
+  alignas(16) uint8_t v[kTokens * kDim * 4];
+  // the two planes of P: 32 rows of 32 columns, 32 of 64
+  alignas(16) uint8_t p[2][kPlaneBytes];
   ChunkScalars scalars[2];
   alignas(16) float weight[kDim];
 };
@@ -63,7 +67,6 @@ struct SearchLds {
   int found[3];
 };
 static_assert(2 * (sizeof(SegmentLds) + sizeof(SearchLds)) <= 160 * 1024, "two workgroups a CU");
-static_assert(2 * kRowsBytes == kTokens * kDim * 4, "O takes the place of k and q");
 
 // x = sum of N bf16 planes (exactly, for three), eight values as an operand each.
 template <int N>
@@ -127,11 +130,18 @@ __device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) {
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+constexpr int kScalarWave = 1;   // makes the chunks' scalars: a wave without blocks of P
+
 // One workgroup's walk over `rows` rows from row `bos`: from the state at `start` (zeros if
 // null), writing outputs if Out, and the state after the last row to `end` (unless null).  Without
-// Out the state is the segment's update; either way returns, on wave 0, the sum of log decays in
-// units of log 2.
-template <bool Out>
+// Out the state is the segment's update; either way returns, on wave kScalarWave, the sum of log
+// decays in units of log 2.
+//
+// Global memory is reached by buffer loads and stores without branches (past the end a resource
+// over 0 bytes or an offset past it: zeros and dropped stores): under a branch the compiler would
+// have to wait for every load in flight before it uses any.  Wide: every address is a multiple of
+// 4 bytes; else elements move one by one.
+template <bool Wide, bool Gated, bool Out>
 __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, int64_t bos, int rows,
                                        int head, const float* start, float* end) {
   const int tid = threadIdx.x;
@@ -148,26 +158,29 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
   } staged;
   const int srow = tid >> 4;
   const int spiece = tid & 15;
-  const uint16_t* const columns = p.qkv + 8 * spiece + key_head * kDim;
-  const int k_col = p.num_k_heads * kDim;
-  const int v_col = (2 * p.num_k_heads + head - key_head) * kDim;
-  auto fetch = [&](int c) __attribute__((always_inline)) {
+  const uint32_t row_bytes = static_cast<uint32_t>(p.qkv_row) * 2;
+  const uint32_t lane_row = srow * row_bytes + spiece * 16;
+  const int q_col = key_head * kTileRow;
+  const int k_col = (p.num_k_heads + key_head) * kTileRow;
+  const int v_col = (2 * p.num_k_heads + head) * kTileRow;
+  const uint32_t width = (2 * p.num_k_heads + p.num_v_heads) * kTileRow;
+  // Chunk c's rows of a tensor as a resource: `row` bytes apart, `used` bytes read of each.
+  auto chunk_rows = [&](const uint16_t* base, int64_t stride, int c, uint32_t row,
+                        uint32_t used) __attribute__((always_inline)) {
     const int live = min(kTokens, rows - c * kTokens);
-    const int64_t first = bos + static_cast<int64_t>(c) * kTokens;
+    return __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint16_t*>(base + (bos + static_cast<int64_t>(c) * kTokens) * stride), 0,
+        live > 0 && c >= 0 ? (live - 1) * row + used : 0, 0x00020000);
+  };
+  auto fetch = [&](int c) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t rs = chunk_rows(p.qkv, p.qkv_row, c, row_bytes, width);
+    const int live = rows - c * kTokens;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint16_t* const row = columns + (first + min(srow + 32 * i, live - 1)) * p.qkv_row;
-      __builtin_memcpy(&staged.k[i], row + k_col, 16);
-      __builtin_memcpy(&staged.v[i], row + v_col, 16);
-      if constexpr (Out) __builtin_memcpy(&staged.q[i], row, 16);
-    }
-    if (live < kTokens) {   // rows past the end are zeros
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (srow + 32 * i >= live) {
-          staged.k[i] = staged.v[i] = u32x4{0u, 0u, 0u, 0u};
-          if constexpr (Out) staged.q[i] = u32x4{0u, 0u, 0u, 0u};
-        }
+      const uint32_t at = srow + 32 * i < live ? lane_row + 32 * i * row_bytes : 0x7ffff000u;
+      staged.k[i] = load_piece<Wide>(rs, at, k_col);
+      if constexpr (Out) staged.q[i] = load_piece<Wide>(rs, at, q_col);
+      staged.v[i] = load_piece<Wide>(rs, at, v_col);
     }
   };
   const uint32_t dst = srow * kTileRow + ((spiece ^ swizzle(srow)) << 4);
@@ -176,27 +189,32 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
     for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4*>(tile + dst + 32 * i * kTileRow) = x[i];
   };
   auto load_decay = [&](int c) __attribute__((always_inline)) {
-    const int t = c * kTokens + lane;
-    return t < rows ? p.log_decay[(bos + t) * p.decay_row + head] : 0.0f;
+    const int live = min(kTokens, rows - c * kTokens);
+    const uint32_t step = static_cast<uint32_t>(p.decay_row) * 4;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<float*>(p.log_decay + (bos + static_cast<int64_t>(c) * kTokens) * p.decay_row + head),
+        0, live > 0 ? (live - 1) * step + 4 : 0, 0x00020000);
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                                         rs, lane < live ? lane * step : 0x7ffff000u, 0, 0));
   };
 
-  double total = 0.0;
-  if (chunks > 0) {
-    fetch(0);
-    if (w == 0) total += chunk_scalars(lds.scalars[0], load_decay(0), p.scale, lane);
-  }
+  fetch(0);
+  float next_g = load_decay(0);
 
   // st[n][a][r] = S[16 w + li][32 n + 8 lg + 4 a + r]
   f32x4 st[4][2];
-  const int tile_at = (16 * w + li) * kDim + 8 * lg;
+  const int tile_at = ((16 * w + li) * kDim + 8 * lg) * 4;
+  {
+    const __amdgpu_buffer_rsrc_t rs = record_resource(
+        start, __builtin_amdgcn_readfirstlane(start != nullptr ? kTileBytes : 0));
 #pragma unroll
-  for (int n = 0; n < 4; ++n)
+    for (int n = 0; n < 4; ++n)
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      st[n][a] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if (start != nullptr)
-        st[n][a] = *reinterpret_cast<const f32x4*>(start + tile_at + 32 * n + 4 * a);
-    }
+      for (int a = 0; a < 2; ++a) st[n][a] = load16(rs, tile_at + 128 * n + 16 * a, 0);
+  }
+  double total = 0.0;
+  if (w == kScalarWave) total += chunk_scalars(lds.scalars[0], next_g, p.scale, lane);
+  next_g = load_decay(1);
 
   // lane addresses of the operands (the parts of the swizzle that depend on the step are XORed in)
   uint32_t a_at = li * kTileRow + ((lg ^ swizzle(li)) << 4);       // ^ (step << 6)
@@ -207,75 +225,145 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
   // transposed v: rows 32 s + 16 h + .., the wave's columns
   const uint32_t vt_at = tr_row + (((2 * w + ((li & 3) >> 1)) ^ (quad << 2) ^ lg) << 4) + (li & 1) * 8;
   // P[t][s] of a plane: the quad of s at 32 i + 16 a + 4 lg is half a of row t's 16-byte piece
-  // 4 i + lg, the pieces of a row XORed with t % 8
-  uint32_t p_at = li * (2 * kTokens) + ((lg ^ (li & 7)) << 4);     // ^ (i << 6)
-  // the wave's part of P: rows of strip w / 2; columns 16 w % 2 of the first two, 32 (w % 2) and
-  // 16 more of the others
+  // 4 i + lg; the pieces of a row are XORed with t / 2 % 4 (rows of 32 columns) or t % 8
+  const uint32_t p_upper = li * 64 + ((lg ^ ((li >> 1) & 3)) << 4);
+  uint32_t p_lower = kPlaneUpper + li * 128 + ((lg ^ (li & 7)) << 4);   // ^ (i << 6)
+  // the wave's part of P: of strip w / 2, the blocks 2 (w % 2) and the next
   const int strip = w >> 1;
-  // O in fp32: row t's 16-byte pieces XORed with 4 (t / 4 % 4)
+  const int block = 2 * (w & 1);
+  const bool has_block = strip >= 2 || block == 0;   // (32 x 32 blocks above the diagonal are not read)
+  // O in LDS: row t's 16-byte pieces XORed with t % 8.  o[tt][r] is token 16 tt + li, column
+  // 16 w + 4 lg + r; a thread finishes columns 8 part + 64 i .. + 7 of one row
+  float* const o_rows = reinterpret_cast<float*>(lds.v);
+  const uint32_t o_put = li * kDim + ((4 * w + lg) ^ (li & 7)) * 4;
   const int row = tid >> 3;
   const int part = tid & 7;
-  const int o_at = row * kDim + (((2 * part) ^ (((row >> 2) & 3) << 2)) << 2);
+  const uint32_t o_get = row * kDim + ((2 * part) ^ (row & 7)) * 4;   // ^ 4 h, + 64 i
+  const uint32_t gate_bytes = static_cast<uint32_t>(p.gate_row) * 2;
+  const uint32_t out_bytes = static_cast<uint32_t>(p.num_v_heads) * kTileRow;
+  u32x4 gate[2];
+  auto load_gate = [&](int c) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t rs =
+        chunk_rows(p.gate + head * kDim, p.gate_row, c, gate_bytes, kTileRow);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) gate[i] = load_piece<Wide>(rs, row * gate_bytes + part * 16 + 128 * i, 0);
+  };
+  auto finish = [&](int c) __attribute__((always_inline)) {   // outputs of chunk c from its O
+    auto read = [&](int i, float (&y)[8]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(o_rows + (o_get ^ (4 * h)) + 64 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[4 * h + e] = x[e];
+      }
+    };
+    float rstd = 1.0f;
+    if constexpr (Gated) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float y[8];
+        read(i, y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
+      }
+      ss += dpp<kDppQuadXor1>(ss);
+      ss += dpp<kDppQuadXor2>(ss);
+      ss += dpp<kDppRowHalfMirror>(ss);
+      rstd = fast_rsqrt(ss * (1.0f / kDim) + p.eps);
+    }
+    const __amdgpu_buffer_rsrc_t rs = chunk_rows(
+        p.out + head * kDim, static_cast<int64_t>(p.num_v_heads) * kDim, c, out_bytes, kTileRow);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (Gated) lds_order();   // (read again: held, the row would cost spills)
+      float y[8];
+      read(i, y);
+      if constexpr (Gated) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t pair = gate[i][e >> 1];
+          const float g = __builtin_bit_cast(float, e & 1 ? pair & 0xffff0000u : pair << 16);
+          y[e] = ((y[e] * rstd) * lds.weight[8 * part + 64 * i + e]) * silu(g);
+        }
+      }
+      u32x4 bits;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bits[e] = bf16_pair(f32x2{y[2 * e], y[2 * e + 1]});
+      const uint32_t at = row * out_bytes + part * 16 + 128 * i;
+      if constexpr (Wide) {
+        __builtin_amdgcn_raw_buffer_store_b128(bits, rs, at, 0, 0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(bits[e]), rs, at + 4 * e, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(bits[e] >> 16), rs, at + 4 * e + 2, 0, 0);
+        }
+      }
+    }
+  };
 
-  if (chunks > 0) {
-    put(lds.k, staged.k);
+  put(lds.k, staged.k);
+  if constexpr (Out)
+    put(lds.q, staged.q);
+  else
     put(lds.v, staged.v);
-    if constexpr (Out) put(lds.q, staged.q);
-  }
+  // (the state's loads are waited for here: in the loop the wait would count against later ones)
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int a = 0; a < 2; ++a) pin(st[n][a]);
   for (int c = 0; c < chunks; ++c) {
     const ChunkScalars& s = lds.scalars[c & 1];
-    const bool more = c + 1 < chunks;
-    float next_g = 0.0f;
     // (opaque here, so that their XORed forms are made where they are used, not held in registers
     // over the loop)
     pin(a_at);
     pin(kt_at);
-    pin(p_at);
-    lds_barrier();   // the chunk's rows and scalars are in LDS
-    if (more) fetch(c + 1);
-    if (more && w == 0) next_g = load_decay(c + 1);
+    pin(p_lower);
+    lds_barrier();   // k, q (without Out: v) and scalars of the chunk are in LDS, O of the last
     f32x4 o[4];
-    const float gamma = s.gamma;
     if constexpr (Out) {
+      if constexpr (Gated) load_gate(c - 1);
       // ---- P ----
-      bf16x8 qf[4];
+      if (has_block) {
+        f32x4 x[2];
 #pragma unroll
-      for (int step = 0; step < 4; ++step)
-        qf[step] = *reinterpret_cast<const bf16x8*>(lds.q + 16 * strip * kTileRow +
-                                                    (a_at ^ (step << 6)));
-      const float thi = s.hi[16 * strip + li], tlo = s.lo[16 * strip + li];
+        for (int i = 0; i < 2; ++i) x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (i == 1 && strip < 2) break;
-        const int j = strip < 2 ? w & 1 : 2 * (w & 1) + i;
-        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (j <= strip) {
+        for (int step = 0; step < 4; ++step) {
+          const bf16x8 q = *reinterpret_cast<const bf16x8*>(lds.q + 16 * strip * kTileRow +
+                                                            (a_at ^ (step << 6)));
 #pragma unroll
-          for (int step = 0; step < 4; ++step)
-            x = mfma16(*reinterpret_cast<const bf16x8*>(lds.k + 16 * j * kTileRow +
-                                                        (a_at ^ (step << 6))),
-                       qf[step], x);
-          const f32x4 shi = *reinterpret_cast<const f32x4*>(&s.hi[16 * j + 4 * lg]);
-          const f32x4 slo = *reinterpret_cast<const f32x4*>(&s.lo[16 * j + 4 * lg]);
+          for (int i = 0; i < 2; ++i)
+            x[i] = mfma16(*reinterpret_cast<const bf16x8*>(lds.k + 16 * (block + i) * kTileRow +
+                                                           (a_at ^ (step << 6))),
+                          q, x[i]);
+        }
+        const float thi = s.hi[16 * strip + li], tlo = s.lo[16 * strip + li];
+        uint8_t* const at = lds.p[0] + (strip < 2 ? p_upper + 16 * 64 * strip
+                                                  : (p_lower ^ (block << 5)) + 16 * 128 * (strip - 2));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int first = 16 * (block + i) + 4 * lg;
+          const f32x4 shi = *reinterpret_cast<const f32x4*>(&s.hi[first]);
+          const f32x4 slo = *reinterpret_cast<const f32x4*>(&s.lo[first]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float d = __builtin_amdgcn_exp2f((thi - shi[r]) + (tlo - slo[r])) * p.scale;
-            x[r] = j < strip || 4 * lg + r <= li ? x[r] * d : 0.0f;
+            x[i][r] = first + r <= 16 * strip + li ? x[i][r] * d : 0.0f;
+          }
+#pragma unroll
+          for (int plane = 0; plane < 2; ++plane) {
+            const uint2 bits = {bf16_pair(f32x2{x[i][0], x[i][1]}), bf16_pair(f32x2{x[i][2], x[i][3]})};
+            *reinterpret_cast<uint2*>(at + 8 * i + plane * kPlaneBytes) = bits;
+            x[i][0] -= __builtin_bit_cast(float, bits.x << 16);
+            x[i][1] -= __builtin_bit_cast(float, bits.x & 0xffff0000u);
+            x[i][2] -= __builtin_bit_cast(float, bits.y << 16);
+            x[i][3] -= __builtin_bit_cast(float, bits.y & 0xffff0000u);
           }
         }
-        uint8_t* const at = lds.p[0] + (16 * strip + li) * (2 * kTokens) +
-                            (((4 * (j >> 1) + lg) ^ (li & 7)) << 4) + (j & 1) * 8;
-#pragma unroll
-        for (int plane = 0; plane < 2; ++plane) {
-          const uint2 bits = {bf16_pair(f32x2{x[0], x[1]}), bf16_pair(f32x2{x[2], x[3]})};
-          *reinterpret_cast<uint2*>(at + plane * sizeof(lds.p[0])) = bits;
-          x[0] -= __builtin_bit_cast(float, bits.x << 16);
-          x[1] -= __builtin_bit_cast(float, bits.x & 0xffff0000u);
-          x[2] -= __builtin_bit_cast(float, bits.y << 16);
-          x[3] -= __builtin_bit_cast(float, bits.y & 0xffff0000u);
-        }
       }
-      // ---- O = Q S^T ----
+      // ---- O^T = S Q^T ----
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) o[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -286,37 +374,30 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
         const Planes<2> split(x);
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
-          const bf16x8 a = *reinterpret_cast<const bf16x8*>(lds.q + 16 * tt * kTileRow +
+          const bf16x8 q = *reinterpret_cast<const bf16x8*>(lds.q + 16 * tt * kTileRow +
                                                             (a_at ^ (n << 6)));
-          o[tt] = mfma16(a, split[1], o[tt]);
-          o[tt] = mfma16(a, split[0], o[tt]);
+          o[tt] = mfma16(split[1], q, o[tt]);
+          o[tt] = mfma16(split[0], q, o[tt]);
         }
       }
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        const f32x4 eq = *reinterpret_cast<const f32x4*>(&s.eq[16 * tt + 4 * lg]);
-        o[tt] *= eq;
-      }
+      for (int tt = 0; tt < 4; ++tt) o[tt] *= s.eq[16 * tt + li];
+      finish(c - 1);
+      lds_barrier();   // O of the last chunk is read
+      put(lds.v, staged.v);
     }
+    const float gamma = s.gamma;
+    fetch(c + 1);
 #pragma unroll
     for (int n = 0; n < 4; ++n)
 #pragma unroll
       for (int a = 0; a < 2; ++a) st[n][a] *= gamma;
-    if constexpr (Out) lds_barrier();   // P is in LDS
-    if (more && w == 0)
+    if (w == kScalarWave)
       total += chunk_scalars(lds.scalars[(c + 1) & 1], next_g, p.scale, lane);
+    next_g = load_decay(c + 2);
+    if constexpr (Out) lds_barrier();   // v is in LDS (and P)
 
-    // ---- O += P V and S += K^T (e V), 32 tokens a step ----
-    u32x4 gate[2];
-    const int64_t token = bos + static_cast<int64_t>(c) * kTokens + row;
-    const bool stored = c * kTokens + row < rows;
-    if constexpr (Out) {
-      if (p.gate != nullptr && stored) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          __builtin_memcpy(&gate[i], p.gate + token * p.gate_row + head * kDim + 8 * part + 64 * i, 16);
-      }
-    }
+    // ---- O^T += V^T P^T and S += K^T (e V), 32 tokens a step ----
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const bf16x8 v = join(read_tr(lds.v + vt_at + 32 * i * kTileRow),
@@ -326,9 +407,11 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
         for (int tt = 2 * i; tt < 4; ++tt)
 #pragma unroll
           for (int plane = 1; plane >= 0; --plane)
-            o[tt] = mfma16(*reinterpret_cast<const bf16x8*>(
-                               lds.p[plane] + 16 * tt * (2 * kTokens) + (p_at ^ (i << 6))),
-                           v, o[tt]);
+            o[tt] = mfma16(v,
+                           *reinterpret_cast<const bf16x8*>(
+                               lds.p[plane] + (tt < 2 ? p_upper + 16 * 64 * tt
+                                                      : (p_lower ^ (i << 6)) + 16 * 128 * (tt - 2))),
+                           o[tt]);
       }
       float x[8];
 #pragma unroll
@@ -350,64 +433,19 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
     }
     lds_barrier();   // every read of the chunk's rows and P is done
     if constexpr (Out) {
-      float* const o_rows = reinterpret_cast<float*>(lds.k);
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          o_rows[(16 * tt + 4 * lg + r) * kDim + (((4 * w + (li >> 2)) ^ (lg << 2)) << 2) + (li & 3)] =
-              o[tt][r];
-      if (more) put(lds.v, staged.v);
-      lds_barrier();   // O is in LDS
-      // ---- an eighth of one row a thread: columns 8 part + 64 i .. + 7 ----
-      float y[2][8];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(
-              o_rows + o_at + 64 * i + 4 * h);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[i][4 * h + e] = x[e];
-        }
-      if (p.gate != nullptr) {
-        float ss = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) ss = fmaf(y[i][e], y[i][e], ss);
-        ss += dpp<kDppQuadXor1>(ss);
-        ss += dpp<kDppQuadXor2>(ss);
-        ss += dpp<kDppRowHalfMirror>(ss);
-        const float rstd = fast_rsqrt(ss * (1.0f / kDim) + p.eps);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint32_t pair = gate[i][e >> 1];
-            const float g = __builtin_bit_cast(float, e & 1 ? pair & 0xffff0000u : pair << 16);
-            y[i][e] = ((y[i][e] * rstd) * lds.weight[8 * part + 64 * i + e]) * silu(g);
-          }
-      }
-      if (stored) {
-        uint16_t* const to = p.out + (token * p.num_v_heads + head) * kDim + 8 * part;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          u32x4 bits;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) bits[e] = bf16_pair(f32x2{y[i][2 * e], y[i][2 * e + 1]});
-          __builtin_memcpy(to + 64 * i, &bits, 16);
-        }
-      }
-      lds_barrier();   // O is read
-      if (more) {
-        put(lds.k, staged.k);
-        put(lds.q, staged.q);
-      }
-    } else if (more) {
-      put(lds.k, staged.k);
-      put(lds.v, staged.v);
+      for (int tt = 0; tt < 4; ++tt) *reinterpret_cast<f32x4*>(o_rows + o_put + 16 * tt * kDim) = o[tt];
     }
+    put(lds.k, staged.k);
+    if constexpr (Out)
+      put(lds.q, staged.q);
+    else
+      put(lds.v, staged.v);
+  }
+  if (Out && chunks > 0) {
+    if constexpr (Gated) load_gate(chunks - 1);
+    lds_barrier();
+    finish(chunks - 1);
   }
 
   if (end != nullptr) {
@@ -415,7 +453,7 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
     for (int n = 0; n < 4; ++n)
 #pragma unroll
       for (int a = 0; a < 2; ++a)
-        *reinterpret_cast<f32x4*>(end + tile_at + 32 * n + 4 * a) = st[n][a];
+        *reinterpret_cast<f32x4*>(reinterpret_cast<char*>(end) + tile_at + 128 * n + 16 * a) = st[n][a];
   }
   return total;
 }
@@ -504,6 +542,7 @@ __device__ __forceinline__ void load_weight(const LinearParams& p, SegmentLds& l
 // The first launch.  Item j < later is later segment j's predecessor: the sequence's first
 // segment, walked from its state, or a middle one, reduced to its update; item later + n is
 // sequence n if it is a single segment.
+template <bool Wide, bool Gated>
 __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(4, 4)))
 void linear_first_kernel(const LinearParams p, const Segments g) {
   __shared__ SegmentLds lds;
@@ -520,9 +559,9 @@ void linear_first_kernel(const LinearParams p, const Segments g) {
   load_weight(p, lds);
   float* const tile = whole ? nullptr : g.tiles + (static_cast<int64_t>(item) * p.num_v_heads + head) * kTileFloats;
   if (index > 0) {
-    const double total = walk<false>(p, lds, bos + (static_cast<int64_t>(index) << g.shift),
+    const double total = walk<Wide, Gated, false>(p, lds, bos + (static_cast<int64_t>(index) << g.shift),
                                      1 << g.shift, head, nullptr, tile);
-    if (threadIdx.x == 0)
+    if (threadIdx.x == 64 * kScalarWave)
       g.decays[static_cast<int64_t>(item) * p.num_v_heads + head] =
           __builtin_amdgcn_exp2f(static_cast<float>(total));
     return;
@@ -530,7 +569,7 @@ void linear_first_kernel(const LinearParams p, const Segments g) {
   const int slot = p.indices[seq];
   const bool live = live_slot(slot, p.num_slots);
   float* const home = p.state + static_cast<int64_t>(live ? slot : 0) * p.state_slot + head * kTileFloats;
-  walk<true>(p, lds, bos, whole ? rows : 1 << g.shift, head,
+  walk<Wide, Gated, true>(p, lds, bos, whole ? rows : 1 << g.shift, head,
              live && p.has_initial[seq] != 0 ? home : nullptr, whole ? (live ? home : nullptr) : tile);
 }
 
@@ -560,6 +599,7 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const LinearParams 
 }
 
 // The third: the later segments, each from its state.
+template <bool Wide, bool Gated>
 __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(4, 4)))
 void linear_later_kernel(const LinearParams p, const Segments g) {
   __shared__ SegmentLds lds;
@@ -575,7 +615,7 @@ void linear_later_kernel(const LinearParams p, const Segments g) {
   const int done = (index + 1) << g.shift;
   const int slot = p.indices[seq];
   float* const home = p.state + static_cast<int64_t>(slot) * p.state_slot + head * kTileFloats;
-  walk<true>(p, lds, bos + done, min(rows - done, 1 << g.shift), head,
+  walk<Wide, Gated, true>(p, lds, bos + done, min(rows - done, 1 << g.shift), head,
              g.tiles + (static_cast<int64_t>(item) * p.num_v_heads + head) * kTileFloats,
              index + 1 == count && live_slot(slot, p.num_slots) ? home : nullptr);
 }
@@ -591,6 +631,27 @@ int segment_shift(int64_t num_tokens, int32_t num_v_heads) {
 // Sequences of more than a segment have at most this many later ones.
 int64_t later_segments(int64_t num_tokens, int32_t num_v_heads) {
   return num_tokens > 0 ? (num_tokens - 1) >> segment_shift(num_tokens, num_v_heads) : 0;
+}
+
+template <bool Wide, bool Gated>
+void launch_segments(const LinearParams& p, const Segments& g, uint32_t first, uint32_t later,
+                     hipStream_t s) {
+  hipLaunchKernelGGL((linear_first_kernel<Wide, Gated>), dim3(first), dim3(kBlock), 0, s, p, g);
+  if (g.later > 1)   // (a lone later segment starts from what the first launch left)
+    hipLaunchKernelGGL(linear_join_kernel, dim3(g.later * p.num_v_heads * kJoinParts), dim3(kBlock),
+                       0, s, p, g);
+  if (g.later > 0)
+    hipLaunchKernelGGL((linear_later_kernel<Wide, Gated>), dim3(later), dim3(kBlock), 0, s, p, g);
+}
+
+void launch_linear_prefill(const LinearParams& p, const Segments& g, uint32_t first, uint32_t later,
+                           hipStream_t s) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(p.qkv) | reinterpret_cast<uintptr_t>(p.gate) |
+                         reinterpret_cast<uintptr_t>(p.out) | (p.qkv_row * 2) | (p.gate_row * 2);
+  const auto launch = (bits & 3) == 0
+                          ? (p.gate != nullptr ? launch_segments<true, true> : launch_segments<true, false>)
+                          : (p.gate != nullptr ? launch_segments<false, true> : launch_segments<false, false>);
+  launch(p, g, first, later, s);
 }
 
 }  // namespace
@@ -613,6 +674,10 @@ extern "C" int ld_linear_prefill(const ld_linear_prefill_args* args, void* strea
   if (!a.slots || !a.has_initial || !a.cu_seqlens || !a.state ||
       (a.num_tokens > 0 && (!a.qkv || !a.log_decay || !a.out)))
     return fail(LD_ERR_INVALID_ARGUMENT, "ld_linear_prefill: NULL tensor pointer");
+  if (a.qkv_row_stride < 0 || a.qkv_row_stride > kMaxRow || a.gate_row_stride < 0 ||
+      a.gate_row_stride > kMaxRow || a.log_decay_row_stride < 0 ||
+      a.log_decay_row_stride > kMaxRow || a.num_v_heads > kMaxRow / kDim)
+    return fail(LD_ERR_INVALID_ARGUMENT, "qkv, log_decay, gate and out rows must be at most 2^23 elements apart");
   if (a.num_tokens > 0x7fffffff) return fail(LD_ERR_INVALID_ARGUMENT, "too many tokens");
   p.indices = a.slots;
   p.cu = a.cu_seqlens;
@@ -634,14 +699,7 @@ extern "C" int ld_linear_prefill(const ld_linear_prefill_args* args, void* strea
   g.later = static_cast<int>(later);
   g.tiles = static_cast<float*>(a.workspace);
   g.decays = g.tiles + later * a.num_v_heads * kTileFloats;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(linear_first_kernel, dim3(static_cast<uint32_t>(blocks_of(later + a.num_sequences))),
-                     dim3(kBlock), 0, s, p, g);
-  if (later > 1)   // (a lone later segment starts from what the first launch left)
-    hipLaunchKernelGGL(linear_join_kernel, dim3(static_cast<uint32_t>(later * a.num_v_heads * kJoinParts)),
-                       dim3(kBlock), 0, s, p, g);
-  if (later > 0)
-    hipLaunchKernelGGL(linear_later_kernel, dim3(static_cast<uint32_t>(blocks_of(later))),
-                       dim3(kBlock), 0, s, p, g);
+  launch_linear_prefill(p, g, static_cast<uint32_t>(blocks_of(later + a.num_sequences)),
+                        static_cast<uint32_t>(blocks_of(later)), static_cast<hipStream_t>(stream));
   return check_launch("ld_linear_prefill");
 }

@@ -96,6 +96,22 @@ __device__ __forceinline__ void lds_barrier() {
 // order).
 __device__ __forceinline__ void lds_order() { asm volatile("" ::: "memory"); }
 
+// Sixteen bytes of a row at a lane's byte offset + a uniform one: one load, or (rows not at
+// 16-byte boundaries) eight of one element.
+template <bool Wide>
+__device__ __forceinline__ u32x4 load_piece(__amdgpu_buffer_rsrc_t rs, uint32_t offset,
+                                            int uniform) {
+  if constexpr (Wide) return load16u(rs, offset, uniform);
+  u32x4 out;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = __builtin_amdgcn_raw_buffer_load_b16(rs, static_cast<int>(offset + 4 * i), uniform, 0);
+    const uint32_t hi = __builtin_amdgcn_raw_buffer_load_b16(rs, static_cast<int>(offset + 4 * i + 2), uniform, 0);
+    out[i] = (lo & 0xffffu) | (hi << 16);
+  }
+  return out;
+}
+
 // The 64-bit value of the lane that Ctrl names (zero where it names none).
 template <int Ctrl>
 __device__ __forceinline__ double dpp64(double x) {

@@ -64,22 +64,6 @@ __device__ __forceinline__ void product(bf16x8 a, bf16x8 b, f32x16& c) {
   pin(c);
 }
 
-// Sixteen bytes of a row at a lane's byte offset + a uniform one: one load, or (rows not at
-// 16-byte boundaries) eight of one element.
-template <bool Wide>
-__device__ __forceinline__ u32x4 load_piece(__amdgpu_buffer_rsrc_t rs, uint32_t offset,
-                                            int uniform) {
-  if constexpr (Wide) return load16u(rs, offset, uniform);
-  u32x4 out;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t lo = __builtin_amdgcn_raw_buffer_load_b16(rs, static_cast<int>(offset + 4 * i), uniform, 0);
-    const uint32_t hi = __builtin_amdgcn_raw_buffer_load_b16(rs, static_cast<int>(offset + 4 * i + 2), uniform, 0);
-    out[i] = (lo & 0xffffu) | (hi << 16);
-  }
-  return out;
-}
-
 // The gated RMSNorm of a chunk's rows, a thread's 16 columns of one token, in slices that fit
 // beside matrix instructions and hold eight independent operations where the arithmetic
 // allows: 0: the raw outputs' reads, 1-4: squares, 5: the row's sum over its 8 threads, 6:
