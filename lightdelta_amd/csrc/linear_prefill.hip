@@ -4,16 +4,14 @@
 //   o_t = scale (e^(c_t) S q_t + sum over s <= t of e^(c_t - c_s) (k_s . q_t) v_s)
 //   S'  = e^(c_63) S + sum over s of k_s (e^(c_63 - c_s) v_s)^T
 //
-// A workgroup of eight waves walks the chunks of one (sequence, v-head).  Wave w owns state rows
-// v = 16 w .. 16 w + 15 as S^T in the accumulators of v_mfma_f32_16x16x32_bf16: for lane l,
-// li = l % 16 and lg = l / 16, an accumulator holds rows 4 lg + r, r < 4, of column li, an operand
-// A[i = li][k = 8 lg + e] or B[k = 8 lg + e][j = li], e < 8.  The summation index may be assigned
-// to (step, lg, e) freely as long as both operands agree, so two accumulators, split into bf16
-// planes, are directly the operand of a step of the next product:
-//   keys     row 4 lg + r of accumulators (n, a) is k = 32 n + 8 lg + 4 a + r, so that step n takes
-//            16 consecutive bytes of a q row
-//   tokens   step i takes token 32 i + 16 (e / 4) + 4 lg + e % 4
-//   P = (K Q^T) . D    16 x 16 blocks over the waves, two planes, exchanged through LDS
+// A workgroup of four waves walks the chunks of one (sequence, v-head).  Wave w owns state rows
+// v = 32 w .. 32 w + 31 as S^T in the accumulators of v_mfma_f32_32x32x16_bf16, with the summation
+// index assigned as in prefill_heads.hip: for lane l, lj = l % 32 and hi = l / 32, an accumulator
+// holds rows i(r) = 8 (r / 4) + 4 hi + r % 4, r < 16, of column lj, so its registers 8 u ..
+// 8 u + 7, split into bf16 planes, are directly the operand of step u of the next product; keys
+// are in an order in which a step takes 16 consecutive bytes of a q row, step u of a sum over
+// tokens takes token 16 u + 8 (e / 4) + 4 hi + e % 4.
+//   P = (K Q^T) . D    32 x 32 blocks over the waves, two planes, exchanged through LDS
 //   O^T = S Q^T        S as two planes
 //   O^T = O^T diag(e^c) + V^T P^T
 //   S' = e^(c_63) S + K^T (e^(c_63 - c) V)    e V as three planes
@@ -36,7 +34,7 @@
 namespace ld {
 namespace {
 
-constexpr int kBlockWaves = 8;
+constexpr int kBlockWaves = 4;
 constexpr int kBlock = 64 * kBlockWaves;
 constexpr int kTokens = 64;                     // tokens per chunk
 constexpr int kRowsBytes = kTokens * kTileRow;  // q, k or v of a chunk
@@ -126,11 +124,15 @@ __device__ __forceinline__ double chunk_scalars(ChunkScalars& s, float g, float 
   return total;
 }
 
+// Keeps LDS reads, matrix instructions and global loads in the program's order (vector and
+// scalar instructions may cross): reads stay the distance ahead of their use that the source gives them.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0x406); }
+
 __device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) {
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-constexpr int kScalarWave = 1;   // makes the chunks' scalars: a wave without blocks of P
+constexpr int kScalarWave = 3;   // makes the chunks' scalars: the wave without a block of P
 
 // One workgroup's walk over `rows` rows from row `bos`: from the state at `start` (zeros if
 // null), writing outputs if Out, and the state after the last row to `end` (unless null).  Without
@@ -147,14 +149,14 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int li = lane & 15;
-  const int lg = lane >> 4;
+  const int lj = lane & 31;
+  const int hi = lane >> 5;
   const int key_head = head / p.group;
   const int chunks = (rows + kTokens - 1) / kTokens;
 
-  // ---- a chunk's rows, in registers on their way to LDS: row 32 i + srow, 16 bytes ----
+  // ---- a chunk's rows, in registers on their way to LDS: row 16 i + srow, 16 bytes ----
   struct Staged {
-    u32x4 q[2], k[2], v[2];
+    u32x4 q[4], k[4], v[4];
   } staged;
   const int srow = tid >> 4;
   const int spiece = tid & 15;
@@ -172,21 +174,25 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
         const_cast<uint16_t*>(base + (bos + static_cast<int64_t>(c) * kTokens) * stride), 0,
         live > 0 && c >= 0 ? (live - 1) * row + used : 0, 0x00020000);
   };
-  auto fetch = [&](int c) __attribute__((always_inline)) {
-    const __amdgpu_buffer_rsrc_t rs = chunk_rows(p.qkv, p.qkv_row, c, row_bytes, width);
-    const int live = rows - c * kTokens;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t at = srow + 32 * i < live ? lane_row + 32 * i * row_bytes : 0x7ffff000u;
-      staged.k[i] = load_piece<Wide>(rs, at, k_col);
-      if constexpr (Out) staged.q[i] = load_piece<Wide>(rs, at, q_col);
-      staged.v[i] = load_piece<Wide>(rs, at, v_col);
-    }
+  // Load i of 12 of a chunk: k and q, then v.  They go out between products: a burst of them would
+  // hold the wave until the last is accepted.
+  auto source = [&](int c) __attribute__((always_inline)) {
+    return chunk_rows(p.qkv, p.qkv_row, c, row_bytes, width);
+  };
+  auto fetch = [&](__amdgpu_buffer_rsrc_t rs, int c, int i) __attribute__((always_inline)) {
+    const int j = i < 8 ? i >> 1 : i - 8;
+    const uint32_t at = srow + 16 * j < rows - c * kTokens ? lane_row + 16 * j * row_bytes : 0x7ffff000u;
+    if (i >= 8)
+      staged.v[j] = load_piece<Wide>(rs, at, v_col);
+    else if ((i & 1) == 0)
+      staged.k[j] = load_piece<Wide>(rs, at, k_col);
+    else if constexpr (Out)
+      staged.q[j] = load_piece<Wide>(rs, at, q_col);
   };
   const uint32_t dst = srow * kTileRow + ((spiece ^ swizzle(srow)) << 4);
-  auto put = [&](uint8_t* tile, const u32x4 (&x)[2]) __attribute__((always_inline)) {
+  auto put = [&](uint8_t* tile, const u32x4 (&x)[4]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4*>(tile + dst + 32 * i * kTileRow) = x[i];
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(tile + dst + 16 * i * kTileRow) = x[i];
   };
   auto load_decay = [&](int c) __attribute__((always_inline)) {
     const int live = min(kTokens, rows - c * kTokens);
@@ -198,106 +204,115 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
                                          rs, lane < live ? lane * step : 0x7ffff000u, 0, 0));
   };
 
-  fetch(0);
+  {
+    const __amdgpu_buffer_rsrc_t rs = source(0);
+#pragma unroll
+    for (int i = 0; i < 12; ++i) fetch(rs, 0, i);
+  }
   float next_g = load_decay(0);
 
-  // st[n][a][r] = S[16 w + li][32 n + 8 lg + 4 a + r]
-  f32x4 st[4][2];
-  const int tile_at = ((16 * w + li) * kDim + 8 * lg) * 4;
+  // st[T][8 u + 4 h + r] = S[32 w + lj][32 T + 16 u + 8 hi + 4 h + r]
+  f32x16 st[4];
+  const int tile_at = ((32 * w + lj) * kDim + 8 * hi) * 4;
   {
     const __amdgpu_buffer_rsrc_t rs = record_resource(
         start, __builtin_amdgcn_readfirstlane(start != nullptr ? kTileBytes : 0));
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
+    for (int T = 0; T < 4; ++T)
 #pragma unroll
-      for (int a = 0; a < 2; ++a) st[n][a] = load16(rs, tile_at + 128 * n + 16 * a, 0);
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 x = load16(rs, tile_at + 128 * T + 64 * (q >> 1) + 16 * (q & 1), 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[T][4 * q + r] = x[r];
+      }
   }
   double total = 0.0;
   if (w == kScalarWave) total += chunk_scalars(lds.scalars[0], next_g, p.scale, lane);
   next_g = load_decay(1);
 
   // lane addresses of the operands (the parts of the swizzle that depend on the step are XORed in)
-  uint32_t a_at = li * kTileRow + ((lg ^ swizzle(li)) << 4);       // ^ (step << 6)
-  const int quad = li >> 2;
-  const uint32_t tr_row = (4 * lg + quad) * kTileRow;
-  // transposed k: rows 32 s + 16 h + .., columns 32 n + 8 (i / 4) + 4 a + i % 4   ^ (n << 6)
-  uint32_t kt_at = tr_row + (((li & 3) ^ (quad << 2) ^ lg) << 4);
-  // transposed v: rows 32 s + 16 h + .., the wave's columns
-  const uint32_t vt_at = tr_row + (((2 * w + ((li & 3) >> 1)) ^ (quad << 2) ^ lg) << 4) + (li & 1) * 8;
-  // P[t][s] of a plane: the quad of s at 32 i + 16 a + 4 lg is half a of row t's 16-byte piece
-  // 4 i + lg; the pieces of a row are XORed with t / 2 % 4 (rows of 32 columns) or t % 8
-  const uint32_t p_upper = li * 64 + ((lg ^ ((li >> 1) & 3)) << 4);
-  uint32_t p_lower = kPlaneUpper + li * 128 + ((lg ^ (li & 7)) << 4);   // ^ (i << 6)
-  // the wave's part of P: of strip w / 2, the blocks 2 (w % 2) and the next
-  const int strip = w >> 1;
-  const int block = 2 * (w & 1);
-  const bool has_block = strip >= 2 || block == 0;   // (32 x 32 blocks above the diagonal are not read)
-  // O in LDS: row t's 16-byte pieces XORed with t % 8.  o[tt][r] is token 16 tt + li, column
-  // 16 w + 4 lg + r; a thread finishes columns 8 part + 64 i .. + 7 of one row
+  uint32_t a_at = lj * kTileRow + ((hi ^ swizzle(lj)) << 4);       // ^ (step << 5)
+  const int m = lane & 15;
+  const int c16 = (lane >> 4) & 1;
+  const uint32_t tr_row = (4 * hi + (m >> 2)) * kTileRow;
+  // transposed k: rows 16 u + 8 h + .., columns in the state's order   ^ (T << 6) ^ (h << 5)
+  uint32_t kt_at = tr_row + (((2 * c16 + (m & 1)) ^ ((m >> 2) << 2) ^ hi) << 4) + ((m >> 1) & 1) * 8;
+  // transposed v: rows 16 u + 8 h + .., the wave's columns   ^ (h << 5)
+  const uint32_t vt_at =
+      tr_row + (((4 * w + 2 * c16 + ((m & 3) >> 1)) ^ ((m >> 2) << 2) ^ hi) << 4) + (m & 1) * 8;
+  // P[t][s] of a plane: the quad of s at 16 u + 8 a + 4 hi is half a of row t's 16-byte piece
+  // 2 u + hi; the pieces of a row are XORed with t / 2 % 4 (rows of 32 columns) or t % 8
+  uint32_t p_upper = lj * 64 + ((hi ^ ((lj >> 1) & 3)) << 4);                // ^ (u << 5)
+  uint32_t p_lower = kPlaneUpper + lj * 128 + ((hi ^ (lj & 7)) << 4);        // ^ (u << 5)
+  // the wave's 32 x 32 block of P (not the one above the diagonal)
+  const int p_rows = w == 0 ? 0 : 1;
+  const int p_columns = w == 2 ? 1 : 0;
+  // O in LDS: row t's 16-byte pieces XORed with t % 8.  o[tt][4 q + r] is token 32 tt + lj, column
+  // 32 w + 8 q + 4 hi + r; a thread finishes columns 8 part + 64 i .. + 7 of rows row and row + 32
   float* const o_rows = reinterpret_cast<float*>(lds.v);
-  const uint32_t o_put = li * kDim + ((4 * w + lg) ^ (li & 7)) * 4;
+  uint32_t o_put = lj * kDim + ((8 * w + hi) ^ (lj & 7)) * 4;                // ^ (8 q)
   const int row = tid >> 3;
   const int part = tid & 7;
   const uint32_t o_get = row * kDim + ((2 * part) ^ (row & 7)) * 4;   // ^ 4 h, + 64 i
   const uint32_t gate_bytes = static_cast<uint32_t>(p.gate_row) * 2;
   const uint32_t out_bytes = static_cast<uint32_t>(p.num_v_heads) * kTileRow;
-  u32x4 gate[2];
+  u32x4 gate[2][2];
   auto load_gate = [&](int c) __attribute__((always_inline)) {
     const __amdgpu_buffer_rsrc_t rs =
         chunk_rows(p.gate + head * kDim, p.gate_row, c, gate_bytes, kTileRow);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) gate[i] = load_piece<Wide>(rs, row * gate_bytes + part * 16 + 128 * i, 0);
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        gate[j][i] = load_piece<Wide>(rs, (row + 32 * j) * gate_bytes + part * 16 + 128 * i, 0);
   };
   auto finish = [&](int c) __attribute__((always_inline)) {   // outputs of chunk c from its O
-    auto read = [&](int i, float (&y)[8]) __attribute__((always_inline)) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(o_rows + (o_get ^ (4 * h)) + 64 * i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[4 * h + e] = x[e];
-      }
-    };
-    float rstd = 1.0f;
-    if constexpr (Gated) {
-      float ss = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float y[8];
-        read(i, y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
-      }
-      ss += dpp<kDppQuadXor1>(ss);
-      ss += dpp<kDppQuadXor2>(ss);
-      ss += dpp<kDppRowHalfMirror>(ss);
-      rstd = fast_rsqrt(ss * (1.0f / kDim) + p.eps);
-    }
     const __amdgpu_buffer_rsrc_t rs = chunk_rows(
         p.out + head * kDim, static_cast<int64_t>(p.num_v_heads) * kDim, c, out_bytes, kTileRow);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if constexpr (Gated) lds_order();   // (read again: held, the row would cost spills)
-      float y[8];
-      read(i, y);
-      if constexpr (Gated) {
+    for (int j = 0; j < 2; ++j) {
+      float y[2][8];
+      float ss = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t pair = gate[i][e >> 1];
-          const float g = __builtin_bit_cast(float, e & 1 ? pair & 0xffff0000u : pair << 16);
-          y[e] = ((y[e] * rstd) * lds.weight[8 * part + 64 * i + e]) * silu(g);
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(o_rows + (o_get ^ (4 * h)) + 64 * i + 32 * j * kDim);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y[i][4 * h + e] = x[e];
+            if constexpr (Gated) ss = fmaf(x[e], x[e], ss);
+          }
         }
+      float rstd = 1.0f;
+      if constexpr (Gated) {
+        ss += dpp<kDppQuadXor1>(ss);
+        ss += dpp<kDppQuadXor2>(ss);
+        ss += dpp<kDppRowHalfMirror>(ss);
+        rstd = fast_rsqrt(ss * (1.0f / kDim) + p.eps);
       }
-      u32x4 bits;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) bits[e] = bf16_pair(f32x2{y[2 * e], y[2 * e + 1]});
-      const uint32_t at = row * out_bytes + part * 16 + 128 * i;
-      if constexpr (Wide) {
-        __builtin_amdgcn_raw_buffer_store_b128(bits, rs, at, 0, 0);
-      } else {
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (Gated) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(bits[e]), rs, at + 4 * e, 0, 0);
-          __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(bits[e] >> 16), rs, at + 4 * e + 2, 0, 0);
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t pair = gate[j][i][e >> 1];
+            const float g = __builtin_bit_cast(float, e & 1 ? pair & 0xffff0000u : pair << 16);
+            y[i][e] = ((y[i][e] * rstd) * lds.weight[8 * part + 64 * i + e]) * silu(g);
+          }
+        }
+        u32x4 bits;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bits[e] = bf16_pair(f32x2{y[i][2 * e], y[i][2 * e + 1]});
+        const uint32_t at = (row + 32 * j) * out_bytes + part * 16 + 128 * i;
+        if constexpr (Wide) {
+          __builtin_amdgcn_raw_buffer_store_b128(bits, rs, at, 0, 0);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(bits[e]), rs, at + 4 * e, 0, 0);
+            __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(bits[e] >> 16), rs, at + 4 * e + 2, 0, 0);
+          }
         }
       }
     }
@@ -310,131 +325,159 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
     put(lds.v, staged.v);
   // (the state's loads are waited for here: in the loop the wait would count against later ones)
 #pragma unroll
-  for (int n = 0; n < 4; ++n)
-#pragma unroll
-    for (int a = 0; a < 2; ++a) pin(st[n][a]);
+  for (int T = 0; T < 4; ++T) pin(st[T]);
   for (int c = 0; c < chunks; ++c) {
     const ChunkScalars& s = lds.scalars[c & 1];
     // (opaque here, so that their XORed forms are made where they are used, not held in registers
     // over the loop)
     pin(a_at);
     pin(kt_at);
+    pin(p_upper);
     pin(p_lower);
+    pin(o_put);
     lds_barrier();   // k, q (without Out: v) and scalars of the chunk are in LDS, O of the last
-    f32x4 o[4];
+    f32x16 o[2];
+    const __amdgpu_buffer_rsrc_t next_rows = source(c + 1);
     if constexpr (Out) {
       if constexpr (Gated) load_gate(c - 1);
       // ---- P ----
-      if (has_block) {
-        f32x4 x[2];
+      if (w != kScalarWave) {
+        f32x16 x = {};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int step = 0; step < 8; ++step)
+          x = mfma32(*reinterpret_cast<const bf16x8*>(lds.k + 32 * p_columns * kTileRow + (a_at ^ (step << 5))),
+                     *reinterpret_cast<const bf16x8*>(lds.q + 32 * p_rows * kTileRow + (a_at ^ (step << 5))),
+                     x);
+        const float thi = s.hi[32 * p_rows + lj], tlo = s.lo[32 * p_rows + lj];
 #pragma unroll
-        for (int step = 0; step < 4; ++step) {
-          const bf16x8 q = *reinterpret_cast<const bf16x8*>(lds.q + 16 * strip * kTileRow +
-                                                            (a_at ^ (step << 6)));
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            x[i] = mfma16(*reinterpret_cast<const bf16x8*>(lds.k + 16 * (block + i) * kTileRow +
-                                                           (a_at ^ (step << 6))),
-                          q, x[i]);
-        }
-        const float thi = s.hi[16 * strip + li], tlo = s.lo[16 * strip + li];
-        uint8_t* const at = lds.p[0] + (strip < 2 ? p_upper + 16 * 64 * strip
-                                                  : (p_lower ^ (block << 5)) + 16 * 128 * (strip - 2));
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int first = 16 * (block + i) + 4 * lg;
-          const f32x4 shi = *reinterpret_cast<const f32x4*>(&s.hi[first]);
-          const f32x4 slo = *reinterpret_cast<const f32x4*>(&s.lo[first]);
+        for (int q = 0; q < 4; ++q) {
+          const int first = 8 * q + 4 * hi;
+          const f32x4 shi = *reinterpret_cast<const f32x4*>(&s.hi[32 * p_columns + first]);
+          const f32x4 slo = *reinterpret_cast<const f32x4*>(&s.lo[32 * p_columns + first]);
+          float y[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float d = __builtin_amdgcn_exp2f((thi - shi[r]) + (tlo - slo[r])) * p.scale;
-            x[i][r] = first + r <= 16 * strip + li ? x[i][r] * d : 0.0f;
+            y[r] = p_rows != p_columns || first + r <= lj ? x[4 * q + r] * d : 0.0f;
           }
+          const int u = 2 * p_columns + (q >> 1);
+          uint8_t* const at = lds.p[0] + 8 * (q & 1) + (p_rows == 0 ? p_upper ^ (u << 5) : p_lower ^ (u << 5));
 #pragma unroll
           for (int plane = 0; plane < 2; ++plane) {
-            const uint2 bits = {bf16_pair(f32x2{x[i][0], x[i][1]}), bf16_pair(f32x2{x[i][2], x[i][3]})};
-            *reinterpret_cast<uint2*>(at + 8 * i + plane * kPlaneBytes) = bits;
-            x[i][0] -= __builtin_bit_cast(float, bits.x << 16);
-            x[i][1] -= __builtin_bit_cast(float, bits.x & 0xffff0000u);
-            x[i][2] -= __builtin_bit_cast(float, bits.y << 16);
-            x[i][3] -= __builtin_bit_cast(float, bits.y & 0xffff0000u);
+            const uint2 bits = {bf16_pair(f32x2{y[0], y[1]}), bf16_pair(f32x2{y[2], y[3]})};
+            *reinterpret_cast<uint2*>(at + plane * kPlaneBytes) = bits;
+            y[0] -= __builtin_bit_cast(float, bits.x << 16);
+            y[1] -= __builtin_bit_cast(float, bits.x & 0xffff0000u);
+            y[2] -= __builtin_bit_cast(float, bits.y << 16);
+            y[3] -= __builtin_bit_cast(float, bits.y & 0xffff0000u);
           }
         }
       }
-      // ---- O^T = S Q^T ----
+      // ---- O^T = S Q^T: 16 keys a step, the next step's operands read ahead ----
+      auto q_operand = [&](int n, int tt) __attribute__((always_inline)) {
+        return *reinterpret_cast<const bf16x8*>(lds.q + 32 * tt * kTileRow + (a_at ^ (n << 5)));
+      };
+      bf16x8 q[2][2];
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) o[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int tt = 0; tt < 2; ++tt) q[0][tt] = q_operand(0, tt);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
+      for (int n = 0; n < 8; ++n) {
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = st[n][e >> 2][e & 3];
+        for (int e = 0; e < 8; ++e) x[e] = st[n >> 1][8 * (n & 1) + e];
         const Planes<2> split(x);
+        if (n < 7) {
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-          const bf16x8 q = *reinterpret_cast<const bf16x8*>(lds.q + 16 * tt * kTileRow +
-                                                            (a_at ^ (n << 6)));
-          o[tt] = mfma16(split[1], q, o[tt]);
-          o[tt] = mfma16(split[0], q, o[tt]);
+          for (int tt = 0; tt < 2; ++tt) q[(n + 1) & 1][tt] = q_operand(n + 1, tt);
         }
+        fetch(next_rows, c + 1, n);
+        in_order();
+#pragma unroll
+        for (int plane = 1; plane >= 0; --plane)
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt)
+            o[tt] = mfma32(split[plane], q[n & 1][tt], n == 0 && plane == 1 ? f32x16{} : o[tt]);
+        in_order();
       }
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) o[tt] *= s.eq[16 * tt + li];
+      for (int tt = 0; tt < 2; ++tt) o[tt] *= s.eq[32 * tt + lj];
       finish(c - 1);
       lds_barrier();   // O of the last chunk is read
       put(lds.v, staged.v);
     }
     const float gamma = s.gamma;
-    fetch(c + 1);
+    if constexpr (!Out) {
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
+      for (int i = 0; i < 12; ++i) fetch(next_rows, c + 1, i);
+    }
 #pragma unroll
-      for (int a = 0; a < 2; ++a) st[n][a] *= gamma;
+    for (int T = 0; T < 4; ++T) st[T] *= gamma;
     if (w == kScalarWave)
       total += chunk_scalars(lds.scalars[(c + 1) & 1], next_g, p.scale, lane);
     next_g = load_decay(c + 2);
     if constexpr (Out) lds_barrier();   // v is in LDS (and P)
 
-    // ---- O^T += V^T P^T and S += K^T (e V), 32 tokens a step ----
+    auto v_operand = [&](int u) __attribute__((always_inline)) {
+      return join(read_tr(lds.v + vt_at + 16 * u * kTileRow),
+                  read_tr(lds.v + (vt_at ^ (1 << 5)) + (16 * u + 8) * kTileRow));
+    };
+    auto k_operand = [&](int u, int T) __attribute__((always_inline)) {
+      return join(read_tr(lds.k + (kt_at ^ (T << 6)) + 16 * u * kTileRow),
+                  read_tr(lds.k + (kt_at ^ (T << 6) ^ (1 << 5)) + (16 * u + 8) * kTileRow));
+    };
+    auto p_operand = [&](int u, int tt, int plane) __attribute__((always_inline)) {
+      return *reinterpret_cast<const bf16x8*>(lds.p[plane] + ((tt == 0 ? p_upper : p_lower) ^ (u << 5)));
+    };
+    // ---- O^T += V^T P^T and S += K^T (e V): 16 tokens a step, operands read a product ahead ----
+    bf16x8 v = v_operand(0);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const bf16x8 v = join(read_tr(lds.v + vt_at + 32 * i * kTileRow),
-                            read_tr(lds.v + vt_at + (32 * i + 16) * kTileRow));
+    for (int u = 0; u < 4; ++u) {
+      bf16x8 k = k_operand(u, 0);
       if constexpr (Out) {
+        bf16x8 ps[2][2];
 #pragma unroll
-        for (int tt = 2 * i; tt < 4; ++tt)
+        for (int tt = u < 2 ? 0 : 1; tt < 2; ++tt)
 #pragma unroll
-          for (int plane = 1; plane >= 0; --plane)
-            o[tt] = mfma16(v,
-                           *reinterpret_cast<const bf16x8*>(
-                               lds.p[plane] + (tt < 2 ? p_upper + 16 * 64 * tt
-                                                      : (p_lower ^ (i << 6)) + 16 * 128 * (tt - 2))),
-                           o[tt]);
+          for (int plane = 0; plane < 2; ++plane) ps[tt][plane] = p_operand(u, tt, plane);
+        in_order();
+#pragma unroll
+        for (int plane = 1; plane >= 0; --plane)
+#pragma unroll
+          for (int tt = u < 2 ? 0 : 1; tt < 2; ++tt) o[tt] = mfma32(v, ps[tt][plane], o[tt]);
       }
       float x[8];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const f32x4 ek = *reinterpret_cast<const f32x4*>(&s.ek[32 * i + 16 * h + 4 * lg]);
+        const f32x4 ek = *reinterpret_cast<const f32x4*>(&s.ek[16 * u + 8 * h + 4 * hi]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[4 * h + r] = static_cast<float>(v[4 * h + r]) * ek[r];
       }
       const Planes<3> split(x);
+      bf16x8 next_v = v;
+      if constexpr (Out) fetch(next_rows, c + 1, 8 + u);
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int T = 0; T < 4; ++T) {
+        bf16x8 next_k = k;
+        if (T < 3)
+          next_k = k_operand(u, T + 1);
+        else if (u < 3)
+          next_v = v_operand(u + 1);
+        in_order();
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          const uint8_t* const at = lds.k + (kt_at ^ (n << 6)) + 8 * a;
-          const bf16x8 k = join(read_tr(at + 32 * i * kTileRow), read_tr(at + (32 * i + 16) * kTileRow));
-#pragma unroll
-          for (int plane = 2; plane >= 0; --plane) st[n][a] = mfma16(k, split[plane], st[n][a]);
-        }
+        for (int plane = 2; plane >= 0; --plane) st[T] = mfma32(k, split[plane], st[T]);
+        in_order();
+        k = next_k;
+      }
+      v = next_v;
     }
     lds_barrier();   // every read of the chunk's rows and P is done
     if constexpr (Out) {
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) *reinterpret_cast<f32x4*>(o_rows + o_put + 16 * tt * kDim) = o[tt];
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<f32x4*>(o_rows + (o_put ^ (8 * q)) + 32 * tt * kDim) =
+              f32x4{o[tt][4 * q], o[tt][4 * q + 1], o[tt][4 * q + 2], o[tt][4 * q + 3]};
     }
     put(lds.k, staged.k);
     if constexpr (Out)
@@ -450,10 +493,11 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
 
   if (end != nullptr) {
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
+    for (int T = 0; T < 4; ++T)
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
-        *reinterpret_cast<f32x4*>(reinterpret_cast<char*>(end) + tile_at + 128 * n + 16 * a) = st[n][a];
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(reinterpret_cast<char*>(end) + tile_at + 128 * T + 64 * (q >> 1) + 16 * (q & 1)) =
+            f32x4{st[T][4 * q], st[T][4 * q + 1], st[T][4 * q + 2], st[T][4 * q + 3]};
   }
   return total;
 }
@@ -543,7 +587,7 @@ __device__ __forceinline__ void load_weight(const LinearParams& p, SegmentLds& l
 // segment, walked from its state, or a middle one, reduced to its update; item later + n is
 // sequence n if it is a single segment.
 template <bool Wide, bool Gated>
-__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(4, 4)))
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void linear_first_kernel(const LinearParams p, const Segments g) {
   __shared__ SegmentLds lds;
   __shared__ SearchLds search;
@@ -573,8 +617,8 @@ void linear_first_kernel(const LinearParams p, const Segments g) {
              live && p.has_initial[seq] != 0 ? home : nullptr, whole ? (live ? home : nullptr) : tile);
 }
 
-// The second: the state at every later segment's start, along each sequence; an eighth of a tile
-// a workgroup.
+// The second: the state at every later segment's start, along each sequence; a sixteenth of a
+// tile a workgroup.
 constexpr int kJoinParts = kTileFloats / 4 / kBlock;
 __global__ __launch_bounds__(kBlock) void linear_join_kernel(const LinearParams p, const Segments g) {
   __shared__ SearchLds search;
@@ -600,7 +644,7 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const LinearParams 
 
 // The third: the later segments, each from its state.
 template <bool Wide, bool Gated>
-__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(4, 4)))
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void linear_later_kernel(const LinearParams p, const Segments g) {
   __shared__ SegmentLds lds;
   __shared__ SearchLds search;
