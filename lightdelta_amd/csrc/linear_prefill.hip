@@ -66,25 +66,33 @@ struct SearchLds {
 };
 static_assert(2 * (sizeof(SegmentLds) + sizeof(SearchLds)) <= 160 * 1024, "two workgroups a CU");
 
-// x = sum of N bf16 planes (exactly, for three), eight values as an operand each.
-template <int N>
-struct Planes {
-  u32x4 w[N];
-  __device__ __forceinline__ explicit Planes(float (&x)[8]) {
+// bf16 of registers 8 u .. 8 u + 7 of an accumulator: an operand of step u.
+__device__ __forceinline__ bf16x8 plane_of(const f32x16& x, int u) {
+  u32x4 w;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+  for (int j = 0; j < 4; ++j) w[j] = bf16_pair(f32x2{x[8 * u + 2 * j], x[8 * u + 2 * j + 1]});
+  return __builtin_bit_cast(bf16x8, w);
+}
+
+// x less its planes, by products with -1: the matrix cores have the room that vector issue, which
+// bounds the kernel, has not (two products instead of 32 vector instructions; exact either way,
+// as fp32 holds what rounding to bf16 leaves).
+struct Remainder {
+  bf16x8 minus[2];   // A[i][k] of step u: -1 where row i is the step's summation index k
+  __device__ __forceinline__ explicit Remainder(int lane) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        w[i][j] = bf16_pair(f32x2{x[2 * j], x[2 * j + 1]});
-        if (i + 1 < N) {
-          x[2 * j] -= __builtin_bit_cast(float, w[i][j] << 16);
-          x[2 * j + 1] -= __builtin_bit_cast(float, w[i][j] & 0xffff0000u);
-        }
+    for (int u = 0; u < 2; ++u) {
+      u32x4 w = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int row = 16 * u + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+        if (row == (lane & 31)) w[e >> 1] |= e & 1 ? 0xbf800000u : 0xbf80u;
       }
+      minus[u] = __builtin_bit_cast(bf16x8, w);
     }
   }
-  __device__ __forceinline__ bf16x8 operator[](int i) const {
-    return __builtin_bit_cast(bf16x8, w[i]);
+  __device__ __forceinline__ f32x16 operator()(const f32x16& x, bf16x8 p0, bf16x8 p1) const {
+    return mfma32(minus[1], p1, mfma32(minus[0], p0, x));
   }
 };
 
@@ -318,6 +326,7 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
     }
   };
 
+  const Remainder less(lane);
   put(lds.k, staged.k);
   if constexpr (Out)
     put(lds.q, staged.q);
@@ -354,50 +363,57 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
           const int first = 8 * q + 4 * hi;
           const f32x4 shi = *reinterpret_cast<const f32x4*>(&s.hi[32 * p_columns + first]);
           const f32x4 slo = *reinterpret_cast<const f32x4*>(&s.lo[32 * p_columns + first]);
-          float y[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float d = __builtin_amdgcn_exp2f((thi - shi[r]) + (tlo - slo[r])) * p.scale;
-            y[r] = p_rows != p_columns || first + r <= lj ? x[4 * q + r] * d : 0.0f;
-          }
-          const int u = 2 * p_columns + (q >> 1);
-          uint8_t* const at = lds.p[0] + 8 * (q & 1) + (p_rows == 0 ? p_upper ^ (u << 5) : p_lower ^ (u << 5));
-#pragma unroll
-          for (int plane = 0; plane < 2; ++plane) {
-            const uint2 bits = {bf16_pair(f32x2{y[0], y[1]}), bf16_pair(f32x2{y[2], y[3]})};
-            *reinterpret_cast<uint2*>(at + plane * kPlaneBytes) = bits;
-            y[0] -= __builtin_bit_cast(float, bits.x << 16);
-            y[1] -= __builtin_bit_cast(float, bits.x & 0xffff0000u);
-            y[2] -= __builtin_bit_cast(float, bits.y << 16);
-            y[3] -= __builtin_bit_cast(float, bits.y & 0xffff0000u);
+            x[4 * q + r] = p_rows != p_columns || first + r <= lj ? x[4 * q + r] * d : 0.0f;
           }
         }
+        auto put_plane = [&](int plane, const bf16x8 (&half)[2]) __attribute__((always_inline)) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            *reinterpret_cast<bf16x8*>(lds.p[plane] + ((p_rows == 0 ? p_upper : p_lower) ^
+                                                       ((2 * p_columns + u) << 5))) = half[u];
+        };
+        const bf16x8 high[2] = {plane_of(x, 0), plane_of(x, 1)};
+        put_plane(0, high);
+        x = less(x, high[0], high[1]);
+        const bf16x8 low[2] = {plane_of(x, 0), plane_of(x, 1)};
+        put_plane(1, low);
       }
-      // ---- O^T = S Q^T: 16 keys a step, the next step's operands read ahead ----
-      auto q_operand = [&](int n, int tt) __attribute__((always_inline)) {
-        return *reinterpret_cast<const bf16x8*>(lds.q + 32 * tt * kTileRow + (a_at ^ (n << 5)));
-      };
+      // ---- O^T = S Q^T: 32 keys at a time, S as two planes; an operand is read again once both
+      // of its products are out ----
       bf16x8 q[2][2];
+      auto read_q = [&](int T, int u) __attribute__((always_inline)) {
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt) q[0][tt] = q_operand(0, tt);
+        for (int tt = 0; tt < 2; ++tt)
+          q[u][tt] = *reinterpret_cast<const bf16x8*>(lds.q + 32 * tt * kTileRow +
+                                                      (a_at ^ ((2 * T + u) << 5)));
+      };
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        float x[8];
+      for (int u = 0; u < 2; ++u) read_q(0, u);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = st[n >> 1][8 * (n & 1) + e];
-        const Planes<2> split(x);
-        if (n < 7) {
+      for (int T = 0; T < 4; ++T) {
+        const bf16x8 high[2] = {plane_of(st[T], 0), plane_of(st[T], 1)};
+        const f32x16 rest = less(st[T], high[0], high[1]);
 #pragma unroll
-          for (int tt = 0; tt < 2; ++tt) q[(n + 1) & 1][tt] = q_operand(n + 1, tt);
-        }
-        fetch(next_rows, c + 1, n);
-        in_order();
-#pragma unroll
-        for (int plane = 1; plane >= 0; --plane)
+        for (int u = 0; u < 2; ++u) {
+          fetch(next_rows, c + 1, 2 * T + u);
+          in_order();
 #pragma unroll
           for (int tt = 0; tt < 2; ++tt)
-            o[tt] = mfma32(split[plane], q[n & 1][tt], n == 0 && plane == 1 ? f32x16{} : o[tt]);
-        in_order();
+            o[tt] = mfma32(high[u], q[u][tt], T == 0 && u == 0 ? f32x16{} : o[tt]);
+          in_order();
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const bf16x8 low = plane_of(rest, u);
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt) o[tt] = mfma32(low, q[u][tt], o[tt]);
+          in_order();
+          if (T < 3) read_q(T + 1, u);
+          in_order();
+        }
       }
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt) o[tt] *= s.eq[32 * tt + lj];
@@ -428,47 +444,63 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
     auto p_operand = [&](int u, int tt, int plane) __attribute__((always_inline)) {
       return *reinterpret_cast<const bf16x8*>(lds.p[plane] + ((tt == 0 ? p_upper : p_lower) ^ (u << 5)));
     };
-    // ---- O^T += V^T P^T and S += K^T (e V): 16 tokens a step, operands read a product ahead ----
-    bf16x8 v = v_operand(0);
+    // ---- O^T += V^T P^T and S += K^T (e V): 32 tokens at a time, operands read a product ahead ----
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      bf16x8 k = k_operand(u, 0);
-      if constexpr (Out) {
-        bf16x8 ps[2][2];
+    for (int i = 0; i < 2; ++i) {
+      const bf16x8 v[2] = {v_operand(2 * i), v_operand(2 * i + 1)};
+      f32x16 x;
 #pragma unroll
-        for (int tt = u < 2 ? 0 : 1; tt < 2; ++tt)
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 ek = *reinterpret_cast<const f32x4*>(&s.ek[32 * i + 8 * q + 4 * hi]);
 #pragma unroll
-          for (int plane = 0; plane < 2; ++plane) ps[tt][plane] = p_operand(u, tt, plane);
-        in_order();
-#pragma unroll
-        for (int plane = 1; plane >= 0; --plane)
-#pragma unroll
-          for (int tt = u < 2 ? 0 : 1; tt < 2; ++tt) o[tt] = mfma32(v, ps[tt][plane], o[tt]);
+        for (int r = 0; r < 4; ++r)
+          x[4 * q + r] = static_cast<float>(v[q >> 1][4 * (q & 1) + r]) * ek[r];
       }
-      float x[8];
+      bf16x8 planes[3][2];
+      auto set_planes = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const f32x4 ek = *reinterpret_cast<const f32x4*>(&s.ek[16 * u + 8 * h + 4 * hi]);
+        for (int u = 0; u < 2; ++u) planes[n][u] = plane_of(x, u);
+      };
+      // O's products, between the steps of the split
+      auto outputs = [&](int u) __attribute__((always_inline)) {
+        if constexpr (Out) {
+          bf16x8 ps[2][2];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[4 * h + r] = static_cast<float>(v[4 * h + r]) * ek[r];
+          for (int tt = i; tt < 2; ++tt)
+#pragma unroll
+            for (int plane = 0; plane < 2; ++plane) ps[tt][plane] = p_operand(2 * i + u, tt, plane);
+          in_order();
+#pragma unroll
+          for (int plane = 1; plane >= 0; --plane)
+#pragma unroll
+            for (int tt = i; tt < 2; ++tt) o[tt] = mfma32(v[u], ps[tt][plane], o[tt]);
+        }
+      };
+      set_planes(0);
+      x = less(x, planes[0][0], planes[0][1]);
+      outputs(0);
+      set_planes(1);
+      x = less(x, planes[1][0], planes[1][1]);
+      outputs(1);
+      set_planes(2);
+      bf16x8 k = k_operand(2 * i, 0);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if constexpr (Out) fetch(next_rows, c + 1, 8 + 2 * i + u);
+#pragma unroll
+        for (int T = 0; T < 4; ++T) {
+          bf16x8 next_k = k;
+          if (T < 3)
+            next_k = k_operand(2 * i + u, T + 1);
+          else if (u == 0)
+            next_k = k_operand(2 * i + 1, 0);
+          in_order();
+#pragma unroll
+          for (int plane = 2; plane >= 0; --plane) st[T] = mfma32(k, planes[plane][u], st[T]);
+          in_order();
+          k = next_k;
+        }
       }
-      const Planes<3> split(x);
-      bf16x8 next_v = v;
-      if constexpr (Out) fetch(next_rows, c + 1, 8 + u);
-#pragma unroll
-      for (int T = 0; T < 4; ++T) {
-        bf16x8 next_k = k;
-        if (T < 3)
-          next_k = k_operand(u, T + 1);
-        else if (u < 3)
-          next_v = v_operand(u + 1);
-        in_order();
-#pragma unroll
-        for (int plane = 2; plane >= 0; --plane) st[T] = mfma32(k, split[plane], st[T]);
-        in_order();
-        k = next_k;
-      }
-      v = next_v;
     }
     lds_barrier();   // every read of the chunk's rows and P is done
     if constexpr (Out) {
