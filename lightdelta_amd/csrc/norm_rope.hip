@@ -4,11 +4,13 @@
 // in fp32, rounded to bf16 once.
 //
 // Bound by memory: 512 bytes a head and token against about 90 vector instructions per 4 heads.
-// A wave takes one token and walks its heads four at a time, 16 lanes a head, 8 consecutive
-// elements (16 bytes) a lane.  A lane's 8 angles are the same for every head of the token, so it
-// forms them once: the product and its reduction to a fraction of a turn in 64 bits (positions
-// of millions times frequencies near 1 leave 32 bits no fraction), sine and cosine in fp32.  No
-// LDS and no barrier.
+// A wave takes one token and four heads at a time, 16 lanes a head, 8 consecutive elements (16
+// bytes) a lane, four rounds of loads in flight.  A lane's 8 angles are the same for every head of
+// the token, so it forms them once: the product and its reduction to a fraction of a turn in 64
+// bits (positions of millions times frequencies near 1 leave 32 bits no fraction), sine and cosine
+// in fp32.  A pair's other element comes from a lane of the same 16 by DPP.  No LDS, no barrier.
+#include <algorithm>
+
 #include "gdn_common.h"
 #include "lightdelta_linear_hip.h"
 
@@ -16,6 +18,8 @@ namespace ld {
 namespace {
 
 constexpr int kHeadsPerRound = 4;
+
+constexpr int kBatch = 4;   // rounds whose loads are in flight together
 
 struct NormRopeParams {
   uint16_t* qkv;
@@ -34,12 +38,25 @@ struct NormRopeParams {
   float eps;
 };
 
-// Interleaved: a pair's elements are neighbours in a lane; else `half` elements apart, the
-// partner's lane half / 8 lanes up (first half) or down.
-template <bool Interleaved>
+// Where a lane finds the other elements of its pairs: its own (neighbours, interleaved), the lane
+// whose number differs in bit D, or (any other half) one that a shuffle names.
+constexpr int kOwn = 0;
+constexpr int kShuffle = -1;
+
+template <int D>
+__device__ __forceinline__ float partner(float y, int lane) {
+  if constexpr (D == 8) return dpp<0x128>(y);                                  // row_ror:8
+  if constexpr (D == 4) return dpp<0x1B>(dpp<kDppRowHalfMirror>(y));           // ^ 7, ^ 3
+  if constexpr (D == 2) return dpp<kDppQuadXor2>(y);
+  if constexpr (D == 1) return dpp<kDppQuadXor1>(y);
+  return __shfl(y, lane);
+}
+
+template <int D>
 __global__ __launch_bounds__(kThreads) void norm_rope_kernel(const NormRopeParams p) {
   const int lane = threadIdx.x & 63;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWaves +
+                       __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t token = unit / p.splits;
   if (token >= p.num_tokens) return;
   const int first = static_cast<int>(unit - token * p.splits) * p.rounds * kHeadsPerRound;
@@ -47,60 +64,81 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(const NormRopeParam
   const int sub = lane >> 4;
   uint16_t* const row = p.qkv + token * p.row + 8 * li;
 
+  // the heads of round r: lanes past the last head repeat it and store nothing
+  u32x4 raw[kBatch];
+  auto head_of = [&](int r) { return first + r * kHeadsPerRound + sub; };
+  auto load = [&](int r) {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+      __builtin_memcpy(&raw[b], row + static_cast<int64_t>(min(head_of(r + b), p.heads - 1)) * kDim, 16);
+  };
+  load(0);
+  float wq[8], wk[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    wq[e] = p.q_heads > 0 ? load_param(p.q_weight, 8 * li + e, p.q_bf16) : 0.0f;
+    wk[e] = p.q_heads < p.heads ? load_param(p.k_weight, 8 * li + e, p.k_bf16) : 0.0f;
+  }
   const double position =
       p.positions64 ? static_cast<double>(static_cast<const int64_t*>(p.positions)[token])
                     : static_cast<double>(static_cast<const int32_t*>(p.positions)[token]);
-  // c[e], s[e]: cosine and signed sine of element 8 li + e; (1, 0) past the rotated ones
+  // c[e], s[e]: cosine and signed sine of element 8 li + e, if it is turned
   float c[8], s[8];
+  bool turned[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int element = 8 * li + e;
-    const bool turned = element < 2 * p.half;
-    const int i = Interleaved ? element >> 1 : (element < p.half ? element : element - p.half);
-    c[e] = 1.0f;
-    s[e] = 0.0f;
-    if (turned) {
-      const double turns = position * static_cast<double>(p.inv_freq[i]) * 0.15915494309189535;
-      const float fraction = static_cast<float>(turns - rint(turns));
-      c[e] = __builtin_amdgcn_cosf(fraction);
-      const float sine = __builtin_amdgcn_sinf(fraction);
-      const bool is_first = Interleaved ? (e & 1) == 0 : element < p.half;
-      s[e] = is_first ? -sine : sine;
-    }
+    turned[e] = element < 2 * p.half;
+    const int i = D == kOwn ? element >> 1 : (element < p.half ? element : element - p.half);
+    const double turns = position * static_cast<double>(p.half > 0 ? p.inv_freq[turned[e] ? i : 0] : 0.0f) *
+                         0.15915494309189535;
+    const float fraction = static_cast<float>(turns - rint(turns));
+    c[e] = __builtin_amdgcn_cosf(fraction);
+    const float sine = __builtin_amdgcn_sinf(fraction);
+    const bool is_first = D == kOwn ? (e & 1) == 0 : element < p.half;
+    s[e] = is_first ? -sine : sine;
   }
-  const int partner = Interleaved ? lane : (8 * li < p.half ? lane + (p.half >> 3)
-                                            : 8 * li < 2 * p.half ? lane - (p.half >> 3)
-                                                                  : lane);
-  for (int round = 0; round < p.rounds; ++round) {
-    const int head = first + round * kHeadsPerRound + sub;
-    const bool live = head < p.heads;
-    if (first + round * kHeadsPerRound >= p.heads) return;
-    const int at = live ? head : p.heads - 1;
-    uint16_t raw[8];
-    __builtin_memcpy(raw, row + static_cast<int64_t>(at) * kDim, 16);
-    const bool is_q = at < p.q_heads;
-    float y[8];
-    float ss = 0.0f;
+  int other_lane = lane;
+  if (D == kShuffle && 8 * li < 2 * p.half)
+    other_lane = 8 * li < p.half ? lane + (p.half >> 3) : lane - (p.half >> 3);
+
+  for (int r = 0; r < p.rounds; r += kBatch) {
+    u32x4 now[kBatch];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      y[e] = bf16_to_f32(raw[e]);
-      ss = fmaf(y[e], y[e], ss);
+    for (int b = 0; b < kBatch; ++b) now[b] = raw[b];
+    if (r + kBatch < p.rounds) load(r + kBatch);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      if (r + b >= p.rounds || first + (r + b) * kHeadsPerRound >= p.heads) break;
+      const int head = head_of(r + b);
+      const bool is_q = head < p.q_heads;
+      float y[8];
+      float ss = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t pair = now[b][e >> 1];
+        y[e] = __uint_as_float(e & 1 ? pair & 0xffff0000u : pair << 16);
+        ss = fmaf(y[e], y[e], ss);
+      }
+      ss += dpp<kDppQuadXor1>(ss);
+      ss += dpp<kDppQuadXor2>(ss);
+      ss += dpp<kDppRowHalfMirror>(ss);
+      ss += dpp<kDppRowMirror>(ss);
+      const float rstd = fast_rsqrt(ss * (1.0f / kDim) + p.eps);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = (y[e] * rstd) * (is_q ? wq[e] : wk[e]);
+      float z[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float other = D == kOwn ? y[e ^ 1] : partner<D>(y[e], other_lane);
+        z[e] = turned[e] ? fmaf(y[e], c[e], other * s[e]) : y[e];
+      }
+      u32x4 bits;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        bits[e] = f32_to_bf16(z[2 * e]) | static_cast<uint32_t>(f32_to_bf16(z[2 * e + 1])) << 16;
+      if (head < p.heads) __builtin_memcpy(row + static_cast<int64_t>(head) * kDim, &bits, 16);
     }
-    ss += dpp<kDppQuadXor1>(ss);
-    ss += dpp<kDppQuadXor2>(ss);
-    ss += dpp<kDppRowHalfMirror>(ss);
-    ss += dpp<kDppRowMirror>(ss);
-    const float rstd = fast_rsqrt(ss * (1.0f / kDim) + p.eps);
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      y[e] = (y[e] * rstd) * load_param(is_q ? p.q_weight : p.k_weight, 8 * li + e,
-                                        is_q ? p.q_bf16 : p.k_bf16);
-    float other[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) other[e] = Interleaved ? y[e ^ 1] : __shfl(y[e], partner);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) raw[e] = f32_to_bf16(fmaf(y[e], c[e], other[e] * s[e]));
-    if (live) __builtin_memcpy(row + static_cast<int64_t>(at) * kDim, raw, 16);
   }
 }
 
@@ -128,7 +166,10 @@ extern "C" int ld_norm_rope(const ld_norm_rope_args* args, void* stream) {
     return fail(LD_ERR_INVALID_ARGUMENT, "ld_norm_rope: NULL tensor pointer");
   if (a.num_tokens > 1 && a.qkv_row_stride < heads * kDim)
     return fail(LD_ERR_INVALID_ARGUMENT, "qkv rows must not overlap");
+  // A wave takes all rounds of its token where tokens fill the chip (four waves a SIMD), else as
+  // many waves as rounds share one.
   const int64_t rounds = (heads + kHeadsPerRound - 1) / kHeadsPerRound;
+  const int64_t splits = a.num_tokens >= 4096 ? 1 : std::min<int64_t>(rounds, 4096 / a.num_tokens);
   NormRopeParams p{};
   p.qkv = static_cast<uint16_t*>(a.qkv);
   p.row = a.qkv_row_stride;
@@ -140,15 +181,20 @@ extern "C" int ld_norm_rope(const ld_norm_rope_args* args, void* stream) {
   p.q_heads = a.q_heads;
   p.heads = static_cast<int32_t>(heads);
   p.half = a.rotary / 2;
-  p.rounds = static_cast<int32_t>(rounds);
-  p.splits = 1;
+  p.rounds = static_cast<int32_t>((rounds + splits - 1) / splits);
+  p.splits = static_cast<int32_t>((rounds + p.rounds - 1) / p.rounds);
   p.q_bf16 = a.q_weight_dtype == LD_DTYPE_BF16;
   p.k_bf16 = a.k_weight_dtype == LD_DTYPE_BF16;
   p.positions64 = a.positions_int64;
   p.eps = a.eps;
   const int64_t blocks = (a.num_tokens * p.splits + kWaves - 1) / kWaves;
   if (blocks > 0xffffff) return fail(LD_ERR_INVALID_ARGUMENT, "too many tokens");
-  const auto kernel = a.interleaved ? norm_rope_kernel<true> : norm_rope_kernel<false>;
+  const auto kernel = a.interleaved    ? norm_rope_kernel<kOwn>
+                      : p.half == 64   ? norm_rope_kernel<8>
+                      : p.half == 32   ? norm_rope_kernel<4>
+                      : p.half == 16   ? norm_rope_kernel<2>
+                      : p.half == 8    ? norm_rope_kernel<1>
+                                       : norm_rope_kernel<kShuffle>;
   hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0,
                      static_cast<hipStream_t>(stream), p);
   return check_launch("ld_norm_rope");
