@@ -3,11 +3,13 @@
 // per (request, v-head), S a 128 x 128 fp32 tile of the state pool.
 //
 // Bound by memory: a tile is read once and written once a token, 4 flops an element and token.
-// One workgroup per tile, its lanes as in gdn_step.h (16 lanes a K row, 4 V rows a wave and
-// piece pair); every tile load goes out first, then the pieces are worked in load order, each
+// One workgroup of 16 waves per tile, its lanes as in gdn_step.h (16 lanes a K row, 4 V rows a
+// wave and piece pair, so that a piece pair of all waves covers half the tile in address order);
+// every tile load goes out first, then the pieces are worked in load order, each
 // row pair scaled, updated, stored and reduced against q (8 products a lane, 4 DPP steps).  A
 // token's q, k and v come straight to registers: the recurrence normalises nothing, so there is
-// nothing to stage.
+// nothing to stage.  Two tiles a CU for one token; for verify steps, whose four tokens' inputs need
+// the registers, one.
 #include "gdn_step.h"
 #include "linear_common.h"
 
@@ -21,14 +23,17 @@ struct LinearToken {
   float decay;
 };
 
-template <int LoadPol, int StorePol, int Width, int Waves>
-__global__ __launch_bounds__(64 * Waves)
+constexpr int kTileWaves = 16;
+
+template <int LoadPol, int StorePol, int Width>
+__global__ __launch_bounds__(64 * kTileWaves)
+__attribute__((amdgpu_waves_per_eu(Width == 1 ? 8 : 4, Width == 1 ? 8 : 4)))
 void linear_decode_kernel(const int32_t* md_indices, const int32_t* md_cu,
                           const int32_t* md_accepted, int md_num_v_heads, const LinearParams p) {
-  constexpr int kBlock = 64 * Waves;
-  constexpr int kPc = kDim / Waves / 2;   // 16-byte tile pieces per lane
-  constexpr int kPair = 4 * Waves;        // rows that a piece pair of every wave covers
-  constexpr int kRows = kPc / 2;          // V rows per lane
+  constexpr int kBlock = 64 * kTileWaves;
+  constexpr int kPc = kDim / kTileWaves / 2;   // 16-byte tile pieces per lane
+  constexpr int kPair = 4 * kTileWaves;        // rows that a piece pair of every wave covers
+  constexpr int kRows = kPc / 2;               // V rows per lane
   const int tile = blockIdx.x;
   const int request = tile / md_num_v_heads;
   const int head = tile - request * md_num_v_heads;
@@ -160,10 +165,32 @@ void linear_decode_kernel(const int32_t* md_indices, const int32_t* md_cu,
   }
 }
 
-template <int LoadPol, int StorePol, int Width, int Waves>
-void launch_linear(const LinearParams& p, uint32_t blocks, hipStream_t stream) {
-  hipLaunchKernelGGL((linear_decode_kernel<LoadPol, StorePol, Width, Waves>), dim3(blocks),
-                     dim3(64 * Waves), 0, stream, p.indices, p.cu, p.accepted, p.num_v_heads, p);
+template <int LoadPol, int StorePol, int Width>
+void launch_width(const LinearParams& p, uint32_t blocks, hipStream_t stream) {
+  hipLaunchKernelGGL((linear_decode_kernel<LoadPol, StorePol, Width>), dim3(blocks),
+                     dim3(64 * kTileWaves), 0, stream, p.indices, p.cu, p.accepted, p.num_v_heads, p);
+}
+
+// Cache policies as measured on MI355X (us; "hot" the same slots every step, "cold" slot sets
+// rotated beyond the 256 MB Infinity Cache), 32 requests x 32 heads hot / cold, 119 x 48 cold, and
+// a 4-token verify of 64 x 32 hot / cold:
+//   non-temporal system-scope loads and stores   25.5 / 25.4   122    81.5 / 85.8   (stream)
+//   plain loads, system-scope stores             21.1 / 27.6   134    88.5 / 98.3   (keep, one token)
+//   plain loads, non-temporal stores             21.8 / 29.9   138    66.1 / 96.3   (keep, verify)
+//   plain loads and stores                       21.8 / 29.4   137    103 / 109
+// Other shapes under the stream policy: 4 waves 25.7 / 25.9, 135, 112 / 115; 8 waves 26.9 / 27.0,
+// 129, 89 / 95.  At 5.1 TB/s, a large copy's rate, these calls' bytes take 26.4, 146 and 92.8 us.
+void launch_linear(const LinearParams& p, int width, bool keep, uint32_t blocks, hipStream_t s) {
+  switch (width) {
+    case 1: return keep ? launch_width<kPolPlain, kPolSys, 1>(p, blocks, s)
+                        : launch_width<kPolNTSys, kPolNTSys, 1>(p, blocks, s);
+    case 2: return keep ? launch_width<kPolPlain, kPolNT, 2>(p, blocks, s)
+                        : launch_width<kPolNTSys, kPolNTSys, 2>(p, blocks, s);
+    case 3: return keep ? launch_width<kPolPlain, kPolNT, 3>(p, blocks, s)
+                        : launch_width<kPolNTSys, kPolNTSys, 3>(p, blocks, s);
+    default: return keep ? launch_width<kPolPlain, kPolNT, 4>(p, blocks, s)
+                         : launch_width<kPolNTSys, kPolNTSys, 4>(p, blocks, s);
+  }
 }
 
 }  // namespace
@@ -187,13 +214,7 @@ extern "C" int ld_linear_decode(const ld_linear_decode_args* args, void* stream)
   p.indices = a.indices;
   p.cu = a.cu;
   p.accepted = a.accepted;
-  const uint32_t n = static_cast<uint32_t>(blocks);
-  const hipStream_t s = static_cast<hipStream_t>(stream);
-  switch (a.width) {
-    case 1: launch_linear<kPolPlain, kPolPlain, 1, 4>(p, n, s); break;
-    case 2: launch_linear<kPolPlain, kPolPlain, 2, 4>(p, n, s); break;
-    case 3: launch_linear<kPolPlain, kPolPlain, 3, 4>(p, n, s); break;
-    default: launch_linear<kPolPlain, kPolPlain, 4, 4>(p, n, s);
-  }
+  launch_linear(p, a.width, a.cache_policy == LD_CACHE_KEEP, static_cast<uint32_t>(blocks),
+                static_cast<hipStream_t>(stream));
   return check_launch("ld_linear_decode");
 }

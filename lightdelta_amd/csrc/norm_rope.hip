@@ -5,10 +5,10 @@
 //
 // Bound by memory: 512 bytes a head and token against about 90 vector instructions per 4 heads.
 // A wave takes one token and four heads at a time, 16 lanes a head, 8 consecutive elements (16
-// bytes) a lane, four rounds of loads in flight.  A lane's 8 angles are the same for every head of
-// the token, so it forms them once: the product and its reduction to a fraction of a turn in 64
-// bits (positions of millions times frequencies near 1 leave 32 bits no fraction), sine and cosine
-// in fp32.  A pair's other element comes from a lane of the same 16 by DPP.  No LDS, no barrier.
+// bytes) a lane, four rounds of loads in flight.  The token's angles are formed once, one a lane,
+// and spread through LDS: the product and its reduction to a fraction of a turn in 64 bits
+// (positions of millions times frequencies near 1 leave 32 bits no fraction), sine and cosine in
+// fp32.  A pair's other element comes from a lane of the same 16 by DPP.
 #include <algorithm>
 
 #include "gdn_common.h"
@@ -52,6 +52,17 @@ __device__ __forceinline__ float partner(float y, int lane) {
   return __shfl(y, lane);
 }
 
+__device__ __forceinline__ void load_weights(float (&w)[8], const void* from, int at, bool bf16) {
+  if (bf16) {
+    uint16_t raw[8];
+    __builtin_memcpy(raw, static_cast<const uint16_t*>(from) + at, 16);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = bf16_to_f32(raw[e]);
+  } else {
+    __builtin_memcpy(w, static_cast<const float*>(from) + at, 32);
+  }
+}
+
 template <int D>
 __global__ __launch_bounds__(kThreads) void norm_rope_kernel(const NormRopeParams p) {
   const int lane = threadIdx.x & 63;
@@ -73,30 +84,34 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(const NormRopeParam
       __builtin_memcpy(&raw[b], row + static_cast<int64_t>(min(head_of(r + b), p.heads - 1)) * kDim, 16);
   };
   load(0);
-  float wq[8], wk[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    wq[e] = p.q_heads > 0 ? load_param(p.q_weight, 8 * li + e, p.q_bf16) : 0.0f;
-    wk[e] = p.q_heads < p.heads ? load_param(p.k_weight, 8 * li + e, p.k_bf16) : 0.0f;
+  float wq[8] = {}, wk[8] = {};
+  if (p.q_heads > 0) load_weights(wq, p.q_weight, 8 * li, p.q_bf16);
+  if (p.q_heads < p.heads) load_weights(wk, p.k_weight, 8 * li, p.k_bf16);
+  // angle `lane` of the token, by one lane each, and from LDS (the wave's own, so without a barrier)
+  // the lane's eight; element 8 li + e has angle first + e (halves) or first + e / 2 (interleaved)
+  __shared__ __attribute__((aligned(16))) float angles[kWaves][2][64];
+  float* const mine = angles[threadIdx.x >> 6][0];
+  if (lane < p.half) {
+    const double position =
+        p.positions64 ? static_cast<double>(static_cast<const int64_t*>(p.positions)[token])
+                      : static_cast<double>(static_cast<const int32_t*>(p.positions)[token]);
+    const double turns = position * static_cast<double>(p.inv_freq[lane]) * 0.15915494309189535;
+    const float fraction = static_cast<float>(turns - rint(turns));
+    mine[lane] = __builtin_amdgcn_cosf(fraction);
+    mine[64 + lane] = __builtin_amdgcn_sinf(fraction);
   }
-  const double position =
-      p.positions64 ? static_cast<double>(static_cast<const int64_t*>(p.positions)[token])
-                    : static_cast<double>(static_cast<const int32_t*>(p.positions)[token]);
-  // c[e], s[e]: cosine and signed sine of element 8 li + e, if it is turned
+  asm volatile("" ::: "memory");   // (a wave's LDS operations run in order)
+  const int element = 8 * li;
+  const bool second = D != kOwn && element >= p.half;   // the lane holds pairs' second elements
+  const int angle = D == kOwn ? element >> 1 : min(second ? element - p.half : element, 56);
   float c[8], s[8];
   bool turned[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const int element = 8 * li + e;
-    turned[e] = element < 2 * p.half;
-    const int i = D == kOwn ? element >> 1 : (element < p.half ? element : element - p.half);
-    const double turns = position * static_cast<double>(p.half > 0 ? p.inv_freq[turned[e] ? i : 0] : 0.0f) *
-                         0.15915494309189535;
-    const float fraction = static_cast<float>(turns - rint(turns));
-    c[e] = __builtin_amdgcn_cosf(fraction);
-    const float sine = __builtin_amdgcn_sinf(fraction);
-    const bool is_first = D == kOwn ? (e & 1) == 0 : element < p.half;
-    s[e] = is_first ? -sine : sine;
+    const int i = angle + (D == kOwn ? e >> 1 : e);
+    c[e] = mine[i];
+    s[e] = (D == kOwn ? (e & 1) != 0 : second) ? mine[64 + i] : -mine[64 + i];
+    turned[e] = element + e < 2 * p.half;
   }
   int other_lane = lane;
   if (D == kShuffle && 8 * li < 2 * p.half)
