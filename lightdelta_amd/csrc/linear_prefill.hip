@@ -25,9 +25,11 @@
 // 2^-9 of the output's own rounding).
 //
 // A sequence longer than a segment is cut into segments, since the recurrence over them is
-// associative: one launch runs every first segment and reduces the middle ones to their update
-// and decay, a second joins these along each sequence, a third runs the later segments from the
-// states the second left.
+// associative: one launch reduces every segment but the last to its update and decay (and walks the
+// sequences of one segment), a second joins these along each sequence, a third walks all segments
+// from the states the second left.
+#include <cstddef>
+
 #include "linear_common.h"
 #include "matrix_common.h"
 
@@ -64,6 +66,7 @@ struct SearchLds {
   int wave_sums[kBlockWaves];
   int found[3];
 };
+static_assert(offsetof(SegmentLds, v) + sizeof(SegmentLds::v) == kTileBytes, "k, q and v are a tile");
 static_assert(2 * (sizeof(SegmentLds) + sizeof(SearchLds)) <= 160 * 1024, "two workgroups a CU");
 
 // bf16 of registers 8 u .. 8 u + 7 of an accumulator: an operand of step u.
@@ -151,7 +154,8 @@ constexpr int kScalarWave = 3;   // makes the chunks' scalars: the wave without 
 // over 0 bytes or an offset past it: zeros and dropped stores): under a branch the compiler would
 // have to wait for every load in flight before it uses any.  Wide: every address is a multiple of
 // 4 bytes; else elements move one by one.
-template <bool Wide, bool Gated, bool Out>
+// StartPol, EndPol: cache policy bits of the state's loads and stores.
+template <bool Wide, bool Gated, bool Out, int StartPol, int EndPol>
 __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, int64_t bos, int rows,
                                        int head, const float* start, float* end) {
   const int tid = threadIdx.x;
@@ -219,20 +223,36 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
   }
   float next_g = load_decay(0);
 
-  // st[T][8 u + 4 h + r] = S[32 w + lj][32 T + 16 u + 8 hi + 4 h + r]
-  f32x16 st[4];
-  const int tile_at = ((32 * w + lj) * kDim + 8 * hi) * 4;
-  {
-    const __amdgpu_buffer_rsrc_t rs = record_resource(
-        start, __builtin_amdgcn_readfirstlane(start != nullptr ? kTileBytes : 0));
+  // st[T][8 u + 4 h + r] = S[32 w + lj][32 T + 16 u + 8 hi + 4 h + r], by way of LDS, so that memory
+  // is read (and at the end written) in whole lines: row v's 16-byte pieces XORed with v % 16
+  f32x16 st[4] = {};
+  uint8_t* const tile = lds.k;
+  const uint32_t tile_at = (32 * w + lj) * (kDim * 4) + (((2 * hi) ^ (lj & 15)) << 4);
+  auto tile_piece = [&](int T, int q) __attribute__((always_inline)) {   // of st[T][4 q ..]
+    return reinterpret_cast<f32x4*>(tile + (tile_at ^ ((8 * T + 4 * (q >> 1) + (q & 1)) << 4)));
+  };
+  const uint32_t line_at = tid * 16;                                     // + 4096 i
+  auto line_piece = [&](int i) __attribute__((always_inline)) {
+    const int v = 8 * i + (tid >> 5);
+    return reinterpret_cast<f32x4*>(tile + v * (kDim * 4) + (((tid & 31) ^ (v & 15)) << 4));
+  };
+  if (start != nullptr) {
+    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(start, kTileBytes);
+    f32x4 lines[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) lines[i] = buffer_load16<StartPol>(rs, line_at + 4096 * i);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) *line_piece(i) = lines[i];
+    lds_barrier();
 #pragma unroll
     for (int T = 0; T < 4; ++T)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const f32x4 x = load16(rs, tile_at + 128 * T + 64 * (q >> 1) + 16 * (q & 1), 0);
+        const f32x4 x = *tile_piece(T, q);
 #pragma unroll
         for (int r = 0; r < 4; ++r) st[T][4 * q + r] = x[r];
       }
+    lds_barrier();
   }
   double total = 0.0;
   if (w == kScalarWave) total += chunk_scalars(lds.scalars[0], next_g, p.scale, lane);
@@ -332,9 +352,6 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
     put(lds.q, staged.q);
   else
     put(lds.v, staged.v);
-  // (the state's loads are waited for here: in the loop the wait would count against later ones)
-#pragma unroll
-  for (int T = 0; T < 4; ++T) pin(st[T]);
   for (int c = 0; c < chunks; ++c) {
     const ChunkScalars& s = lds.scalars[c & 1];
     // (opaque here, so that their XORed forms are made where they are used, not held in registers
@@ -524,12 +541,16 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
   }
 
   if (end != nullptr) {
+    lds_barrier();   // (the last chunk's reads of LDS)
 #pragma unroll
     for (int T = 0; T < 4; ++T)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<f32x4*>(reinterpret_cast<char*>(end) + tile_at + 128 * T + 64 * (q >> 1) + 16 * (q & 1)) =
-            f32x4{st[T][4 * q], st[T][4 * q + 1], st[T][4 * q + 2], st[T][4 * q + 3]};
+        *tile_piece(T, q) = f32x4{st[T][4 * q], st[T][4 * q + 1], st[T][4 * q + 2], st[T][4 * q + 3]};
+    lds_barrier();
+    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(end, kTileBytes);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) buffer_store16<EndPol>(*line_piece(i), rs, line_at + 4096 * i);
   }
   return total;
 }
@@ -540,13 +561,33 @@ __device__ __forceinline__ void sequence_rows(const LinearParams& p, int seq, in
   rows = static_cast<int>(max(row_of(p.cu[seq + 1], p.num_tokens) - bos, int64_t{0}));
 }
 
+// Inclusive sums over the workgroup, and the total; `sums` is free again after a barrier.
+__device__ __forceinline__ int inclusive_sum(int mine, int (&sums)[kBlockWaves], int& all) {
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  int sum = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int below = __shfl_up(sum, d);
+    if (lane >= d) sum += below;
+  }
+  if (lane == 63) sums[wave] = sum;
+  __syncthreads();
+  all = 0;
+#pragma unroll
+  for (int v = 0; v < kBlockWaves; ++v) {
+    if (v < wave) sum += sums[v];
+    all += sums[v];
+  }
+  return sum;
+}
+
 // Later segments (all but the first) of the sequences are numbered in order: finds the j-th, i.e.
 // its sequence, which of the sequence's later segments it is, and how many that has.  False past
 // the last.  By the whole workgroup.
 __device__ bool find_segment(const LinearParams& p, SearchLds& lds, int num_sequences, int shift,
                              int j, int& seq, int& index, int& count) {
   const int tid = threadIdx.x;
-  const int lane = tid & 63;
   int base = 0;
   for (int first = 0; first < num_sequences; first += kBlock) {
     const int n = first + tid;
@@ -557,20 +598,8 @@ __device__ bool find_segment(const LinearParams& p, SearchLds& lds, int num_sequ
       sequence_rows(p, n, bos, rows);
       mine = rows > 0 ? (rows - 1) >> shift : 0;
     }
-    int sum = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int below = __shfl_up(sum, d);
-      if (lane >= d) sum += below;
-    }
-    if (lane == 63) lds.wave_sums[tid >> 6] = sum;
-    __syncthreads();
-    int all = 0;
-#pragma unroll
-    for (int v = 0; v < kBlockWaves; ++v) {
-      if (v < tid >> 6) sum += lds.wave_sums[v];
-      all += lds.wave_sums[v];
-    }
+    int all;
+    const int sum = inclusive_sum(mine, lds.wave_sums, all);
     const int at = j - base;
     if (at < sum && at >= sum - mine) {
       lds.found[0] = n;
@@ -593,8 +622,10 @@ struct Segments {
   int num_sequences;
   int shift;        // log2 of a segment's tokens
   int later;        // at most this many later segments
-  float* tiles;     // per (later segment, head): the state it starts from, S or (before the
-                    // second launch) the update of the segment ahead of it
+  float* tiles;     // per (later segment, head): the state it starts from (before the second
+                    // launch, the update of the segment ahead of it)
+  float* firsts;    // in the places of the first later segments: the state the sequence starts
+                    // from, as its last segment replaces it in the pool
   float* decays;    // per (later segment, head): the decay over the segment ahead of it
 };
 
@@ -615,9 +646,12 @@ __device__ __forceinline__ void load_weight(const LinearParams& p, SegmentLds& l
     lds.weight[threadIdx.x] = load_param(p.norm_weight, threadIdx.x, p.weight_bf16);
 }
 
-// The first launch.  Item j < later is later segment j's predecessor: the sequence's first
-// segment, walked from its state, or a middle one, reduced to its update; item later + n is
-// sequence n if it is a single segment.
+__device__ __forceinline__ int64_t tile_of(const LinearParams& p, int segment, int head) {
+  return static_cast<int64_t>(segment) * p.num_v_heads + head;
+}
+
+// The first launch.  Item j < later reduces the segment ahead of later segment j to its update and
+// decay; item later + n walks sequence n if it is a single segment.
 template <bool Wide, bool Gated>
 __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void linear_first_kernel(const LinearParams p, const Segments g) {
@@ -625,75 +659,122 @@ void linear_first_kernel(const LinearParams p, const Segments g) {
   __shared__ SearchLds search;
   int item, head;
   if (!unit_of(p, g.later + g.num_sequences, item, head)) return;
-  int seq = item - g.later, index = 0, count = 0;
-  const bool whole = item >= g.later;
-  if (!whole && !find_segment(p, search, g.num_sequences, g.shift, item, seq, index, count)) return;
   int64_t bos;
   int rows;
-  sequence_rows(p, seq, bos, rows);
-  if (whole && rows > 0 && (rows - 1) >> g.shift != 0) return;
-  load_weight(p, lds);
-  float* const tile = whole ? nullptr : g.tiles + (static_cast<int64_t>(item) * p.num_v_heads + head) * kTileFloats;
-  if (index > 0) {
-    const double total = walk<Wide, Gated, false>(p, lds, bos + (static_cast<int64_t>(index) << g.shift),
-                                     1 << g.shift, head, nullptr, tile);
-    if (threadIdx.x == 64 * kScalarWave)
-      g.decays[static_cast<int64_t>(item) * p.num_v_heads + head] =
-          __builtin_amdgcn_exp2f(static_cast<float>(total));
+  if (item < g.later) {
+    int seq, index, count;
+    if (!find_segment(p, search, g.num_sequences, g.shift, item, seq, index, count)) return;
+    sequence_rows(p, seq, bos, rows);
+    const int64_t at = tile_of(p, item, head);
+    const double total = walk<Wide, Gated, false, kPolPlain, kPolPlain>(
+        p, lds, bos + (static_cast<int64_t>(index) << g.shift), 1 << g.shift, head, nullptr,
+        g.tiles + at * kTileFloats);
+    if (threadIdx.x == 64 * kScalarWave) g.decays[at] = __builtin_amdgcn_exp2f(static_cast<float>(total));
     return;
   }
+  const int seq = item - g.later;
+  sequence_rows(p, seq, bos, rows);
+  if (rows > 0 && (rows - 1) >> g.shift != 0) return;
+  load_weight(p, lds);
   const int slot = p.indices[seq];
   const bool live = live_slot(slot, p.num_slots);
   float* const home = p.state + static_cast<int64_t>(live ? slot : 0) * p.state_slot + head * kTileFloats;
-  walk<Wide, Gated, true>(p, lds, bos, whole ? rows : 1 << g.shift, head,
-             live && p.has_initial[seq] != 0 ? home : nullptr, whole ? (live ? home : nullptr) : tile);
+  walk<Wide, Gated, true, kPolNTSys, kPolNTSys>(
+      p, lds, bos, rows, head, live && p.has_initial[seq] != 0 ? home : nullptr, live ? home : nullptr);
 }
 
-// The second: the state at every later segment's start, along each sequence; a sixteenth of a
-// tile a workgroup.
+// The second: the state at every later segment's start, along each sequence, and the sequence's own
+// start set aside.  A workgroup takes a sixteenth of one head's tile through every sequence.
 constexpr int kJoinParts = kTileFloats / 4 / kBlock;
 __global__ __launch_bounds__(kBlock) void linear_join_kernel(const LinearParams p, const Segments g) {
-  __shared__ SearchLds search;
+  __shared__ int longer[kBlock], counts[kBlock], bases[kBlock];   // the sequences of several segments
+  __shared__ int sums[2][kBlockWaves];
+  const int tid = threadIdx.x;
   const int part = blockIdx.x % kJoinParts;
-  const int pair = blockIdx.x / kJoinParts;
-  const int j = pair / p.num_v_heads;
-  const int head = pair - j * p.num_v_heads;
-  int seq, index, count;
-  if (!find_segment(p, search, g.num_sequences, g.shift, j, seq, index, count) || index != 0) return;
-  count = min(count, g.later - j);
+  const int head = blockIdx.x / kJoinParts;
+  const int64_t at = (part * kBlock + tid) * 4;
   const int64_t step = p.num_v_heads * kTileFloats;
-  float* at = g.tiles + (static_cast<int64_t>(j) * p.num_v_heads + head) * kTileFloats +
-              (part * kBlock + threadIdx.x) * 4;
-  const float* decay = g.decays + static_cast<int64_t>(j) * p.num_v_heads + head;
-  f32x4 s = *reinterpret_cast<const f32x4*>(at);
-  for (int i = 1; i < count; ++i) {
-    at += step;
-    decay += p.num_v_heads;
-    s = s * *decay + *reinterpret_cast<const f32x4*>(at);
-    *reinterpret_cast<f32x4*>(at) = s;
+  int base = 0;
+  for (int first = 0; first < g.num_sequences; first += kBlock) {
+    // later segments of each of kBlock sequences, and of those ahead of it
+    const int n = first + tid;
+    int mine = 0;
+    if (n < g.num_sequences) {
+      int64_t bos;
+      int rows;
+      sequence_rows(p, n, bos, rows);
+      mine = rows > 0 ? (rows - 1) >> g.shift : 0;
+    }
+    int all, several;
+    const int sum = inclusive_sum(mine, sums[0], all);
+    const int place = inclusive_sum(mine > 0 ? 1 : 0, sums[1], several) - 1;
+    if (mine > 0) {
+      longer[place] = n;
+      counts[place] = mine;
+      bases[place] = base + sum - mine;
+    }
+    __syncthreads();
+    base += all;
+    for (int i = 0; i < several; ++i) {
+      const int j = __builtin_amdgcn_readfirstlane(bases[i]);
+      const int seq = __builtin_amdgcn_readfirstlane(longer[i]);
+      const int count = min(__builtin_amdgcn_readfirstlane(counts[i]), g.later - j);
+      if (count <= 0) break;
+      const int slot = p.indices[seq];
+      f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (live_slot(slot, p.num_slots) && p.has_initial[seq] != 0)
+        s = *reinterpret_cast<const f32x4*>(p.state + slot * p.state_slot + head * kTileFloats + at);
+      *reinterpret_cast<f32x4*>(g.firsts + tile_of(p, j, head) * kTileFloats + at) = s;
+      float* tile = g.tiles + tile_of(p, j, head) * kTileFloats + at;
+      const float* decay = g.decays + tile_of(p, j, head);
+      constexpr int kAhead = 8;   // updates and decays in flight
+      f32x4 update[kAhead];
+      float by[kAhead];
+      auto load = [&](int a, int k) __attribute__((always_inline)) {   // (past the last, that again)
+        const int64_t from = min(k, count - 1);
+        update[a] = *reinterpret_cast<const f32x4*>(tile + from * step);
+        by[a] = decay[from * p.num_v_heads];
+      };
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) load(a, a);
+      for (int k = 0; k < count; k += kAhead) {
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          s = s * by[a] + update[a];
+          load(a, k + a + kAhead);
+          if (k + a < count) *reinterpret_cast<f32x4*>(tile + (k + a) * step) = s;
+        }
+      }
+    }
+    __syncthreads();
   }
 }
 
-// The third: the later segments, each from its state.
+// The third: every segment of the sequences of several, each from its state.  Item j < later is
+// later segment j; item later + j the sequence's first, if j is its first later one.
 template <bool Wide, bool Gated>
 __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void linear_later_kernel(const LinearParams p, const Segments g) {
   __shared__ SegmentLds lds;
   __shared__ SearchLds search;
   int item, head, seq, index, count;
-  if (!unit_of(p, g.later, item, head) ||
-      !find_segment(p, search, g.num_sequences, g.shift, item, seq, index, count))
+  if (!unit_of(p, 2 * g.later, item, head)) return;
+  const bool is_first = item >= g.later;
+  if (is_first) item -= g.later;
+  if (!find_segment(p, search, g.num_sequences, g.shift, item, seq, index, count) ||
+      (is_first && index != 0))
     return;
   int64_t bos;
   int rows;
   sequence_rows(p, seq, bos, rows);
   load_weight(p, lds);
-  const int done = (index + 1) << g.shift;
+  const int done = is_first ? 0 : (index + 1) << g.shift;
   const int slot = p.indices[seq];
   float* const home = p.state + static_cast<int64_t>(slot) * p.state_slot + head * kTileFloats;
-  walk<Wide, Gated, true>(p, lds, bos + done, min(rows - done, 1 << g.shift), head,
-             g.tiles + (static_cast<int64_t>(item) * p.num_v_heads + head) * kTileFloats,
-             index + 1 == count && live_slot(slot, p.num_slots) ? home : nullptr);
+  walk<Wide, Gated, true, kPolPlain, kPolNTSys>(
+      p, lds, bos + done, min(rows - done, 1 << g.shift), head,
+      (is_first ? g.firsts : g.tiles) + tile_of(p, item, head) * kTileFloats,
+      !is_first && index + 1 == count && live_slot(slot, p.num_slots) ? home : nullptr);
 }
 
 // log2 of a segment's tokens: the share of a workgroup where about 512 run at once (two a CU),
@@ -713,11 +794,9 @@ template <bool Wide, bool Gated>
 void launch_segments(const LinearParams& p, const Segments& g, uint32_t first, uint32_t later,
                      hipStream_t s) {
   hipLaunchKernelGGL((linear_first_kernel<Wide, Gated>), dim3(first), dim3(kBlock), 0, s, p, g);
-  if (g.later > 1)   // (a lone later segment starts from what the first launch left)
-    hipLaunchKernelGGL(linear_join_kernel, dim3(g.later * p.num_v_heads * kJoinParts), dim3(kBlock),
-                       0, s, p, g);
-  if (g.later > 0)
-    hipLaunchKernelGGL((linear_later_kernel<Wide, Gated>), dim3(later), dim3(kBlock), 0, s, p, g);
+  if (g.later == 0) return;
+  hipLaunchKernelGGL(linear_join_kernel, dim3(p.num_v_heads * kJoinParts), dim3(kBlock), 0, s, p, g);
+  hipLaunchKernelGGL((linear_later_kernel<Wide, Gated>), dim3(later), dim3(kBlock), 0, s, p, g);
 }
 
 void launch_linear_prefill(const LinearParams& p, const Segments& g, uint32_t first, uint32_t later,
@@ -737,7 +816,7 @@ extern "C" int64_t ld_linear_prefill_workspace_bytes(int64_t num_tokens, int32_t
                                                      int32_t num_v_heads) {
   if (num_tokens < 0 || num_sequences <= 0 || num_v_heads <= 0) return 0;
   return ld::later_segments(num_tokens, num_v_heads) * num_v_heads *
-         static_cast<int64_t>((ld::kTileFloats + 4) * sizeof(float));
+         static_cast<int64_t>((2 * ld::kTileFloats + 4) * sizeof(float));
 }
 
 extern "C" int ld_linear_prefill(const ld_linear_prefill_args* args, void* stream) {
@@ -767,15 +846,16 @@ extern "C" int ld_linear_prefill(const ld_linear_prefill_args* args, void* strea
   auto blocks_of = [&](int64_t items) {
     return (items * a.num_k_heads + 7) / 8 * 8 * p.group;
   };
-  if (blocks_of(later + a.num_sequences) > 0x7fffff || later * a.num_v_heads * kJoinParts > 0x7fffff)
+  if (blocks_of(2 * later + a.num_sequences) > 0x7fffff || a.num_v_heads > 0x7fffff / kJoinParts)
     return fail(LD_ERR_INVALID_ARGUMENT, "too many (sequence, head) tiles");
   Segments g{};
   g.num_sequences = a.num_sequences;
   g.shift = segment_shift(a.num_tokens, a.num_v_heads);
   g.later = static_cast<int>(later);
   g.tiles = static_cast<float*>(a.workspace);
-  g.decays = g.tiles + later * a.num_v_heads * kTileFloats;
+  g.firsts = g.tiles + later * a.num_v_heads * kTileFloats;
+  g.decays = g.firsts + later * a.num_v_heads * kTileFloats;
   launch_linear_prefill(p, g, static_cast<uint32_t>(blocks_of(later + a.num_sequences)),
-                        static_cast<uint32_t>(blocks_of(later)), static_cast<hipStream_t>(stream));
+                        static_cast<uint32_t>(blocks_of(2 * later)), static_cast<hipStream_t>(stream));
   return check_launch("ld_linear_prefill");
 }
