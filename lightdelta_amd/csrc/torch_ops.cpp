@@ -441,7 +441,7 @@ Args linear_args(const at::Tensor& qkv, const at::Tensor& log_decay, const at::T
   args.log_decay_row_stride = log_decay.dim() == 2 ? log_decay.stride(0) : 0;
   args.state = static_cast<float*>(state.data_ptr());
   args.state_slot_stride = state.stride(0);
-  if (gate.has_value()) {
+  if (gate.has_value() && gate->size(0) > 0) {   // (without tokens its pointer is NULL)
     args.gate = gate->data_ptr();
     args.gate_row_stride = gate->stride(0);
     args.norm_weight = weight->data_ptr();

@@ -281,3 +281,42 @@ def test_c_abi_refuses_without_launching():
     refused(lib.ld_norm_rope, r, "too many heads")
     r.q_heads, r.k_heads = 0, 0
     assert lib.ld_norm_rope(ctypes.byref(r), None) == 0
+
+
+def test_c_abi_prefill_limits():
+    """A prefill's own refusals, all ahead of any launch: row strides past what a chunk's offsets
+    hold, tokens and tiles past what a grid does, and a missing, short or misaligned workspace."""
+    lib = _lib.load()
+    good = dict(qkv=16, qkv_row_stride=1024, log_decay=16, slots=16, has_initial=16, cu_seqlens=16,
+                state=16, out=16, num_tokens=4096, num_slots=4, num_sequences=1, num_k_heads=2,
+                num_v_heads=4, eps=1e-6, workspace=16, workspace_bytes=1 << 40)
+    for change, message in [
+            (dict(qkv_row_stride=2**23 + 1), "2^23 elements"),
+            (dict(qkv_row_stride=-1), "2^23 elements"),
+            (dict(log_decay_row_stride=2**23 + 1), "2^23 elements"),
+            (dict(gate=16, norm_weight=16, gate_row_stride=2**23 + 1), "2^23 elements"),
+            (dict(num_v_heads=2**16 + 2), "2^23 elements"),
+            (dict(num_tokens=2**31), "too many tokens"),
+            (dict(num_sequences=2**30), "too many (sequence, head) tiles"),
+            (dict(workspace=None), "workspace missing or too small"),
+            (dict(workspace=8), "workspace missing or too small"),
+            (dict(workspace_bytes=lib.ld_linear_prefill_workspace_bytes(4096, 1, 4) - 1),
+             "workspace missing or too small"),
+            (dict(state_slot_stride=2), "16-byte aligned")]:
+        refused(lib.ld_linear_prefill, _lib.LinearPrefillArgs(**dict(good, **change)), message)
+
+
+@pytest.mark.parametrize("tokens,heads,segment", [
+    (256, 4, 256), (257, 4, 256), (4096, 32, 256), (4096, 33, 512), (2**17, 32, 2**13),
+    (2**31 - 1, 1, 2**22)])
+def test_prefill_workspace(tokens, heads, segment):
+    """Two states and a decay for each segment of a head but the first, of at least 256 tokens,
+    doubled until about 512 workgroups hold all: 64 MiB and little more at the most."""
+    got = _lib.load().ld_linear_prefill_workspace_bytes(tokens, 3, heads)
+    assert got == (tokens - 1) // segment * heads * (2 * DIM * DIM + 4) * 4
+    assert got <= 512 * (2 * DIM * DIM + 4) * 4
+
+
+def test_prefill_workspace_of_nothing():
+    call = _lib.load().ld_linear_prefill_workspace_bytes
+    assert [call(*a) for a in [(0, 1, 4), (-1, 1, 4), (10, 0, 4), (10, 1, 0), (256, 1, 4)]] == [0] * 5
