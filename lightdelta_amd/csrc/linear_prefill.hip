@@ -28,6 +28,7 @@
 // associative: one launch reduces every segment but the last to its update and decay (and walks the
 // sequences of one segment), a second joins these along each sequence, a third walks all segments
 // from the states the second left.
+#include <algorithm>
 #include <cstddef>
 
 #include "linear_common.h"
@@ -582,10 +583,21 @@ __device__ __forceinline__ int inclusive_sum(int mine, int (&sums)[kBlockWaves],
   return sum;
 }
 
+// A sequence of `rows` rows is cut into as few segments as `most` rows a segment (a multiple of a
+// chunk's) allow, each but the last of the same whole chunks: no workgroup walks longer than the
+// sequence needs.
+__device__ __forceinline__ int later_of(int rows, int most) {
+  return rows > 0 ? static_cast<int>(static_cast<uint32_t>(rows - 1) / static_cast<uint32_t>(most)) : 0;
+}
+__device__ __forceinline__ int segment_rows(int rows, int later) {
+  const uint32_t count = static_cast<uint32_t>(later) + 1;
+  return static_cast<int>((rows + count - 1) / count + kTokens - 1) / kTokens * kTokens;
+}
+
 // Later segments (all but the first) of the sequences are numbered in order: finds the j-th, i.e.
 // its sequence, which of the sequence's later segments it is, and how many that has.  False past
 // the last.  By the whole workgroup.
-__device__ bool find_segment(const LinearParams& p, SearchLds& lds, int num_sequences, int shift,
+__device__ bool find_segment(const LinearParams& p, SearchLds& lds, int num_sequences, int most,
                              int j, int& seq, int& index, int& count) {
   const int tid = threadIdx.x;
   int base = 0;
@@ -596,7 +608,7 @@ __device__ bool find_segment(const LinearParams& p, SearchLds& lds, int num_sequ
       int64_t bos;
       int rows;
       sequence_rows(p, n, bos, rows);
-      mine = rows > 0 ? (rows - 1) >> shift : 0;
+      mine = later_of(rows, most);
     }
     int all;
     const int sum = inclusive_sum(mine, lds.wave_sums, all);
@@ -620,7 +632,7 @@ __device__ bool find_segment(const LinearParams& p, SearchLds& lds, int num_sequ
 
 struct Segments {
   int num_sequences;
-  int shift;        // log2 of a segment's tokens
+  int most;         // tokens of a segment, at most
   int later;        // at most this many later segments
   float* tiles;     // per (later segment, head): the state it starts from (before the second
                     // launch, the update of the segment ahead of it)
@@ -663,18 +675,18 @@ void linear_first_kernel(const LinearParams p, const Segments g) {
   int rows;
   if (item < g.later) {
     int seq, index, count;
-    if (!find_segment(p, search, g.num_sequences, g.shift, item, seq, index, count)) return;
+    if (!find_segment(p, search, g.num_sequences, g.most, item, seq, index, count)) return;
     sequence_rows(p, seq, bos, rows);
     const int64_t at = tile_of(p, item, head);
+    const int each = segment_rows(rows, count);
     const double total = walk<Wide, Gated, false, kPolPlain, kPolPlain>(
-        p, lds, bos + (static_cast<int64_t>(index) << g.shift), 1 << g.shift, head, nullptr,
-        g.tiles + at * kTileFloats);
+        p, lds, bos + index * each, each, head, nullptr, g.tiles + at * kTileFloats);
     if (threadIdx.x == 64 * kScalarWave) g.decays[at] = __builtin_amdgcn_exp2f(static_cast<float>(total));
     return;
   }
   const int seq = item - g.later;
   sequence_rows(p, seq, bos, rows);
-  if (rows > 0 && (rows - 1) >> g.shift != 0) return;
+  if (later_of(rows, g.most) != 0) return;
   load_weight(p, lds);
   const int slot = p.indices[seq];
   const bool live = live_slot(slot, p.num_slots);
@@ -703,7 +715,7 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const LinearParams 
       int64_t bos;
       int rows;
       sequence_rows(p, n, bos, rows);
-      mine = rows > 0 ? (rows - 1) >> g.shift : 0;
+      mine = later_of(rows, g.most);
     }
     int all, several;
     const int sum = inclusive_sum(mine, sums[0], all);
@@ -761,33 +773,36 @@ void linear_later_kernel(const LinearParams p, const Segments g) {
   if (!unit_of(p, 2 * g.later, item, head)) return;
   const bool is_first = item >= g.later;
   if (is_first) item -= g.later;
-  if (!find_segment(p, search, g.num_sequences, g.shift, item, seq, index, count) ||
+  if (!find_segment(p, search, g.num_sequences, g.most, item, seq, index, count) ||
       (is_first && index != 0))
     return;
   int64_t bos;
   int rows;
   sequence_rows(p, seq, bos, rows);
   load_weight(p, lds);
-  const int done = is_first ? 0 : (index + 1) << g.shift;
+  const int each = segment_rows(rows, count);
+  const int done = is_first ? 0 : (index + 1) * each;
   const int slot = p.indices[seq];
   float* const home = p.state + static_cast<int64_t>(slot) * p.state_slot + head * kTileFloats;
   walk<Wide, Gated, true, kPolPlain, kPolNTSys>(
-      p, lds, bos + done, min(rows - done, 1 << g.shift), head,
+      p, lds, bos + done, min(rows - done, each), head,
       (is_first ? g.firsts : g.tiles) + tile_of(p, item, head) * kTileFloats,
       !is_first && index + 1 == count && live_slot(slot, p.num_slots) ? home : nullptr);
 }
 
-// log2 of a segment's tokens: the share of a workgroup where about 512 run at once (two a CU),
-// at least 256.
-int segment_shift(int64_t num_tokens, int32_t num_v_heads) {
-  int shift = 8;
-  while (shift < 30 && (int64_t{512} << shift) < num_tokens * num_v_heads) ++shift;
-  return shift;
+// A segment's tokens, at most: the share of a workgroup where 512 run at once (two a CU), in whole
+// chunks and at least 4 of them, as a segment is walked twice.  Rounded to a power of two the share
+// left CUs idle behind one long prompt (32 heads, us: 5000 tokens 117 / 97, 9000 180 / 149, 20000
+// 368 / 300) and gained and lost by turns on mixed ones; 1.14 or 1.33 shares likewise.
+int64_t segment_tokens(int64_t num_tokens, int32_t num_v_heads) {
+  constexpr int64_t kAtOnce = 512;
+  const int64_t share = (num_tokens * num_v_heads + kAtOnce - 1) / kAtOnce;
+  return std::clamp<int64_t>((share + kTokens - 1) / kTokens * kTokens, 4 * kTokens, 1 << 30);
 }
 
 // Sequences of more than a segment have at most this many later ones.
 int64_t later_segments(int64_t num_tokens, int32_t num_v_heads) {
-  return num_tokens > 0 ? (num_tokens - 1) >> segment_shift(num_tokens, num_v_heads) : 0;
+  return num_tokens > 0 ? (num_tokens - 1) / segment_tokens(num_tokens, num_v_heads) : 0;
 }
 
 template <bool Wide, bool Gated>
@@ -850,7 +865,7 @@ extern "C" int ld_linear_prefill(const ld_linear_prefill_args* args, void* strea
     return fail(LD_ERR_INVALID_ARGUMENT, "too many (sequence, head) tiles");
   Segments g{};
   g.num_sequences = a.num_sequences;
-  g.shift = segment_shift(a.num_tokens, a.num_v_heads);
+  g.most = static_cast<int>(segment_tokens(a.num_tokens, a.num_v_heads));
   g.later = static_cast<int>(later);
   g.tiles = static_cast<float*>(a.workspace);
   g.firsts = g.tiles + later * a.num_v_heads * kTileFloats;

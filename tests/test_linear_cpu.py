@@ -307,11 +307,12 @@ def test_c_abi_prefill_limits():
 
 
 @pytest.mark.parametrize("tokens,heads,segment", [
-    (256, 4, 256), (257, 4, 256), (4096, 32, 256), (4096, 33, 512), (2**17, 32, 2**13),
-    (2**31 - 1, 1, 2**22)])
+    (256, 4, 256), (257, 4, 256), (4096, 32, 256), (4097, 32, 320), (5000, 32, 320),
+    (2**17, 32, 2**13), (10**6, 48, 93760), (2**31 - 1, 1, 2**22)])
 def test_prefill_workspace(tokens, heads, segment):
-    """Two states and a decay for each segment of a head but the first, of at least 256 tokens,
-    doubled until about 512 workgroups hold all: 64 MiB and little more at the most."""
+    """Two states and a decay for each segment of a head but the first: a segment has a 512th of all
+    heads' tokens in whole chunks of 64, at least 256, so that it is 64 MiB and little more at the
+    most."""
     got = _lib.load().ld_linear_prefill_workspace_bytes(tokens, 3, heads)
     assert got == (tokens - 1) // segment * heads * (2 * DIM * DIM + 4) * 4
     assert got <= 512 * (2 * DIM * DIM + 4) * 4

@@ -284,3 +284,16 @@ def test_far_rows(gpu):
     rope = rope_case(tokens, 1, 1, 64, seed=6, device=gpu)
     rope["qkv"] = far
     check_rope(rope, False)
+
+
+# ---- segments ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("lengths,heads", [([513], (1, 1)), ([767, 768, 769], (1, 2)),
+                                           ([1023, 256, 1025, 257], (1, 1)), ([9000], (2, 8)),
+                                           ([2300, 700, 2], (4, 16))])
+def test_prefill_segments(gpu, lengths, heads):
+    """Sequences cut into segments of equal whole chunks: a token to either side of a further
+    segment, and more heads than leave a segment at its least."""
+    announce(test="linear_prefill_segments", lengths=lengths, heads=heads)
+    check_prefill(prefill_case(lengths, *heads, seed=11, device=gpu, decay=0.05))
