@@ -25,9 +25,9 @@
 // 2^-9 of the output's own rounding).
 //
 // A sequence longer than a segment is cut into segments, since the recurrence over them is
-// associative: one launch reduces every segment but the last to its update and decay (and walks the
-// sequences of one segment), a second joins these along each sequence, a third walks all segments
-// from the states the second left.
+// associative: one launch reduces every segment but a sequence's last to its update and decay, a
+// second joins these along each sequence, a third walks all segments from the states the second
+// left, and the sequences of one segment.
 #include <algorithm>
 #include <cstddef>
 
@@ -146,19 +146,205 @@ __device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) {
 
 constexpr int kScalarWave = 3;   // makes the chunks' scalars: the wave without a block of P
 
+// The state in a wave's accumulators, st[T][8 u + 4 h + r] = S[32 w + lj][32 T + 16 u + 8 hi + 4 h + r],
+// to and from memory by way of LDS, so that memory is read and written in whole lines: row v's
+// 16-byte pieces are XORed with v % 16.
+struct StateTile {
+  uint8_t* tile;
+  uint32_t at;
+  __device__ __forceinline__ explicit StateTile(SegmentLds& lds) : tile(lds.k) {
+    const int tid = threadIdx.x, lj = tid & 31, hi = (tid >> 5) & 1;
+    at = (32 * (tid >> 6) + lj) * (kDim * 4) + (((2 * hi) ^ (lj & 15)) << 4);
+  }
+  __device__ __forceinline__ f32x4* piece(int T, int q) const {   // of st[T][4 q ..]
+    return reinterpret_cast<f32x4*>(tile + (at ^ ((8 * T + 4 * (q >> 1) + (q & 1)) << 4)));
+  }
+  __device__ __forceinline__ f32x4* line(int i) const {           // the thread's 16 bytes of line i
+    const int tid = threadIdx.x, v = 8 * i + (tid >> 5);
+    return reinterpret_cast<f32x4*>(tile + v * (kDim * 4) + (((tid & 31) ^ (v & 15)) << 4));
+  }
+  template <int Pol>
+  __device__ __forceinline__ void load(const float* from, f32x16 (&st)[4]) const {
+    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(from, kTileBytes);
+    f32x4 lines[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) lines[i] = buffer_load16<Pol>(rs, threadIdx.x * 16 + 4096 * i);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) *line(i) = lines[i];
+    lds_barrier();
+#pragma unroll
+    for (int T = 0; T < 4; ++T)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 x = *piece(T, q);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[T][4 * q + r] = x[r];
+      }
+    lds_barrier();
+  }
+  template <int Pol>
+  __device__ __forceinline__ void store(float* to, const f32x16 (&st)[4]) const {
+    lds_barrier();   // (the last chunk's reads of LDS)
+#pragma unroll
+    for (int T = 0; T < 4; ++T)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) *piece(T, q) = quad(st[T], q);
+    lds_barrier();
+    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(to, kTileBytes);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) buffer_store16<Pol>(*line(i), rs, threadIdx.x * 16 + 4096 * i);
+  }
+};
+
+// Transposed operands of a lane, as byte offsets: k's rows 16 u + 8 h + .. in the state's order of
+// columns (^ (T << 6) ^ (h << 5)), v's in the wave's columns (^ (h << 5)).
+__device__ __forceinline__ uint32_t k_offset(int lane) {
+  const int m = lane & 15, c16 = (lane >> 4) & 1, hi = lane >> 5;
+  return (4 * hi + (m >> 2)) * kTileRow + (((2 * c16 + (m & 1)) ^ ((m >> 2) << 2) ^ hi) << 4) +
+         ((m >> 1) & 1) * 8;
+}
+__device__ __forceinline__ uint32_t v_offset(int lane, int w) {
+  const int m = lane & 15, c16 = (lane >> 4) & 1, hi = lane >> 5;
+  return (4 * hi + (m >> 2)) * kTileRow +
+         (((4 * w + 2 * c16 + ((m & 3) >> 1)) ^ ((m >> 2) << 2) ^ hi) << 4) + (m & 1) * 8;
+}
+__device__ __forceinline__ bf16x8 v_operand(const uint8_t* v, uint32_t at, int u) {
+  return join(read_tr(v + at + 16 * u * kTileRow), read_tr(v + (at ^ (1 << 5)) + (16 * u + 8) * kTileRow));
+}
+__device__ __forceinline__ bf16x8 k_operand(const uint8_t* k, uint32_t at, int u, int T) {
+  return join(read_tr(k + (at ^ (T << 6)) + 16 * u * kTileRow),
+              read_tr(k + (at ^ (T << 6) ^ (1 << 5)) + (16 * u + 8) * kTileRow));
+}
+// e V of 32 tokens (from token `first`) in accumulator order.
+__device__ __forceinline__ f32x16 decayed(const bf16x8 (&v)[2], const float* ek, int first, int hi) {
+  f32x16 x;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const f32x4 e = *reinterpret_cast<const f32x4*>(ek + first + 8 * q + 4 * hi);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[4 * q + r] = static_cast<float>(v[q >> 1][4 * (q & 1) + r]) * e[r];
+  }
+  return x;
+}
+
+// A segment of `rows` rows (whole chunks) from row `bos`, reduced to its update, the state after it
+// from zeros, at `end`; returns, on wave kScalarWave, the sum of log decays in units of log 2.
+// Rows of k and v go to one half of the tile's LDS while the other is worked on: one barrier a
+// chunk.
+template <bool Wide>
+__device__ __forceinline__ double reduce(const LinearParams& p, SegmentLds& lds, int64_t bos, int rows,
+                                         int head, float* end) {
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hi = lane >> 5;
+  const int key_head = head / p.group;
+  const int chunks = rows / kTokens;
+  u32x4 next_k[4], next_v[4];
+  const int srow = tid >> 4;
+  const int spiece = tid & 15;
+  const uint32_t row_bytes = static_cast<uint32_t>(p.qkv_row) * 2;
+  const uint32_t lane_row = srow * row_bytes + spiece * 16;
+  const int k_col = (p.num_k_heads + key_head) * kTileRow;
+  const int v_col = (2 * p.num_k_heads + head) * kTileRow;
+  const uint32_t width = (2 * p.num_k_heads + p.num_v_heads) * kTileRow;
+  auto fetch = [&](int c) __attribute__((always_inline)) {   // (past the end zeros)
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint16_t*>(p.qkv + (bos + static_cast<int64_t>(c) * kTokens) * p.qkv_row), 0,
+        c < chunks ? (kTokens - 1) * row_bytes + width : 0, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      next_k[i] = load_piece<Wide>(rs, lane_row + 16 * i * row_bytes, k_col);
+      next_v[i] = load_piece<Wide>(rs, lane_row + 16 * i * row_bytes, v_col);
+    }
+  };
+  const uint32_t dst = srow * kTileRow + ((spiece ^ swizzle(srow)) << 4);
+  auto put = [&](int c) __attribute__((always_inline)) {
+    uint8_t* const at = lds.k + (c & 1) * 2 * kRowsBytes + dst;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      *reinterpret_cast<u32x4*>(at + 16 * i * kTileRow) = next_k[i];
+      *reinterpret_cast<u32x4*>(at + kRowsBytes + 16 * i * kTileRow) = next_v[i];
+    }
+  };
+  auto load_decay = [&](int c) __attribute__((always_inline)) {
+    const uint32_t step = static_cast<uint32_t>(p.decay_row) * 4;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<float*>(p.log_decay + (bos + static_cast<int64_t>(c) * kTokens) * p.decay_row + head),
+        0, c < chunks ? (kTokens - 1) * step + 4 : 0, 0x00020000);
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, lane * step, 0, 0));
+  };
+  const uint32_t kt_at = k_offset(lane);
+  const uint32_t vt_at = v_offset(lane, w);
+  const Remainder less(lane);
+  f32x16 st[4] = {};
+  double total = 0.0;
+  float next_g = load_decay(0);
+  fetch(0);
+  if (w == kScalarWave) total += chunk_scalars(lds.scalars[0], next_g, p.scale, lane);
+  next_g = load_decay(1);
+  put(0);
+  fetch(1);
+  for (int c = 0; c < chunks; ++c) {
+    const ChunkScalars& s = lds.scalars[c & 1];
+    const uint8_t* const k_rows = lds.k + (c & 1) * 2 * kRowsBytes;
+    const uint8_t* const v_rows = k_rows + kRowsBytes;
+    lds_barrier();   // the chunk's rows and scalars are in LDS, the last's read
+    const float gamma = s.gamma;
+#pragma unroll
+    for (int T = 0; T < 4; ++T) st[T] *= gamma;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bf16x8 v[2] = {v_operand(v_rows, vt_at, 2 * i), v_operand(v_rows, vt_at, 2 * i + 1)};
+      f32x16 x = decayed(v, s.ek, 32 * i, hi);
+      bf16x8 planes[3][2];
+#pragma unroll
+      for (int n = 0; n < 3; ++n) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) planes[n][u] = plane_of(x, u);
+        if (n < 2) x = less(x, planes[n][0], planes[n][1]);
+      }
+      bf16x8 k = k_operand(k_rows, kt_at, 2 * i, 0);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int T = 0; T < 4; ++T) {
+          bf16x8 next = k;
+          if (T < 3)
+            next = k_operand(k_rows, kt_at, 2 * i + u, T + 1);
+          else if (u == 0)
+            next = k_operand(k_rows, kt_at, 2 * i + 1, 0);
+          in_order();
+#pragma unroll
+          for (int plane = 2; plane >= 0; --plane) st[T] = mfma32(k, planes[plane][u], st[T]);
+          in_order();
+          k = next;
+        }
+      if (i == 0) {
+        put(c + 1);
+        fetch(c + 2);
+        if (w == kScalarWave)
+          total += chunk_scalars(lds.scalars[(c + 1) & 1], next_g, p.scale, lane);
+        next_g = load_decay(c + 2);
+      }
+    }
+  }
+  StateTile(lds).store<kPolPlain>(end, st);
+  return total;
+}
+
 // One workgroup's walk over `rows` rows from row `bos`: from the state at `start` (zeros if
-// null), writing outputs if Out, and the state after the last row to `end` (unless null).  Without
-// Out the state is the segment's update; either way returns, on wave kScalarWave, the sum of log
-// decays in units of log 2.
+// null), writing outputs, and the state after the last row to `end` (unless null).
 //
 // Global memory is reached by buffer loads and stores without branches (past the end a resource
 // over 0 bytes or an offset past it: zeros and dropped stores): under a branch the compiler would
 // have to wait for every load in flight before it uses any.  Wide: every address is a multiple of
 // 4 bytes; else elements move one by one.
-// StartPol, EndPol: cache policy bits of the state's loads and stores.
-template <bool Wide, bool Gated, bool Out, int StartPol, int EndPol>
-__device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, int64_t bos, int rows,
-                                       int head, const float* start, float* end) {
+// The pool (`end`, and `start` if pooled) is passed by, the workspace read as the second launch
+// left it in the caches.
+template <bool Wide, bool Gated>
+__device__ __forceinline__ void walk(const LinearParams& p, SegmentLds& lds, int64_t bos, int rows,
+                                     int head, const float* start, bool pooled, float* end) {
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -199,7 +385,7 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
       staged.v[j] = load_piece<Wide>(rs, at, v_col);
     else if ((i & 1) == 0)
       staged.k[j] = load_piece<Wide>(rs, at, k_col);
-    else if constexpr (Out)
+    else
       staged.q[j] = load_piece<Wide>(rs, at, q_col);
   };
   const uint32_t dst = srow * kTileRow + ((spiece ^ swizzle(srow)) << 4);
@@ -224,51 +410,21 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
   }
   float next_g = load_decay(0);
 
-  // st[T][8 u + 4 h + r] = S[32 w + lj][32 T + 16 u + 8 hi + 4 h + r], by way of LDS, so that memory
-  // is read (and at the end written) in whole lines: row v's 16-byte pieces XORed with v % 16
   f32x16 st[4] = {};
-  uint8_t* const tile = lds.k;
-  const uint32_t tile_at = (32 * w + lj) * (kDim * 4) + (((2 * hi) ^ (lj & 15)) << 4);
-  auto tile_piece = [&](int T, int q) __attribute__((always_inline)) {   // of st[T][4 q ..]
-    return reinterpret_cast<f32x4*>(tile + (tile_at ^ ((8 * T + 4 * (q >> 1) + (q & 1)) << 4)));
-  };
-  const uint32_t line_at = tid * 16;                                     // + 4096 i
-  auto line_piece = [&](int i) __attribute__((always_inline)) {
-    const int v = 8 * i + (tid >> 5);
-    return reinterpret_cast<f32x4*>(tile + v * (kDim * 4) + (((tid & 31) ^ (v & 15)) << 4));
-  };
+  const StateTile tile(lds);
   if (start != nullptr) {
-    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(start, kTileBytes);
-    f32x4 lines[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) lines[i] = buffer_load16<StartPol>(rs, line_at + 4096 * i);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) *line_piece(i) = lines[i];
-    lds_barrier();
-#pragma unroll
-    for (int T = 0; T < 4; ++T)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x4 x = *tile_piece(T, q);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) st[T][4 * q + r] = x[r];
-      }
-    lds_barrier();
+    if (pooled)
+      tile.load<kPolNTSys>(start, st);
+    else
+      tile.load<kPolPlain>(start, st);
   }
-  double total = 0.0;
-  if (w == kScalarWave) total += chunk_scalars(lds.scalars[0], next_g, p.scale, lane);
+  if (w == kScalarWave) chunk_scalars(lds.scalars[0], next_g, p.scale, lane);
   next_g = load_decay(1);
 
   // lane addresses of the operands (the parts of the swizzle that depend on the step are XORed in)
   uint32_t a_at = lj * kTileRow + ((hi ^ swizzle(lj)) << 4);       // ^ (step << 5)
-  const int m = lane & 15;
-  const int c16 = (lane >> 4) & 1;
-  const uint32_t tr_row = (4 * hi + (m >> 2)) * kTileRow;
-  // transposed k: rows 16 u + 8 h + .., columns in the state's order   ^ (T << 6) ^ (h << 5)
-  uint32_t kt_at = tr_row + (((2 * c16 + (m & 1)) ^ ((m >> 2) << 2) ^ hi) << 4) + ((m >> 1) & 1) * 8;
-  // transposed v: rows 16 u + 8 h + .., the wave's columns   ^ (h << 5)
-  const uint32_t vt_at =
-      tr_row + (((4 * w + 2 * c16 + ((m & 3) >> 1)) ^ ((m >> 2) << 2) ^ hi) << 4) + (m & 1) * 8;
+  uint32_t kt_at = k_offset(lane);
+  const uint32_t vt_at = v_offset(lane, w);
   // P[t][s] of a plane: the quad of s at 16 u + 8 a + 4 hi is half a of row t's 16-byte piece
   // 2 u + hi; the pieces of a row are XORed with t / 2 % 4 (rows of 32 columns) or t % 8
   uint32_t p_upper = lj * 64 + ((hi ^ ((lj >> 1) & 3)) << 4);                // ^ (u << 5)
@@ -349,10 +505,7 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
 
   const Remainder less(lane);
   put(lds.k, staged.k);
-  if constexpr (Out)
-    put(lds.q, staged.q);
-  else
-    put(lds.v, staged.v);
+  put(lds.q, staged.q);
   for (int c = 0; c < chunks; ++c) {
     const ChunkScalars& s = lds.scalars[c & 1];
     // (opaque here, so that their XORed forms are made where they are used, not held in registers
@@ -362,118 +515,96 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
     pin(p_upper);
     pin(p_lower);
     pin(o_put);
-    lds_barrier();   // k, q (without Out: v) and scalars of the chunk are in LDS, O of the last
+    lds_barrier();   // k, q and scalars of the chunk are in LDS, O of the last
     f32x16 o[2];
     const __amdgpu_buffer_rsrc_t next_rows = source(c + 1);
-    if constexpr (Out) {
-      if constexpr (Gated) load_gate(c - 1);
-      // ---- P ----
-      if (w != kScalarWave) {
-        f32x16 x = {};
+    if constexpr (Gated) load_gate(c - 1);
+    // ---- P ----
+    if (w != kScalarWave) {
+      f32x16 x = {};
 #pragma unroll
-        for (int step = 0; step < 8; ++step)
-          x = mfma32(*reinterpret_cast<const bf16x8*>(lds.k + 32 * p_columns * kTileRow + (a_at ^ (step << 5))),
-                     *reinterpret_cast<const bf16x8*>(lds.q + 32 * p_rows * kTileRow + (a_at ^ (step << 5))),
-                     x);
-        const float thi = s.hi[32 * p_rows + lj], tlo = s.lo[32 * p_rows + lj];
+      for (int step = 0; step < 8; ++step)
+        x = mfma32(*reinterpret_cast<const bf16x8*>(lds.k + 32 * p_columns * kTileRow + (a_at ^ (step << 5))),
+                   *reinterpret_cast<const bf16x8*>(lds.q + 32 * p_rows * kTileRow + (a_at ^ (step << 5))),
+                   x);
+      const float thi = s.hi[32 * p_rows + lj], tlo = s.lo[32 * p_rows + lj];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int first = 8 * q + 4 * hi;
-          const f32x4 shi = *reinterpret_cast<const f32x4*>(&s.hi[32 * p_columns + first]);
-          const f32x4 slo = *reinterpret_cast<const f32x4*>(&s.lo[32 * p_columns + first]);
+      for (int q = 0; q < 4; ++q) {
+        const int first = 8 * q + 4 * hi;
+        const f32x4 shi = *reinterpret_cast<const f32x4*>(&s.hi[32 * p_columns + first]);
+        const f32x4 slo = *reinterpret_cast<const f32x4*>(&s.lo[32 * p_columns + first]);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float d = __builtin_amdgcn_exp2f((thi - shi[r]) + (tlo - slo[r])) * p.scale;
-            x[4 * q + r] = p_rows != p_columns || first + r <= lj ? x[4 * q + r] * d : 0.0f;
-          }
+        for (int r = 0; r < 4; ++r) {
+          const float d = __builtin_amdgcn_exp2f((thi - shi[r]) + (tlo - slo[r])) * p.scale;
+          x[4 * q + r] = p_rows != p_columns || first + r <= lj ? x[4 * q + r] * d : 0.0f;
         }
-        auto put_plane = [&](int plane, const bf16x8 (&half)[2]) __attribute__((always_inline)) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            *reinterpret_cast<bf16x8*>(lds.p[plane] + ((p_rows == 0 ? p_upper : p_lower) ^
-                                                       ((2 * p_columns + u) << 5))) = half[u];
-        };
-        const bf16x8 high[2] = {plane_of(x, 0), plane_of(x, 1)};
-        put_plane(0, high);
-        x = less(x, high[0], high[1]);
-        const bf16x8 low[2] = {plane_of(x, 0), plane_of(x, 1)};
-        put_plane(1, low);
       }
-      // ---- O^T = S Q^T: 32 keys at a time, S as two planes; an operand is read again once both
-      // of its products are out ----
-      bf16x8 q[2][2];
-      auto read_q = [&](int T, int u) __attribute__((always_inline)) {
+      auto put_plane = [&](int plane, const bf16x8 (&half)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          *reinterpret_cast<bf16x8*>(lds.p[plane] + ((p_rows == 0 ? p_upper : p_lower) ^
+                                                     ((2 * p_columns + u) << 5))) = half[u];
+      };
+      const bf16x8 high[2] = {plane_of(x, 0), plane_of(x, 1)};
+      put_plane(0, high);
+      x = less(x, high[0], high[1]);
+      const bf16x8 low[2] = {plane_of(x, 0), plane_of(x, 1)};
+      put_plane(1, low);
+    }
+    // ---- O^T = S Q^T: 32 keys at a time, S as two planes; an operand is read again once both
+    // of its products are out ----
+    bf16x8 q[2][2];
+    auto read_q = [&](int T, int u) __attribute__((always_inline)) {
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+        q[u][tt] = *reinterpret_cast<const bf16x8*>(lds.q + 32 * tt * kTileRow +
+                                                    (a_at ^ ((2 * T + u) << 5)));
+    };
+#pragma unroll
+    for (int u = 0; u < 2; ++u) read_q(0, u);
+#pragma unroll
+    for (int T = 0; T < 4; ++T) {
+      const bf16x8 high[2] = {plane_of(st[T], 0), plane_of(st[T], 1)};
+      const f32x16 rest = less(st[T], high[0], high[1]);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        fetch(next_rows, c + 1, 2 * T + u);
+        in_order();
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
-          q[u][tt] = *reinterpret_cast<const bf16x8*>(lds.q + 32 * tt * kTileRow +
-                                                      (a_at ^ ((2 * T + u) << 5)));
-      };
-#pragma unroll
-      for (int u = 0; u < 2; ++u) read_q(0, u);
-#pragma unroll
-      for (int T = 0; T < 4; ++T) {
-        const bf16x8 high[2] = {plane_of(st[T], 0), plane_of(st[T], 1)};
-        const f32x16 rest = less(st[T], high[0], high[1]);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          fetch(next_rows, c + 1, 2 * T + u);
-          in_order();
-#pragma unroll
-          for (int tt = 0; tt < 2; ++tt)
-            o[tt] = mfma32(high[u], q[u][tt], T == 0 && u == 0 ? f32x16{} : o[tt]);
-          in_order();
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const bf16x8 low = plane_of(rest, u);
-#pragma unroll
-          for (int tt = 0; tt < 2; ++tt) o[tt] = mfma32(low, q[u][tt], o[tt]);
-          in_order();
-          if (T < 3) read_q(T + 1, u);
-          in_order();
-        }
+          o[tt] = mfma32(high[u], q[u][tt], T == 0 && u == 0 ? f32x16{} : o[tt]);
+        in_order();
       }
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt) o[tt] *= s.eq[32 * tt + lj];
-      finish(c - 1);
-      lds_barrier();   // O of the last chunk is read
-      put(lds.v, staged.v);
-    }
-    const float gamma = s.gamma;
-    if constexpr (!Out) {
+      for (int u = 0; u < 2; ++u) {
+        const bf16x8 low = plane_of(rest, u);
 #pragma unroll
-      for (int i = 0; i < 12; ++i) fetch(next_rows, c + 1, i);
+        for (int tt = 0; tt < 2; ++tt) o[tt] = mfma32(low, q[u][tt], o[tt]);
+        in_order();
+        if (T < 3) read_q(T + 1, u);
+        in_order();
+      }
     }
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt) o[tt] *= s.eq[32 * tt + lj];
+    finish(c - 1);
+    lds_barrier();   // O of the last chunk is read
+    put(lds.v, staged.v);
+    const float gamma = s.gamma;
 #pragma unroll
     for (int T = 0; T < 4; ++T) st[T] *= gamma;
-    if (w == kScalarWave)
-      total += chunk_scalars(lds.scalars[(c + 1) & 1], next_g, p.scale, lane);
+    if (w == kScalarWave) chunk_scalars(lds.scalars[(c + 1) & 1], next_g, p.scale, lane);
     next_g = load_decay(c + 2);
-    if constexpr (Out) lds_barrier();   // v is in LDS (and P)
+    lds_barrier();   // v is in LDS (and P)
 
-    auto v_operand = [&](int u) __attribute__((always_inline)) {
-      return join(read_tr(lds.v + vt_at + 16 * u * kTileRow),
-                  read_tr(lds.v + (vt_at ^ (1 << 5)) + (16 * u + 8) * kTileRow));
-    };
-    auto k_operand = [&](int u, int T) __attribute__((always_inline)) {
-      return join(read_tr(lds.k + (kt_at ^ (T << 6)) + 16 * u * kTileRow),
-                  read_tr(lds.k + (kt_at ^ (T << 6) ^ (1 << 5)) + (16 * u + 8) * kTileRow));
-    };
     auto p_operand = [&](int u, int tt, int plane) __attribute__((always_inline)) {
       return *reinterpret_cast<const bf16x8*>(lds.p[plane] + ((tt == 0 ? p_upper : p_lower) ^ (u << 5)));
     };
     // ---- O^T += V^T P^T and S += K^T (e V): 32 tokens at a time, operands read a product ahead ----
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const bf16x8 v[2] = {v_operand(2 * i), v_operand(2 * i + 1)};
-      f32x16 x;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x4 ek = *reinterpret_cast<const f32x4*>(&s.ek[32 * i + 8 * q + 4 * hi]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          x[4 * q + r] = static_cast<float>(v[q >> 1][4 * (q & 1) + r]) * ek[r];
-      }
+      const bf16x8 v[2] = {v_operand(lds.v, vt_at, 2 * i), v_operand(lds.v, vt_at, 2 * i + 1)};
+      f32x16 x = decayed(v, s.ek, 32 * i, hi);
       bf16x8 planes[3][2];
       auto set_planes = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
@@ -481,18 +612,16 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
       };
       // O's products, between the steps of the split
       auto outputs = [&](int u) __attribute__((always_inline)) {
-        if constexpr (Out) {
-          bf16x8 ps[2][2];
+        bf16x8 ps[2][2];
 #pragma unroll
-          for (int tt = i; tt < 2; ++tt)
+        for (int tt = i; tt < 2; ++tt)
 #pragma unroll
-            for (int plane = 0; plane < 2; ++plane) ps[tt][plane] = p_operand(2 * i + u, tt, plane);
-          in_order();
+          for (int plane = 0; plane < 2; ++plane) ps[tt][plane] = p_operand(2 * i + u, tt, plane);
+        in_order();
 #pragma unroll
-          for (int plane = 1; plane >= 0; --plane)
+        for (int plane = 1; plane >= 0; --plane)
 #pragma unroll
-            for (int tt = i; tt < 2; ++tt) o[tt] = mfma32(v[u], ps[tt][plane], o[tt]);
-        }
+          for (int tt = i; tt < 2; ++tt) o[tt] = mfma32(v[u], ps[tt][plane], o[tt]);
       };
       set_planes(0);
       x = less(x, planes[0][0], planes[0][1]);
@@ -501,17 +630,17 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
       x = less(x, planes[1][0], planes[1][1]);
       outputs(1);
       set_planes(2);
-      bf16x8 k = k_operand(2 * i, 0);
+      bf16x8 k = k_operand(lds.k, kt_at, 2 * i, 0);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        if constexpr (Out) fetch(next_rows, c + 1, 8 + 2 * i + u);
+        fetch(next_rows, c + 1, 8 + 2 * i + u);
 #pragma unroll
         for (int T = 0; T < 4; ++T) {
           bf16x8 next_k = k;
           if (T < 3)
-            next_k = k_operand(2 * i + u, T + 1);
+            next_k = k_operand(lds.k, kt_at, 2 * i + u, T + 1);
           else if (u == 0)
-            next_k = k_operand(2 * i + 1, 0);
+            next_k = k_operand(lds.k, kt_at, 2 * i + 1, 0);
           in_order();
 #pragma unroll
           for (int plane = 2; plane >= 0; --plane) st[T] = mfma32(k, planes[plane][u], st[T]);
@@ -521,39 +650,21 @@ __device__ __forceinline__ double walk(const LinearParams& p, SegmentLds& lds, i
       }
     }
     lds_barrier();   // every read of the chunk's rows and P is done
-    if constexpr (Out) {
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
+    for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<f32x4*>(o_rows + (o_put ^ (8 * q)) + 32 * tt * kDim) =
-              f32x4{o[tt][4 * q], o[tt][4 * q + 1], o[tt][4 * q + 2], o[tt][4 * q + 3]};
-    }
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(o_rows + (o_put ^ (8 * q)) + 32 * tt * kDim) = quad(o[tt], q);
     put(lds.k, staged.k);
-    if constexpr (Out)
-      put(lds.q, staged.q);
-    else
-      put(lds.v, staged.v);
+    put(lds.q, staged.q);
   }
-  if (Out && chunks > 0) {
+  if (chunks > 0) {
     if constexpr (Gated) load_gate(chunks - 1);
     lds_barrier();
     finish(chunks - 1);
   }
 
-  if (end != nullptr) {
-    lds_barrier();   // (the last chunk's reads of LDS)
-#pragma unroll
-    for (int T = 0; T < 4; ++T)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *tile_piece(T, q) = f32x4{st[T][4 * q], st[T][4 * q + 1], st[T][4 * q + 2], st[T][4 * q + 3]};
-    lds_barrier();
-    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(end, kTileBytes);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) buffer_store16<EndPol>(*line_piece(i), rs, line_at + 4096 * i);
-  }
-  return total;
+  if (end != nullptr) tile.store<kPolNTSys>(end, st);
 }
 
 // A sequence's rows, clamped to those there are.
@@ -653,46 +764,28 @@ __device__ __forceinline__ bool unit_of(const LinearParams& p, int items, int& i
   return true;
 }
 
-__device__ __forceinline__ void load_weight(const LinearParams& p, SegmentLds& lds) {
-  if (p.gate != nullptr && threadIdx.x < kDim)
-    lds.weight[threadIdx.x] = load_param(p.norm_weight, threadIdx.x, p.weight_bf16);
-}
-
 __device__ __forceinline__ int64_t tile_of(const LinearParams& p, int segment, int head) {
   return static_cast<int64_t>(segment) * p.num_v_heads + head;
 }
 
-// The first launch.  Item j < later reduces the segment ahead of later segment j to its update and
-// decay; item later + n walks sequence n if it is a single segment.
-template <bool Wide, bool Gated>
+// The first launch: item j reduces the segment ahead of later segment j to its update and decay.
+template <bool Wide>
 __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void linear_first_kernel(const LinearParams p, const Segments g) {
+void linear_reduce_kernel(const LinearParams p, const Segments g) {
   __shared__ SegmentLds lds;
   __shared__ SearchLds search;
-  int item, head;
-  if (!unit_of(p, g.later + g.num_sequences, item, head)) return;
+  int item, head, seq, index, count;
+  if (!unit_of(p, g.later, item, head) ||
+      !find_segment(p, search, g.num_sequences, g.most, item, seq, index, count))
+    return;
   int64_t bos;
   int rows;
-  if (item < g.later) {
-    int seq, index, count;
-    if (!find_segment(p, search, g.num_sequences, g.most, item, seq, index, count)) return;
-    sequence_rows(p, seq, bos, rows);
-    const int64_t at = tile_of(p, item, head);
-    const int each = segment_rows(rows, count);
-    const double total = walk<Wide, Gated, false, kPolPlain, kPolPlain>(
-        p, lds, bos + index * each, each, head, nullptr, g.tiles + at * kTileFloats);
-    if (threadIdx.x == 64 * kScalarWave) g.decays[at] = __builtin_amdgcn_exp2f(static_cast<float>(total));
-    return;
-  }
-  const int seq = item - g.later;
   sequence_rows(p, seq, bos, rows);
-  if (later_of(rows, g.most) != 0) return;
-  load_weight(p, lds);
-  const int slot = p.indices[seq];
-  const bool live = live_slot(slot, p.num_slots);
-  float* const home = p.state + static_cast<int64_t>(live ? slot : 0) * p.state_slot + head * kTileFloats;
-  walk<Wide, Gated, true, kPolNTSys, kPolNTSys>(
-      p, lds, bos, rows, head, live && p.has_initial[seq] != 0 ? home : nullptr, live ? home : nullptr);
+  const int64_t at = tile_of(p, item, head);
+  const int each = segment_rows(rows, count);
+  const double total =
+      reduce<Wide>(p, lds, bos + index * each, each, head, g.tiles + at * kTileFloats);
+  if (threadIdx.x == 64 * kScalarWave) g.decays[at] = __builtin_amdgcn_exp2f(static_cast<float>(total));
 }
 
 // The second: the state at every later segment's start, along each sequence, and the sequence's own
@@ -762,32 +855,42 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const LinearParams 
   }
 }
 
-// The third: every segment of the sequences of several, each from its state.  Item j < later is
-// later segment j; item later + j the sequence's first, if j is its first later one.
+// The third: every segment's outputs, and the sequences' last states.  Item j < later is later
+// segment j; item later + j the first segment of its sequence, if j is the sequence's first later
+// one; item 2 later + n sequence n, if it is a single segment (the shortest last).
 template <bool Wide, bool Gated>
 __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void linear_later_kernel(const LinearParams p, const Segments g) {
+void linear_walk_kernel(const LinearParams p, const Segments g) {
   __shared__ SegmentLds lds;
   __shared__ SearchLds search;
-  int item, head, seq, index, count;
-  if (!unit_of(p, 2 * g.later, item, head)) return;
-  const bool is_first = item >= g.later;
-  if (is_first) item -= g.later;
-  if (!find_segment(p, search, g.num_sequences, g.most, item, seq, index, count) ||
-      (is_first && index != 0))
-    return;
+  int item, head, seq, index = -1, count = 0;
+  if (!unit_of(p, 2 * g.later + g.num_sequences, item, head)) return;
+  const bool single = item >= 2 * g.later;
+  if (single) {
+    seq = item - 2 * g.later;
+  } else {
+    const bool is_first = item >= g.later;
+    if (is_first) item -= g.later;
+    if (!find_segment(p, search, g.num_sequences, g.most, item, seq, index, count) ||
+        (is_first && index != 0))
+      return;
+    if (is_first) index = -1;
+  }
   int64_t bos;
   int rows;
   sequence_rows(p, seq, bos, rows);
-  load_weight(p, lds);
+  if (single && later_of(rows, g.most) != 0) return;
+  if (p.gate != nullptr && threadIdx.x < kDim)
+    lds.weight[threadIdx.x] = load_param(p.norm_weight, threadIdx.x, p.weight_bf16);
   const int each = segment_rows(rows, count);
-  const int done = is_first ? 0 : (index + 1) * each;
+  const int done = (index + 1) * each;
   const int slot = p.indices[seq];
-  float* const home = p.state + static_cast<int64_t>(slot) * p.state_slot + head * kTileFloats;
-  walk<Wide, Gated, true, kPolPlain, kPolNTSys>(
-      p, lds, bos + done, min(rows - done, each), head,
-      (is_first ? g.firsts : g.tiles) + tile_of(p, item, head) * kTileFloats,
-      !is_first && index + 1 == count && live_slot(slot, p.num_slots) ? home : nullptr);
+  const bool live = live_slot(slot, p.num_slots);
+  float* const home = p.state + static_cast<int64_t>(live ? slot : 0) * p.state_slot + head * kTileFloats;
+  const float* start = (index < 0 ? g.firsts : g.tiles) + tile_of(p, item, head) * kTileFloats;
+  if (single) start = live && p.has_initial[seq] != 0 ? home : nullptr;
+  walk<Wide, Gated>(p, lds, bos + done, min(rows - done, each), head, start, single,
+                    live && index + 1 == count ? home : nullptr);
 }
 
 // A segment's tokens, at most: the share of a workgroup where 512 run at once (two a CU), in whole
@@ -805,23 +908,25 @@ int64_t later_segments(int64_t num_tokens, int32_t num_v_heads) {
   return num_tokens > 0 ? (num_tokens - 1) / segment_tokens(num_tokens, num_v_heads) : 0;
 }
 
-template <bool Wide, bool Gated>
-void launch_segments(const LinearParams& p, const Segments& g, uint32_t first, uint32_t later,
+template <bool Wide>
+void launch_segments(const LinearParams& p, const Segments& g, uint32_t reduced, uint32_t walked,
                      hipStream_t s) {
-  hipLaunchKernelGGL((linear_first_kernel<Wide, Gated>), dim3(first), dim3(kBlock), 0, s, p, g);
-  if (g.later == 0) return;
-  hipLaunchKernelGGL(linear_join_kernel, dim3(p.num_v_heads * kJoinParts), dim3(kBlock), 0, s, p, g);
-  hipLaunchKernelGGL((linear_later_kernel<Wide, Gated>), dim3(later), dim3(kBlock), 0, s, p, g);
+  if (g.later > 0) {
+    hipLaunchKernelGGL((linear_reduce_kernel<Wide>), dim3(reduced), dim3(kBlock), 0, s, p, g);
+    hipLaunchKernelGGL(linear_join_kernel, dim3(p.num_v_heads * kJoinParts), dim3(kBlock), 0, s, p, g);
+  }
+  const auto walk = p.gate != nullptr ? linear_walk_kernel<Wide, true> : linear_walk_kernel<Wide, false>;
+  hipLaunchKernelGGL(walk, dim3(walked), dim3(kBlock), 0, s, p, g);
 }
 
-void launch_linear_prefill(const LinearParams& p, const Segments& g, uint32_t first, uint32_t later,
-                           hipStream_t s) {
+void launch_linear_prefill(const LinearParams& p, const Segments& g, uint32_t reduced,
+                           uint32_t walked, hipStream_t s) {
   const uintptr_t bits = reinterpret_cast<uintptr_t>(p.qkv) | reinterpret_cast<uintptr_t>(p.gate) |
                          reinterpret_cast<uintptr_t>(p.out) | (p.qkv_row * 2) | (p.gate_row * 2);
-  const auto launch = (bits & 3) == 0
-                          ? (p.gate != nullptr ? launch_segments<true, true> : launch_segments<true, false>)
-                          : (p.gate != nullptr ? launch_segments<false, true> : launch_segments<false, false>);
-  launch(p, g, first, later, s);
+  if ((bits & 3) == 0)
+    launch_segments<true>(p, g, reduced, walked, s);
+  else
+    launch_segments<false>(p, g, reduced, walked, s);
 }
 
 }  // namespace
@@ -870,7 +975,8 @@ extern "C" int ld_linear_prefill(const ld_linear_prefill_args* args, void* strea
   g.tiles = static_cast<float*>(a.workspace);
   g.firsts = g.tiles + later * a.num_v_heads * kTileFloats;
   g.decays = g.firsts + later * a.num_v_heads * kTileFloats;
-  launch_linear_prefill(p, g, static_cast<uint32_t>(blocks_of(later + a.num_sequences)),
-                        static_cast<uint32_t>(blocks_of(2 * later)), static_cast<hipStream_t>(stream));
+  launch_linear_prefill(p, g, static_cast<uint32_t>(blocks_of(later)),
+                        static_cast<uint32_t>(blocks_of(2 * later + a.num_sequences)),
+                        static_cast<hipStream_t>(stream));
   return check_launch("ld_linear_prefill");
 }
