@@ -39,8 +39,10 @@ extern "C" {
  *              NULL: no norm
  *   norm_weight fp32 or bf16 [128] (norm_weight_dtype)
  *   out        bf16 [tokens, HV, 128] contiguous
+ * out and state overlap no other argument, nor do two slots or two rows of out.
  * A slot outside 1 .. num_slots - 1 is padding: never read, never written.  Non-finite values of
- * a request's activations reach outputs and state of that request alone.
+ * a request's activations reach outputs and state of that request alone (in a prompt also outputs
+ * of up to 63 tokens ahead of the value's).
  */
 
 /*
@@ -83,7 +85,8 @@ int ld_linear_decode(const ld_linear_decode_args* args, void* stream);
  * cu_seqlens[n] .. cu_seqlens[n+1]-1; its state starts from state[slots[n]] when slots[n] is not
  * padding and has_initial[n] != 0, else from zeros, and the state after its last token goes to
  * state[slots[n]] (an empty sequence writes its initial state back).  Rows outside every
- * sequence are left as they were.  Slots are distinct.
+ * sequence are left as they were.  Slots are distinct.  Row strides of qkv, gate and log_decay are
+ * 0 .. 2^23 elements, rows of out likewise (num_v_heads <= 2^16), num_tokens < 2^31.
  */
 typedef struct ld_linear_prefill_args {
   const void* qkv;
@@ -113,7 +116,12 @@ typedef struct ld_linear_prefill_args {
 
 int ld_linear_prefill(const ld_linear_prefill_args* args, void* stream);
 
-/* Workspace bytes of ld_linear_prefill for these sizes; 0 where it needs none. */
+/*
+ * Workspace bytes of ld_linear_prefill for these sizes, 64 MiB and little more at most; 0 where
+ * it needs none.  Two states and a decay for each segment of a head but the first, segments of at
+ * least 256 tokens.  Nothing is kept in it from one call for the next; calls that may run at once
+ * need one each.
+ */
 int64_t ld_linear_prefill_workspace_bytes(int64_t num_tokens, int32_t num_sequences,
                                           int32_t num_v_heads);
 

@@ -19,4 +19,8 @@ Modules and what pins each one (details in each module's header):
   state_io  numpy gather / scatter / slot copy (csrc/state_io.cu:11-27).  Pinned by brute
             force element loops on tiny pools and by the reference test's fixed expectations
             (tests/test_gdn.py:125-143).
+  linear    the linear-attention ops and norm_rope from their definitions in 64 bits, with
+            the error that a correct fp32 implementation may have.  Pinned by the sum over
+            token pairs, by decode steps against a prefill, and by the rotation's invariants
+            (tests/test_linear_cpu.py).
 """
