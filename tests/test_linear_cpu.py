@@ -146,6 +146,10 @@ SHARED = [
     (dict(weight=lambda m: None), "gate and weight must be given together"),
     (dict(gate=lambda m: bf16(m, 4, 4, 64)), "gate must be CUDA BF16"),
     (dict(weight=lambda m: bf16(m, 64)), "weight must be contiguous"),
+    (dict(state=lambda m: torch.zeros(10, 4, DIM, DIM)), "state must be CUDA FP32"),
+    (dict(log_decay=lambda m: torch.zeros(4)), "log_decay must be CUDA FP32"),
+    (dict(out=lambda m: torch.zeros(4, 4, DIM, dtype=torch.bfloat16)), "out must be contiguous CUDA"),
+    (dict(weight=lambda m: torch.zeros(DIM)), "weight must be contiguous CUDA"),
     (dict(scale=lambda m: float("nan")), "scale must be finite"),
     (dict(eps=lambda m: 0.0), "epsilon must be positive"),
 ]
@@ -154,11 +158,13 @@ DECODE_ONLY = [
     (dict(indices=lambda m: torch.empty(4, 1, dtype=torch.int64, device=m)), "metadata must be"),
     (dict(cu=lambda m: i32(m, 4)), "invalid request metadata shapes"),
     (dict(accepted=lambda m: i32(m, 8)[::2]), "metadata must be"),
+    (dict(indices=lambda m: torch.zeros(4, 1, dtype=torch.int32)), "metadata must be"),
 ]
 PREFILL_ONLY = [
     (dict(slots=lambda m: i32(m, 3, 1)), "metadata must be"),
     (dict(has_initial=lambda m: i32(m, 3)), "has_initial must be"),
     (dict(cu_seqlens=lambda m: i32(m, 3)), "invalid sequence metadata shapes"),
+    (dict(slots=lambda m: torch.zeros(3, dtype=torch.int32)), "metadata must be"),
 ]
 ROPE = [
     (dict(qkv=lambda m: f32(m, 5, 7 * DIM)), "qkv must be CUDA BF16"),
@@ -171,6 +177,8 @@ ROPE = [
     (dict(inv_freq=lambda m: f32(m, 65)), "inv_freq must be"),
     (dict(inv_freq=lambda m: f32(m, 12)), "inv_freq must be"),
     (dict(eps=lambda m: -1.0), "epsilon must be positive"),
+    (dict(positions=lambda m: torch.zeros(5, dtype=torch.int64)), "positions must be"),
+    (dict(inv_freq=lambda m: torch.zeros(32)), "inv_freq must be"),
 ]
 KINDS = {
     "linear_decode": (decode_args, ops.check_linear_decode, SHARED + DECODE_ONLY),
