@@ -33,10 +33,11 @@
 // (against eight of 16, which read every K and Q operand twice: 415 us and 332 at one time).
 //
 // A sequence longer than a segment is cut into segments, since the recurrence over them is
-// associative: one launch reduces every segment but a sequence's last to its update and decay, a
-// second joins these along each sequence, a third walks all segments from the states the second
-// left, and the sequences of one segment.  One prompt of 4096 tokens and 32 heads, 16 segments: 23,
-// 13 and 50 us (walked in one piece by 32 workgroups, 64 chunks' chain alone would be 330).
+// associative: one launch reduces every segment but a sequence's last to the state after it from zeros
+// and its decay, a second (where there are many) joins these along each sequence, a third walks all
+// segments from the joined states, and the sequences of one segment.  One prompt of 4096 tokens and
+// 32 heads, 16 segments: 23 and 57 us (walked in one piece by 32 workgroups, 64 chunks' chain alone
+// would be 330).
 #include <algorithm>
 #include <cstddef>
 
@@ -172,14 +173,54 @@ struct StateTile {
     const int tid = threadIdx.x, v = 8 * i + (tid >> 5);
     return reinterpret_cast<f32x4*>(tile + v * (kDim * 4) + (((tid & 31) ^ (v & 15)) << 4));
   }
-  template <int Pol>
-  __device__ __forceinline__ void load(const float* from, f32x16 (&st)[4]) const {
+  // From the pool, and a copy in `kept` unless null.
+  __device__ __forceinline__ void load(const float* from, float* kept, f32x16 (&st)[4]) const {
     const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(from, kTileBytes);
     f32x4 lines[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) lines[i] = buffer_load16<Pol>(rs, threadIdx.x * 16 + 4096 * i);
+    for (int i = 0; i < 16; ++i) lines[i] = buffer_load16<kPolNTSys>(rs, threadIdx.x * 16 + 4096 * i);
+    if (kept != nullptr) {
+      const __amdgpu_buffer_rsrc_t copy = buffer_rsrc(kept, kTileBytes);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) buffer_store16<kPolPlain>(lines[i], copy, threadIdx.x * 16 + 4096 * i);
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) *line(i) = lines[i];
+    take(st);
+  }
+  // From the workspace: `count` tiles, each (but the first) added to its decay times those ahead.
+  __device__ __forceinline__ void load_joined(const float* tiles, const float* decays, int count,
+                                              int num_v_heads, f32x16 (&st)[4]) const {
+    constexpr int kAhead = 2, kLines = 8;   // tiles in flight, half of their lines at a time
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      f32x4 sum[kLines] = {}, part[kAhead][kLines];
+      auto fetch = [&](int a, int k) __attribute__((always_inline)) {   // (past the last, that again)
+        const __amdgpu_buffer_rsrc_t rs =
+            buffer_rsrc(tiles + min(k, count - 1) * (num_v_heads * kTileFloats), kTileBytes);
+#pragma unroll
+        for (int i = 0; i < kLines; ++i)
+          part[a][i] = buffer_load16<kPolPlain>(rs, threadIdx.x * 16 + 4096 * (kLines * half + i));
+      };
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) fetch(a, a);
+      for (int k = 0; k < count; k += kAhead) {
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          if (k + a < count) {
+            const float by = k + a == 0 ? 0.0f : decays[(k + a) * num_v_heads];
+#pragma unroll
+            for (int i = 0; i < kLines; ++i) sum[i] = sum[i] * by + part[a][i];
+          }
+          fetch(a, k + a + kAhead);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kLines; ++i) *line(kLines * half + i) = sum[i];
+    }
+    take(st);
+  }
+  __device__ __forceinline__ void take(f32x16 (&st)[4]) const {   // from LDS
     lds_barrier();
 #pragma unroll
     for (int T = 0; T < 4; ++T)
@@ -236,13 +277,14 @@ __device__ __forceinline__ f32x16 decayed(const bf16x8 (&v)[2], const float* ek,
   return x;
 }
 
-// A segment of `rows` rows (whole chunks) from row `bos`, reduced to its update, the state after it
-// from zeros, at `end`; returns, on wave kScalarWave, the sum of log decays in units of log 2.
+// A segment of `rows` rows (whole chunks) from row `bos`, reduced to the state after it, from the
+// state at `start` (kept in `kept`) or, if null, from zeros, at `end`; returns, on wave kScalarWave,
+// the sum of log decays in units of log 2.
 // Rows of k and v go to one half of the tile's LDS while the other is worked on: one barrier a
 // chunk.
 template <bool Wide>
 __device__ __forceinline__ double reduce(const LinearParams& p, SegmentLds& lds, int64_t bos, int rows,
-                                         int head, float* end) {
+                                         int head, const float* start, float* kept, float* end) {
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -290,6 +332,8 @@ __device__ __forceinline__ double reduce(const LinearParams& p, SegmentLds& lds,
   double total = 0.0;
   float next_g = load_decay(0);
   fetch(0);
+  const StateTile tile(lds);
+  if (start != nullptr) tile.load(start, kept, st);
   if (w == kScalarWave) total += chunk_scalars(lds.scalars[0], next_g, p.scale, lane);
   next_g = load_decay(1);
   put(0);
@@ -338,7 +382,7 @@ __device__ __forceinline__ double reduce(const LinearParams& p, SegmentLds& lds,
       }
     }
   }
-  StateTile(lds).store<kPolPlain>(end, st);
+  tile.store<kPolPlain>(end, st);
   return total;
 }
 
@@ -349,11 +393,12 @@ __device__ __forceinline__ double reduce(const LinearParams& p, SegmentLds& lds,
 // over 0 bytes or an offset past it: zeros and dropped stores): under a branch the compiler would
 // have to wait for every load in flight before it uses any.  Wide: every address is a multiple of
 // 4 bytes; else elements move one by one.
-// The pool (`end`, and `start` if pooled) is passed by, the workspace read as the second launch
-// left it in the caches.
+// The pool (`end`, and `start` if `joined` is 0) is passed by, the workspace read as the launches
+// ahead left it in the caches: `joined` tiles from `start`, with `decays`.
 template <bool Wide, bool Gated>
 __device__ __forceinline__ void walk(const LinearParams& p, SegmentLds& lds, int64_t bos, int rows,
-                                     int head, const float* start, bool pooled, float* end) {
+                                     int head, const float* start, int joined, const float* decays,
+                                     float* end) {
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -422,10 +467,10 @@ __device__ __forceinline__ void walk(const LinearParams& p, SegmentLds& lds, int
   f32x16 st[4] = {};
   const StateTile tile(lds);
   if (start != nullptr) {
-    if (pooled)
-      tile.load<kPolNTSys>(start, st);
+    if (joined == 0)
+      tile.load(start, nullptr, st);
     else
-      tile.load<kPolPlain>(start, st);
+      tile.load_joined(start, decays, joined, p.num_v_heads, st);
   }
   if (w == kScalarWave) chunk_scalars(lds.scalars[0], next_g, p.scale, lane);
   next_g = load_decay(1);
@@ -754,8 +799,15 @@ struct Segments {
   int num_sequences;
   int most;         // tokens of a segment, at most
   int later;        // at most this many later segments
-  float* tiles;     // per (later segment, head): the state it starts from (before the second
-                    // launch, the update of the segment ahead of it)
+  // Each segment sums the states ahead of it by itself, without the second launch: up to 16 of them,
+  // or 32 among several sequences, most of which have far fewer (us, with the second launch and
+  // without: 13 prompts of 1 to 3000 tokens 149 / 136, 16 of 64 to 1024 106 / 92, one of 4096 88 / 83;
+  // one of 8192 with 8 heads, 31 ahead of the last, 55 / 63, of 16384 85 / 130).
+  bool direct;
+  // per (later segment, head): the state after the segment ahead of it, for a sequence's first one
+  // from the state that the sequence starts from, for the others from zeros (behind the join: the
+  // state that the segment starts from)
+  float* tiles;
   float* firsts;    // in the places of the first later segments: the state the sequence starts
                     // from, as its last segment replaces it in the pool
   float* decays;    // per (later segment, head): the decay over the segment ahead of it
@@ -777,7 +829,8 @@ __device__ __forceinline__ int64_t tile_of(const LinearParams& p, int segment, i
   return static_cast<int64_t>(segment) * p.num_v_heads + head;
 }
 
-// The first launch: item j reduces the segment ahead of later segment j to its update and decay.
+// The first launch: item j reduces the segment ahead of later segment j to the state after it and
+// its decay.
 template <bool Wide>
 __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void linear_reduce_kernel(const LinearParams p, const Segments g) {
@@ -792,19 +845,22 @@ void linear_reduce_kernel(const LinearParams p, const Segments g) {
   sequence_rows(p, seq, bos, rows);
   const int64_t at = tile_of(p, item, head);
   const int each = segment_rows(rows, count);
-  const double total =
-      reduce<Wide>(p, lds, bos + index * each, each, head, g.tiles + at * kTileFloats);
+  const int slot = p.indices[seq];
+  const float* start = index == 0 && live_slot(slot, p.num_slots) && p.has_initial[seq] != 0
+                           ? p.state + slot * p.state_slot + head * kTileFloats
+                           : nullptr;
+  const double total = reduce<Wide>(p, lds, bos + index * each, each, head, start,
+                                    g.firsts + at * kTileFloats, g.tiles + at * kTileFloats);
   if (threadIdx.x == 64 * kScalarWave) g.decays[at] = __builtin_amdgcn_exp2f(static_cast<float>(total));
 }
 
-// The second: the state at every later segment's start, along each sequence, and the sequence's own
-// start set aside.  A workgroup takes a sixteenth of one head's tile through every fourth of the
-// sequences of several segments: they wait for memory side by side (13 prompts of 1 to 3000 tokens 152
-// to 150 us, 20 of 1 to 2500 175 to 171; where there are none four times the workgroups cost nothing).
+// The second, unless direct: the state at every later segment's start, along each sequence.  A
+// workgroup takes a sixteenth of one head's tile through every fourth of the sequences of several
+// segments: they wait for memory side by side.
 constexpr int kJoinParts = kTileFloats / 4 / kBlock;
 constexpr int kJoinSequences = 4;
 __global__ __launch_bounds__(kBlock) void linear_join_kernel(const LinearParams p, const Segments g) {
-  __shared__ int longer[kBlock], counts[kBlock], bases[kBlock];   // the sequences of several segments
+  __shared__ int counts[kBlock], bases[kBlock];   // of the sequences of several segments
   __shared__ int sums[2][kBlockWaves];
   const int tid = threadIdx.x;
   const int part = blockIdx.x % kJoinParts;
@@ -826,7 +882,6 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const LinearParams 
     const int sum = inclusive_sum(mine, sums[0], all);
     const int place = inclusive_sum(mine > 0 ? 1 : 0, sums[1], several) - 1;
     if (mine > 0) {
-      longer[place] = n;
       counts[place] = mine;
       bases[place] = base + sum - mine;
     }
@@ -834,14 +889,9 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const LinearParams 
     base += all;
     for (int i = blockIdx.y; i < several; i += gridDim.y) {
       const int j = __builtin_amdgcn_readfirstlane(bases[i]);
-      const int seq = __builtin_amdgcn_readfirstlane(longer[i]);
       const int count = min(__builtin_amdgcn_readfirstlane(counts[i]), g.later - j);
-      if (count <= 0) break;
-      const int slot = p.indices[seq];
+      if (count <= 1) continue;
       f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (live_slot(slot, p.num_slots) && p.has_initial[seq] != 0)
-        s = *reinterpret_cast<const f32x4*>(p.state + slot * p.state_slot + head * kTileFloats + at);
-      *reinterpret_cast<f32x4*>(g.firsts + tile_of(p, j, head) * kTileFloats + at) = s;
       float* tile = g.tiles + tile_of(p, j, head) * kTileFloats + at;
       const float* decay = g.decays + tile_of(p, j, head);
       constexpr int kAhead = 8;   // updates and decays in flight
@@ -850,7 +900,7 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const LinearParams 
       auto load = [&](int a, int k) __attribute__((always_inline)) {   // (past the last, that again)
         const int64_t from = min(k, count - 1);
         update[a] = *reinterpret_cast<const f32x4*>(tile + from * step);
-        by[a] = decay[from * p.num_v_heads];
+        by[a] = from == 0 ? 0.0f : decay[from * p.num_v_heads];
       };
 #pragma unroll
       for (int a = 0; a < kAhead; ++a) load(a, a);
@@ -859,7 +909,7 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const LinearParams 
         for (int a = 0; a < kAhead; ++a) {
           s = s * by[a] + update[a];
           load(a, k + a + kAhead);
-          if (k + a < count) *reinterpret_cast<f32x4*>(tile + (k + a) * step) = s;
+          if (k + a > 0 && k + a < count) *reinterpret_cast<f32x4*>(tile + (k + a) * step) = s;
         }
       }
     }
@@ -899,9 +949,14 @@ void linear_walk_kernel(const LinearParams p, const Segments g) {
   const int slot = p.indices[seq];
   const bool live = live_slot(slot, p.num_slots);
   float* const home = p.state + static_cast<int64_t>(live ? slot : 0) * p.state_slot + head * kTileFloats;
-  const float* start = (index < 0 ? g.firsts : g.tiles) + tile_of(p, item, head) * kTileFloats;
-  if (single) start = live && p.has_initial[seq] != 0 ? home : nullptr;
-  walk<Wide, Gated>(p, lds, bos + done, min(rows - done, each), head, start, single,
+  const bool initial = live && p.has_initial[seq] != 0;
+  // later segments: the tile that the join left, or all of the sequence's up to theirs
+  const int joined = single ? 0 : index < 0 || !g.direct ? 1 : index + 1;
+  const int64_t at = tile_of(p, item - (index < 0 ? 0 : joined - 1), head);
+  const float* start = g.tiles + at * kTileFloats;
+  if (single) start = initial ? home : nullptr;
+  if (!single && index < 0) start = initial ? g.firsts + at * kTileFloats : nullptr;
+  walk<Wide, Gated>(p, lds, bos + done, min(rows - done, each), head, start, joined, g.decays + at,
                     live && index + 1 == count ? home : nullptr);
 }
 
@@ -909,22 +964,26 @@ void linear_walk_kernel(const LinearParams p, const Segments g) {
 // chunks and at least 4 of them, as a segment is walked twice.  Rounded to a power of two the share
 // left CUs idle behind one long prompt (32 heads, us: 5000 tokens 117 / 97, 9000 180 / 149, 20000
 // 368 / 300) and gained and lost by turns on mixed ones; 1.14 or 1.33 shares likewise.
-int64_t segment_tokens(int64_t num_tokens, int32_t num_v_heads) {
+// Several sequences of 512 tokens in all are left whole: most likely none is long, and a reduction in
+// vain takes 5 us of their 20.
+int64_t segment_tokens(int64_t num_tokens, int32_t num_sequences, int32_t num_v_heads) {
   constexpr int64_t kAtOnce = 512;
+  if (num_sequences > 1 && num_tokens <= 512) return 512;
   const int64_t share = (num_tokens * num_v_heads + kAtOnce - 1) / kAtOnce;
   return std::clamp<int64_t>((share + kTokens - 1) / kTokens * kTokens, 4 * kTokens, 1 << 30);
 }
 
 // Sequences of more than a segment have at most this many later ones.
-int64_t later_segments(int64_t num_tokens, int32_t num_v_heads) {
-  return num_tokens > 0 ? (num_tokens - 1) / segment_tokens(num_tokens, num_v_heads) : 0;
+int64_t later_segments(int64_t num_tokens, int32_t num_sequences, int32_t num_v_heads) {
+  return num_tokens > 0 ? (num_tokens - 1) / segment_tokens(num_tokens, num_sequences, num_v_heads) : 0;
 }
 
 template <bool Wide>
 void launch_segments(const LinearParams& p, const Segments& g, uint32_t reduced, uint32_t walked,
                      hipStream_t s) {
-  if (g.later > 0) {
+  if (g.later > 0)
     hipLaunchKernelGGL((linear_reduce_kernel<Wide>), dim3(reduced), dim3(kBlock), 0, s, p, g);
+  if (g.later > 0 && !g.direct) {
     const dim3 parts(p.num_v_heads * kJoinParts,
                      std::min({g.num_sequences, g.later, kJoinSequences}));
     hipLaunchKernelGGL(linear_join_kernel, parts, dim3(kBlock), 0, s, p, g);
@@ -949,7 +1008,7 @@ void launch_linear_prefill(const LinearParams& p, const Segments& g, uint32_t re
 extern "C" int64_t ld_linear_prefill_workspace_bytes(int64_t num_tokens, int32_t num_sequences,
                                                      int32_t num_v_heads) {
   if (num_tokens < 0 || num_sequences <= 0 || num_v_heads <= 0) return 0;
-  return ld::later_segments(num_tokens, num_v_heads) * num_v_heads *
+  return ld::later_segments(num_tokens, num_sequences, num_v_heads) * num_v_heads *
          static_cast<int64_t>((2 * ld::kTileFloats + 4) * sizeof(float));
 }
 
@@ -971,7 +1030,7 @@ extern "C" int ld_linear_prefill(const ld_linear_prefill_args* args, void* strea
   p.indices = a.slots;
   p.cu = a.cu_seqlens;
   p.has_initial = a.has_initial;
-  const int64_t later = later_segments(a.num_tokens, a.num_v_heads);
+  const int64_t later = later_segments(a.num_tokens, a.num_sequences, a.num_v_heads);
   if (later > 0 && (!aligned16(a.workspace) || a.workspace == nullptr ||
                     a.workspace_bytes < ld_linear_prefill_workspace_bytes(
                                             a.num_tokens, a.num_sequences, a.num_v_heads)))
@@ -984,8 +1043,9 @@ extern "C" int ld_linear_prefill(const ld_linear_prefill_args* args, void* strea
     return fail(LD_ERR_INVALID_ARGUMENT, "too many (sequence, head) tiles");
   Segments g{};
   g.num_sequences = a.num_sequences;
-  g.most = static_cast<int>(segment_tokens(a.num_tokens, a.num_v_heads));
+  g.most = static_cast<int>(segment_tokens(a.num_tokens, a.num_sequences, a.num_v_heads));
   g.later = static_cast<int>(later);
+  g.direct = later <= (a.num_sequences == 1 ? 16 : 32);
   g.tiles = static_cast<float*>(a.workspace);
   g.firsts = g.tiles + later * a.num_v_heads * kTileFloats;
   g.decays = g.firsts + later * a.num_v_heads * kTileFloats;

@@ -314,14 +314,15 @@ def test_c_abi_prefill_limits():
         refused(lib.ld_linear_prefill, _lib.LinearPrefillArgs(**dict(good, **change)), message)
 
 
-@pytest.mark.parametrize("tokens,heads,segment", [
-    (256, 4, 256), (257, 4, 256), (4096, 32, 256), (4097, 32, 320), (5000, 32, 320),
-    (2**17, 32, 2**13), (10**6, 48, 93760), (2**31 - 1, 1, 2**22)])
-def test_prefill_workspace(tokens, heads, segment):
+@pytest.mark.parametrize("tokens,sequences,heads,segment", [
+    (256, 1, 4, 256), (257, 1, 4, 256), (512, 2, 4, 512), (513, 2, 4, 256), (4096, 3, 32, 256),
+    (4097, 1, 32, 320), (5000, 3, 32, 320), (2**17, 3, 32, 2**13), (10**6, 9, 48, 93760),
+    (2**31 - 1, 1, 1, 2**22)])
+def test_prefill_workspace(tokens, sequences, heads, segment):
     """Two states and a decay for each segment of a head but the first: a segment has a 512th of all
-    heads' tokens in whole chunks of 64, at least 256, so that it is 64 MiB and little more at the
-    most."""
-    got = _lib.load().ld_linear_prefill_workspace_bytes(tokens, 3, heads)
+    heads' tokens in whole chunks of 64, at least 256 (several sequences of 512 in all are whole),
+    so that it is 64 MiB and little more at the most."""
+    got = _lib.load().ld_linear_prefill_workspace_bytes(tokens, sequences, heads)
     assert got == (tokens - 1) // segment * heads * (2 * DIM * DIM + 4) * 4
     assert got <= 512 * (2 * DIM * DIM + 4) * 4
 

@@ -292,9 +292,13 @@ def test_far_rows(gpu):
 @pytest.mark.parametrize("lengths,heads", [([513], (1, 1)), ([767, 768, 769], (1, 2)),
                                            ([1023, 256, 1025, 257], (1, 1)), ([9000], (2, 8)),
                                            ([2300, 700, 2], (4, 16)),
-                                           ([3] * 250 + [300] * 8 + [2] * 20 + [520], (1, 1))])
+                                           ([3] * 250 + [300] * 8 + [2] * 20 + [520], (1, 1)),
+                                           ([200, 312], (1, 2)), ([512], (1, 2)),
+                                           ([8000, 450], (1, 1)), ([4352], (1, 1)),
+                                           ([4353], (1, 1))])
 def test_prefill_segments(gpu, lengths, heads):
     """Sequences cut into segments of equal whole chunks: a token to either side of a further
-    segment, more heads than leave a segment at its least, long sequences among many short ones."""
+    segment, more heads than leave a segment at its least, long sequences among many short ones,
+    segments that sum the states ahead of them by themselves and ones that find them joined."""
     announce(test="linear_prefill_segments", lengths=lengths[-3:], heads=heads)
     check_prefill(prefill_case(lengths, *heads, seed=11, device=gpu, decay=0.05))
