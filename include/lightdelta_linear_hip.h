@@ -119,7 +119,7 @@ int ld_linear_prefill(const ld_linear_prefill_args* args, void* stream);
 /*
  * Workspace bytes of ld_linear_prefill for these sizes, 64 MiB and little more at most; 0 where
  * it needs none.  Two states and a decay for each segment of a head but the first, segments of at
- * least 256 tokens.  Nothing is kept in it from one call for the next; calls that may run at once
+ * least 128 tokens (of several sequences 256).  Nothing is kept in it from one call for the next; calls that may run at once
  * need one each.
  */
 int64_t ld_linear_prefill_workspace_bytes(int64_t num_tokens, int32_t num_sequences,

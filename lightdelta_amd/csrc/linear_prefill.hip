@@ -191,10 +191,10 @@ struct StateTile {
   // From the workspace: `count` tiles, each (but the first) added to its decay times those ahead.
   __device__ __forceinline__ void load_joined(const float* tiles, const float* decays, int count,
                                               int num_v_heads, f32x16 (&st)[4]) const {
-    constexpr int kAhead = 2, kLines = 8;   // tiles in flight, half of their lines at a time
+    constexpr int kFlight = 2, kLines = 8;   // tiles in flight, half of their lines at a time
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      f32x4 sum[kLines] = {}, part[kAhead][kLines];
+      f32x4 sum[kLines] = {}, part[kFlight][kLines];
       auto fetch = [&](int a, int k) __attribute__((always_inline)) {   // (past the last, that again)
         const __amdgpu_buffer_rsrc_t rs =
             buffer_rsrc(tiles + min(k, count - 1) * (num_v_heads * kTileFloats), kTileBytes);
@@ -203,16 +203,16 @@ struct StateTile {
           part[a][i] = buffer_load16<kPolPlain>(rs, threadIdx.x * 16 + 4096 * (kLines * half + i));
       };
 #pragma unroll
-      for (int a = 0; a < kAhead; ++a) fetch(a, a);
-      for (int k = 0; k < count; k += kAhead) {
+      for (int a = 0; a < kFlight; ++a) fetch(a, a);
+      for (int k = 0; k < count; k += kFlight) {
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) {
+        for (int a = 0; a < kFlight; ++a) {
           if (k + a < count) {
             const float by = k + a == 0 ? 0.0f : decays[(k + a) * num_v_heads];
 #pragma unroll
             for (int i = 0; i < kLines; ++i) sum[i] = sum[i] * by + part[a][i];
           }
-          fetch(a, k + a + kAhead);
+          fetch(a, k + a + kFlight);
         }
       }
 #pragma unroll
@@ -795,12 +795,14 @@ __device__ bool find_segment(const LinearParams& p, SearchLds& lds, int num_sequ
   return false;
 }
 
+constexpr int kAhead = 16;
+
 struct Segments {
   int num_sequences;
   int most;         // tokens of a segment, at most
   int later;        // at most this many later segments
-  // Each segment sums the states ahead of it by itself, without the second launch: up to 16 of them,
-  // or 32 among several sequences, most of which have far fewer (us, with the second launch and
+  // Each segment sums the states ahead of it by itself, without the second launch: up to kAhead of
+  // them, or twice that among several sequences, most of which have far fewer (us, with the second launch and
   // without: 13 prompts of 1 to 3000 tokens 149 / 136, 16 of 64 to 1024 106 / 92, one of 4096 88 / 83;
   // one of 8192 with 8 heads, 31 ahead of the last, 55 / 63, of 16384 85 / 130).
   bool direct;
@@ -894,21 +896,21 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const LinearParams 
       f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
       float* tile = g.tiles + tile_of(p, j, head) * kTileFloats + at;
       const float* decay = g.decays + tile_of(p, j, head);
-      constexpr int kAhead = 8;   // updates and decays in flight
-      f32x4 update[kAhead];
-      float by[kAhead];
+      constexpr int kFlight = 8;   // updates and decays in flight
+      f32x4 update[kFlight];
+      float by[kFlight];
       auto load = [&](int a, int k) __attribute__((always_inline)) {   // (past the last, that again)
         const int64_t from = min(k, count - 1);
         update[a] = *reinterpret_cast<const f32x4*>(tile + from * step);
         by[a] = from == 0 ? 0.0f : decay[from * p.num_v_heads];
       };
 #pragma unroll
-      for (int a = 0; a < kAhead; ++a) load(a, a);
-      for (int k = 0; k < count; k += kAhead) {
+      for (int a = 0; a < kFlight; ++a) load(a, a);
+      for (int k = 0; k < count; k += kFlight) {
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) {
+        for (int a = 0; a < kFlight; ++a) {
           s = s * by[a] + update[a];
-          load(a, k + a + kAhead);
+          load(a, k + a + kFlight);
           if (k + a > 0 && k + a < count) *reinterpret_cast<f32x4*>(tile + (k + a) * step) = s;
         }
       }
@@ -960,17 +962,25 @@ void linear_walk_kernel(const LinearParams p, const Segments g) {
                     live && index + 1 == count ? home : nullptr);
 }
 
-// A segment's tokens, at most: the share of a workgroup where 512 run at once (two a CU), in whole
-// chunks and at least 4 of them, as a segment is walked twice.  Rounded to a power of two the share
-// left CUs idle behind one long prompt (32 heads, us: 5000 tokens 117 / 97, 9000 180 / 149, 20000
-// 368 / 300) and gained and lost by turns on mixed ones; 1.14 or 1.33 shares likewise.
-// Several sequences of 512 tokens in all are left whole: most likely none is long, and a reduction in
-// vain takes 5 us of their 20.
+// A segment's tokens, at most, in whole chunks: the share of a workgroup where 512 run at once (two
+// a CU), and at least 256, as a segment is walked twice.  Rounded to a power of two the share left
+// CUs idle behind one long prompt (32 heads, us: 5000 tokens 117 / 97, 9000 180 / 149, 20000 368 /
+// 300) and gained and lost by turns on mixed ones; 1.14 or 1.33 shares likewise.
+// One prompt is cut finer, to 128 tokens, while a CU gets one workgroup and a segment has 16 ahead
+// of it (us: 512 tokens of 32 heads 40 / 31, 1024 44 / 37; to 128 in any case 2048 50 / 56, 4096 of 8
+// heads 55 / 62).  Several of 512 tokens in all are left whole: most likely none is long, and a
+// reduction in vain takes 5 us of their 20.
 int64_t segment_tokens(int64_t num_tokens, int32_t num_sequences, int32_t num_v_heads) {
-  constexpr int64_t kAtOnce = 512;
   if (num_sequences > 1 && num_tokens <= 512) return 512;
-  const int64_t share = (num_tokens * num_v_heads + kAtOnce - 1) / kAtOnce;
-  return std::clamp<int64_t>((share + kTokens - 1) / kTokens * kTokens, 4 * kTokens, 1 << 30);
+  const auto share = [](int64_t tokens, int64_t parts) {
+    const int64_t each = (tokens + parts - 1) / parts;
+    return (each + kTokens - 1) / kTokens * kTokens;
+  };
+  int64_t least = 256;
+  if (num_sequences == 1)
+    least = std::clamp<int64_t>(
+        std::max(share(num_tokens * num_v_heads, 256), share(num_tokens, kAhead + 1)), 128, least);
+  return std::clamp<int64_t>(share(num_tokens * num_v_heads, 512), least, 1 << 30);
 }
 
 // Sequences of more than a segment have at most this many later ones.
@@ -1007,7 +1017,7 @@ void launch_linear_prefill(const LinearParams& p, const Segments& g, uint32_t re
 
 extern "C" int64_t ld_linear_prefill_workspace_bytes(int64_t num_tokens, int32_t num_sequences,
                                                      int32_t num_v_heads) {
-  if (num_tokens < 0 || num_sequences <= 0 || num_v_heads <= 0) return 0;
+  if (num_tokens < 0 || num_tokens > 0x7fffffff || num_sequences <= 0 || num_v_heads <= 0) return 0;
   return ld::later_segments(num_tokens, num_sequences, num_v_heads) * num_v_heads *
          static_cast<int64_t>((2 * ld::kTileFloats + 4) * sizeof(float));
 }
@@ -1045,7 +1055,7 @@ extern "C" int ld_linear_prefill(const ld_linear_prefill_args* args, void* strea
   g.num_sequences = a.num_sequences;
   g.most = static_cast<int>(segment_tokens(a.num_tokens, a.num_sequences, a.num_v_heads));
   g.later = static_cast<int>(later);
-  g.direct = later <= (a.num_sequences == 1 ? 16 : 32);
+  g.direct = later <= (a.num_sequences == 1 ? kAhead : 2 * kAhead);
   g.tiles = static_cast<float*>(a.workspace);
   g.firsts = g.tiles + later * a.num_v_heads * kTileFloats;
   g.decays = g.firsts + later * a.num_v_heads * kTileFloats;

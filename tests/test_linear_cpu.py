@@ -315,13 +315,14 @@ def test_c_abi_prefill_limits():
 
 
 @pytest.mark.parametrize("tokens,sequences,heads,segment", [
-    (256, 1, 4, 256), (257, 1, 4, 256), (512, 2, 4, 512), (513, 2, 4, 256), (4096, 3, 32, 256),
+    (128, 1, 4, 128), (129, 1, 4, 128), (1024, 1, 33, 192), (2048, 1, 32, 256), (3000, 1, 4, 192),
+    (256, 2, 4, 512), (512, 2, 4, 512), (513, 2, 4, 256), (4096, 3, 32, 256), (2176, 1, 1, 128),
     (4097, 1, 32, 320), (5000, 3, 32, 320), (2**17, 3, 32, 2**13), (10**6, 9, 48, 93760),
     (2**31 - 1, 1, 1, 2**22)])
 def test_prefill_workspace(tokens, sequences, heads, segment):
     """Two states and a decay for each segment of a head but the first: a segment has a 512th of all
-    heads' tokens in whole chunks of 64, at least 256 (several sequences of 512 in all are whole),
-    so that it is 64 MiB and little more at the most."""
+    heads' tokens in whole chunks of 64, at least 256 (several sequences of 512 in all are whole,
+    one alone may have segments of 128), so that it is 64 MiB and little more at the most."""
     got = _lib.load().ld_linear_prefill_workspace_bytes(tokens, sequences, heads)
     assert got == (tokens - 1) // segment * heads * (2 * DIM * DIM + 4) * 4
     assert got <= 512 * (2 * DIM * DIM + 4) * 4
@@ -329,4 +330,5 @@ def test_prefill_workspace(tokens, sequences, heads, segment):
 
 def test_prefill_workspace_of_nothing():
     call = _lib.load().ld_linear_prefill_workspace_bytes
-    assert [call(*a) for a in [(0, 1, 4), (-1, 1, 4), (10, 0, 4), (10, 1, 0), (256, 1, 4)]] == [0] * 5
+    assert [call(*a) for a in [(0, 1, 4), (-1, 1, 4), (10, 0, 4), (10, 1, 0), (128, 1, 4),
+                                 (2**31, 1, 4)]] == [0] * 6
