@@ -26,7 +26,7 @@
 //
 // Bound by issue, with memory close behind.  32 prompts of 1024 tokens, 32 v-heads and a norm: 303 to
 // 340 us as clock and power allow (290 without the norm; their bytes at a large copy's rate, 236), in
-// which two waves a SIMD keep the vector unit busy 43% and the matrix cores 38% of the time, mostly by
+// which two waves a SIMD keep the vector unit busy 42% and the matrix cores 38% of the time, mostly by
 // turns: two workgroups a CU finish a chunk each in 8.3 us, one alone in 5.1.  512 prompts of 8 to 56
 // tokens: 415 to 450 us of 394, states read and written at 4.9 TB/s.  Hence the layout: operands that
 // stay in registers, remainders by matrix products, no branch around a load, four waves of 32 columns
@@ -36,7 +36,7 @@
 // associative: one launch reduces every segment but a sequence's last to the state after it from zeros
 // and its decay, a second (where there are many) joins these along each sequence, a third walks all
 // segments from the joined states, and the sequences of one segment.  One prompt of 4096 tokens and
-// 32 heads, 16 segments: 23 and 57 us (walked in one piece by 32 workgroups, 64 chunks' chain alone
+// 32 heads, 16 segments: 23 and 55 us (walked in one piece by 32 workgroups, 64 chunks' chain alone
 // would be 330).
 #include <algorithm>
 #include <cstddef>
