@@ -16,6 +16,7 @@
 
 #include <atomic>
 #include <cmath>
+#include <limits>
 #include <optional>
 
 #include "lightdelta_hip.h"
@@ -422,7 +423,7 @@ std::pair<int64_t, int64_t> check_linear(const at::Tensor& qkv, const at::Tensor
                     weight->numel() == kDim,
                 "weight must be contiguous CUDA FP32/BF16 [128]");
   }
-  TORCH_CHECK(std::isfinite(scale), "scale must be finite");
+  TORCH_CHECK(std::abs(scale) <= std::numeric_limits<float>::max(), "scale must be finite");
   TORCH_CHECK(eps > 0, "norm epsilon must be positive");
   TORCH_CHECK(state.size(0) <= INT32_MAX && hv <= INT32_MAX / kDim, "state pool too large");
   return {h, hv};

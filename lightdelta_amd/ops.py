@@ -67,7 +67,6 @@ can run without a GPU.
 from __future__ import annotations
 
 import ctypes
-import math
 import os
 from pathlib import Path
 
@@ -585,7 +584,7 @@ def _linear_layout(qkv, log_decay, state, gate, weight, out, scale, eps):
             and weight.numel() == HEAD_DIM,
             "weight must be contiguous CUDA FP32/BF16 [128]",
         )
-    _require(math.isfinite(scale), "scale must be finite")
+    _require(abs(scale) <= torch.finfo(torch.float32).max, "scale must be finite")
     _require(eps > 0, "norm epsilon must be positive")
     return h, hv
 

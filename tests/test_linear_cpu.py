@@ -151,6 +151,7 @@ SHARED = [
     (dict(out=lambda m: torch.zeros(4, 4, DIM, dtype=torch.bfloat16)), "out must be contiguous CUDA"),
     (dict(weight=lambda m: torch.zeros(DIM)), "weight must be contiguous CUDA"),
     (dict(scale=lambda m: float("nan")), "scale must be finite"),
+    (dict(scale=lambda m: 1e39), "scale must be finite"),
     (dict(eps=lambda m: 0.0), "epsilon must be positive"),
 ]
 DECODE_ONLY = [
