@@ -11,18 +11,19 @@
 // 8 u + 7, split into bf16 planes, are directly the operand of step u of the next product; keys
 // are in an order in which a step takes 16 consecutive bytes of a q row, step u of a sum over
 // tokens takes token 16 u + 8 (e / 4) + 4 hi + e % 4.
-//   P = (K Q^T) . D    32 x 32 blocks over the waves, two planes, exchanged through LDS
-//   O^T = S Q^T        S as two planes
+//   O^T = S Q^T        S as three planes
+//   P = (K Q^T) . D    32 x 32 blocks over the waves, three planes, exchanged through LDS
 //   O^T = O^T diag(e^c) + V^T P^T
 //   S' = e^(c_63) S + K^T (e^(c_63 - c) V)    e V as three planes
 // O crosses LDS in fp32, in the place of v, to whole rows, whose norm and 16-byte stores run
 // beside the next chunk's first products.  The transposed operands come by ds_read_b64_tr_b16.
 //
 // Decays come from differences of 64-bit prefix sums: their error over thousands of tokens would
-// be the state's.  Roundings to fewer than 32 bits, each of operands of the bf16 matrix cores
-// whose sums are fp32: the state's update takes its operand exactly (three planes hold fp32's 24
-// bits), what only reaches bf16 outputs takes two planes (relative error 2^-17 a term, against
-// 2^-9 of the output's own rounding).
+// be the state's.  Operands of the bf16 matrix cores, whose sums are fp32, are taken exactly: three
+// planes hold fp32's 24 bits.  (Two planes of S and P, 16 bits, leave the outputs' error what bf16's
+// rounding, up to 2^-8 of a value, makes it, but round one output in 500 to the other neighbour,
+// against one in 9,000; 32 prompts of 1024 tokens then take 328 us, with three of S alone 359, with
+// three of both 370.)
 //
 // Bound by issue, with memory close behind.  32 prompts of 1024 tokens, 32 v-heads and a norm: 303 to
 // 340 us as clock and power allow (290 without the norm; their bytes at a large copy's rate, 236), in
@@ -68,7 +69,7 @@ struct SegmentLds {
   alignas(16) uint8_t q[kRowsBytes];
   // v; behind it, in its place and another 16 KiB, the chunk's O in fp32
   alignas(16) uint8_t v[kTokens * kDim * 4];
-  // the two planes of P: 32 rows of 32 columns, 32 of 64
+  // two planes of P: 32 rows of 32 columns, 32 of 64; the third is behind v
   alignas(16) uint8_t p[2][kPlaneBytes];
   ChunkScalars scalars[2];
   alignas(16) float weight[kDim];
@@ -483,6 +484,10 @@ __device__ __forceinline__ void walk(const LinearParams& p, SegmentLds& lds, int
   // 2 u + hi; the pieces of a row are XORed with t / 2 % 4 (rows of 32 columns) or t % 8
   uint32_t p_upper = lj * 64 + ((hi ^ ((lj >> 1) & 3)) << 4);                // ^ (u << 5)
   uint32_t p_lower = kPlaneUpper + lj * 128 + ((hi ^ (lj & 7)) << 4);        // ^ (u << 5)
+  // (between the reads of the last chunk's O and the writes of the next the half behind v is free)
+  auto p_plane = [&](int plane) __attribute__((always_inline)) {
+    return plane < 2 ? lds.p[plane] : lds.v + kRowsBytes;
+  };
   // the wave's 32 x 32 block of P (not the one above the diagonal)
   const int p_rows = w == 0 ? 0 : 1;
   const int p_columns = w == 2 ? 1 : 0;
@@ -573,6 +578,54 @@ __device__ __forceinline__ void walk(const LinearParams& p, SegmentLds& lds, int
     f32x16 o[2];
     const __amdgpu_buffer_rsrc_t next_rows = source(c + 1);
     if constexpr (Gated) load_gate(c - 1);
+    // ---- O^T = S Q^T: 32 keys at a time, S as three planes; an operand is read again once all
+    // of its products are out ----
+    bf16x8 q[2][2];
+    auto read_q = [&](int T, int u) __attribute__((always_inline)) {
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+        q[u][tt] = *reinterpret_cast<const bf16x8*>(lds.q + 32 * tt * kTileRow +
+                                                    (a_at ^ ((2 * T + u) << 5)));
+    };
+#pragma unroll
+    for (int u = 0; u < 2; ++u) read_q(0, u);
+#pragma unroll
+    for (int T = 0; T < 4; ++T) {
+      const bf16x8 high[2] = {plane_of(st[T], 0), plane_of(st[T], 1)};
+      f32x16 rest = less(st[T], high[0], high[1]);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        fetch(next_rows, c + 1, 2 * T + u);
+        in_order();
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+          o[tt] = mfma32(high[u], q[u][tt], T == 0 && u == 0 ? f32x16{} : o[tt]);
+        in_order();
+      }
+      const bf16x8 middle[2] = {plane_of(rest, 0), plane_of(rest, 1)};
+      rest = less(rest, middle[0], middle[1]);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) o[tt] = mfma32(middle[u], q[u][tt], o[tt]);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const bf16x8 low = plane_of(rest, u);
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) o[tt] = mfma32(low, q[u][tt], o[tt]);
+        in_order();
+        if (T < 3) read_q(T + 1, u);
+        in_order();
+      }
+    }
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt) o[tt] *= s.eq[32 * tt + lj];
+    finish(c - 1);
+    lds_barrier();   // O of the last chunk is read
+    put(lds.v, staged.v);
+    const float gamma = s.gamma;
+#pragma unroll
+    for (int T = 0; T < 4; ++T) st[T] *= gamma;
     // ---- P ----
     if (w != kScalarWave) {
       f32x16 x = {};
@@ -596,63 +649,24 @@ __device__ __forceinline__ void walk(const LinearParams& p, SegmentLds& lds, int
       auto put_plane = [&](int plane, const bf16x8 (&half)[2]) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-          *reinterpret_cast<bf16x8*>(lds.p[plane] + ((p_rows == 0 ? p_upper : p_lower) ^
-                                                     ((2 * p_columns + u) << 5))) = half[u];
+          *reinterpret_cast<bf16x8*>(p_plane(plane) + ((p_rows == 0 ? p_upper : p_lower) ^
+                                                       ((2 * p_columns + u) << 5))) = half[u];
       };
       const bf16x8 high[2] = {plane_of(x, 0), plane_of(x, 1)};
       put_plane(0, high);
       x = less(x, high[0], high[1]);
+      const bf16x8 middle[2] = {plane_of(x, 0), plane_of(x, 1)};
+      put_plane(1, middle);
+      x = less(x, middle[0], middle[1]);
       const bf16x8 low[2] = {plane_of(x, 0), plane_of(x, 1)};
-      put_plane(1, low);
+      put_plane(2, low);
     }
-    // ---- O^T = S Q^T: 32 keys at a time, S as two planes; an operand is read again once both
-    // of its products are out ----
-    bf16x8 q[2][2];
-    auto read_q = [&](int T, int u) __attribute__((always_inline)) {
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-        q[u][tt] = *reinterpret_cast<const bf16x8*>(lds.q + 32 * tt * kTileRow +
-                                                    (a_at ^ ((2 * T + u) << 5)));
-    };
-#pragma unroll
-    for (int u = 0; u < 2; ++u) read_q(0, u);
-#pragma unroll
-    for (int T = 0; T < 4; ++T) {
-      const bf16x8 high[2] = {plane_of(st[T], 0), plane_of(st[T], 1)};
-      const f32x16 rest = less(st[T], high[0], high[1]);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        fetch(next_rows, c + 1, 2 * T + u);
-        in_order();
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-          o[tt] = mfma32(high[u], q[u][tt], T == 0 && u == 0 ? f32x16{} : o[tt]);
-        in_order();
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const bf16x8 low = plane_of(rest, u);
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt) o[tt] = mfma32(low, q[u][tt], o[tt]);
-        in_order();
-        if (T < 3) read_q(T + 1, u);
-        in_order();
-      }
-    }
-#pragma unroll
-    for (int tt = 0; tt < 2; ++tt) o[tt] *= s.eq[32 * tt + lj];
-    finish(c - 1);
-    lds_barrier();   // O of the last chunk is read
-    put(lds.v, staged.v);
-    const float gamma = s.gamma;
-#pragma unroll
-    for (int T = 0; T < 4; ++T) st[T] *= gamma;
     if (w == kScalarWave) chunk_scalars(lds.scalars[(c + 1) & 1], next_g, p.scale, lane);
     next_g = load_decay(c + 2);
-    lds_barrier();   // v is in LDS (and P)
+    lds_barrier();   // v and P are in LDS
 
     auto p_operand = [&](int u, int tt, int plane) __attribute__((always_inline)) {
-      return *reinterpret_cast<const bf16x8*>(lds.p[plane] + ((tt == 0 ? p_upper : p_lower) ^ (u << 5)));
+      return *reinterpret_cast<const bf16x8*>(p_plane(plane) + ((tt == 0 ? p_upper : p_lower) ^ (u << 5)));
     };
     // ---- O^T += V^T P^T and S += K^T (e V): 32 tokens at a time, operands read a product ahead ----
 #pragma unroll
@@ -666,14 +680,14 @@ __device__ __forceinline__ void walk(const LinearParams& p, SegmentLds& lds, int
       };
       // O's products, between the steps of the split
       auto outputs = [&](int u) __attribute__((always_inline)) {
-        bf16x8 ps[2][2];
+        bf16x8 ps[2][3];
 #pragma unroll
         for (int tt = i; tt < 2; ++tt)
 #pragma unroll
-          for (int plane = 0; plane < 2; ++plane) ps[tt][plane] = p_operand(2 * i + u, tt, plane);
+          for (int plane = 0; plane < 3; ++plane) ps[tt][plane] = p_operand(2 * i + u, tt, plane);
         in_order();
 #pragma unroll
-        for (int plane = 1; plane >= 0; --plane)
+        for (int plane = 2; plane >= 0; --plane)
 #pragma unroll
           for (int tt = i; tt < 2; ++tt) o[tt] = mfma32(v[u], ps[tt][plane], o[tt]);
       };

@@ -9,9 +9,8 @@ same recurrence over absolute values (what a term's rounding is relative to):
   state   A * (n + 64) * 2^-22: an entry's term is decayed over up to n tokens, each decay within
           2^-22 (an exponential's and a product's rounding), and is one of up to 128 summed terms
           of a chunk or an update, a few roundings of 2^-24 each
-  o       A * (n + 64) * 2^-22 + A * 2^-14: the state's, and sums over 128 keys and 64 tokens
-          (192 * 2^-24), operands held as two bf16 planes (2^-17 each of S, the scores and both
-          decays)
+  o       A * (n + 64) * 2^-22 + A * 2^-16: the state's, and sums over 128 keys and 64 tokens
+          (192 * 2^-24)
   out     half a bf16 step (2^-8 of the value), and what o's bound comes to behind the norm:
           its own element's, and through the root mean square at most the row's
 """
@@ -59,7 +58,7 @@ def _finish(o, o_bound, gate, weight, eps):
 
 def _bounds(n, magnitude, state):
     held = (n + 64) * 2.0**-22
-    return magnitude * (held + 2.0**-14), state[1] * held
+    return magnitude * (held + 2.0**-16), state[1] * held
 
 
 def expected_linear_decode(qkv, log_decay, indices, cu, accepted, pool, gate, weight, out, scale,
