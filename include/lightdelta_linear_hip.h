@@ -41,8 +41,7 @@ extern "C" {
  *   out        bf16 [tokens, HV, 128] contiguous
  * out and state overlap no other argument, nor do two slots or two rows of out.
  * A slot outside 1 .. num_slots - 1 is padding: never read, never written.  Non-finite values of
- * a request's activations reach outputs and state of that request alone (in a prompt also outputs
- * of up to 63 tokens ahead of the value's).
+ * a token's activations reach that token's and later outputs, and the state, of its request alone.
  */
 
 /*

@@ -73,6 +73,7 @@ struct SegmentLds {
   alignas(16) uint8_t p[2][kPlaneBytes];
   ChunkScalars scalars[2];
   alignas(16) float weight[kDim];
+  int nonfinite[kDim];   // per column, where a wave says so, the chunk's first v that is not finite
 };
 struct SearchLds {
   int wave_sums[kBlockWaves];
@@ -276,6 +277,28 @@ __device__ __forceinline__ f32x16 decayed(const bf16x8 (&v)[2], const float* ek,
     for (int r = 0; r < 4; ++r) x[4 * q + r] = static_cast<float>(v[q >> 1][4 * (q & 1) + r]) * e[r];
   }
   return x;
+}
+
+// A v that is not finite must not meet the outputs ahead of it in a product, whose scores with it
+// are zeros: it becomes a zero in `v`, a lane's operands of the 32 tokens from `first`.  Returns the
+// first such token of the lane's column, kTokens without one.
+__device__ __forceinline__ int take_nonfinite(bf16x8 (&v)[2], int first, int hi) {
+  int from = kTokens;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    u32x4 x = __builtin_bit_cast(u32x4, v[u]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t exponent = e & 1 ? 0x7f800000u : 0x7f80u;
+      if ((x[e >> 1] & exponent) == exponent) {
+        from = min(from, first + 16 * u + 8 * (e >> 2) + 4 * hi + (e & 3));
+        x[e >> 1] &= e & 1 ? 0xffffu : 0xffff0000u;
+      }
+      __builtin_amdgcn_sched_barrier(0);   // (one at a time: the path is rare, registers are not)
+    }
+    v[u] = __builtin_bit_cast(bf16x8, x);
+  }
+  return min(from, __shfl_xor(from, 32));
 }
 
 // A segment of `rows` rows (whole chunks) from row `bos`, reduced to the state after it, from the
@@ -668,10 +691,11 @@ __device__ __forceinline__ void walk(const LinearParams& p, SegmentLds& lds, int
     auto p_operand = [&](int u, int tt, int plane) __attribute__((always_inline)) {
       return *reinterpret_cast<const bf16x8*>(p_plane(plane) + ((tt == 0 ? p_upper : p_lower) ^ (u << 5)));
     };
+    bool nonfinite = false;   // a v of the wave's columns is not finite
     // ---- O^T += V^T P^T and S += K^T (e V): 32 tokens at a time, operands read a product ahead ----
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const bf16x8 v[2] = {v_operand(lds.v, vt_at, 2 * i), v_operand(lds.v, vt_at, 2 * i + 1)};
+      bf16x8 v[2] = {v_operand(lds.v, vt_at, 2 * i), v_operand(lds.v, vt_at, 2 * i + 1)};
       f32x16 x = decayed(v, s.ek, 32 * i, hi);
       bf16x8 planes[3][2];
       auto set_planes = [&](int n) __attribute__((always_inline)) {
@@ -693,8 +717,16 @@ __device__ __forceinline__ void walk(const LinearParams& p, SegmentLds& lds, int
       };
       set_planes(0);
       x = less(x, planes[0][0], planes[0][1]);
-      outputs(0);
       set_planes(1);
+      // A v that is not finite, times the zeros of `less`, has made its whole column of x NaN.
+      // (32 prompts of 1024 tokens: 375 us; asked right behind `less`, which has to end first, 378;
+      // without 369.)
+      if (__builtin_expect(__any(x[0] != x[0]), 0)) {
+        int* const from = &lds.nonfinite[32 * w + lj];
+        *from = min(nonfinite ? *from : kTokens, take_nonfinite(v, 32 * i, hi));
+        nonfinite = true;
+      }
+      outputs(0);
       x = less(x, planes[1][0], planes[1][1]);
       outputs(1);
       set_planes(2);
@@ -723,6 +755,11 @@ __device__ __forceinline__ void walk(const LinearParams& p, SegmentLds& lds, int
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         *reinterpret_cast<f32x4*>(o_rows + (o_put ^ (8 * q)) + 32 * tt * kDim) = quad(o[tt], q);
+    if (__builtin_expect(nonfinite, 0)) {   // the outputs behind it are NaN
+      lds_order();
+      for (int t = lds.nonfinite[32 * w + lj]; t < kTokens; ++t)
+        o_rows[t * kDim + (((8 * w + (lj >> 2)) ^ (t & 7)) << 2) + (lj & 3)] = __builtin_nanf("");
+    }
     put(lds.k, staged.k);
     put(lds.q, staged.q);
   }

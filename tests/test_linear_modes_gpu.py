@@ -1,4 +1,5 @@
-"""linear_prefill where a mode or a value is what matters: outputs whose every bit is known."""
+"""linear_prefill where a mode or a value is what matters: outputs whose every bit is known, values
+that are not finite."""
 
 from __future__ import annotations
 
@@ -69,3 +70,50 @@ def test_prefill_reads_every_bit_of_the_scores(gpu, lengths, scale):
     run_prefill(case, scale=scale)
     torch.cuda.synchronize()
     assert torch.equal(case["out"], (v[source] * scale).bfloat16().to(gpu))
+
+
+@pytest.mark.parametrize("lengths,token", [([130], t) for t in (0, 17, 31, 32, 45, 63, 64, 100, 129)] +
+                         [([700, 20], t) for t in (100, 128, 383, 390, 699)])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_prefill_nonfinite_v_goes_forward(gpu, lengths, token, gated, value):
+    """One v that is not finite: its column of the outputs from its token on (every column where
+    they are normed), its row of the state, and nothing else."""
+    announce(test="linear_prefill_nonfinite_v", lengths=lengths, token=token, gated=gated, value=value)
+    clean = prefill_case(lengths, 1, 2, seed=21, device=gpu, gated=gated)
+    case = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in clean.items()}
+    case["qkv"][token, 2 * DIM + 77] = value
+    run_prefill(clean)
+    run_prefill(case)
+    torch.cuda.synchronize()
+    bad = torch.zeros_like(clean["out"], dtype=torch.bool)
+    bad[token:lengths[0], 0, slice(None) if gated else 77] = True
+    assert not torch.isfinite(case["out"][bad]).any()
+    assert torch.equal(case["out"][~bad], clean["out"][~bad])
+    bad = torch.zeros_like(clean["pool"], dtype=torch.bool)
+    bad[int(clean["slots"][0]), 0, 77] = True
+    assert not torch.isfinite(case["pool"][bad]).any()
+    assert torch.equal(case["pool"][~bad], clean["pool"][~bad])
+
+
+@pytest.mark.parametrize("column", [5, DIM + 5, 2 * DIM + 5], ids=["q", "k", "v"])
+@pytest.mark.parametrize("tokens", [[20], [40, 50, 41], [3, 3, 70, 129]])
+def test_prefill_nonfinite_rows_go_forward(gpu, column, tokens):
+    """Several of them in one column, and in all heads at once: earlier tokens keep their bits, and
+    behind a q all but its own do."""
+    announce(test="linear_prefill_nonfinite_rows", column=column, tokens=tokens)
+    clean = prefill_case([130], 1, 2, seed=22, device=gpu, gated=False)
+    case = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in clean.items()}
+    for i, token in enumerate(tokens):
+        case["qkv"][token, column] = float("-inf" if i % 2 else "nan")
+    run_prefill(clean)
+    run_prefill(case)
+    torch.cuda.synchronize()
+    keep = torch.ones(130, dtype=torch.bool, device=gpu)
+    if column < DIM:
+        keep[tokens] = False
+        assert torch.equal(case["pool"], clean["pool"])
+    else:
+        keep[min(tokens):] = False
+    assert torch.equal(case["out"][keep], clean["out"][keep])
+    assert not torch.isfinite(case["out"][~keep][:, 0, 5]).any()
