@@ -1,12 +1,12 @@
 """linear_prefill where a mode or a value is what matters: outputs whose every bit is known, values
-that are not finite."""
+that are not finite, and every mode of a call on sequences that are cut into segments."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
-from tests.test_linear_gpu import DIM, announce, prefill_case, run_prefill
+from tests.test_linear_gpu import DIM, announce, check_prefill, prefill_case, run_prefill
 
 pytestmark = pytest.mark.gpu
 
@@ -117,3 +117,81 @@ def test_prefill_nonfinite_rows_go_forward(gpu, column, tokens):
         keep[min(tokens):] = False
     assert torch.equal(case["out"][keep], clean["out"][keep])
     assert not torch.isfinite(case["out"][~keep][:, 0, 5]).any()
+
+
+# ---- segments ------------------------------------------------------------------------------
+
+# Of these the first prompts are cut: into 11 segments of 128 tokens, 6 of 256 (and the last prompt
+# into two of 192), 18 of 256 behind a join.
+CUT = [([1300], (1, 2)), ([1300, 3, 257], (1, 2)), ([4400], (1, 1))]
+
+
+def odd_rows(x, device):
+    """The same rows at odd elements of wider ones."""
+    flat = x.flatten(1)
+    wide = torch.zeros(flat.shape[0], flat.shape[1] + 7, dtype=x.dtype, device=device)
+    wide[:, 3:-4] = flat
+    return wide[:, 3:-4].unflatten(1, x.shape[1:]) if x.dim() == 3 else wide[:, 3:-4]
+
+
+def cut_case(lengths, heads, device, **kw):
+    case = prefill_case(lengths, *heads, seed=31, device=device, decay=0.05, **kw)
+    case["has_initial"][0] = True
+    return case
+
+
+@pytest.mark.parametrize("lengths,heads", CUT)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("odd", [False, True])
+def test_cut_prompts_layouts(gpu, lengths, heads, gated, odd):
+    """With and without the norm, one constant decay a head, bf16 weight, rows at odd elements."""
+    announce(test="linear_prefill_cut_layouts", lengths=lengths, gated=gated, odd=odd)
+    case = cut_case(lengths, heads, gpu, gated=gated, per_token=False, weight_dtype=torch.bfloat16)
+    if odd:
+        case["qkv"] = odd_rows(case["qkv"], gpu)
+        if gated:
+            case["gate"] = odd_rows(case["gate"], gpu)
+    check_prefill(case, eps=1e-3, scale=0.3)
+
+
+@pytest.mark.parametrize("lengths,heads", CUT)
+@pytest.mark.parametrize("slot", [0, -1, 5])
+def test_cut_prompts_padding_and_outside_rows(gpu, lengths, heads, slot):
+    """A cut prompt whose slot is padding; rows that are not finite ahead of and behind all."""
+    announce(test="linear_prefill_cut_padding", lengths=lengths, slot=slot)
+    case = cut_case(lengths, heads, gpu, front=7, behind=70)
+    case["slots"][0] = slot if slot < 1 else case["pool"].shape[0]
+    case["qkv"][:7] = float("nan")
+    case["qkv"][-70:] = float("-inf")
+    case["gate"][-70:] = float("nan")
+    case["log_decay"][:7] = float("nan")
+    case["log_decay"][-70:] = float("nan")
+    check_prefill(case)
+    assert (case["out"][:7] == 7).all() and (case["out"][-70:] == 7).all()
+
+
+@pytest.mark.parametrize("lengths,heads", CUT)
+@pytest.mark.parametrize("value", [float("-inf"), -200.0])
+@pytest.mark.parametrize("tokens", [[0, 128, 256, 512], [127, 255, 511], [192, 300], [1299]])
+def test_cut_prompts_extreme_decays(gpu, lengths, heads, value, tokens):
+    """Tokens that empty the state: a segment's first, its last, one inside, a prompt's last."""
+    announce(test="linear_prefill_cut_decays", lengths=lengths, value=value, tokens=tokens)
+    case = cut_case(lengths, heads, gpu)
+    case["log_decay"][tokens] = value
+    case["log_decay"][[t - lengths[-1] for t in tokens if t < lengths[-1]]] = value   # (the last prompt's)
+    check_prefill(case)
+
+
+def test_cut_prompt_far_rows(gpu):
+    """One prompt in five segments over rows 16 MiB apart: all but the first start past 2 GiB, the
+    last two past 4 GiB."""
+    announce(test="linear_prefill_cut_far")
+    tokens, apart = 600, 2**23
+    case = cut_case([tokens], (1, 2), gpu)
+    flat = torch.zeros((tokens - 1) * apart + 6 * DIM, dtype=torch.bfloat16, device=gpu)
+    far = flat.as_strided((tokens, 4 * DIM), (apart, 1))
+    gate = flat[4 * DIM:].as_strided((tokens, 2, DIM), (apart, DIM, 1))
+    far.copy_(case["qkv"])
+    gate.copy_(case["gate"])
+    case.update(qkv=far, gate=gate)
+    check_prefill(case)
