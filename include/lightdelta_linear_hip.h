@@ -85,7 +85,8 @@ int ld_linear_decode(const ld_linear_decode_args* args, void* stream);
  * padding and has_initial[n] != 0, else from zeros, and the state after its last token goes to
  * state[slots[n]] (an empty sequence writes its initial state back).  Rows outside every
  * sequence are left as they were.  Slots are distinct.  Row strides of qkv, gate and log_decay are
- * 0 .. 2^23 elements, rows of out likewise (num_v_heads <= 2^16), num_tokens < 2^31.
+ * 0 .. 2^23 elements (of a single row anything), rows of out likewise (num_v_heads <= 2^16),
+ * num_tokens < 2^31.
  */
 typedef struct ld_linear_prefill_args {
   const void* qkv;

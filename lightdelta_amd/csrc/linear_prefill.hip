@@ -1083,9 +1083,9 @@ extern "C" int ld_linear_prefill(const ld_linear_prefill_args* args, void* strea
   if (!a.slots || !a.has_initial || !a.cu_seqlens || !a.state ||
       (a.num_tokens > 0 && (!a.qkv || !a.log_decay || !a.out)))
     return fail(LD_ERR_INVALID_ARGUMENT, "ld_linear_prefill: NULL tensor pointer");
-  if (a.qkv_row_stride < 0 || a.qkv_row_stride > kMaxRow || a.gate_row_stride < 0 ||
-      a.gate_row_stride > kMaxRow || a.log_decay_row_stride < 0 ||
-      a.log_decay_row_stride > kMaxRow || a.num_v_heads > kMaxRow / kDim)
+  if (a.num_tokens <= 1) p.qkv_row = p.gate_row = p.decay_row = 0;   // (the distance to no other row)
+  if (p.qkv_row < 0 || p.qkv_row > kMaxRow || p.gate_row < 0 || p.gate_row > kMaxRow ||
+      p.decay_row < 0 || p.decay_row > kMaxRow || a.num_v_heads > kMaxRow / kDim)
     return fail(LD_ERR_INVALID_ARGUMENT, "qkv, log_decay, gate and out rows must be at most 2^23 elements apart");
   if (a.num_tokens > 0x7fffffff) return fail(LD_ERR_INVALID_ARGUMENT, "too many tokens");
   p.indices = a.slots;

@@ -11,6 +11,22 @@ from tests.test_linear_gpu import DIM, announce, check_prefill, prefill_case, ru
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("has_initial", [False, True])
+def test_prefill_of_one_far_row(gpu, has_initial):
+    """The last tokens of buffers whose rows are further apart than several rows may be: with one
+    row there is no distance to keep."""
+    announce(test="linear_prefill_one_row", has_initial=has_initial)
+    case = prefill_case([1], 1, 2, seed=8, device=gpu)
+    case["has_initial"].fill_(has_initial)
+    for name, rows in (("qkv", 2**14 + 1), ("gate", 2**15 + 1), ("log_decay", 2**22 + 1)):
+        x = case[name]
+        wide = torch.zeros(1, rows, *x.shape[1:], dtype=x.dtype, device=gpu)
+        wide[:, -1] = x
+        case[name] = wide[:, -1]
+        assert case[name].stride(0) > 2**23
+    check_prefill(case)
+
+
 def near_ties(shape, seed, device):
     """fp32 values 1 to 16 units in the last place to either side of the middle between two bf16
     neighbours: 16 bits of them are the middle itself, which rounds to even."""
