@@ -121,6 +121,7 @@ SCHEMAS = {
 }
 
 HEAD_DIM = _lib.HEAD_DIM
+_INT32_MAX = 2**31 - 1
 QK_SCALE = HEAD_DIM**-0.5  # reference csrc/gdn_decode.cu:417
 
 # State cache policy of the decode kernel (never changes results, only which kernel shape and
@@ -586,6 +587,7 @@ def _linear_layout(qkv, log_decay, state, gate, weight, out, scale, eps):
         )
     _require(abs(scale) <= torch.finfo(torch.float32).max, "scale must be finite")
     _require(eps > 0, "norm epsilon must be positive")
+    _require(state.shape[0] <= _INT32_MAX and hv <= _INT32_MAX // HEAD_DIM, "state pool too large")
     return h, hv
 
 
@@ -599,9 +601,14 @@ def check_linear_decode(qkv, log_decay, indices, cu, accepted, state, gate, weig
     _require(indices.dim() == 2 and 1 <= indices.shape[1] <= _lib.MAX_TOKENS,
              "decode/MTP supports 1 through 4 tokens per request")
     requests = indices.shape[0]
-    _require(tuple(cu.shape) == (requests + 1,) and tuple(accepted.shape) == (requests,),
-             "invalid request metadata shapes")
+    _require(tuple(cu.shape) == (requests + 1,) and tuple(accepted.shape) == (requests,)
+             and requests <= _INT32_MAX, "invalid request metadata shapes")
     return heads
+
+
+# Elements between rows, at most, and tokens of ld_linear_prefill (include/lightdelta_linear_hip.h).
+LINEAR_PREFILL_MAX_ROW = 1 << 23
+LINEAR_PREFILL_MAX_TOKENS = _INT32_MAX
 
 
 def check_linear_prefill(qkv, log_decay, slots, has_initial, cu_seqlens, state, gate, weight, out,
@@ -614,8 +621,17 @@ def check_linear_prefill(qkv, log_decay, slots, has_initial, cu_seqlens, state, 
     _require(has_initial.device == qkv.device and has_initial.dtype == torch.bool
              and has_initial.dim() == 1 and has_initial.is_contiguous(),
              "has_initial must be a contiguous CUDA bool vector")
-    _require(cu_seqlens.numel() == slots.numel() + 1 and has_initial.numel() == slots.numel(),
-             "invalid sequence metadata shapes")
+    _require(cu_seqlens.numel() == slots.numel() + 1 and has_initial.numel() == slots.numel()
+             and slots.numel() <= _INT32_MAX, "invalid sequence metadata shapes")
+    if slots.numel() == 0:
+        return heads
+    rows = [x for x in (qkv, gate, log_decay if log_decay.dim() == 2 else None) if x is not None]
+    _require(
+        heads[1] <= LINEAR_PREFILL_MAX_ROW // HEAD_DIM
+        and (qkv.shape[0] <= 1 or all(x.stride(0) <= LINEAR_PREFILL_MAX_ROW for x in rows)),
+        "qkv, log_decay, gate and out rows must be at most 2^23 elements apart",
+    )
+    _require(qkv.shape[0] <= LINEAR_PREFILL_MAX_TOKENS, "too many tokens")
     return heads
 
 
@@ -624,8 +640,8 @@ def check_norm_rope(qkv, q_weight, k_weight, positions, inv_freq, q_heads, k_hea
     """Validation of norm_rope."""
     _require(_is_gpu(qkv) and qkv.dtype == torch.bfloat16, "qkv must be CUDA BF16")
     columns = (q_heads + k_heads) * HEAD_DIM
-    _require(q_heads >= 0 and k_heads >= 0 and qkv.dim() == 2 and qkv.shape[1] >= columns
-             and qkv.stride(1) == 1,
+    _require(q_heads >= 0 and k_heads >= 0 and max(q_heads, k_heads) <= _INT32_MAX // HEAD_DIM
+             and qkv.dim() == 2 and qkv.shape[1] >= columns and qkv.stride(1) == 1,
              "qkv must be [tokens,>=(q_heads+k_heads)*128] with dense rows")
     n = qkv.shape[0]
     _require(n <= 1 or qkv.stride(0) >= columns, "qkv rows must not overlap")
