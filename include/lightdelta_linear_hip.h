@@ -130,11 +130,12 @@ int64_t ld_linear_prefill_workspace_bytes(int64_t num_tokens, int32_t num_sequen
  * first q_heads + k_heads heads of a row of qkv (bf16, row stride qkv_row_stride; later columns
  * are left alone):
  *   y = x * rsqrt(mean(x^2) + eps) * w         (w: q_weight or k_weight [128], weight_dtype)
- *   a = positions[token] * inv_freq[i]         (in 64 bits), i < rotary / 2
+ *   a = positions[token] * inv_freq[i]         i < rotary / 2
  *   halves:      (y[i], y[i + rotary/2])  turned by a
  *   interleaved: (y[2 i], y[2 i + 1])     turned by a
  * and rounded to bf16 once; elements from `rotary` on are only normalised.  positions int32 or
- * int64 [tokens] (any value); inv_freq fp32 [rotary / 2].  rotary <= 128: a multiple of 16
+ * int64 [tokens] (any value: angles are those of the exact product, reduced within 2^-44 of a turn for
+ * |inv_freq| <= 1); inv_freq fp32 [rotary / 2].  rotary <= 128: a multiple of 16
  * (halves) or of 2 (interleaved); 0 for the norm alone.
  */
 typedef struct ld_norm_rope_args {

@@ -6,9 +6,8 @@
 // Bound by memory: 512 bytes a head and token against about 90 vector instructions per 4 heads.
 // A wave takes one token and four heads at a time, 16 lanes a head, 8 consecutive elements (16
 // bytes) a lane, four rounds of loads in flight.  The token's angles are formed once, one a lane,
-// and spread through LDS: the product and its reduction to a fraction of a turn in 64 bits
-// (positions of millions times frequencies near 1 leave 32 bits no fraction), sine and cosine in
-// fp32.  A pair's other element comes from a lane of the same 16 by DPP.
+// and spread through LDS: the product and its reduction to a fraction of a turn in pairs of doubles
+// (turn_fraction), sine and cosine in fp32.  A pair's other element comes from a lane of the same 16 by DPP.
 //
 // 32,768 tokens of 16 + 16 heads: 99 us, 5.4 TB/s (260 with a round at a time, an angle per element and
 // pairs by shuffles); one token of them 2.5 us.  Few tokens are split over waves by rounds, so that a
@@ -46,6 +45,23 @@ struct NormRopeParams {
 // whose number differs in bit D, or (any other half) one that a shuffle names.
 constexpr int kOwn = 0;
 constexpr int kShuffle = -1;
+
+// position * inv_freq / (2 pi) less the nearest whole number, for any position: positions of millions
+// leave 32 bits no fraction, 2^50 none to 64.  1 / (2 pi), and with it a turn a position, is a sum
+// of two doubles, and the position one of its upper and lower 32 bits, so that what a product with
+// the first double rounds off comes back by fma: within 2^-44 of a turn for frequencies up to 1.
+__device__ __forceinline__ double turn_part(double position, double first, double second) {
+  return fma(position, first, -rint(position * first)) + position * second;
+}
+__device__ __forceinline__ float turn_fraction(int64_t position, float inv_freq) {
+  constexpr double kTurn = 0x1.45f306dc9c883p-3, kTurnRest = -0x1.6b01ec5417056p-57;
+  const double first = inv_freq * kTurn;
+  const double second = fma(static_cast<double>(inv_freq), kTurn, -first) + inv_freq * kTurnRest;
+  const double upper = static_cast<double>(static_cast<int32_t>(position >> 32)) * 0x1p32;
+  const double lower = static_cast<double>(static_cast<uint32_t>(position));
+  const double turns = turn_part(upper, first, second) + turn_part(lower, first, second);
+  return static_cast<float>(turns - rint(turns));
+}
 
 template <int D>
 __device__ __forceinline__ float partner(float y, int lane) {
@@ -96,11 +112,9 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(const NormRopeParam
   __shared__ __attribute__((aligned(16))) float angles[kWaves][2][64];
   float* const mine = angles[threadIdx.x >> 6][0];
   if (lane < p.half) {
-    const double position =
-        p.positions64 ? static_cast<double>(static_cast<const int64_t*>(p.positions)[token])
-                      : static_cast<double>(static_cast<const int32_t*>(p.positions)[token]);
-    const double turns = position * static_cast<double>(p.inv_freq[lane]) * 0.15915494309189535;
-    const float fraction = static_cast<float>(turns - rint(turns));
+    const int64_t position = p.positions64 ? static_cast<const int64_t*>(p.positions)[token]
+                                           : static_cast<const int32_t*>(p.positions)[token];
+    const float fraction = turn_fraction(position, p.inv_freq[lane]);
     mine[lane] = __builtin_amdgcn_cosf(fraction);
     mine[64 + lane] = __builtin_amdgcn_sinf(fraction);
   }

@@ -115,6 +115,32 @@ def expected_linear_prefill(qkv, log_decay, slots, has_initial, cu_seqlens, pool
     return out, out_bound, new_pool, pool_bound
 
 
+def exact_angles(positions, inv_freq):
+    """positions x inv_freq.  From 2^29 on a product with an fp32 frequency has more than a double's
+    53 bits: there by whole numbers, in units of 2^-320, less the whole turns."""
+    if positions.numel() == 0 or -(2**29) < int(positions.min()) <= int(positions.max()) < 2**29:
+        return positions.double()[:, None] * inv_freq.double()
+    unit = 1 << 320
+
+    def arctan(n):   # of 1 / n
+        term = total = unit // n
+        k = 1
+        while term:
+            term //= -n * n
+            k += 2
+            total += term // k
+        return total
+
+    turn = 8 * (4 * arctan(5) - arctan(239))
+    angles = []
+    for position in positions.tolist():
+        for frequency in inv_freq.tolist():
+            above, below = frequency.as_integer_ratio()
+            angles.append(position * above * unit // below % turn / unit)
+    return torch.tensor(angles, dtype=torch.float64, device=positions.device).view(
+        len(positions), -1)
+
+
 def expected_norm_rope(qkv, q_weight, k_weight, positions, inv_freq, q_heads, k_heads, eps,
                        interleaved):
     """(qkv, bound) of norm_rope.  The bound: half a bf16 step, and 2^-18 of the normalised pair
@@ -122,7 +148,7 @@ def expected_norm_rope(qkv, q_weight, k_weight, positions, inv_freq, q_heads, k_
     result = qkv.double()
     bound = torch.zeros_like(result)
     half = inv_freq.numel()
-    angle = positions.double()[:, None] * inv_freq.double()
+    angle = exact_angles(positions, inv_freq)
     cos, sin = angle.cos(), angle.sin()
     lower = torch.arange(half, device=qkv.device) * (2 if interleaved else 1)
     upper = lower + (1 if interleaved else half)
