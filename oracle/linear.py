@@ -143,8 +143,9 @@ def exact_angles(positions, inv_freq):
 
 def expected_norm_rope(qkv, q_weight, k_weight, positions, inv_freq, q_heads, k_heads, eps,
                        interleaved):
-    """(qkv, bound) of norm_rope.  The bound: half a bf16 step, and 2^-18 of the normalised pair
-    (sine and cosine within 2^-20 of a turn's unit circle, fp32 norm and products)."""
+    """(qkv, bound) of norm_rope.  The bound: half a bf16 step, and 2^-20 of the normalised pair
+    (2^-23.3 for an angle that is an fp32 fraction of a turn, below 2^-22 each for its sine and
+    cosine, and for the norm's root and the products)."""
     result = qkv.double()
     bound = torch.zeros_like(result)
     half = inv_freq.numel()
@@ -165,5 +166,5 @@ def expected_norm_rope(qkv, q_weight, k_weight, positions, inv_freq, q_heads, k_
         size[:, lower] = pair
         size[:, upper] = pair
         result[:, columns] = z
-        bound[:, columns] = z.abs() * 2.0**-8 + size * 2.0**-18 + 1e-30
+        bound[:, columns] = z.abs() * 2.0**-8 + size * 2.0**-20 + 1e-30
     return result, bound

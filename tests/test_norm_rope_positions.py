@@ -1,12 +1,13 @@
-"""norm_rope's angles at any position: int64 ones far past what a double's product holds."""
+"""norm_rope's angles at any position, int64 ones far past what a double's product holds, and their
+sines and cosines."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
-from oracle.linear import exact_angles
-from tests.test_linear_gpu import check_rope, rope_case
+from oracle.linear import exact_angles, expected_norm_rope
+from tests.test_linear_gpu import EPS, check_rope, rope_case, within
 
 FAR = [2**31 - 1, -(2**31), 2**32, 2**35 + 3, 2**40 + 12345, -(2**45) - 1, 2**53 + 1,
        2**62 + 987654321, 2**63 - 1, -(2**63)]
@@ -51,3 +52,22 @@ def test_far_positions_int32(gpu):
     case = rope_case(400, 1, 1, 64, seed=8, device=gpu, far=2**31 - 1)
     case["positions"][::2] *= -1
     check_rope(dict(case, positions=case["positions"].int()), True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("zeros", ["first", "second"])
+def test_small_sines_and_cosines(gpu, zeros):
+    """Where one element of a pair is 0 the other's sine or cosine alone is what an output holds, and
+    a small one shows its error: that of an fp32 fraction of a turn (2^-26 of one, 2^-23.3 of the
+    element), and some roundings of the value itself, far below bf16's."""
+    case = rope_case(32768, 1, 1, 128, seed=9, device=gpu, extra=0, far=2**20)
+    x = case["qkv"].view(-1, 2, 2, 64)
+    x.copy_(torch.where(x < 0, -1.0, 1.0))
+    x[:, :, 0 if zeros == "first" else 1] = 0
+    case["q_weight"].fill_(1.0)
+    case["k_weight"].fill_(1.0)
+    want, _ = expected_norm_rope(*case.values(), EPS, False)
+    torch.ops.lightdelta.norm_rope(*case.values(), EPS, False)
+    torch.cuda.synchronize()
+    assert (want.abs() < 2.0**-13).sum() > 100
+    within(case["qkv"], want, want.abs() * (2.0**-8 + 2.0**-20) + 2**0.5 * 2.0**-23, "qkv")
