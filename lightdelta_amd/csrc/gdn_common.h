@@ -89,6 +89,19 @@ __device__ __forceinline__ void buffer_store16(f32x4 v, __amdgpu_buffer_rsrc_t r
   __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, offset, 0, Pol);
 }
 
+// ---- LDS of a wave and of a workgroup --------------------------------------------------------
+
+// Keeps the compiler from moving LDS accesses across this point: values written as 16-byte pieces
+// and read back as 2-byte columns (or the reverse) type-based alias analysis would otherwise let it
+// reorder.  The hardware runs a wave's LDS operations in program order, so no wait is needed.
+__device__ __forceinline__ void lds_order() { asm volatile("" ::: "memory"); }
+
+// Waits for this wave's LDS traffic, then joins the workgroup barrier.  Global loads that
+// are still in flight stay in flight (a __syncthreads() fence would drain them).
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 __device__ __forceinline__ float load_param(const void* p, int i, bool bf16) {
   return bf16 ? bf16_to_f32(static_cast<const uint16_t*>(p)[i])
               : static_cast<const float*>(p)[i];

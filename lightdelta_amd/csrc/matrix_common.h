@@ -88,14 +88,6 @@ __device__ __forceinline__ bf16x4 read_tr(const uint8_t* at) {
   return __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
 }
 
-__device__ __forceinline__ void lds_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-
-// Keeps LDS accesses of a wave in program order past the compiler (the hardware runs them in
-// order).
-__device__ __forceinline__ void lds_order() { asm volatile("" ::: "memory"); }
-
 // Sixteen bytes of a row at a lane's byte offset + a uniform one: one load, or (rows not at
 // 16-byte boundaries) eight of one element.
 template <bool Wide>
