@@ -438,7 +438,7 @@ __device__ __forceinline__ void walk(const LinearParams& p, SegmentLds& lds, int
   const int srow = tid >> 4;
   const int spiece = tid & 15;
   const uint32_t row_bytes = static_cast<uint32_t>(p.qkv_row) * 2;
-  const uint32_t lane_row = srow * row_bytes + spiece * 16;
+  uint32_t lane_row = srow * row_bytes + spiece * 16;
   const int q_col = key_head * kTileRow;
   const int k_col = (p.num_k_heads + key_head) * kTileRow;
   const int v_col = (2 * p.num_k_heads + head) * kTileRow;
@@ -458,7 +458,7 @@ __device__ __forceinline__ void walk(const LinearParams& p, SegmentLds& lds, int
   };
   auto fetch = [&](__amdgpu_buffer_rsrc_t rs, int c, int i) __attribute__((always_inline)) {
     const int j = i < 8 ? i >> 1 : i - 8;
-    const uint32_t at = srow + 16 * j < rows - c * kTokens ? lane_row + 16 * j * row_bytes : 0x7ffff000u;
+    const uint32_t at = srow < rows - c * kTokens - 16 * j ? lane_row + 16 * j * row_bytes : 0x7ffff000u;
     if (i >= 8)
       staged.v[j] = load_piece<Wide>(rs, at, v_col);
     else if ((i & 1) == 0)
@@ -590,13 +590,19 @@ __device__ __forceinline__ void walk(const LinearParams& p, SegmentLds& lds, int
   put(lds.q, staged.q);
   for (int c = 0; c < chunks; ++c) {
     const ChunkScalars& s = lds.scalars[c & 1];
-    // (opaque here, so that their XORed forms are made where they are used, not held in registers
-    // over the loop)
+    // (opaque here, so that what follows from them is made where it is used, not held in registers
+    // over the loop: spilled, it came back with a wait for every load ahead of it, 376 us of 32
+    // prompts of 1024 tokens against 360)
+    pin(lane_row);
     pin(a_at);
     pin(kt_at);
     pin(p_upper);
     pin(p_lower);
     pin(o_put);
+    int here = lane;
+    pin(here);
+    const int lj = here & 31;
+    const int hi = here >> 5;
     lds_barrier();   // k, q and scalars of the chunk are in LDS, O of the last
     f32x16 o[2];
     const __amdgpu_buffer_rsrc_t next_rows = source(c + 1);
