@@ -33,6 +33,7 @@ extern "C" {
  *              column kh*128, k at H*128 + kh*128, v of v-head h at 2*H*128 + h*128
  *   log_decay  fp32, g of (token, head) at token*log_decay_row_stride + head; a row stride of 0
  *              is one constant decay a head.  g <= 0; -inf empties the state
+ *              (of finite values: those that are not stay, as 0 times them is NaN)
  *   state      fp32 [num_slots, HV, 128(V), 128(K)], slot stride state_slot_stride, 16-byte
  *              aligned
  *   gate       bf16 [tokens, HV, 128], row stride gate_row_stride, or NULL with norm_weight

@@ -22,14 +22,14 @@
 // be the state's.  Operands of the bf16 matrix cores, whose sums are fp32, are taken exactly: three
 // planes hold fp32's 24 bits.  (Two planes of S and P, 16 bits, leave the outputs' error what bf16's
 // rounding, up to 2^-8 of a value, makes it, but round one output in 500 to the other neighbour,
-// against one in 9,000; 32 prompts of 1024 tokens then take 328 us, with three of S alone 359, with
-// three of both 370.)
+// against one in 9,000; 32 prompts of 1024 tokens then take 326 us, with three of S alone 355, with
+// three of both 366.)
 //
-// Bound by issue, with memory close behind.  32 prompts of 1024 tokens, 32 v-heads and a norm: 303 to
-// 340 us as clock and power allow (290 without the norm; their bytes at a large copy's rate, 236), in
-// which two waves a SIMD keep the vector unit busy 42% and the matrix cores 38% of the time, mostly by
-// turns: two workgroups a CU finish a chunk each in 8.3 us, one alone in 5.1.  512 prompts of 8 to 56
-// tokens: 415 to 450 us of 394, states read and written at 4.9 TB/s.  Hence the layout: operands that
+// Bound by issue, with memory close behind.  32 prompts of 1024 tokens, 32 v-heads and a norm: 329 to
+// 367 us as clock and power allow (313 to 318 without the norm; their bytes at a large copy's rate,
+// 236), in which two waves a SIMD keep the vector unit busy 43% and the matrix cores 44% of the time,
+// mostly by turns: two workgroups a CU finish a chunk each in 10.7 us, one alone in 5.0.  512 prompts of
+// 8 to 56 tokens: 427 to 433 us of 394, states read and written at 4.7 TB/s.  Hence the layout: operands that
 // stay in registers, remainders by matrix products, no branch around a load, four waves of 32 columns
 // (against eight of 16, which read every K and Q operand twice: 415 us and 332 at one time).
 //
@@ -37,8 +37,8 @@
 // associative: one launch reduces every segment but a sequence's last to the state after it from zeros
 // and its decay, a second (where there are many) joins these along each sequence, a third walks all
 // segments from the joined states, and the sequences of one segment.  One prompt of 4096 tokens and
-// 32 heads, 16 segments: 23 and 55 us (walked in one piece by 32 workgroups, 64 chunks' chain alone
-// would be 330).
+// 32 heads, 16 segments: 23 and 63 us by the kernel trace, 78 to 84 a call in a loop (walked in one
+// piece by 32 workgroups, 64 chunks' chain alone would be 320).
 #include <algorithm>
 #include <cstddef>
 
@@ -725,8 +725,7 @@ __device__ __forceinline__ void walk(const LinearParams& p, SegmentLds& lds, int
       x = less(x, planes[0][0], planes[0][1]);
       set_planes(1);
       // A v that is not finite, times the zeros of `less`, has made its whole column of x NaN.
-      // (32 prompts of 1024 tokens: 375 us; asked right behind `less`, which has to end first, 378;
-      // without 369.)
+      // (4 of the 366 us of 32 prompts of 1024 tokens.)
       if (__builtin_expect(__any(x[0] != x[0]), 0)) {
         int* const from = &lds.nonfinite[32 * w + lj];
         *from = min(nonfinite ? *from : kTokens, take_nonfinite(v, 32 * i, hi));
@@ -860,8 +859,9 @@ struct Segments {
   int later;        // at most this many later segments
   // Each segment sums the states ahead of it by itself, without the second launch: up to kAhead of
   // them, or twice that among several sequences, most of which have far fewer (us, with the second launch and
-  // without: 13 prompts of 1 to 3000 tokens 149 / 136, 16 of 64 to 1024 106 / 92, one of 4096 88 / 83;
-  // one of 8192 with 8 heads, 31 ahead of the last, 55 / 63, of 16384 85 / 130).
+  // without: 13 prompts of 1 to 3000 tokens 140 / 131, 16 of 64 to 1024 107 / 100, one of 4096 80 / 78;
+  // one of 8192 with 8 heads, 31 ahead of the last, 56 / 63, of 16384 85 / 127).  Among several one that
+  // has nearly all of the tokens loses by it, as one alone would (8192 and an empty one 56 / 62).
   bool direct;
   // per (later segment, head): the state after the segment ahead of it, for a sequence's first one
   // from the state that the sequence starts from, for the others from zeros (behind the join: the
@@ -980,8 +980,8 @@ __global__ __launch_bounds__(kBlock) void linear_join_kernel(const LinearParams 
 // segment j; item later + j the first segment of its sequence, if j is the sequence's first later
 // one; item 2 later + n sequence n, if it is a single segment (the shortest last).
 // Two workgroups a CU; one where elements are loaded one by one, whose 96 loads in flight take a
-// register each: with the registers of two, 82 of them spilled (32 prompts of 1024 tokens with a norm
-// 1111 us against 791, without 876 against 691).
+// register each: with the registers of two, 49 of them spilled (32 prompts of 1024 tokens with a norm
+// 926 us against 797, without 735 against 682).
 template <bool Wide, bool Gated>
 __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(Wide ? 2 : 1, Wide ? 2 : 1)))
 void linear_walk_kernel(const LinearParams p, const Segments g) {
@@ -1023,12 +1023,12 @@ void linear_walk_kernel(const LinearParams p, const Segments g) {
 }
 
 // A segment's tokens, at most, in whole chunks: the share of a workgroup where 512 run at once (two
-// a CU), and at least 256, as a segment is walked twice.  Rounded to a power of two the share left
-// CUs idle behind one long prompt (32 heads, us: 5000 tokens 117 / 97, 9000 180 / 149, 20000 368 /
-// 300) and gained and lost by turns on mixed ones; 1.14 or 1.33 shares likewise.
+// a CU), and at least 256, as a segment is walked twice.  Rounded to a power of two the share leaves
+// CUs idle (32 heads, us: 5000 tokens 105 / 88, 9000 173 / 147, 20000 375 / 301, 16 prompts of 64 to
+// 1024 119 / 100).
 // One prompt is cut finer, to 128 tokens, while a CU gets one workgroup and a segment has 16 ahead
-// of it (us: 512 tokens of 32 heads 40 / 31, 1024 44 / 37; to 128 in any case 2048 50 / 56, 4096 of 8
-// heads 55 / 62).  Several of 512 tokens in all are left whole: most likely none is long, and a
+// of it (us: 512 tokens of 32 heads 42 / 32, 1024 46 / 37; to 128 in any case 2048 55 against 51, 8192 of
+// 8 heads 62 against 56, though 4096 of those 43 against 53).  Several of 512 tokens in all are left whole: most likely none is long, and a
 // reduction in vain takes 5 us of their 20.
 int64_t segment_tokens(int64_t num_tokens, int32_t num_sequences, int32_t num_v_heads) {
   if (num_sequences > 1 && num_tokens <= 512) return 512;

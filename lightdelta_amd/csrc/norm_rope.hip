@@ -3,13 +3,13 @@
 //   y = x * rsqrt(mean(x^2) + eps) * w ;  pairs of y turned by positions[token] * inv_freq[i]
 // in fp32, rounded to bf16 once.
 //
-// Bound by memory: 512 bytes a head and token against about 90 vector instructions per 4 heads.
+// Bound by memory: 512 bytes a head and token against 164 vector instructions per 4 heads.
 // A wave takes one token and four heads at a time, 16 lanes a head, 8 consecutive elements (16
 // bytes) a lane, four rounds of loads in flight.  The token's angles are formed once, one a lane,
 // and spread through LDS: the product and its reduction to a fraction of a turn in pairs of doubles
 // (turn_fraction), sine and cosine in fp32.  A pair's other element comes from a lane of the same 16 by DPP.
 //
-// 32,768 tokens of 16 + 16 heads: 99 us, 5.4 TB/s (260 with a round at a time, an angle per element and
+// 32,768 tokens of 16 + 16 heads: 101 us, 5.3 TB/s (260 with a round at a time, an angle per element and
 // pairs by shuffles); one token of them 2.5 us.  Few tokens are split over waves by rounds, so that a
 // small launch's latency is one batch's.
 #include <algorithm>

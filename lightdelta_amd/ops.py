@@ -58,8 +58,8 @@ Every kernel launches on the caller's current stream and reads no device memory 
 so it can be captured in a HIP graph.  None allocates, except prefill's chunked form, which
 keeps one workspace per device and stream for later eager calls (release_prefill_workspaces
 frees them) and gives a call under graph capture a workspace the graph keeps, and
-linear_prefill, which takes a long prompt's workspace (64 MiB at most) from torch's allocator
-for the call.  The kernels of every op but prefill are C++ (csrc/torch_ops.cpp,
+linear_prefill, which takes a long prompt's workspace (64 MiB and little more at most) from
+torch's allocator for the call.  The kernels of every op but prefill are C++ (csrc/torch_ops.cpp,
 liblightdelta_torch.so); the check_* functions below restate their argument checks so they
 can run without a GPU.
 """
