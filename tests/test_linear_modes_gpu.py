@@ -135,6 +135,24 @@ def test_prefill_nonfinite_rows_go_forward(gpu, column, tokens):
     assert not torch.isfinite(case["out"][~keep][:, 0, 5]).any()
 
 
+@pytest.mark.parametrize("lengths,token", [([130], 45), ([700], 300)])
+@pytest.mark.parametrize("odd", [False, True])
+def test_prefill_nonfinite_token_goes_forward(gpu, lengths, token, odd):
+    """A token of which nothing is finite, also in rows at odd elements."""
+    announce(test="linear_prefill_nonfinite_token", lengths=lengths, token=token, odd=odd)
+    clean = prefill_case(lengths, 2, 4, seed=23, device=gpu)
+    if odd:
+        clean["qkv"] = odd_rows(clean["qkv"], gpu)
+    case = {k: v.clone() if k in ("pool", "out") else v for k, v in clean.items()}
+    run_prefill(clean)
+    clean["qkv"][token] = float("nan")
+    run_prefill(case)
+    torch.cuda.synchronize()
+    assert torch.equal(case["out"][:token], clean["out"][:token])
+    assert not torch.isfinite(case["out"][token:]).any()
+    assert not torch.isfinite(case["pool"][case["slots"].long()]).any()
+
+
 # ---- segments ------------------------------------------------------------------------------
 
 # Of these the first prompts are cut: into 11 segments of 128 tokens, 6 of 256 (and the last prompt
