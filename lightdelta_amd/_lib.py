@@ -1,5 +1,5 @@
-"""ctypes binding of liblightdelta_hip.so (the C ABI declared in include/lightdelta_hip.h and
-include/lightdelta_linear_hip.h).
+"""ctypes binding of liblightdelta_hip.so (the C ABI declared in include/lightdelta_hip.h,
+include/lightdelta_linear_hip.h and include/lightdelta_attention_hip.h).
 
 torch is imported first on purpose: torch ships its own libamdhip64.so.7, and loading it
 before the library makes the library's `libamdhip64.so.7` dependency resolve to that same
@@ -199,6 +199,69 @@ class NormRopeArgs(ctypes.Structure):
     ]
 
 
+class PagedCache(ctypes.Structure):
+    """Mirror of ld_paged_cache (include/lightdelta_attention_hip.h)."""
+
+    _fields_ = [
+        ("k", _vp),
+        ("v", _vp),
+        ("k_scale", _vp),
+        ("v_scale", _vp),
+        ("k_page_stride", _c_i64),
+        ("v_page_stride", _c_i64),
+        ("k_scale_stride", _c_i64),
+        ("v_scale_stride", _c_i64),
+        ("pages", _vp),
+        ("pages_row_stride", _c_i64),
+        ("cu", _vp),
+        ("lengths", _vp),
+        ("num_tokens", _c_i64),
+        ("table_width", _c_i32),
+        ("num_pages", _c_i32),
+        ("page_size", _c_i32),
+        ("num_kv_heads", _c_i32),
+        ("num_requests", _c_i32),
+    ]
+
+
+class CacheRows(ctypes.Structure):
+    """Mirror of ld_cache_rows (include/lightdelta_attention_hip.h)."""
+
+    _fields_ = [
+        ("k", _vp),
+        ("v", _vp),
+        ("k_row_stride", _c_i64),
+        ("v_row_stride", _c_i64),
+    ]
+
+
+class AttentionArgs(ctypes.Structure):
+    """Mirror of ld_attention_args (include/lightdelta_attention_hip.h)."""
+
+    _fields_ = [
+        ("q", _vp),
+        ("q_row_stride", _c_i64),
+        ("gate", _vp),
+        ("gate_row_stride", _c_i64),
+        ("out", _vp),
+        ("num_q_heads", _c_i32),
+        ("width", _c_i32),
+        ("scale", ctypes.c_float),
+        ("workspace", _vp),
+        ("workspace_bytes", _c_i64),
+    ]
+
+
+class RopeAxes(ctypes.Structure):
+    """Mirror of ld_rope_axes (include/lightdelta_attention_hip.h)."""
+
+    _fields_ = [
+        ("axes", _vp),
+        ("position_axis_stride", _c_i64),
+        ("num_axes", _c_i32),
+    ]
+
+
 PREFILL_AUTO, PREFILL_TOKEN_SERIAL, PREFILL_CHUNKED, PREFILL_CHUNKED_32 = 0, 1, 2, 3
 PREFILL_STATIC_SCRATCH_BYTES = 64 << 20
 
@@ -238,6 +301,21 @@ LINEAR_SIGNATURES = {
     "ld_norm_rope": ([ctypes.POINTER(NormRopeArgs), _vp], ctypes.c_int),
 }
 
+# include/lightdelta_attention_hip.h's.
+_cache = ctypes.POINTER(PagedCache)
+ATTENTION_SIGNATURES = {
+    "ld_cache_write": ([_cache, ctypes.POINTER(CacheRows), _vp], ctypes.c_int),
+    "ld_cache_read": ([_cache, ctypes.POINTER(CacheRows), _vp], ctypes.c_int),
+    "ld_attention_decode": ([_cache, ctypes.POINTER(AttentionArgs), _vp], ctypes.c_int),
+    "ld_attention_prefill": ([_cache, ctypes.POINTER(AttentionArgs), _vp], ctypes.c_int),
+    "ld_attention_decode_workspace_bytes": ([_cache, ctypes.POINTER(AttentionArgs)], _c_i64),
+    "ld_attention_prefill_workspace_bytes": ([_cache, ctypes.POINTER(AttentionArgs)], _c_i64),
+    "ld_norm_rope_axes": (
+        [ctypes.POINTER(NormRopeArgs), ctypes.POINTER(RopeAxes), _vp],
+        ctypes.c_int,
+    ),
+}
+
 _lock = threading.Lock()
 _lib = None
 
@@ -255,7 +333,8 @@ def load() -> ctypes.CDLL:
                     "(hipcc, gfx950) before using the lightdelta ops"
                 )
             lib = ctypes.CDLL(str(LIBRARY_PATH))
-            for name, (argtypes, restype) in {**SIGNATURES, **LINEAR_SIGNATURES}.items():
+            for name, (argtypes, restype) in {**SIGNATURES, **LINEAR_SIGNATURES,
+                                              **ATTENTION_SIGNATURES}.items():
                 fn = getattr(lib, name)
                 fn.argtypes = argtypes
                 fn.restype = restype

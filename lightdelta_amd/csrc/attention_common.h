@@ -1,0 +1,165 @@
+// Definitions shared by the paged 8-bit cache and the attention over it (cache_io.hip,
+// attention_decode.hip, attention_prefill.hip).
+#pragma once
+
+#include "gdn_common.h"
+#include "lightdelta_attention_hip.h"
+
+namespace ld {
+
+constexpr int kScaleLow = -100, kScaleHigh = 119;   // exponents of a scale
+constexpr int kScaleBias = 127;
+
+struct Cache {
+  uint8_t* k;
+  uint8_t* v;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  int64_t k_page, v_page;              // bytes
+  int64_t k_scale_page, v_scale_page;
+  const int32_t* pages;
+  int64_t pages_row;
+  const int32_t* cu;
+  const int32_t* lengths;
+  int64_t num_tokens;
+  int32_t table_width;
+  int32_t num_pages;
+  int32_t page_log2;
+  int32_t kv_heads;
+  int32_t requests;
+};
+
+// The checks and parameters of every entry point; LD_OK, or an error code with its message.
+inline int cache_params(const ld_paged_cache* from, Cache& c) {
+  if (from == nullptr) return fail(LD_ERR_INVALID_ARGUMENT, "cache is NULL");
+  const ld_paged_cache& a = *from;
+  if (a.num_requests < 0 || a.num_tokens < 0 || a.num_pages < 0 || a.table_width < 0)
+    return fail(LD_ERR_INVALID_ARGUMENT,
+                "num_requests, num_tokens, num_pages and table_width must be >= 0");
+  if (a.num_kv_heads <= 0 || a.num_kv_heads > 1 << 16)
+    return fail(LD_ERR_INVALID_ARGUMENT, "num_kv_heads must be 1 through 2^16");
+  if (a.page_size != 16 && a.page_size != 32 && a.page_size != 64 && a.page_size != 128)
+    return fail(LD_ERR_INVALID_ARGUMENT, "page_size must be 16, 32, 64 or 128");
+  if (a.num_tokens >= int64_t{1} << 31)
+    return fail(LD_ERR_INVALID_ARGUMENT, "too many tokens");
+  c = Cache{};
+  if (a.num_requests == 0 || a.num_tokens == 0) return LD_OK;
+  if ((a.num_pages > 0 && (!a.k || !a.v || !a.k_scale || !a.v_scale)) || !a.cu || !a.lengths ||
+      (a.table_width > 0 && !a.pages))
+    return fail(LD_ERR_INVALID_ARGUMENT, "cache: NULL tensor pointer");
+  if (!aligned16(a.k) || !aligned16(a.v) || (a.k_page_stride & 15) != 0 ||
+      (a.v_page_stride & 15) != 0)
+    return fail(LD_ERR_INVALID_ARGUMENT, "cache pages must be 16-byte aligned");
+  c.k = static_cast<uint8_t*>(a.k);
+  c.v = static_cast<uint8_t*>(a.v);
+  c.k_scale = a.k_scale;
+  c.v_scale = a.v_scale;
+  c.k_page = a.k_page_stride;
+  c.v_page = a.v_page_stride;
+  c.k_scale_page = a.k_scale_stride;
+  c.v_scale_page = a.v_scale_stride;
+  c.pages = a.pages;
+  c.pages_row = a.pages_row_stride;
+  c.cu = a.cu;
+  c.lengths = a.lengths;
+  c.num_tokens = a.num_tokens;
+  c.table_width = a.table_width;
+  c.num_pages = a.num_pages;
+  c.page_log2 = __builtin_ctz(a.page_size);
+  c.kv_heads = a.num_kv_heads;
+  c.requests = a.num_requests;
+  return LD_OK;
+}
+
+struct Attention {
+  const uint16_t* q;
+  int64_t q_row;
+  const uint16_t* gate;   // NULL: none
+  int64_t gate_row;
+  uint16_t* out;
+  float* workspace;
+  int32_t q_heads;
+  int32_t group;          // q_heads / kv_heads
+  int32_t width;          // decode: rows of a request at most
+  float log2_scale;       // scale * log2(e)
+};
+
+// The same of the attention entry points.
+inline int attention_params(const ld_paged_cache& c, const ld_attention_args* from, Attention& p) {
+  if (from == nullptr) return fail(LD_ERR_INVALID_ARGUMENT, "args is NULL");
+  const ld_attention_args& a = *from;
+  if (a.num_q_heads <= 0 || a.num_q_heads > 1 << 16 || a.num_q_heads % c.num_kv_heads != 0)
+    return fail(LD_ERR_INVALID_ARGUMENT,
+                "num_q_heads must be a positive multiple of num_kv_heads, at most 2^16");
+  if (!(a.scale > 0.0f && a.scale <= 3.4028235e38f))
+    return fail(LD_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+  p = Attention{};
+  if (c.num_requests == 0 || c.num_tokens == 0) return LD_OK;
+  if (!a.q || !a.out) return fail(LD_ERR_INVALID_ARGUMENT, "attention: NULL tensor pointer");
+  p.q = static_cast<const uint16_t*>(a.q);
+  p.q_row = a.q_row_stride;
+  p.gate = static_cast<const uint16_t*>(a.gate);
+  p.gate_row = a.gate_row_stride;
+  p.out = static_cast<uint16_t*>(a.out);
+  p.workspace = static_cast<float*>(a.workspace);
+  p.q_heads = a.num_q_heads;
+  p.group = a.num_q_heads / c.num_kv_heads;
+  p.width = a.width;
+  p.log2_scale = a.scale * 1.44269504088896340736f;
+  return LD_OK;
+}
+
+namespace {
+
+// What a request has in this call: rows first .. last - 1 of the activations, of which row i is at
+// position i + shift (64 bits: lengths and cu are any int32), and the tokens that its table holds.
+struct Request {
+  int64_t first, last, shift;
+  int32_t tokens;
+};
+
+__device__ __forceinline__ Request request_of(const Cache& c, int r) {
+  Request q;
+  const int64_t end = c.cu[r + 1];
+  q.first = max(static_cast<int64_t>(c.cu[r]), int64_t{0});
+  q.last = min(end, c.num_tokens);
+  const int64_t length = c.lengths[r];
+  q.shift = length - end;
+  q.tokens = static_cast<int32_t>(
+      max(min(length, static_cast<int64_t>(c.table_width) << c.page_log2), int64_t{0}));
+  return q;
+}
+
+// The last request that begins at or before `row` (0 if none does).
+__device__ __forceinline__ int request_at(const Cache& c, int64_t row) {
+  int low = 0, high = c.requests - 1;
+  while (low < high) {
+    const int mid = low + (high - low + 1) / 2;
+    if (c.cu[mid] <= row) low = mid;
+    else high = mid - 1;
+  }
+  return low;
+}
+
+__device__ __forceinline__ bool live_page(const Cache& c, int page) {
+  return page > 0 && page < c.num_pages;
+}
+
+// Bytes of a page and head: 128 a token.
+__device__ __forceinline__ const uint8_t* k_tile(const Cache& c, int page, int head) {
+  return c.k + page * c.k_page + (static_cast<int64_t>(head) << (7 + c.page_log2));
+}
+__device__ __forceinline__ const uint8_t* v_tile(const Cache& c, int page, int head) {
+  return c.v + page * c.v_page + (static_cast<int64_t>(head) << (7 + c.page_log2));
+}
+
+// 2^e for -126 <= e <= 127.
+__device__ __forceinline__ float power_of_two(int e) {
+  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+__device__ __forceinline__ float scale_value(uint8_t b) {
+  return power_of_two(min(max(static_cast<int>(b) - kScaleBias, kScaleLow), kScaleHigh));
+}
+
+}  // namespace
+}  // namespace ld

@@ -13,9 +13,10 @@
 // pairs by shuffles); one token of them 2.5 us.  Few tokens are split over waves by rounds, so that a
 // small launch's latency is one batch's.
 #include <algorithm>
+#include <type_traits>
 
 #include "gdn_common.h"
-#include "lightdelta_linear_hip.h"
+#include "lightdelta_attention_hip.h"
 
 namespace ld {
 namespace {
@@ -39,6 +40,9 @@ struct NormRopeParams {
   int32_t splits;   // waves a token
   int32_t q_bf16, k_bf16, positions64;
   float eps;
+  const int32_t* axes;   // with several axes: that of each angle
+  int64_t axis_stride;   // between the positions of two axes
+  int32_t num_axes;
 };
 
 // Where a lane finds the other elements of its pairs: its own (neighbours, interleaved), the lane
@@ -83,7 +87,7 @@ __device__ __forceinline__ void load_weights(float (&w)[8], const void* from, in
   }
 }
 
-template <int D>
+template <int D, bool Axes>
 __global__ __launch_bounds__(kThreads) void norm_rope_kernel(const NormRopeParams p) {
   const int lane = threadIdx.x & 63;
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWaves +
@@ -112,8 +116,16 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(const NormRopeParam
   __shared__ __attribute__((aligned(16))) float angles[kWaves][2][64];
   float* const mine = angles[threadIdx.x >> 6][0];
   if (lane < p.half) {
-    const int64_t position = p.positions64 ? static_cast<const int64_t*>(p.positions)[token]
-                                           : static_cast<const int32_t*>(p.positions)[token];
+    int64_t at = token;
+    bool turns = true;
+    if constexpr (Axes) {   // (an axis that there is not: no turn)
+      const int axis = p.axes[lane];
+      turns = axis >= 0 && axis < p.num_axes;
+      at += (turns ? axis : 0) * p.axis_stride;
+    }
+    const int64_t position = !turns          ? 0
+                             : p.positions64 ? static_cast<const int64_t*>(p.positions)[at]
+                                             : static_cast<const int32_t*>(p.positions)[at];
     const float fraction = turn_fraction(position, p.inv_freq[lane]);
     mine[lane] = __builtin_amdgcn_cosf(fraction);
     mine[64 + lane] = __builtin_amdgcn_sinf(fraction);
@@ -178,8 +190,11 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(const NormRopeParam
 }  // namespace
 }  // namespace ld
 
-extern "C" int ld_norm_rope(const ld_norm_rope_args* args, void* stream) {
-  using namespace ld;
+namespace ld {
+namespace {
+
+int launch_norm_rope(const ld_norm_rope_args* args, const ld_rope_axes* axes, const char* what,
+                     void* stream) {
   if (args == nullptr) return fail(LD_ERR_INVALID_ARGUMENT, "ld_norm_rope: args is NULL");
   const ld_norm_rope_args& a = *args;
   if (a.num_tokens < 0 || a.q_heads < 0 || a.k_heads < 0)
@@ -220,15 +235,41 @@ extern "C" int ld_norm_rope(const ld_norm_rope_args* args, void* stream) {
   p.k_bf16 = a.k_weight_dtype == LD_DTYPE_BF16;
   p.positions64 = a.positions_int64;
   p.eps = a.eps;
+  if (axes != nullptr) {
+    p.axes = axes->axes;
+    p.axis_stride = axes->position_axis_stride;
+    p.num_axes = axes->num_axes;
+  }
   const int64_t blocks = (a.num_tokens * p.splits + kWaves - 1) / kWaves;
   if (blocks > 0xffffff) return fail(LD_ERR_INVALID_ARGUMENT, "too many tokens");
-  const auto kernel = a.interleaved    ? norm_rope_kernel<kOwn>
-                      : p.half == 64   ? norm_rope_kernel<8>
-                      : p.half == 32   ? norm_rope_kernel<4>
-                      : p.half == 16   ? norm_rope_kernel<2>
-                      : p.half == 8    ? norm_rope_kernel<1>
-                                       : norm_rope_kernel<kShuffle>;
+  const auto pick = [&](auto several) {
+    constexpr bool kAxes = decltype(several)::value;
+    return a.interleaved    ? norm_rope_kernel<kOwn, kAxes>
+           : p.half == 64   ? norm_rope_kernel<8, kAxes>
+           : p.half == 32   ? norm_rope_kernel<4, kAxes>
+           : p.half == 16   ? norm_rope_kernel<2, kAxes>
+           : p.half == 8    ? norm_rope_kernel<1, kAxes>
+                            : norm_rope_kernel<kShuffle, kAxes>;
+  };
+  const auto kernel = axes != nullptr ? pick(std::true_type{}) : pick(std::false_type{});
   hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0,
                      static_cast<hipStream_t>(stream), p);
-  return check_launch("ld_norm_rope");
+  return check_launch(what);
+}
+
+}  // namespace
+}  // namespace ld
+
+extern "C" int ld_norm_rope(const ld_norm_rope_args* args, void* stream) {
+  return ld::launch_norm_rope(args, nullptr, "ld_norm_rope", stream);
+}
+
+extern "C" int ld_norm_rope_axes(const ld_norm_rope_args* args, const ld_rope_axes* axes,
+                                 void* stream) {
+  using namespace ld;
+  if (axes == nullptr) return fail(LD_ERR_INVALID_ARGUMENT, "ld_norm_rope_axes: axes is NULL");
+  if (axes->num_axes < 1) return fail(LD_ERR_INVALID_ARGUMENT, "num_axes must be >= 1");
+  if (args != nullptr && args->rotary > 0 && args->num_tokens > 0 && axes->axes == nullptr)
+    return fail(LD_ERR_INVALID_ARGUMENT, "ld_norm_rope_axes: NULL tensor pointer");
+  return launch_norm_rope(args, axes, "ld_norm_rope_axes", stream);
 }

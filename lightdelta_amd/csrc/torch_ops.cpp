@@ -3,9 +3,10 @@
 // (csrc/gdn_decode.cu:366-403), generalised to any H, HV with HV % H == 0, with its
 // messages; the state-pool ops with the checks of the reference's state_io
 // (csrc/state_io.cu:29-49) and of the additive ones; the linear-attention ops (linear_decode,
-// linear_prefill, norm_rope); then the C ABI of liblightdelta_hip.so on the current HIP stream
-// of the tensors' device.  The schemas are defined by
-// lightdelta_amd/ops.py, which loads this library (prefill keeps a Python kernel).
+// linear_prefill, norm_rope) and the softmax-attention ones (norm_rope_axes, cache_write,
+// cache_read, attention_decode, attention_prefill); then the C ABI of liblightdelta_hip.so on the
+// current HIP stream of the tensors' device.  The schemas are defined by lightdelta_amd/ops.py, which
+// loads this library (prefill keeps a Python kernel).
 // Host-only C++ (no device code): one eager call costs a few microseconds of host time, as
 // the reference's C++ launcher does, where a Python kernel costs about twelve.
 #include <ATen/core/Tensor.h>
@@ -14,11 +15,13 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <limits>
 #include <optional>
 
+#include "lightdelta_attention_hip.h"
 #include "lightdelta_hip.h"
 #include "lightdelta_linear_hip.h"
 
@@ -524,9 +527,11 @@ void linear_prefill(const at::Tensor& qkv, const at::Tensor& log_decay, const at
   TORCH_CHECK(rc == LD_OK, ld_last_error());
 }
 
-void norm_rope(at::Tensor qkv, const at::Tensor& q_weight, const at::Tensor& k_weight,
-               const at::Tensor& positions, const at::Tensor& inv_freq, int64_t q_heads,
-               int64_t k_heads, double eps, bool interleaved) {
+// What norm_rope and norm_rope_axes share (ops.py _rope_layout restates the checks): the C ABI's
+// arguments but for the positions.
+ld_norm_rope_args rope_args(const at::Tensor& qkv, const at::Tensor& q_weight,
+                            const at::Tensor& k_weight, const at::Tensor& inv_freq,
+                            int64_t q_heads, int64_t k_heads, double eps, bool interleaved) {
   TORCH_CHECK(qkv.is_cuda() && qkv.scalar_type() == at::kBFloat16, "qkv must be CUDA BF16");
   TORCH_CHECK(q_heads >= 0 && k_heads >= 0 && q_heads <= INT32_MAX / kDim &&
                   k_heads <= INT32_MAX / kDim && qkv.dim() == 2 &&
@@ -538,10 +543,6 @@ void norm_rope(at::Tensor qkv, const at::Tensor& q_weight, const at::Tensor& k_w
     TORCH_CHECK(t->device() == qkv.device() && t->is_contiguous() && floats(*t) &&
                     t->numel() == kDim,
                 "weights must be contiguous CUDA FP32/BF16 [128]");
-  TORCH_CHECK(positions.device() == qkv.device() &&
-                  (positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong) &&
-                  positions.dim() == 1 && positions.size(0) == n && positions.is_contiguous(),
-              "positions must be contiguous CUDA int32/int64 [tokens]");
   const int64_t rotary = 2 * inv_freq.numel();
   TORCH_CHECK(inv_freq.device() == qkv.device() && inv_freq.scalar_type() == at::kFloat &&
                   inv_freq.dim() == 1 && inv_freq.is_contiguous() && rotary <= kDim &&
@@ -549,7 +550,6 @@ void norm_rope(at::Tensor qkv, const at::Tensor& q_weight, const at::Tensor& k_w
               "inv_freq must be contiguous CUDA FP32 [rotary/2], rotary at most 128 and a multiple "
               "of 16 unless interleaved");
   TORCH_CHECK(eps > 0, "norm epsilon must be positive");
-  if (n == 0 || q_heads + k_heads == 0) return;
   ld_norm_rope_args args{};
   args.qkv = qkv.data_ptr();
   args.qkv_row_stride = qkv.stride(0);
@@ -557,8 +557,6 @@ void norm_rope(at::Tensor qkv, const at::Tensor& q_weight, const at::Tensor& k_w
   args.k_weight = k_weight.data_ptr();
   args.q_weight_dtype = dtype_code(q_weight);
   args.k_weight_dtype = dtype_code(k_weight);
-  args.positions = positions.data_ptr();
-  args.positions_int64 = positions.scalar_type() == at::kLong;
   args.rotary = static_cast<int32_t>(rotary);
   args.inv_freq = static_cast<const float*>(inv_freq.data_ptr());
   args.num_tokens = n;
@@ -566,9 +564,218 @@ void norm_rope(at::Tensor qkv, const at::Tensor& q_weight, const at::Tensor& k_w
   args.k_heads = static_cast<int32_t>(k_heads);
   args.interleaved = interleaved;
   args.eps = static_cast<float>(eps);
+  return args;
+}
+
+bool is_index(const at::Tensor& t) {
+  return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong;
+}
+
+void norm_rope(at::Tensor qkv, const at::Tensor& q_weight, const at::Tensor& k_weight,
+               const at::Tensor& positions, const at::Tensor& inv_freq, int64_t q_heads,
+               int64_t k_heads, double eps, bool interleaved) {
+  auto args = rope_args(qkv, q_weight, k_weight, inv_freq, q_heads, k_heads, eps, interleaved);
+  TORCH_CHECK(positions.device() == qkv.device() && is_index(positions) && positions.dim() == 1 &&
+                  positions.size(0) == args.num_tokens && positions.is_contiguous(),
+              "positions must be contiguous CUDA int32/int64 [tokens]");
+  if (args.num_tokens == 0 || q_heads + k_heads == 0) return;
+  args.positions = positions.data_ptr();
+  args.positions_int64 = positions.scalar_type() == at::kLong;
   const c10::DeviceGuard guard(qkv.device());
   const int rc = ld_norm_rope(&args, stream_of(qkv));
   TORCH_CHECK(rc == LD_OK, ld_last_error());
+}
+
+// ---- softmax attention over a paged cache in 8 bits ----------------------------------------
+
+void norm_rope_axes(at::Tensor qkv, const at::Tensor& q_weight, const at::Tensor& k_weight,
+                    const at::Tensor& positions, const at::Tensor& axes,
+                    const at::Tensor& inv_freq, int64_t q_heads, int64_t k_heads, double eps,
+                    bool interleaved) {
+  auto args = rope_args(qkv, q_weight, k_weight, inv_freq, q_heads, k_heads, eps, interleaved);
+  const int64_t n = args.num_tokens;
+  TORCH_CHECK(positions.device() == qkv.device() && is_index(positions) && positions.dim() == 2 &&
+                  positions.size(0) >= 1 && positions.size(0) <= INT32_MAX &&
+                  positions.size(1) == n && (n <= 1 || positions.stride(1) == 1),
+              "positions must be CUDA int32/int64 [axes,tokens] with dense rows");
+  TORCH_CHECK(axes.device() == qkv.device() && axes.scalar_type() == at::kInt && axes.dim() == 1 &&
+                  axes.size(0) == inv_freq.size(0) && axes.is_contiguous(),
+              "axes must be contiguous CUDA int32 [rotary/2]");
+  if (n == 0 || q_heads + k_heads == 0) return;
+  args.positions = positions.data_ptr();
+  args.positions_int64 = positions.scalar_type() == at::kLong;
+  ld_rope_axes several{};
+  several.axes = static_cast<const int32_t*>(axes.data_ptr());
+  several.position_axis_stride = positions.stride(0);
+  several.num_axes = static_cast<int32_t>(positions.size(0));
+  const c10::DeviceGuard guard(qkv.device());
+  const int rc = ld_norm_rope_axes(&args, &several, stream_of(qkv));
+  TORCH_CHECK(rc == LD_OK, ld_last_error());
+}
+
+// The cache and its requests, for activations like `rows` (ops.py _cache_layout restates the
+// checks).
+ld_paged_cache paged_cache(const at::Tensor& rows, const at::Tensor& pages, const at::Tensor& cu,
+                           const at::Tensor& lengths, const at::Tensor& k_cache,
+                           const at::Tensor& v_cache, const at::Tensor& k_scale,
+                           const at::Tensor& v_scale) {
+  const c10::Device device = rows.device();
+  for (const at::Tensor* t : {&k_cache, &v_cache})
+    TORCH_CHECK(t->device() == device && t->scalar_type() == at::kFloat8_e4m3fn &&
+                    t->dim() == 5 && dense_inner(*t) &&
+                    reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0 &&
+                    (t->size(0) <= 1 || (t->stride(0) % 16 == 0 && t->stride(0) >= row_bytes(*t))),
+                "caches must be CUDA float8_e4m3fn with dense pages, 16-byte aligned");
+  const int64_t count = k_cache.size(0), heads = k_cache.size(1), page = k_cache.size(3);
+  TORCH_CHECK((page == 16 || page == 32 || page == 64 || page == 128) && k_cache.size(2) == 8 &&
+                  k_cache.size(4) == 16 && heads >= 1 && heads <= 1 << 16,
+              "k_cache must be [pages,kv_heads,8,page,16], page 16, 32, 64 or 128");
+  TORCH_CHECK(v_cache.size(0) == count && v_cache.size(1) == heads &&
+                  v_cache.size(2) == page / 16 && v_cache.size(3) == kDim && v_cache.size(4) == 16,
+              "v_cache must be [pages,kv_heads,page/16,128,16]");
+  for (const at::Tensor* t : {&k_scale, &v_scale})
+    TORCH_CHECK(t->device() == device && t->scalar_type() == at::kFloat8_e8m0fnu &&
+                    t->dim() == 2 && t->size(0) == count && t->size(1) == heads &&
+                    dense_inner(*t) && (count <= 1 || t->stride(0) >= heads),
+                "scales must be CUDA float8_e8m0fnu [pages,kv_heads] with dense rows");
+  for (const at::Tensor* t : {&pages, &cu, &lengths})
+    TORCH_CHECK(t->device() == device && t->scalar_type() == at::kInt,
+                "metadata must be CUDA int32");
+  const int64_t requests = lengths.numel();
+  TORCH_CHECK(lengths.dim() == 1 && lengths.is_contiguous() && cu.dim() == 1 &&
+                  cu.numel() == requests + 1 && cu.is_contiguous() && pages.dim() == 2 &&
+                  pages.size(0) == requests && (pages.size(1) <= 1 || pages.stride(1) == 1) &&
+                  std::max({requests, pages.size(1), count}) <= INT32_MAX,
+              "invalid request metadata shapes");
+  ld_paged_cache cache{};
+  cache.k = k_cache.data_ptr();
+  cache.v = v_cache.data_ptr();
+  cache.k_scale = static_cast<uint8_t*>(k_scale.data_ptr());
+  cache.v_scale = static_cast<uint8_t*>(v_scale.data_ptr());
+  cache.k_page_stride = count > 1 ? k_cache.stride(0) : 0;
+  cache.v_page_stride = count > 1 ? v_cache.stride(0) : 0;
+  cache.k_scale_stride = count > 1 ? k_scale.stride(0) : 0;
+  cache.v_scale_stride = count > 1 ? v_scale.stride(0) : 0;
+  cache.pages = static_cast<const int32_t*>(pages.data_ptr());
+  cache.pages_row_stride = pages.stride(0);
+  cache.cu = static_cast<const int32_t*>(cu.data_ptr());
+  cache.lengths = static_cast<const int32_t*>(lengths.data_ptr());
+  cache.num_tokens = rows.dim() > 0 ? rows.size(0) : 0;
+  cache.table_width = static_cast<int32_t>(pages.size(1));
+  cache.num_pages = static_cast<int32_t>(count);
+  cache.page_size = static_cast<int32_t>(page);
+  cache.num_kv_heads = static_cast<int32_t>(heads);
+  cache.num_requests = static_cast<int32_t>(requests);
+  return cache;
+}
+
+ld_cache_rows cache_rows(const at::Tensor& k, const at::Tensor& v, int64_t heads) {
+  for (const at::Tensor* t : {&k, &v})
+    TORCH_CHECK(t->device() == k.device() && t->scalar_type() == at::kBFloat16 && t->dim() == 3 &&
+                    t->size(0) == k.size(0) && t->size(1) == heads && t->size(2) == kDim &&
+                    dense_inner(*t),
+                "k and v must be CUDA BF16 [tokens,kv_heads,128] with dense rows");
+  TORCH_CHECK(k.size(0) <= INT32_MAX, "too many tokens");
+  return ld_cache_rows{k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0)};
+}
+
+bool nothing(const ld_paged_cache& cache) {
+  return cache.num_requests == 0 || cache.num_tokens == 0;
+}
+
+void cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& pages,
+                 const at::Tensor& cu, const at::Tensor& lengths, at::Tensor k_cache,
+                 at::Tensor v_cache, at::Tensor k_scale, at::Tensor v_scale) {
+  TORCH_CHECK(k.is_cuda(), "k and v must be CUDA BF16 [tokens,kv_heads,128] with dense rows");
+  auto cache = paged_cache(k, pages, cu, lengths, k_cache, v_cache, k_scale, v_scale);
+  const auto rows = cache_rows(k, v, cache.num_kv_heads);
+  if (nothing(cache)) return;
+  const c10::DeviceGuard guard(k.device());
+  const int rc = ld_cache_write(&cache, &rows, stream_of(k));
+  TORCH_CHECK(rc == LD_OK, ld_last_error());
+}
+
+void cache_read(const at::Tensor& pages, const at::Tensor& cu, const at::Tensor& lengths,
+                const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& k_scale,
+                const at::Tensor& v_scale, at::Tensor k, at::Tensor v) {
+  TORCH_CHECK(k.is_cuda(), "k and v must be CUDA BF16 [tokens,kv_heads,128] with dense rows");
+  auto cache = paged_cache(k, pages, cu, lengths, k_cache, v_cache, k_scale, v_scale);
+  const auto rows = cache_rows(k, v, cache.num_kv_heads);
+  TORCH_CHECK(k.size(0) <= 1 || std::min(k.stride(0), v.stride(0)) >= cache.num_kv_heads * kDim,
+              "rows of k and v must not overlap");
+  if (nothing(cache)) return;
+  const c10::DeviceGuard guard(k.device());
+  const int rc = ld_cache_read(&cache, &rows, stream_of(k));
+  TORCH_CHECK(rc == LD_OK, ld_last_error());
+}
+
+// attention_decode (a width) and attention_prefill (none).
+void attend(const at::Tensor& q, const at::Tensor& pages, const at::Tensor& cu,
+            const at::Tensor& lengths, const at::Tensor& k_cache, const at::Tensor& v_cache,
+            const at::Tensor& k_scale, const at::Tensor& v_scale,
+            const std::optional<at::Tensor>& gate, const at::Tensor& out,
+            std::optional<int64_t> width, double scale) {
+  TORCH_CHECK(!width || (*width >= 1 && *width <= LD_MAX_TOKENS),
+              "decode/MTP supports 1 through 4 tokens per request");
+  TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.dim() == 3 &&
+                  q.size(2) == kDim && dense_inner(q),
+              "q must be CUDA BF16 [tokens,q_heads,128] with dense rows");
+  auto cache = paged_cache(q, pages, cu, lengths, k_cache, v_cache, k_scale, v_scale);
+  const int64_t heads = q.size(1);
+  TORCH_CHECK(heads > 0 && heads <= 1 << 16 && heads % cache.num_kv_heads == 0,
+              "q_heads must be a positive multiple of kv_heads");
+  TORCH_CHECK(!gate.has_value() ||
+                  (gate->device() == q.device() && gate->scalar_type() == at::kBFloat16 &&
+                   gate->sizes() == q.sizes() && dense_inner(*gate)),
+              "gate must be CUDA BF16 [tokens,q_heads,128] with dense rows");
+  TORCH_CHECK(out.device() == q.device() && out.scalar_type() == at::kBFloat16 &&
+                  out.sizes() == q.sizes() && out.is_contiguous(),
+              "out must be contiguous CUDA BF16 [tokens,q_heads,128]");
+  TORCH_CHECK(scale > 0 && scale <= std::numeric_limits<float>::max(),
+              "scale must be positive and finite");
+  TORCH_CHECK(q.size(0) <= INT32_MAX, "too many tokens");
+  if (nothing(cache)) return;
+  ld_attention_args args{};
+  args.q = q.data_ptr();
+  args.q_row_stride = q.stride(0);
+  if (gate.has_value()) {
+    args.gate = gate->data_ptr();
+    args.gate_row_stride = gate->stride(0);
+  }
+  args.out = out.data_ptr();
+  args.num_q_heads = static_cast<int32_t>(heads);
+  args.width = static_cast<int32_t>(width.value_or(0));
+  args.scale = static_cast<float>(scale);
+  const c10::DeviceGuard guard(q.device());
+  // (a workspace as linear_prefill's: from torch's allocator for this call alone)
+  at::Tensor workspace;
+  const int64_t bytes = width ? ld_attention_decode_workspace_bytes(&cache, &args)
+                              : ld_attention_prefill_workspace_bytes(&cache, &args);
+  if (bytes > 0) {
+    workspace = at::empty({bytes}, q.options().dtype(at::kByte));
+    args.workspace = workspace.data_ptr();
+    args.workspace_bytes = bytes;
+  }
+  const int rc = width ? ld_attention_decode(&cache, &args, stream_of(q))
+                       : ld_attention_prefill(&cache, &args, stream_of(q));
+  TORCH_CHECK(rc == LD_OK, ld_last_error());
+}
+
+void attention_decode(const at::Tensor& q, const at::Tensor& pages, const at::Tensor& cu,
+                      const at::Tensor& lengths, const at::Tensor& k_cache,
+                      const at::Tensor& v_cache, const at::Tensor& k_scale,
+                      const at::Tensor& v_scale, const std::optional<at::Tensor>& gate,
+                      at::Tensor out, int64_t width, double scale) {
+  attend(q, pages, cu, lengths, k_cache, v_cache, k_scale, v_scale, gate, out, width, scale);
+}
+
+void attention_prefill(const at::Tensor& q, const at::Tensor& pages, const at::Tensor& cu,
+                       const at::Tensor& lengths, const at::Tensor& k_cache,
+                       const at::Tensor& v_cache, const at::Tensor& k_scale,
+                       const at::Tensor& v_scale, const std::optional<at::Tensor>& gate,
+                       at::Tensor out, double scale) {
+  attend(q, pages, cu, lengths, k_cache, v_cache, k_scale, v_scale, gate, out, std::nullopt,
+         scale);
 }
 
 }  // namespace
@@ -587,6 +794,11 @@ TORCH_LIBRARY_IMPL(lightdelta, CUDA, m) {
   m.impl("linear_decode", &linear_decode);
   m.impl("linear_prefill", &linear_prefill);
   m.impl("norm_rope", &norm_rope);
+  m.impl("norm_rope_axes", &norm_rope_axes);
+  m.impl("cache_write", &cache_write);
+  m.impl("cache_read", &cache_read);
+  m.impl("attention_decode", &attention_decode);
+  m.impl("attention_prefill", &attention_prefill);
 }
 
 // The state cache policy these kernels pass (LD_CACHE_KEEP / LD_CACHE_STREAM), set from

@@ -53,13 +53,29 @@ Additive ops (no reference counterpart):
                                         rotation of its first 2 * len(inv_freq) elements by
                                         positions * inv_freq, in place on qkv's first
                                         (q_heads + k_heads) * 128 columns
+  norm_rope_axes(qkv, q_weight, k_weight, positions, axes, inv_freq, q_heads, k_heads, eps,
+                 interleaved)           the same with positions [axes, tokens] of several axes
+                                        (time, height, width); axes int32 [rotary/2] names each
+                                        frequency's
+  cache_write(k, v, pages, cu, lengths, k_cache, v_cache, k_scale, v_scale)
+                                        keys and values of the last tokens of each request into a
+                                        paged cache in e4m3, a power of two as the scale of each
+                                        page and head (attention_cache allocates one)
+  cache_read(pages, cu, lengths, k_cache, v_cache, k_scale, v_scale, k, v)
+                                        the values at the same places back in bf16
+  attention_decode(q, pages, cu, lengths, k_cache, v_cache, k_scale, v_scale, gate, out, width,
+                   scale)               softmax attention of up to `width` (1 to 4) new tokens a
+                                        request to all tokens up to their own, over that cache;
+                                        gate None, or out times sigmoid(gate)
+  attention_prefill(q, pages, cu, lengths, k_cache, v_cache, k_scale, v_scale, gate, out, scale)
+                                        the same for any number of new tokens
 
 Every kernel launches on the caller's current stream and reads no device memory on the host,
 so it can be captured in a HIP graph.  None allocates, except prefill's chunked form, which
 keeps one workspace per device and stream for later eager calls (release_prefill_workspaces
 frees them) and gives a call under graph capture a workspace the graph keeps, and
-linear_prefill, which takes a long prompt's workspace (64 MiB and little more at most) from
-torch's allocator for the call.  The kernels of every op but prefill are C++ (csrc/torch_ops.cpp,
+linear_prefill, attention_decode and attention_prefill, which take what workspace they need (for
+linear_prefill 64 MiB and little more at most) from torch's allocator for the call.  The kernels of every op but prefill are C++ (csrc/torch_ops.cpp,
 liblightdelta_torch.so); the check_* functions below restate their argument checks so they
 can run without a GPU.
 """
@@ -117,6 +133,29 @@ SCHEMAS = {
     "norm_rope": (
         "norm_rope(Tensor(q!) qkv, Tensor q_weight, Tensor k_weight, Tensor positions, "
         "Tensor inv_freq, int q_heads, int k_heads, float eps, bool interleaved) -> ()"
+    ),
+    "norm_rope_axes": (
+        "norm_rope_axes(Tensor(q!) qkv, Tensor q_weight, Tensor k_weight, Tensor positions, "
+        "Tensor axes, Tensor inv_freq, int q_heads, int k_heads, float eps, bool interleaved) "
+        "-> ()"
+    ),
+    "cache_write": (
+        "cache_write(Tensor k, Tensor v, Tensor pages, Tensor cu, Tensor lengths, "
+        "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, Tensor(d!) v_scale) -> ()"
+    ),
+    "cache_read": (
+        "cache_read(Tensor pages, Tensor cu, Tensor lengths, Tensor k_cache, Tensor v_cache, "
+        "Tensor k_scale, Tensor v_scale, Tensor(k!) k, Tensor(v!) v) -> ()"
+    ),
+    "attention_decode": (
+        "attention_decode(Tensor q, Tensor pages, Tensor cu, Tensor lengths, Tensor k_cache, "
+        "Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor? gate, Tensor(o!) out, int width, "
+        "float scale) -> ()"
+    ),
+    "attention_prefill": (
+        "attention_prefill(Tensor q, Tensor pages, Tensor cu, Tensor lengths, Tensor k_cache, "
+        "Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor? gate, Tensor(o!) out, "
+        "float scale) -> ()"
     ),
 }
 
@@ -638,6 +677,27 @@ def check_linear_prefill(qkv, log_decay, slots, has_initial, cu_seqlens, state, 
 def check_norm_rope(qkv, q_weight, k_weight, positions, inv_freq, q_heads, k_heads, eps,
                     interleaved):
     """Validation of norm_rope."""
+    n = _rope_layout(qkv, q_weight, k_weight, inv_freq, q_heads, k_heads, eps, interleaved)
+    _require(positions.device == qkv.device and positions.dtype in (torch.int32, torch.int64)
+             and tuple(positions.shape) == (n,) and positions.is_contiguous(),
+             "positions must be contiguous CUDA int32/int64 [tokens]")
+
+
+def check_norm_rope_axes(qkv, q_weight, k_weight, positions, axes, inv_freq, q_heads, k_heads, eps,
+                         interleaved):
+    """Validation of norm_rope_axes."""
+    n = _rope_layout(qkv, q_weight, k_weight, inv_freq, q_heads, k_heads, eps, interleaved)
+    _require(positions.device == qkv.device and positions.dtype in (torch.int32, torch.int64)
+             and positions.dim() == 2 and 1 <= positions.shape[0] <= _INT32_MAX
+             and positions.shape[1] == n and (n <= 1 or positions.stride(1) == 1),
+             "positions must be CUDA int32/int64 [axes,tokens] with dense rows")
+    _require(axes.device == qkv.device and axes.dtype == torch.int32
+             and tuple(axes.shape) == tuple(inv_freq.shape) and axes.is_contiguous(),
+             "axes must be contiguous CUDA int32 [rotary/2]")
+
+
+def _rope_layout(qkv, q_weight, k_weight, inv_freq, q_heads, k_heads, eps, interleaved):
+    """What norm_rope and norm_rope_axes share; returns the tokens."""
     _require(_is_gpu(qkv) and qkv.dtype == torch.bfloat16, "qkv must be CUDA BF16")
     columns = (q_heads + k_heads) * HEAD_DIM
     _require(q_heads >= 0 and k_heads >= 0 and max(q_heads, k_heads) <= _INT32_MAX // HEAD_DIM
@@ -648,9 +708,6 @@ def check_norm_rope(qkv, q_weight, k_weight, positions, inv_freq, q_heads, k_hea
     for t in (q_weight, k_weight):
         _require(t.device == qkv.device and t.is_contiguous() and t.dtype in _FLOATS
                  and t.numel() == HEAD_DIM, "weights must be contiguous CUDA FP32/BF16 [128]")
-    _require(positions.device == qkv.device and positions.dtype in (torch.int32, torch.int64)
-             and tuple(positions.shape) == (n,) and positions.is_contiguous(),
-             "positions must be contiguous CUDA int32/int64 [tokens]")
     rotary = 2 * inv_freq.numel()
     _require(inv_freq.device == qkv.device and inv_freq.dtype == torch.float32
              and inv_freq.dim() == 1 and inv_freq.is_contiguous() and rotary <= HEAD_DIM
@@ -658,6 +715,113 @@ def check_norm_rope(qkv, q_weight, k_weight, positions, inv_freq, q_heads, k_hea
              "inv_freq must be contiguous CUDA FP32 [rotary/2], rotary at most 128 and a "
              "multiple of 16 unless interleaved")
     _require(eps > 0, "norm epsilon must be positive")
+    return n
+
+
+# ---------------------------------------------------------------------------------------
+# softmax attention over a paged cache in 8 bits: the checks of the C++ kernels, restated
+# ---------------------------------------------------------------------------------------
+
+PAGE_SIZES = (16, 32, 64, 128)
+ATTENTION_MAX_HEADS = 1 << 16
+
+
+def attention_cache(num_pages: int, kv_heads: int, page_size: int = 64, device="cuda"):
+    """(k_cache, v_cache, k_scale, v_scale) of a paged cache, all zeros: e4m3
+    [pages, kv_heads, 8, page, 16] and [pages, kv_heads, page / 16, 128, 16] (element d of token t
+    of a page at [d / 16, t, d % 16], and at [t / 16, d, t % 16]), scales e8m0 [pages, kv_heads].
+    Page 0 is padding."""
+    _require(page_size in PAGE_SIZES, "page size must be 16, 32, 64 or 128")
+    k = torch.zeros(num_pages, kv_heads, 8, page_size, 16, dtype=torch.uint8, device=device)
+    v = torch.zeros(num_pages, kv_heads, page_size // 16, HEAD_DIM, 16, dtype=torch.uint8,
+                    device=device)
+    scales = torch.full((2, num_pages, kv_heads), 127, dtype=torch.uint8, device=device)
+    return (k.view(torch.float8_e4m3fn), v.view(torch.float8_e4m3fn),
+            *scales.view(torch.float8_e8m0fnu).unbind(0))
+
+
+def _cache_layout(rows, pages, cu, lengths, k_cache, v_cache, k_scale, v_scale):
+    """The cache and its requests, for activations like `rows`; returns the kv heads."""
+    device = rows.device
+    for t in (k_cache, v_cache):
+        _require(t.device == device and t.dtype == torch.float8_e4m3fn and t.dim() == 5
+                 and _dense_inner(t) and t.data_ptr() % 16 == 0
+                 and (t.shape[0] <= 1 or (t.stride(0) % 16 == 0
+                                          and t.stride(0) >= t.shape[1:].numel())),
+                 "caches must be CUDA float8_e4m3fn with dense pages, 16-byte aligned")
+    count, heads, _, page, _ = k_cache.shape
+    _require(page in PAGE_SIZES and tuple(k_cache.shape[2:]) == (8, page, 16)
+             and 1 <= heads <= ATTENTION_MAX_HEADS,
+             "k_cache must be [pages,kv_heads,8,page,16], page 16, 32, 64 or 128")
+    _require(tuple(v_cache.shape) == (count, heads, page // 16, HEAD_DIM, 16),
+             "v_cache must be [pages,kv_heads,page/16,128,16]")
+    for t in (k_scale, v_scale):
+        _require(t.device == device and t.dtype == torch.float8_e8m0fnu
+                 and tuple(t.shape) == (count, heads) and _dense_inner(t)
+                 and (count <= 1 or t.stride(0) >= heads),
+                 "scales must be CUDA float8_e8m0fnu [pages,kv_heads] with dense rows")
+    for t in (pages, cu, lengths):
+        _require(t.device == device and t.dtype == torch.int32, "metadata must be CUDA int32")
+    requests = lengths.numel()
+    _require(lengths.dim() == 1 and lengths.is_contiguous() and cu.dim() == 1
+             and cu.numel() == requests + 1 and cu.is_contiguous()
+             and pages.dim() == 2 and pages.shape[0] == requests
+             and (pages.shape[1] <= 1 or pages.stride(1) == 1)
+             and max(requests, pages.shape[1], count) <= _INT32_MAX,
+             "invalid request metadata shapes")
+    return heads
+
+
+def _cache_rows(k, v, heads):
+    for t in (k, v):
+        _require(t.device == k.device and t.dtype == torch.bfloat16 and t.dim() == 3
+                 and tuple(t.shape) == (k.shape[0], heads, HEAD_DIM) and _dense_inner(t),
+                 "k and v must be CUDA BF16 [tokens,kv_heads,128] with dense rows")
+    _require(k.shape[0] <= _INT32_MAX, "too many tokens")
+
+
+def check_cache_write(k, v, pages, cu, lengths, k_cache, v_cache, k_scale, v_scale):
+    """Validation of cache_write; returns the kv heads."""
+    _require(_is_gpu(k), "k and v must be CUDA BF16 [tokens,kv_heads,128] with dense rows")
+    heads = _cache_layout(k, pages, cu, lengths, k_cache, v_cache, k_scale, v_scale)
+    _cache_rows(k, v, heads)
+    return heads
+
+
+def check_cache_read(pages, cu, lengths, k_cache, v_cache, k_scale, v_scale, k, v):
+    """Validation of cache_read; returns the kv heads."""
+    heads = check_cache_write(k, v, pages, cu, lengths, k_cache, v_cache, k_scale, v_scale)
+    _require(k.shape[0] <= 1 or min(k.stride(0), v.stride(0)) >= heads * HEAD_DIM,
+             "rows of k and v must not overlap")
+    return heads
+
+
+def check_attention_prefill(q, pages, cu, lengths, k_cache, v_cache, k_scale, v_scale, gate, out,
+                            scale):
+    """Validation of attention_prefill; returns (q heads, kv heads)."""
+    _require(_is_gpu(q) and q.dtype == torch.bfloat16 and q.dim() == 3 and q.shape[2] == HEAD_DIM
+             and _dense_inner(q), "q must be CUDA BF16 [tokens,q_heads,128] with dense rows")
+    heads = _cache_layout(q, pages, cu, lengths, k_cache, v_cache, k_scale, v_scale)
+    q_heads = q.shape[1]
+    _require(0 < q_heads <= ATTENTION_MAX_HEADS and q_heads % heads == 0,
+             "q_heads must be a positive multiple of kv_heads")
+    _require(gate is None or (gate.device == q.device and gate.dtype == torch.bfloat16
+                              and tuple(gate.shape) == tuple(q.shape) and _dense_inner(gate)),
+             "gate must be CUDA BF16 [tokens,q_heads,128] with dense rows")
+    _require(out.device == q.device and out.dtype == torch.bfloat16
+             and tuple(out.shape) == tuple(q.shape) and out.is_contiguous(),
+             "out must be contiguous CUDA BF16 [tokens,q_heads,128]")
+    _require(0 < scale <= torch.finfo(torch.float32).max, "scale must be positive and finite")
+    _require(q.shape[0] <= _INT32_MAX, "too many tokens")
+    return q_heads, heads
+
+
+def check_attention_decode(q, pages, cu, lengths, k_cache, v_cache, k_scale, v_scale, gate, out,
+                           width, scale):
+    """Validation of attention_decode; returns (q heads, kv heads)."""
+    _require(1 <= width <= _lib.MAX_TOKENS, "decode/MTP supports 1 through 4 tokens per request")
+    return check_attention_prefill(q, pages, cu, lengths, k_cache, v_cache, k_scale, v_scale, gate,
+                                   out, scale)
 
 
 # ---------------------------------------------------------------------------------------
@@ -669,7 +833,8 @@ def check_norm_rope(qkv, q_weight, k_weight, positions, inv_freq, q_heads, k_hea
 # chunked form's workspace cache and the algorithm choice).
 _CXX_KERNELS = ("decode", "decode_conv", "gather_state", "scatter_state", "gather_slots",
                 "scatter_slots", "copy_state", "copy_state_checked", "zero_slots", "packed_plan",
-                "linear_decode", "linear_prefill", "norm_rope")
+                "linear_decode", "linear_prefill", "norm_rope", "norm_rope_axes", "cache_write",
+                "cache_read", "attention_decode", "attention_prefill")
 _IMPLS = {
     "prefill": _prefill_impl,
 }
