@@ -22,7 +22,8 @@ LIBRARY = PACKAGE / "liblightdelta_hip.so"
 TORCH_LIBRARY = PACKAGE / "liblightdelta_torch.so"
 SOURCES = ("abi.hip", "gdn_decode.hip", "prefill_serial.hip", "prefill_chunked.hip",
            "prefill_heads.hip", "state_io.hip", "linear_decode.hip", "linear_prefill.hip",
-           "norm_rope.hip", "cache_io.hip", "attention_decode.hip")
+           "norm_rope.hip", "cache_io.hip", "attention_decode.hip",
+           "attention_prefill.hip")
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [

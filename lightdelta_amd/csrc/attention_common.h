@@ -2,7 +2,7 @@
 // attention_decode.hip, attention_prefill.hip).
 #pragma once
 
-#include "gdn_common.h"
+#include "matrix_common.h"
 #include "lightdelta_attention_hip.h"
 
 namespace ld {
@@ -63,7 +63,7 @@ inline int cache_params(const ld_paged_cache* from, Cache& c) {
   c.cu = a.cu;
   c.lengths = a.lengths;
   c.num_tokens = a.num_tokens;
-  c.table_width = a.table_width;
+  c.table_width = a.num_pages > 1 ? a.table_width : 0;   // (without a page none has a place)
   c.num_pages = a.num_pages;
   c.page_log2 = __builtin_ctz(a.page_size);
   c.kv_heads = a.num_kv_heads;
@@ -152,6 +152,40 @@ __device__ __forceinline__ const uint8_t* k_tile(const Cache& c, int page, int h
 __device__ __forceinline__ const uint8_t* v_tile(const Cache& c, int page, int head) {
   return c.v + page * c.v_page + (static_cast<int64_t>(head) << (7 + c.page_log2));
 }
+
+// Codes 4 w .. 4 w + 3 of each word as operands: e4m3 times a power of two is exact in bf16.
+__device__ __forceinline__ bf16x8 operand8(uint32_t lo, uint32_t hi, float scale) {
+  u32x4 r;
+  r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
+  r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
+  r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
+  r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
+  return __builtin_bit_cast(bf16x8, r);
+}
+
+// Of four codes, 0x80 in the byte of each that is NaN.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t codes) {
+  return ((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
+// A word whose first `count` bytes are kept.
+__device__ __forceinline__ uint32_t first_bytes(int count) {
+  return count >= 4 ? 0xffffffffu : count <= 0 ? 0u : (1u << (8 * count)) - 1;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A value of this lane and of lane i ^ 16, then i ^ 32: their largest.
+__device__ __forceinline__ float max_over_quarters(float x) {
+  uint32_t u = __float_as_uint(x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  u = __float_as_uint(x);
+  const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+constexpr float kLowest = -3.4028234663852886e38f;
 
 // 2^e for -126 <= e <= 127.
 __device__ __forceinline__ float power_of_two(int e) {

@@ -1,124 +1,549 @@
-// Attention over the paged 8-bit cache.
+// Attention of up to four rows a request to its tokens in the paged 8-bit cache.
+//
+// Bound by memory: 256 bytes a token and kv head against 4 * 128 operations a query.  All tiles of
+// 64 tokens, request after request and head after head, are cut into equal runs, one a workgroup,
+// whatever the lengths are (they are known on the device alone); runs that begin or end inside a
+// head's tiles leave sums in the workspace, which a second launch joins.
+//
+// A wave takes every fourth tile of its workgroup's run, straight from memory into the operands of
+// v_mfma_f32_16x16x32_bf16: the cache's order of bytes is theirs.  With m = lane % 16 and h = lane / 16,
+//   scores [token, column]: operand A holds the keys of token 16 (m / 4) + 4 t + m % 4 of the tile
+//     in product t (0 .. 3), so that a lane finds the scores of tokens 16 h .. 16 h + 15 of column m;
+//   outputs [element, column]: operand B is these sixteen weights, A sixteen bytes of a page's v,
+//     the same tokens of element 16 b + m.
+// Columns are the request's rows times the q heads of a kv head, CT tiles of 16.  e4m3 times its
+// scale is exact in bf16; weights are rounded to bf16, their sum is not.
+#include <algorithm>
+
 #include "attention_common.h"
 
 namespace ld {
 namespace {
 
-struct AttentionParams {
+constexpr int kTile = 64;        // tokens
+constexpr int kLeastRun = kWaves;  // tiles of a workgroup's run at the least
+
+struct DecodeAttention {
   Cache cache;
   Attention a;
+  int32_t workers;
+  int32_t columns;   // width * group
 };
 
-// A wave takes one row and q head: 64 tokens at a time, a token's score by a lane, then two
-// elements of the output by a lane, with the running maximum and sum of the softmax.
-__global__ __launch_bounds__(64) void attention_rows_kernel(const AttentionParams p) {
-  const Cache& c = p.cache;
-  const Attention& a = p.a;
-  const int64_t row = blockIdx.x / a.q_heads;
-  const int head = static_cast<int>(blockIdx.x - row * a.q_heads);
-  const int r = request_at(c, row);
-  const Request req = request_of(c, r);
-  if (row < req.first || row >= req.last) return;
-  const int lane = threadIdx.x;
-  const int kv = head / a.group;
-  const int64_t position = row + req.shift;
-  int64_t sees = min(position + 1, static_cast<int64_t>(req.tokens));
-  if (a.width > 0 && req.last - req.first > a.width) sees = 0;
-  __shared__ float query[kDim];
-  __shared__ float weight[64];
-  for (int d = lane; d < kDim; d += 64) query[d] = bf16_to_f32(a.q[row * a.q_row + head * kDim + d]);
-  __syncthreads();
-  float top = -3.4028235e38f, total = 0.0f, o0 = 0.0f, o1 = 0.0f;
-  bool any = false;
-  for (int64_t t0 = 0; t0 < sees; t0 += 64) {
-    const int64_t t = t0 + lane;
-    const int page = t < sees ? c.pages[r * c.pages_row + (t >> c.page_log2)] : 0;
-    const bool live = live_page(c, page);
-    float s = -__builtin_inff();
-    if (live) {
-      const int at = static_cast<int>(t) & ((1 << c.page_log2) - 1);
-      const uint32_t* const k = reinterpret_cast<const uint32_t*>(k_tile(c, page, kv));
-      float sum = 0.0f;
-      for (int d = 0; d < kDim; d += 4) {
-        const uint32_t x = k[((d >> 4 << c.page_log2) + at) * 4 + (d >> 2 & 3)];
-        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(x, false);
-        const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(x, true);
-        sum = fmaf(lo[0], query[d], fmaf(lo[1], query[d + 1], sum));
-        sum = fmaf(hi[0], query[d + 2], fmaf(hi[1], query[d + 3], sum));
-      }
-      s = sum * scale_value(c.k_scale[page * c.k_scale_page + kv]);
-    }
-    float most = s;
-    for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-    const float now = fmaxf(top, most);
-    const float keep = exp2f((top - now) * a.log2_scale);
-    const float w = live ? exp2f((s - now) * a.log2_scale) : 0.0f;
-    any = any || __any(live);
-    float sum = w;
-    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-    total = total * keep + sum;
-    o0 *= keep;
-    o1 *= keep;
-    top = now;
-    weight[lane] = w;
-    __syncthreads();
-    for (int j = 0; j < 64 && t0 + j < sees; ++j) {
-      const int pg = __shfl(page, j);
-      if (!live_page(c, pg)) continue;
-      const int at = static_cast<int>(t0 + j) & ((1 << c.page_log2) - 1);
-      const uint8_t* const v = v_tile(c, pg, kv) + (at >> 4) * (kDim * 16) + (at & 15);
-      const auto x = __builtin_amdgcn_cvt_pk_f32_fp8(v[lane * 32] | v[lane * 32 + 16] << 8, false);
-      const float vs = scale_value(c.v_scale[pg * c.v_scale_page + kv]);
-      o0 = fmaf(weight[j] * vs, x[0], o0);
-      o1 = fmaf(weight[j] * vs, x[1], o1);
-    }
-    __syncthreads();
-  }
-  const float inverse = 1.0f / total;
-  o0 = any ? o0 * inverse : 0.0f;
-  o1 = any ? o1 * inverse : 0.0f;
-  if (a.gate != nullptr && any) {
-    const uint16_t* const g = a.gate + row * a.gate_row + head * kDim + 2 * lane;
-    o0 *= sigmoid(bf16_to_f32(g[0]));
-    o1 *= sigmoid(bf16_to_f32(g[1]));
-  }
-  const uint32_t bits = f32_to_bf16(o0) | static_cast<uint32_t>(f32_to_bf16(o1)) << 16;
-  __builtin_memcpy(a.out + (row * a.q_heads + head) * kDim + 2 * lane, &bits, 4);
+__device__ __forceinline__ uint32_t tiles_of(const DecodeAttention& p, int r) {
+  if (r >= p.cache.requests) return 0;
+  const Request q = request_of(p.cache, r);
+  const int64_t rows = q.last - q.first;
+  return rows <= 0 || rows > p.a.width ? 0 : (static_cast<uint32_t>(q.tokens) + kTile - 1) / kTile;
 }
 
-int launch(const ld_paged_cache* cache, const ld_attention_args* args, bool decode, void* stream) {
-  AttentionParams p{};
+// Requests and their tiles, 64 requests at a time, one a lane; every lane of a wave calls it.
+struct Walk {
+  int base = 0;            // the first of the 64
+  uint64_t before = 0;     // tiles of the requests before it
+  uint32_t mine = 0;       // this lane's request's tiles
+  uint32_t behind = 0;     // tiles of the 64 up to and with it
+  uint32_t all = 0;        // of the 64
+
+  __device__ __forceinline__ void load(const DecodeAttention& p, int first) {
+    const int lane = threadIdx.x & 63;
+    base = first;
+    mine = tiles_of(p, first + lane);
+    behind = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t x = __shfl_up(behind, d);
+      behind += lane >= d ? x : 0;
+    }
+    all = __builtin_amdgcn_readlane(behind, 63);
+  }
+  // Tiles of all requests; ends at the first 64 again.
+  __device__ __forceinline__ uint64_t total(const DecodeAttention& p) {
+    load(p, 0);
+    uint64_t sum = all;
+    if (p.cache.requests > 64) {
+      for (int first = 64; first < p.cache.requests; first += 64) {
+        load(p, first);
+        sum += all;
+      }
+      load(p, 0);
+    }
+    return sum;
+  }
+  // The request that has tile `at` of all (which there is, and which is not before the 64), and
+  // the tiles of those before it.
+  __device__ __forceinline__ int find(const DecodeAttention& p, uint64_t at, uint64_t& first,
+                                      uint32_t& tiles) {
+    while (at >= before + all) {
+      before += all;
+      load(p, base + 64);
+    }
+    const uint32_t local = static_cast<uint32_t>(at - before);
+    const int k = __popcll(__ballot(behind <= local));
+    tiles = __builtin_amdgcn_readlane(mine, k);
+    first = before + __builtin_amdgcn_readlane(behind, k) - tiles;
+    return base + k;
+  }
+};
+
+__device__ __forceinline__ uint64_t run_length(const DecodeAttention& p, uint64_t total) {
+  const uint64_t run = (total * p.cache.kv_heads + p.workers - 1) / p.workers;
+  return run > kLeastRun ? run : kLeastRun;
+}
+
+// Sums of a run in the workspace: two a workgroup (a run's first piece and, where it is another
+// one, its last), of `stride` columns each: outputs, then the maximum and sum of each column.
+__device__ __forceinline__ float* piece_at(const DecodeAttention& p, uint64_t worker, int which,
+                                           int stride) {
+  return p.a.workspace + (((worker * 2 + which) * gridDim.y + blockIdx.y) * stride) * (kDim + 2);
+}
+
+__device__ __forceinline__ u32x4 eight_bf16(const float (&x)[8]) {
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = bf16_pair(f32x2{x[2 * i], x[2 * i + 1]});
+  return r;
+}
+
+// Eight elements of an output: divided, gated and rounded.
+__device__ __forceinline__ void store_out(const Attention& a, int64_t row, int head, int d,
+                                          float (&o)[8], float top, float total) {
+  const bool some = top > -__builtin_inff();   // the row sees a token
+  const float inverse = 1.0f / total;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = some ? o[i] * inverse : 0.0f;
+  if (a.gate != nullptr && some) {
+    uint16_t g[8];
+    __builtin_memcpy(g, a.gate + row * a.gate_row + head * kDim + d, 16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] *= sigmoid(bf16_to_f32(g[i]));
+  }
+  const u32x4 bits = eight_bf16(o);
+  __builtin_memcpy(a.out + (row * a.q_heads + head) * kDim + d, &bits, 16);
+}
+
+template <int CT>
+__global__ __launch_bounds__(kThreads, CT <= 2 ? 2 : 1) void attention_decode_kernel(
+    const DecodeAttention p) {
+  const Cache& c = p.cache;
+  const Attention& a = p.a;
+  constexpr int kCols = 16 * CT;
+  constexpr int kPad = kDim + 4;
+  __shared__ __attribute__((aligned(16))) float sums[kWaves][16][kPad];
+  __shared__ float stats[kWaves][2][kCols];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m = lane & 15, h = lane >> 4;
+  const int column0 = blockIdx.y * kCols;
+
+  Walk walk;
+  const uint64_t total = walk.total(p);
+  const uint64_t run = run_length(p, total);
+  const uint64_t start = blockIdx.x * run;
+  const uint64_t end = min(start + run, total * c.kv_heads);
+  for (uint64_t at = start; at < end;) {
+    uint64_t first;
+    uint32_t tiles;
+    const int r = walk.find(p, at / c.kv_heads, first, tiles);
+    const uint32_t local = static_cast<uint32_t>(at - first * c.kv_heads);
+    const int head = static_cast<int>(local / tiles);
+    const uint32_t from = local - head * tiles;
+    const uint32_t to = static_cast<uint32_t>(min(static_cast<uint64_t>(tiles), from + (end - at)));
+    const Request q = request_of(c, r);
+    const int rows = static_cast<int>(q.last - q.first);
+    const int32_t* const table = c.pages + r * c.pages_row;
+
+    // the columns' queries, and how many tokens each sees (a column that there is not: all)
+    bf16x8 query[CT][4];
+    int limit[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int column = column0 + 16 * ct + m;
+      const int t = column / a.group;
+      const bool real = column < p.columns && t < rows;
+      limit[ct] = real ? static_cast<int>(max(min(q.first + t + q.shift + 1,
+                                                  static_cast<int64_t>(q.tokens)), int64_t{0}))
+                       : q.tokens;
+      const uint16_t* const from_q = a.q + (q.first + (real ? t : 0)) * a.q_row +
+                                     (head * a.group + (real ? column - t * a.group : 0)) * kDim;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        u32x4 x;
+        __builtin_memcpy(&x, from_q + 16 * (4 * (s >> 1) + h) + 8 * (s & 1), 16);
+        query[ct][s] = __builtin_bit_cast(bf16x8, real ? x : u32x4{0, 0, 0, 0});
+      }
+    }
+    const int least = static_cast<int>(max(min(q.first + q.shift + 1, static_cast<int64_t>(q.tokens)),
+                                           int64_t{0}));   // what the first row sees
+
+    f32x4 o[CT][8];
+    float top[CT], sum[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      top[ct] = -__builtin_inff();
+      sum[ct] = 0.0f;
+#pragma unroll
+      for (int b = 0; b < 8; ++b) o[ct][b] = f32x4{0, 0, 0, 0};
+    }
+
+    // A tile's pages: that of tokens 16 (m / 4) .. for the keys, 16 h .. for the values (0, whose
+    // bytes are read and not used, where there is none).
+    auto page_of = [&](uint32_t tile, int group) {
+      const int token = static_cast<int>(tile) * kTile + 16 * group;
+      const int page = tile < to && token < q.tokens ? table[token >> c.page_log2] : 0;
+      return live_page(c, page) ? page : 0;
+    };
+    u32x4 keys[4][2], values[8];
+    float k_scale, v_scale;
+    auto load_keys = [&](uint32_t tile, int page) {
+      const int in = (static_cast<int>(tile) * kTile + 16 * (m >> 2)) & ((1 << c.page_log2) - 1);
+      const uint8_t* const at_k = k_tile(c, page, head) + (((h << c.page_log2) + in + (m & 3)) << 4);
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          keys[t][s] = *reinterpret_cast<const u32x4*>(at_k + 64 * t + (s << (6 + c.page_log2)));
+      k_scale = scale_value(c.k_scale[page * c.k_scale_page + head]);
+    };
+    auto load_values = [&](uint32_t tile, int page) {
+      const int in = (static_cast<int>(tile) * kTile + 16 * h) & ((1 << c.page_log2) - 1);
+      const uint8_t* const at_v = v_tile(c, page, head) + (in >> 4) * (kDim * 16) + m * 16;
+#pragma unroll
+      for (int b = 0; b < 8; ++b) values[b] = *reinterpret_cast<const u32x4*>(at_v + b * 256);
+      v_scale = scale_value(c.v_scale[page * c.v_scale_page + head]);
+    };
+
+    uint32_t tile = from + wave;
+    int k_page = page_of(tile, m >> 2), v_page = page_of(tile, h);
+    int k_next = page_of(tile + kWaves, m >> 2), v_next = page_of(tile + kWaves, h);
+    if (tile < to) {
+      load_keys(tile, k_page);
+      load_values(tile, v_page);
+    }
+    for (; tile < to; tile += kWaves) {
+      const int token0 = static_cast<int>(tile) * kTile;
+      const bool live = v_page > 0;
+      f32x4 score[CT][4];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) score[ct][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const u32x4 x = keys[t][s >> 1];
+          const bf16x8 k = operand8(x[2 * (s & 1)], x[2 * (s & 1) + 1], k_scale);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) score[ct][t] = mfma16(k, query[ct][s], score[ct][t]);
+        }
+      const bool more = tile + kWaves < to;
+      if (more) load_keys(tile + kWaves, k_next);
+      k_page = k_next;
+      const int v_now = v_next;
+      k_next = page_of(tile + 2 * kWaves, m >> 2);
+      v_next = page_of(tile + 2 * kWaves, h);
+
+      // a tile that some column does not see whole: scores of -inf, weights of zero
+      const bool whole = token0 + kTile <= least && __all(live);
+      bf16x8 weight[CT][2];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        if (!whole) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (!live || token0 + 16 * h + 4 * t + i >= limit[ct]) score[ct][t][i] = -__builtin_inff();
+        }
+        float most = kLowest;   // (of a score of -inf that is seen: a weight of zero, not none)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) most = fmaxf(most, score[ct][t][i]);
+        if (!whole && (!live || token0 + 16 * h >= limit[ct])) most = -__builtin_inff();
+        most = max_over_quarters(most);
+        const float now = fmaxf(top[ct], most);
+        if (__any(now > top[ct])) {
+          const float keep = now == top[ct] ? 1.0f : exp2_fast((top[ct] - now) * a.log2_scale);
+          sum[ct] *= keep;
+#pragma unroll
+          for (int b = 0; b < 8; ++b) o[ct][b] *= keep;
+          top[ct] = now;
+        }
+        const float less = now == -__builtin_inff() ? 0.0f : -now * a.log2_scale;
+        u32x4 bits[2];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          float w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            w[i] = exp2_fast(fmaf(score[ct][t][i], a.log2_scale, less));
+            sum[ct] += w[i];
+          }
+          bits[t >> 1][2 * (t & 1)] = bf16_pair(f32x2{w[0], w[1]});
+          bits[t >> 1][2 * (t & 1) + 1] = bf16_pair(f32x2{w[2], w[3]});
+        }
+        weight[ct][0] = __builtin_bit_cast(bf16x8, bits[0]);
+        weight[ct][1] = __builtin_bit_cast(bf16x8, bits[1]);
+      }
+
+      if (!whole) {
+        // values behind the last token, or without a page, take no part; a value that is not
+        // finite reaches the columns that see its token alone
+        const int kept = live ? q.tokens - (token0 + 16 * h) : 0;
+        uint32_t strange = 0;
+#pragma unroll
+        for (int b = 0; b < 8; ++b)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            values[b][w] &= first_bytes(kept - 4 * w);
+            strange |= nan_bytes(values[b][w]);
+          }
+        if (__any(strange != 0)) {
+          bf16x8 seen[CT][2];
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              u32x4 bits;
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                const int token = token0 + 16 * h + 8 * u + 2 * w;
+                bits[w] = (live && token < limit[ct] ? 0x3f80u : 0u) |
+                          (live && token + 1 < limit[ct] ? 0x3f800000u : 0u);
+              }
+              seen[ct][u] = __builtin_bit_cast(bf16x8, bits);
+            }
+#pragma unroll
+          for (int b = 0; b < 8; ++b) {
+            u32x4 ones;   // e4m3's 1 where a value is NaN
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t at_nan = nan_bytes(values[b][w]) >> 7;
+              ones[w] = at_nan * 0x38u;
+              values[b][w] &= ~(at_nan * 0xffu);
+            }
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+              f32x4 count = {0, 0, 0, 0};
+#pragma unroll
+              for (int u = 0; u < 2; ++u)
+                count = mfma16(operand8(ones[2 * u], ones[2 * u + 1], 1.0f), seen[ct][u], count);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (count[i] > 0.0f) o[ct][b][i] = __builtin_nanf("");
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < 8; ++b)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const bf16x8 v = operand8(values[b][2 * u], values[b][2 * u + 1], v_scale);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) o[ct][b] = mfma16(v, weight[ct][u], o[ct][b]);
+        }
+      v_page = v_now;
+      if (more) load_values(tile + kWaves, v_page);
+    }
+
+    // the waves' sums joined, sixteen columns at a time: thread (column, eight elements)
+    const bool entire = from == 0 && to == tiles;
+    float* const piece = piece_at(p, blockIdx.x, at == start ? 0 : 1, kCols);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float s = sum[ct];
+      s = add_partner<32>(add_partner<16>(s));
+      if (h == 0) {
+        stats[wave][0][16 * ct + m] = top[ct];
+        stats[wave][1][16 * ct + m] = s;
+      }
+#pragma unroll
+      for (int b = 0; b < 8; ++b)
+        *reinterpret_cast<f32x4*>(&sums[wave][m][16 * b + 4 * h]) = o[ct][b];
+      __syncthreads();
+      const int mine = threadIdx.x >> 4, d = 8 * (threadIdx.x & 15);
+      const int column = column0 + 16 * ct + mine;
+      const int t = column / a.group;
+      float best = -__builtin_inff();
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) best = fmaxf(best, stats[w][0][16 * ct + mine]);
+      float all = 0.0f, x[8] = {};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float theirs = stats[w][0][16 * ct + mine];
+        const float keep = theirs == best ? 1.0f : exp2_fast((theirs - best) * a.log2_scale);
+        if (theirs > -__builtin_inff()) {
+          all = fmaf(stats[w][1][16 * ct + mine], keep, all);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = fmaf(sums[w][mine][d + i], keep, x[i]);
+        }
+      }
+      if (column < p.columns && t < rows) {
+        if (entire) {
+          store_out(a, q.first + t, head * a.group + column - t * a.group, d, x, best, all);
+        } else {
+          float* const to_o = piece + (16 * ct + mine) * kDim + d;
+          *reinterpret_cast<f32x4*>(to_o) = f32x4{x[0], x[1], x[2], x[3]};
+          *reinterpret_cast<f32x4*>(to_o + 4) = f32x4{x[4], x[5], x[6], x[7]};
+          if (d == 0) {
+            piece[kCols * kDim + 2 * (16 * ct + mine)] = best;
+            piece[kCols * kDim + 2 * (16 * ct + mine) + 1] = all;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    at += to - from;
+  }
+}
+
+// One column of a request and kv head a workgroup: joins the sums of the runs that its tiles were
+// cut into, in their order; zeros for a request without tokens or with more rows than the width.
+// Each wave takes every fourth piece, two elements a lane.
+__global__ __launch_bounds__(kThreads) void attention_join_kernel(const DecodeAttention p, int cols) {
+  const Cache& c = p.cache;
+  const Attention& a = p.a;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int q_head = blockIdx.x % a.q_heads;
+  const int64_t rest = blockIdx.x / a.q_heads;
+  const int t = static_cast<int>(rest % a.width);
+  const int r = static_cast<int>(rest / a.width);
+  const Request q = request_of(c, r);
+  const int64_t rows = q.last - q.first;
+  if (t >= rows) return;
+  Walk walk;
+  const uint64_t total = walk.total(p);
+  if (tiles_of(p, r) == 0) {
+    for (int64_t row = q.first + t; row < q.last; row += a.width)
+      if (threadIdx.x < 64)
+        reinterpret_cast<uint32_t*>(a.out + (row * a.q_heads + q_head) * kDim)[lane] = 0;
+    return;
+  }
+  while (walk.base + 64 <= r) {
+    walk.before += walk.all;
+    walk.load(p, walk.base + 64);
+  }
+  const uint32_t tiles = __builtin_amdgcn_readlane(walk.mine, r & 63);
+  const uint64_t first = walk.before + __builtin_amdgcn_readlane(walk.behind, r & 63) - tiles;
+  const uint64_t run = run_length(p, total);
+  const int head = q_head / a.group;
+  const uint64_t begin = first * c.kv_heads + static_cast<uint64_t>(head) * tiles;
+  const uint64_t w0 = begin / run, w1 = (begin + tiles - 1) / run;
+  if (w0 == w1) return;   // one run had them all
+  const int column = t * a.group + q_head - head * a.group;
+  const int y = column / cols, within = column % cols;
+  const int grid_y = (p.columns + cols - 1) / cols;
+  auto piece = [&](uint64_t w) {
+    const int which = w == w0 && begin != w * run ? 1 : 0;
+    return a.workspace + (((w * 2 + which) * grid_y + y) * cols) * (kDim + 2);
+  };
+  // the largest of the pieces' maxima
+  float best = -__builtin_inff();
+  for (uint64_t w = w0 + threadIdx.x; w <= w1; w += kThreads)
+    best = fmaxf(best, piece(w)[cols * kDim + 2 * within]);
+  __shared__ float shared[kWaves];
+  __shared__ float outs[kWaves][kDim + 1];
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) best = fmaxf(best, __shfl_xor(best, d));
+  if (lane == 0) shared[wave] = best;
+  __syncthreads();
+  best = fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
+  float x0 = 0.0f, x1 = 0.0f, all = 0.0f;
+#pragma unroll 4
+  for (uint64_t w = w0 + wave; w <= w1; w += kWaves) {
+    const float* const from = piece(w);
+    const float top = from[cols * kDim + 2 * within];
+    const float keep = top == best ? 1.0f : exp2_fast((top - best) * a.log2_scale);
+    const float s = from[cols * kDim + 2 * within + 1];
+    const float o0 = from[within * kDim + 2 * lane], o1 = from[within * kDim + 2 * lane + 1];
+    if (top > -__builtin_inff()) {
+      all = fmaf(s, keep, all);
+      x0 = fmaf(o0, keep, x0);
+      x1 = fmaf(o1, keep, x1);
+    }
+  }
+  outs[wave][2 * lane] = x0;
+  outs[wave][2 * lane + 1] = x1;
+  if (lane == 0) outs[wave][kDim] = all;
+  __syncthreads();
+  if (threadIdx.x < kDim / 8) {
+    const int d = 8 * threadIdx.x;
+    float o[8], s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) s += outs[w][kDim];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = (outs[0][d + i] + outs[1][d + i]) + (outs[2][d + i] + outs[3][d + i]);
+    store_out(a, q.first + t, q_head, d, o, best, s);
+  }
+}
+
+// Workgroups of the first launch: two a CU (one with 64 columns), fewer where no table is long
+// enough for a least run each; tiles of 16 columns of each; and the rest of the columns' blocks.
+struct Shape {
+  int64_t workers;
+  int tiles, blocks;
+  int64_t bytes;
+};
+
+Shape decode_shape(const ld_paged_cache& c, int64_t q_heads, int64_t width) {
+  Shape s{};
+  const int64_t columns = width * (q_heads / c.num_kv_heads);
+  s.tiles = columns <= 16 ? 1 : columns <= 32 ? 2 : 4;
+  s.blocks = static_cast<int>((columns + 16 * s.tiles - 1) / (16 * s.tiles));
+  const int64_t tiles = (static_cast<int64_t>(c.table_width) * c.page_size + kTile - 1) / kTile;
+  const double most = static_cast<double>(tiles) * c.num_requests * c.num_kv_heads / kLeastRun;
+  const int64_t chip = std::max<int64_t>(64, (s.tiles == 4 ? 256 : 512) / s.blocks);
+  s.workers = most >= chip ? chip : static_cast<int64_t>(most) + 1;
+  s.bytes = s.workers * 2 * s.blocks * 16 * s.tiles * (kDim + 2) * 4;
+  return s;
+}
+
+int check_decode(const ld_paged_cache* cache, const ld_attention_args* args, DecodeAttention& p) {
   if (const int rc = cache_params(cache, p.cache)) return rc;
   if (const int rc = attention_params(*cache, args, p.a)) return rc;
-  if (decode && (args->width < 1 || args->width > LD_MAX_TOKENS))
+  if (args->width < 1 || args->width > LD_MAX_TOKENS)
     return fail(LD_ERR_INVALID_ARGUMENT, "decode/MTP supports 1 through 4 tokens per request");
-  if (p.cache.requests == 0) return LD_OK;
-  if (!decode) p.a.width = 0;
-  const int64_t blocks = p.cache.num_tokens * p.a.q_heads;
-  if (blocks > 0x7fffffff) return fail(LD_ERR_INVALID_ARGUMENT, "too many rows and heads");
-  hipLaunchKernelGGL(attention_rows_kernel, dim3(static_cast<uint32_t>(blocks)), dim3(64), 0,
-                     static_cast<hipStream_t>(stream), p);
-  return check_launch(decode ? "ld_attention_decode" : "ld_attention_prefill");
+  return LD_OK;
 }
 
 }  // namespace
 }  // namespace ld
 
-extern "C" int64_t ld_attention_decode_workspace_bytes(const ld_paged_cache*,
-                                                       const ld_attention_args*) {
-  return 0;
-}
-extern "C" int64_t ld_attention_prefill_workspace_bytes(const ld_paged_cache*,
-                                                        const ld_attention_args*) {
-  return 0;
+extern "C" int64_t ld_attention_decode_workspace_bytes(const ld_paged_cache* cache,
+                                                       const ld_attention_args* args) {
+  using namespace ld;
+  if (cache == nullptr || args == nullptr || cache->num_requests <= 0 || cache->num_tokens <= 0 ||
+      cache->num_kv_heads <= 0 || args->num_q_heads < cache->num_kv_heads || args->width < 1 ||
+      args->width > LD_MAX_TOKENS || cache->table_width < 0)
+    return 0;
+  return decode_shape(*cache, args->num_q_heads, args->width).bytes;
 }
 
 extern "C" int ld_attention_decode(const ld_paged_cache* cache, const ld_attention_args* args,
                                    void* stream) {
-  return ld::launch(cache, args, true, stream);
-}
-
-extern "C" int ld_attention_prefill(const ld_paged_cache* cache, const ld_attention_args* args,
-                                    void* stream) {
-  return ld::launch(cache, args, false, stream);
+  using namespace ld;
+  DecodeAttention p{};
+  if (const int rc = check_decode(cache, args, p)) return rc;
+  if (p.cache.requests == 0) return LD_OK;
+  const Shape s = decode_shape(*cache, p.a.q_heads, p.a.width);
+  if (p.a.workspace == nullptr || !aligned16(p.a.workspace) || args->workspace_bytes < s.bytes)
+    return fail(LD_ERR_INVALID_ARGUMENT, "workspace missing or too small");
+  const int64_t joins = static_cast<int64_t>(p.cache.requests) * p.a.width * p.a.q_heads;
+  if (joins > 0x7fffffff) return fail(LD_ERR_INVALID_ARGUMENT, "too many requests and heads");
+  p.workers = static_cast<int32_t>(s.workers);
+  p.columns = p.a.width * p.a.group;
+  const auto kernel = s.tiles == 1   ? attention_decode_kernel<1>
+                      : s.tiles == 2 ? attention_decode_kernel<2>
+                                     : attention_decode_kernel<4>;
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(s.workers), s.blocks), dim3(kThreads), 0, on, p);
+  if (const int rc = check_launch("ld_attention_decode")) return rc;
+  hipLaunchKernelGGL(attention_join_kernel, dim3(static_cast<uint32_t>(joins)), dim3(kThreads), 0,
+                     on, p, 16 * s.tiles);
+  return check_launch("ld_attention_decode");
 }
