@@ -21,7 +21,6 @@ namespace ld {
 namespace {
 
 constexpr int kTile = 64;        // tokens
-constexpr int kLeastRun = kWaves;  // tiles of a workgroup's run at the least
 
 struct DecodeAttention {
   Cache cache;
@@ -30,26 +29,38 @@ struct DecodeAttention {
   int32_t columns;   // width * group
 };
 
-__device__ __forceinline__ uint32_t tiles_of(const DecodeAttention& p, int r) {
-  if (r >= p.cache.requests) return 0;
-  const Request q = request_of(p.cache, r);
-  const int64_t rows = q.last - q.first;
-  return rows <= 0 || rows > p.a.width ? 0 : (static_cast<uint32_t>(q.tokens) + kTile - 1) / kTile;
+// The workspace: the sums of runs, two a workgroup (a run's first piece and, where it is another
+// one, its last), `blocks` x 16 CT columns each: outputs, then the maximum and sum of each column.  Ahead
+// of them the run's length and of each request the tiles ahead of it, for the second launch.
+struct Layout {
+  int64_t plan;      // floats
+  int64_t columns;   // of a piece
+  __device__ __host__ int64_t piece(int64_t worker, int which) const {
+    return plan + (worker * 2 + which) * columns * (kDim + 2);
+  }
+};
+__device__ __host__ inline Layout layout_of(int64_t requests, int64_t columns) {
+  return Layout{(2 * (requests + 2) + 3) & ~int64_t{3}, columns};
 }
 
 // Requests and their tiles, 64 requests at a time, one a lane; every lane of a wave calls it.
 struct Walk {
   int base = 0;            // the first of the 64
   uint64_t before = 0;     // tiles of the requests before it
-  uint32_t mine = 0;       // this lane's request's tiles
+  Request mine;            // this lane's request
+  uint32_t tiles = 0;      // its tiles
   uint32_t behind = 0;     // tiles of the 64 up to and with it
   uint32_t all = 0;        // of the 64
 
   __device__ __forceinline__ void load(const DecodeAttention& p, int first) {
     const int lane = threadIdx.x & 63;
     base = first;
-    mine = tiles_of(p, first + lane);
-    behind = mine;
+    const bool real = first + lane < p.cache.requests;
+    mine = request_of(p.cache, real ? first + lane : 0);
+    const int64_t rows = mine.last - mine.first;
+    tiles = real && rows > 0 && rows <= p.a.width
+                ? (static_cast<uint32_t>(mine.tokens) + kTile - 1) / kTile : 0;
+    behind = tiles;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const uint32_t x = __shfl_up(behind, d);
@@ -57,45 +68,48 @@ struct Walk {
     }
     all = __builtin_amdgcn_readlane(behind, 63);
   }
-  // Tiles of all requests; ends at the first 64 again.
-  __device__ __forceinline__ uint64_t total(const DecodeAttention& p) {
-    load(p, 0);
-    uint64_t sum = all;
-    if (p.cache.requests > 64) {
-      for (int first = 64; first < p.cache.requests; first += 64) {
-        load(p, first);
-        sum += all;
-      }
-      load(p, 0);
+  // Tiles of all requests; ends at the first 64 again.  `plan`: where those ahead of each request
+  // are written (NULL: nowhere).
+  __device__ __forceinline__ uint64_t total(const DecodeAttention& p, uint64_t* plan) {
+    uint64_t sum = 0;
+    for (int first = 0;; first += 64) {
+      load(p, first);
+      const int r = first + (threadIdx.x & 63);
+      if (plan != nullptr && r < p.cache.requests) plan[1 + r] = sum + behind - tiles;
+      sum += all;
+      if (first + 64 >= p.cache.requests) break;
     }
+    if (p.cache.requests > 64) load(p, 0);
     return sum;
   }
-  // The request that has tile `at` of all (which there is, and which is not before the 64), and
-  // the tiles of those before it.
-  __device__ __forceinline__ int find(const DecodeAttention& p, uint64_t at, uint64_t& first,
-                                      uint32_t& tiles) {
+  // The request that has tile `at` of all (which there is, and which is not before the 64): its
+  // tiles, those of the requests before it, its number and what it has in the call.
+  __device__ __forceinline__ uint32_t find(const DecodeAttention& p, uint64_t at, uint64_t& first,
+                                           int& number, Request& q) {
     while (at >= before + all) {
       before += all;
       load(p, base + 64);
     }
     const uint32_t local = static_cast<uint32_t>(at - before);
     const int k = __popcll(__ballot(behind <= local));
-    tiles = __builtin_amdgcn_readlane(mine, k);
-    first = before + __builtin_amdgcn_readlane(behind, k) - tiles;
-    return base + k;
+    const uint32_t n = __builtin_amdgcn_readlane(tiles, k);
+    first = before + __builtin_amdgcn_readlane(behind, k) - n;
+    number = base + k;
+    // (rows are below 2^31)
+    q.first = __builtin_amdgcn_readlane(static_cast<int>(mine.first), k);
+    q.last = __builtin_amdgcn_readlane(static_cast<int>(mine.last), k);
+    q.shift = static_cast<int64_t>(
+        static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine.shift >> 32), k))) << 32 |
+        static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine.shift), k)));
+    q.tokens = __builtin_amdgcn_readlane(mine.tokens, k);
+    return n;
   }
 };
 
+// Tiles of a workgroup's run: a whole number for each of its waves.
 __device__ __forceinline__ uint64_t run_length(const DecodeAttention& p, uint64_t total) {
   const uint64_t run = (total * p.cache.kv_heads + p.workers - 1) / p.workers;
-  return run > kLeastRun ? run : kLeastRun;
-}
-
-// Sums of a run in the workspace: two a workgroup (a run's first piece and, where it is another
-// one, its last), of `stride` columns each: outputs, then the maximum and sum of each column.
-__device__ __forceinline__ float* piece_at(const DecodeAttention& p, uint64_t worker, int which,
-                                           int stride) {
-  return p.a.workspace + (((worker * 2 + which) * gridDim.y + blockIdx.y) * stride) * (kDim + 2);
+  return max((run + kWaves - 1) / kWaves, uint64_t{1}) * kWaves;
 }
 
 __device__ __forceinline__ u32x4 eight_bf16(const float (&x)[8]) {
@@ -131,31 +145,40 @@ __global__ __launch_bounds__(kThreads, CT <= 2 ? 2 : 1) void attention_decode_ke
   constexpr int kPad = kDim + 4;
   __shared__ __attribute__((aligned(16))) float sums[kWaves][16][kPad];
   __shared__ float stats[kWaves][2][kCols];
+  // the columns' queries as operands, where registers hold no more than sixteen columns'
+  __shared__ __attribute__((aligned(16))) u32x4 queries[CT > 1 ? CT : 1][4][CT > 1 ? 64 : 1];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, h = lane >> 4;
   const int column0 = blockIdx.y * kCols;
 
+  const Layout layout = layout_of(c.requests, static_cast<int64_t>(gridDim.y) * kCols);
+  const bool planner = blockIdx.x == 0 && blockIdx.y == 0 && wave == 0;
+  uint64_t* const plan = planner ? reinterpret_cast<uint64_t*>(a.workspace) : nullptr;
   Walk walk;
-  const uint64_t total = walk.total(p);
+  const uint64_t total = walk.total(p, plan);
   const uint64_t run = run_length(p, total);
+  if (planner && lane == 0) {
+    plan[0] = run;
+    plan[1 + c.requests] = total;
+  }
   const uint64_t start = blockIdx.x * run;
   const uint64_t end = min(start + run, total * c.kv_heads);
   for (uint64_t at = start; at < end;) {
     uint64_t first;
-    uint32_t tiles;
-    const int r = walk.find(p, at / c.kv_heads, first, tiles);
+    int r;
+    Request q;
+    const uint32_t tiles = walk.find(p, at / c.kv_heads, first, r, q);
     const uint32_t local = static_cast<uint32_t>(at - first * c.kv_heads);
     const int head = static_cast<int>(local / tiles);
     const uint32_t from = local - head * tiles;
     const uint32_t to = static_cast<uint32_t>(min(static_cast<uint64_t>(tiles), from + (end - at)));
-    const Request q = request_of(c, r);
     const int rows = static_cast<int>(q.last - q.first);
     const int32_t* const table = c.pages + r * c.pages_row;
 
     // the columns' queries, and how many tokens each sees (a column that there is not: all)
-    bf16x8 query[CT][4];
+    bf16x8 query[4];
     int limit[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
@@ -167,13 +190,19 @@ __global__ __launch_bounds__(kThreads, CT <= 2 ? 2 : 1) void attention_decode_ke
                        : q.tokens;
       const uint16_t* const from_q = a.q + (q.first + (real ? t : 0)) * a.q_row +
                                      (head * a.group + (real ? column - t * a.group : 0)) * kDim;
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
+      auto load_query = [&](int s) {
         u32x4 x;
         __builtin_memcpy(&x, from_q + 16 * (4 * (s >> 1) + h) + 8 * (s & 1), 16);
-        query[ct][s] = __builtin_bit_cast(bf16x8, real ? x : u32x4{0, 0, 0, 0});
+        return real ? x : u32x4{0, 0, 0, 0};
+      };
+      if constexpr (CT == 1) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) query[s] = __builtin_bit_cast(bf16x8, load_query(s));
+      } else {
+        queries[ct][wave][lane] = load_query(wave);
       }
     }
+    if constexpr (CT > 1) __syncthreads();
     const int least = static_cast<int>(max(min(q.first + q.shift + 1, static_cast<int64_t>(q.tokens)),
                                            int64_t{0}));   // what the first row sees
 
@@ -236,7 +265,9 @@ __global__ __launch_bounds__(kThreads, CT <= 2 ? 2 : 1) void attention_decode_ke
           const u32x4 x = keys[t][s >> 1];
           const bf16x8 k = operand8(x[2 * (s & 1)], x[2 * (s & 1) + 1], k_scale);
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct) score[ct][t] = mfma16(k, query[ct][s], score[ct][t]);
+          for (int ct = 0; ct < CT; ++ct)
+            score[ct][t] = mfma16(k, CT == 1 ? query[s] : __builtin_bit_cast(bf16x8, queries[ct][s][lane]),
+                                  score[ct][t]);
         }
       const bool more = tile + kWaves < to;
       if (more) load_keys(tile + kWaves, k_next);
@@ -352,7 +383,7 @@ __global__ __launch_bounds__(kThreads, CT <= 2 ? 2 : 1) void attention_decode_ke
 
     // the waves' sums joined, sixteen columns at a time: thread (column, eight elements)
     const bool entire = from == 0 && to == tiles;
-    float* const piece = piece_at(p, blockIdx.x, at == start ? 0 : 1, kCols);
+    float* const piece = a.workspace + layout.piece(blockIdx.x, at == start ? 0 : 1);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       float s = sum[ct];
@@ -386,13 +417,11 @@ __global__ __launch_bounds__(kThreads, CT <= 2 ? 2 : 1) void attention_decode_ke
         if (entire) {
           store_out(a, q.first + t, head * a.group + column - t * a.group, d, x, best, all);
         } else {
-          float* const to_o = piece + (16 * ct + mine) * kDim + d;
+          float* const to_o = piece + static_cast<int64_t>(column) * kDim + d;
           *reinterpret_cast<f32x4*>(to_o) = f32x4{x[0], x[1], x[2], x[3]};
           *reinterpret_cast<f32x4*>(to_o + 4) = f32x4{x[4], x[5], x[6], x[7]};
-          if (d == 0) {
-            piece[kCols * kDim + 2 * (16 * ct + mine)] = best;
-            piece[kCols * kDim + 2 * (16 * ct + mine) + 1] = all;
-          }
+          if (d == 0)
+            *reinterpret_cast<f32x2*>(piece + layout.columns * kDim + 2 * column) = f32x2{best, all};
         }
       }
       __syncthreads();
@@ -401,89 +430,87 @@ __global__ __launch_bounds__(kThreads, CT <= 2 ? 2 : 1) void attention_decode_ke
   }
 }
 
-// One column of a request and kv head a workgroup: joins the sums of the runs that its tiles were
-// cut into, in their order; zeros for a request without tokens or with more rows than the width.
-// Each wave takes every fourth piece, two elements a lane.
-__global__ __launch_bounds__(kThreads) void attention_join_kernel(const DecodeAttention p, int cols) {
+// Sixteen columns of a request and kv head a workgroup: joins the sums of the runs that its tiles
+// were cut into; zeros for a request without tokens or with more rows than the width.  Four groups
+// of threads take every fourth piece, a thread eight elements of a column.
+constexpr int kJoinThreads = 1024;
+__global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const DecodeAttention p,
+                                                                      Layout layout, int tiles16) {
   const Cache& c = p.cache;
   const Attention& a = p.a;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int q_head = blockIdx.x % a.q_heads;
-  const int64_t rest = blockIdx.x / a.q_heads;
-  const int t = static_cast<int>(rest % a.width);
-  const int r = static_cast<int>(rest / a.width);
+  const int tile16 = blockIdx.x % tiles16;
+  const int rest = blockIdx.x / tiles16;
+  const int head = rest % c.kv_heads;
+  const int r = rest / c.kv_heads;
+  const uint64_t* const plan = reinterpret_cast<const uint64_t*>(a.workspace);
+  const uint64_t run = plan[0], first = plan[1 + r];
+  const uint64_t tiles = plan[2 + r] - first;
   const Request q = request_of(c, r);
   const int64_t rows = q.last - q.first;
-  if (t >= rows) return;
-  Walk walk;
-  const uint64_t total = walk.total(p);
-  if (tiles_of(p, r) == 0) {
-    for (int64_t row = q.first + t; row < q.last; row += a.width)
-      if (threadIdx.x < 64)
-        reinterpret_cast<uint32_t*>(a.out + (row * a.q_heads + q_head) * kDim)[lane] = 0;
+  const int group = threadIdx.x >> 8;
+  const int mine = threadIdx.x >> 4 & 15, d = 8 * (threadIdx.x & 15);
+  const int column = 16 * tile16 + mine;
+  const int t = column / a.group;
+  const int q_head = head * a.group + column - t * a.group;
+  if (tiles == 0) {
+    if (group == 0 && column < p.columns)
+      for (int64_t row = q.first + t; row < q.last; row += a.width)
+        *reinterpret_cast<u32x4*>(a.out + (row * a.q_heads + q_head) * kDim + d) = u32x4{0, 0, 0, 0};
     return;
   }
-  while (walk.base + 64 <= r) {
-    walk.before += walk.all;
-    walk.load(p, walk.base + 64);
-  }
-  const uint32_t tiles = __builtin_amdgcn_readlane(walk.mine, r & 63);
-  const uint64_t first = walk.before + __builtin_amdgcn_readlane(walk.behind, r & 63) - tiles;
-  const uint64_t run = run_length(p, total);
-  const int head = q_head / a.group;
-  const uint64_t begin = first * c.kv_heads + static_cast<uint64_t>(head) * tiles;
+  const uint64_t begin = first * c.kv_heads + head * tiles;
   const uint64_t w0 = begin / run, w1 = (begin + tiles - 1) / run;
   if (w0 == w1) return;   // one run had them all
-  const int column = t * a.group + q_head - head * a.group;
-  const int y = column / cols, within = column % cols;
-  const int grid_y = (p.columns + cols - 1) / cols;
-  auto piece = [&](uint64_t w) {
-    const int which = w == w0 && begin != w * run ? 1 : 0;
-    return a.workspace + (((w * 2 + which) * grid_y + y) * cols) * (kDim + 2);
-  };
-  // the largest of the pieces' maxima
-  float best = -__builtin_inff();
-  for (uint64_t w = w0 + threadIdx.x; w <= w1; w += kThreads)
-    best = fmaxf(best, piece(w)[cols * kDim + 2 * within]);
-  __shared__ float shared[kWaves];
-  __shared__ float outs[kWaves][kDim + 1];
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) best = fmaxf(best, __shfl_xor(best, d));
-  if (lane == 0) shared[wave] = best;
-  __syncthreads();
-  best = fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
-  float x0 = 0.0f, x1 = 0.0f, all = 0.0f;
+  const bool real = column < p.columns && t < rows;
+  float best = -__builtin_inff(), all = 0.0f, x[8] = {};
+  if (real) {
 #pragma unroll 4
-  for (uint64_t w = w0 + wave; w <= w1; w += kWaves) {
-    const float* const from = piece(w);
-    const float top = from[cols * kDim + 2 * within];
-    const float keep = top == best ? 1.0f : exp2_fast((top - best) * a.log2_scale);
-    const float s = from[cols * kDim + 2 * within + 1];
-    const float o0 = from[within * kDim + 2 * lane], o1 = from[within * kDim + 2 * lane + 1];
-    if (top > -__builtin_inff()) {
-      all = fmaf(s, keep, all);
-      x0 = fmaf(o0, keep, x0);
-      x1 = fmaf(o1, keep, x1);
+    for (uint64_t w = w0 + group; w <= w1; w += 4) {
+      const float* const from = a.workspace + layout.piece(w, w == w0 && begin != w * run);
+      const f32x2 stat = *reinterpret_cast<const f32x2*>(from + layout.columns * kDim + 2 * column);
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(from + static_cast<int64_t>(column) * kDim + d);
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(from + static_cast<int64_t>(column) * kDim + d + 4);
+      const float now = fmaxf(best, stat[0]);
+      if (stat[0] > -__builtin_inff()) {   // (what saw nothing has sums of zero)
+        const float keep = best == now ? 1.0f : exp2_fast((best - now) * a.log2_scale);
+        const float add = stat[0] == now ? 1.0f : exp2_fast((stat[0] - now) * a.log2_scale);
+        best = now;
+        all = all * keep + stat[1] * add;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = x[i] * keep + lo[i] * add;
+          x[4 + i] = x[4 + i] * keep + hi[i] * add;
+        }
+      }
     }
   }
-  outs[wave][2 * lane] = x0;
-  outs[wave][2 * lane + 1] = x1;
-  if (lane == 0) outs[wave][kDim] = all;
+  __shared__ __attribute__((aligned(16))) float sums[4][16][kDim + 4];
+  __shared__ f32x2 stats[4][16];
+  *reinterpret_cast<f32x4*>(&sums[group][mine][d]) = f32x4{x[0], x[1], x[2], x[3]};
+  *reinterpret_cast<f32x4*>(&sums[group][mine][d + 4]) = f32x4{x[4], x[5], x[6], x[7]};
+  if (d == 0) stats[group][mine] = f32x2{best, all};
   __syncthreads();
-  if (threadIdx.x < kDim / 8) {
-    const int d = 8 * threadIdx.x;
-    float o[8], s = 0.0f;
+  if (group > 0 || !real) return;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) s += outs[w][kDim];
+  for (int g = 0; g < 4; ++g) best = fmaxf(best, stats[g][mine][0]);
+  all = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = (outs[0][d + i] + outs[1][d + i]) + (outs[2][d + i] + outs[3][d + i]);
-    store_out(a, q.first + t, q_head, d, o, best, s);
+  for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x2 stat = stats[g][mine];
+    if (stat[0] > -__builtin_inff()) {
+      const float add = stat[0] == best ? 1.0f : exp2_fast((stat[0] - best) * a.log2_scale);
+      all = fmaf(stat[1], add, all);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = fmaf(sums[g][mine][d + i], add, x[i]);
+    }
   }
+  store_out(a, q.first + t, q_head, d, x, best, all);
 }
 
 // Workgroups of the first launch: two a CU (one with 64 columns), fewer where no table is long
-// enough for a least run each; tiles of 16 columns of each; and the rest of the columns' blocks.
+// enough for a tile a wave each; tiles of 16 columns of each; and the rest of the columns' blocks.
 struct Shape {
   int64_t workers;
   int tiles, blocks;
@@ -496,10 +523,10 @@ Shape decode_shape(const ld_paged_cache& c, int64_t q_heads, int64_t width) {
   s.tiles = columns <= 16 ? 1 : columns <= 32 ? 2 : 4;
   s.blocks = static_cast<int>((columns + 16 * s.tiles - 1) / (16 * s.tiles));
   const int64_t tiles = (static_cast<int64_t>(c.table_width) * c.page_size + kTile - 1) / kTile;
-  const double most = static_cast<double>(tiles) * c.num_requests * c.num_kv_heads / kLeastRun;
+  const double most = static_cast<double>(tiles) * c.num_requests * c.num_kv_heads / kWaves;
   const int64_t chip = std::max<int64_t>(64, (s.tiles == 4 ? 256 : 512) / s.blocks);
   s.workers = most >= chip ? chip : static_cast<int64_t>(most) + 1;
-  s.bytes = s.workers * 2 * s.blocks * 16 * s.tiles * (kDim + 2) * 4;
+  s.bytes = layout_of(c.num_requests, 16 * s.tiles * s.blocks).piece(s.workers, 0) * 4;
   return s;
 }
 
@@ -533,17 +560,18 @@ extern "C" int ld_attention_decode(const ld_paged_cache* cache, const ld_attenti
   const Shape s = decode_shape(*cache, p.a.q_heads, p.a.width);
   if (p.a.workspace == nullptr || !aligned16(p.a.workspace) || args->workspace_bytes < s.bytes)
     return fail(LD_ERR_INVALID_ARGUMENT, "workspace missing or too small");
-  const int64_t joins = static_cast<int64_t>(p.cache.requests) * p.a.width * p.a.q_heads;
+  p.columns = p.a.width * p.a.group;
+  const int tiles16 = (p.columns + 15) / 16;
+  const int64_t joins = static_cast<int64_t>(p.cache.requests) * p.cache.kv_heads * tiles16;
   if (joins > 0x7fffffff) return fail(LD_ERR_INVALID_ARGUMENT, "too many requests and heads");
   p.workers = static_cast<int32_t>(s.workers);
-  p.columns = p.a.width * p.a.group;
   const auto kernel = s.tiles == 1   ? attention_decode_kernel<1>
                       : s.tiles == 2 ? attention_decode_kernel<2>
                                      : attention_decode_kernel<4>;
   const hipStream_t on = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(s.workers), s.blocks), dim3(kThreads), 0, on, p);
   if (const int rc = check_launch("ld_attention_decode")) return rc;
-  hipLaunchKernelGGL(attention_join_kernel, dim3(static_cast<uint32_t>(joins)), dim3(kThreads), 0,
-                     on, p, 16 * s.tiles);
+  hipLaunchKernelGGL(attention_join_kernel, dim3(static_cast<uint32_t>(joins)), dim3(kJoinThreads),
+                     0, on, p, layout_of(p.cache.requests, 16 * s.tiles * s.blocks), tiles16);
   return check_launch("ld_attention_decode");
 }
