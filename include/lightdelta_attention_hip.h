@@ -108,7 +108,8 @@ typedef struct ld_attention_args {
   int64_t workspace_bytes;
 } ld_attention_args;
 
-/* Decode and speculative verify: requests of at most `width` rows (one with more gets zeros). */
+/* Decode and speculative verify: requests of at most `width` rows (one with more gets zeros).
+ * num_requests * num_kv_heads * (tokens of a table, in 64s) is below 2^30. */
 int ld_attention_decode(const ld_paged_cache* cache, const ld_attention_args* args, void* stream);
 
 /* Requests of any number of rows. */

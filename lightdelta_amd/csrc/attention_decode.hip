@@ -40,13 +40,20 @@ struct Layout {
   }
 };
 __device__ __host__ inline Layout layout_of(int64_t requests, int64_t columns) {
-  return Layout{(2 * (requests + 2) + 3) & ~int64_t{3}, columns};
+  return Layout{(requests + 2 + 3) & ~int64_t{3}, columns};
+}
+
+// The value of the lane that Ctrl names, in the rows of RowMask; 0 where there is none.
+template <int Ctrl, int RowMask>
+__device__ __forceinline__ uint32_t shifted(uint32_t x) {
+  return static_cast<uint32_t>(
+      __builtin_amdgcn_update_dpp(0, static_cast<int>(x), Ctrl, RowMask, 0xF, false));
 }
 
 // Requests and their tiles, 64 requests at a time, one a lane; every lane of a wave calls it.
 struct Walk {
   int base = 0;            // the first of the 64
-  uint64_t before = 0;     // tiles of the requests before it
+  uint32_t before = 0;     // tiles of the requests before it
   Request mine;            // this lane's request
   uint32_t tiles = 0;      // its tiles
   uint32_t behind = 0;     // tiles of the 64 up to and with it
@@ -61,17 +68,19 @@ struct Walk {
     tiles = real && rows > 0 && rows <= p.a.width
                 ? (static_cast<uint32_t>(mine.tokens) + kTile - 1) / kTile : 0;
     behind = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t x = __shfl_up(behind, d);
-      behind += lane >= d ? x : 0;
-    }
+    // (within rows of 16 lanes, then from each row's last lane to the next row, then to the upper half)
+    behind += shifted<0x111, 0xf>(behind);
+    behind += shifted<0x112, 0xf>(behind);
+    behind += shifted<0x114, 0xf>(behind);
+    behind += shifted<0x118, 0xf>(behind);
+    behind += shifted<0x142, 0xa>(behind);
+    behind += shifted<0x143, 0xc>(behind);
     all = __builtin_amdgcn_readlane(behind, 63);
   }
   // Tiles of all requests; ends at the first 64 again.  `plan`: where those ahead of each request
   // are written (NULL: nowhere).
-  __device__ __forceinline__ uint64_t total(const DecodeAttention& p, uint64_t* plan) {
-    uint64_t sum = 0;
+  __device__ __forceinline__ uint32_t total(const DecodeAttention& p, uint32_t* plan) {
+    uint32_t sum = 0;
     for (int first = 0;; first += 64) {
       load(p, first);
       const int r = first + (threadIdx.x & 63);
@@ -84,13 +93,13 @@ struct Walk {
   }
   // The request that has tile `at` of all (which there is, and which is not before the 64): its
   // tiles, those of the requests before it, its number and what it has in the call.
-  __device__ __forceinline__ uint32_t find(const DecodeAttention& p, uint64_t at, uint64_t& first,
+  __device__ __forceinline__ uint32_t find(const DecodeAttention& p, uint32_t at, uint32_t& first,
                                            int& number, Request& q) {
     while (at >= before + all) {
       before += all;
       load(p, base + 64);
     }
-    const uint32_t local = static_cast<uint32_t>(at - before);
+    const uint32_t local = at - before;
     const int k = __popcll(__ballot(behind <= local));
     const uint32_t n = __builtin_amdgcn_readlane(tiles, k);
     first = before + __builtin_amdgcn_readlane(behind, k) - n;
@@ -107,9 +116,9 @@ struct Walk {
 };
 
 // Tiles of a workgroup's run: a whole number for each of its waves.
-__device__ __forceinline__ uint64_t run_length(const DecodeAttention& p, uint64_t total) {
-  const uint64_t run = (total * p.cache.kv_heads + p.workers - 1) / p.workers;
-  return max((run + kWaves - 1) / kWaves, uint64_t{1}) * kWaves;
+__device__ __forceinline__ uint32_t run_length(const DecodeAttention& p, uint32_t total) {
+  const uint32_t each = static_cast<uint32_t>(p.workers) * kWaves;
+  return max((total * p.cache.kv_heads + each - 1) / each, 1u) * kWaves;
 }
 
 __device__ __forceinline__ u32x4 eight_bf16(const float (&x)[8]) {
@@ -155,30 +164,44 @@ __global__ __launch_bounds__(kThreads, CT <= 2 ? 2 : 1) void attention_decode_ke
 
   const Layout layout = layout_of(c.requests, static_cast<int64_t>(gridDim.y) * kCols);
   const bool planner = blockIdx.x == 0 && blockIdx.y == 0 && wave == 0;
-  uint64_t* const plan = planner ? reinterpret_cast<uint64_t*>(a.workspace) : nullptr;
+  uint32_t* const plan = planner ? reinterpret_cast<uint32_t*>(a.workspace) : nullptr;
   Walk walk;
-  const uint64_t total = walk.total(p, plan);
-  const uint64_t run = run_length(p, total);
+  const uint32_t total = walk.total(p, plan);
+  const uint32_t run = run_length(p, total);
   if (planner && lane == 0) {
     plan[0] = run;
     plan[1 + c.requests] = total;
   }
-  const uint64_t start = blockIdx.x * run;
-  const uint64_t end = min(start + run, total * c.kv_heads);
-  for (uint64_t at = start; at < end;) {
-    uint64_t first;
+  // (the host has seen to it that all tiles and two runs are below 2^32)
+  const uint32_t start = blockIdx.x * run;
+  const uint32_t end = min(start + run, total * c.kv_heads);
+  for (uint32_t at = start; at < end;) {
+    uint32_t first;
     int r;
     Request q;
     const uint32_t tiles = walk.find(p, at / c.kv_heads, first, r, q);
-    const uint32_t local = static_cast<uint32_t>(at - first * c.kv_heads);
+    const uint32_t local = at - first * c.kv_heads;
     const int head = static_cast<int>(local / tiles);
     const uint32_t from = local - head * tiles;
-    const uint32_t to = static_cast<uint32_t>(min(static_cast<uint64_t>(tiles), from + (end - at)));
+    const uint32_t to = min(tiles, from + (end - at));
     const int rows = static_cast<int>(q.last - q.first);
     const int32_t* const table = c.pages + r * c.pages_row;
 
+    // the tiles' pages first: the keys wait for them
+    // A tile's pages: that of tokens 16 (m / 4) .. for the keys, 16 h .. for the values (0, whose
+    // bytes are read and not used, where there is none).
+    auto page_of = [&](uint32_t tile, int group) {
+      const int token = static_cast<int>(tile) * kTile + 16 * group;
+      const int page = tile < to && token < q.tokens ? table[token >> c.page_log2] : 0;
+      return live_page(c, page) ? page : 0;
+    };
+    uint32_t tile = from + wave;
+    int k_page = page_of(tile, m >> 2), v_page = page_of(tile, h);
+    int k_next = page_of(tile + kWaves, m >> 2), v_next = page_of(tile + kWaves, h);
+
     // the columns' queries, and how many tokens each sees (a column that there is not: all)
     bf16x8 query[4];
+    u32x4 staged[CT];
     int limit[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
@@ -199,10 +222,9 @@ __global__ __launch_bounds__(kThreads, CT <= 2 ? 2 : 1) void attention_decode_ke
 #pragma unroll
         for (int s = 0; s < 4; ++s) query[s] = __builtin_bit_cast(bf16x8, load_query(s));
       } else {
-        queries[ct][wave][lane] = load_query(wave);
+        staged[ct] = load_query(wave);
       }
     }
-    if constexpr (CT > 1) __syncthreads();
     const int least = static_cast<int>(max(min(q.first + q.shift + 1, static_cast<int64_t>(q.tokens)),
                                            int64_t{0}));   // what the first row sees
 
@@ -216,13 +238,6 @@ __global__ __launch_bounds__(kThreads, CT <= 2 ? 2 : 1) void attention_decode_ke
       for (int b = 0; b < 8; ++b) o[ct][b] = f32x4{0, 0, 0, 0};
     }
 
-    // A tile's pages: that of tokens 16 (m / 4) .. for the keys, 16 h .. for the values (0, whose
-    // bytes are read and not used, where there is none).
-    auto page_of = [&](uint32_t tile, int group) {
-      const int token = static_cast<int>(tile) * kTile + 16 * group;
-      const int page = tile < to && token < q.tokens ? table[token >> c.page_log2] : 0;
-      return live_page(c, page) ? page : 0;
-    };
     u32x4 keys[4][2], values[8];
     float k_scale, v_scale;
     auto load_keys = [&](uint32_t tile, int page) {
@@ -243,12 +258,14 @@ __global__ __launch_bounds__(kThreads, CT <= 2 ? 2 : 1) void attention_decode_ke
       v_scale = scale_value(c.v_scale[page * c.v_scale_page + head]);
     };
 
-    uint32_t tile = from + wave;
-    int k_page = page_of(tile, m >> 2), v_page = page_of(tile, h);
-    int k_next = page_of(tile + kWaves, m >> 2), v_next = page_of(tile + kWaves, h);
     if (tile < to) {
       load_keys(tile, k_page);
       load_values(tile, v_page);
+    }
+    if constexpr (CT > 1) {   // (the last reads of earlier ones are behind a barrier)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) queries[ct][wave][lane] = staged[ct];
+      lds_barrier();
     }
     for (; tile < to; tile += kWaves) {
       const int token0 = static_cast<int>(tile) * kTile;
@@ -442,9 +459,9 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Deco
   const int rest = blockIdx.x / tiles16;
   const int head = rest % c.kv_heads;
   const int r = rest / c.kv_heads;
-  const uint64_t* const plan = reinterpret_cast<const uint64_t*>(a.workspace);
-  const uint64_t run = plan[0], first = plan[1 + r];
-  const uint64_t tiles = plan[2 + r] - first;
+  const uint32_t* const plan = reinterpret_cast<const uint32_t*>(a.workspace);
+  const uint32_t run = plan[0], first = plan[1 + r];
+  const uint32_t tiles = plan[2 + r] - first;
   const Request q = request_of(c, r);
   const int64_t rows = q.last - q.first;
   const int group = threadIdx.x >> 8;
@@ -458,14 +475,14 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Deco
         *reinterpret_cast<u32x4*>(a.out + (row * a.q_heads + q_head) * kDim + d) = u32x4{0, 0, 0, 0};
     return;
   }
-  const uint64_t begin = first * c.kv_heads + head * tiles;
-  const uint64_t w0 = begin / run, w1 = (begin + tiles - 1) / run;
+  const uint32_t begin = first * c.kv_heads + head * tiles;
+  const uint32_t w0 = begin / run, w1 = (begin + tiles - 1) / run;
   if (w0 == w1) return;   // one run had them all
   const bool real = column < p.columns && t < rows;
   float best = -__builtin_inff(), all = 0.0f, x[8] = {};
   if (real) {
 #pragma unroll 4
-    for (uint64_t w = w0 + group; w <= w1; w += 4) {
+    for (uint32_t w = w0 + group; w <= w1; w += 4) {
       const float* const from = a.workspace + layout.piece(w, w == w0 && begin != w * run);
       const f32x2 stat = *reinterpret_cast<const f32x2*>(from + layout.columns * kDim + 2 * column);
       const f32x4 lo = *reinterpret_cast<const f32x4*>(from + static_cast<int64_t>(column) * kDim + d);
@@ -514,6 +531,7 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Deco
 struct Shape {
   int64_t workers;
   int tiles, blocks;
+  double most;       // tiles of 64 tokens, were every table full
   int64_t bytes;
 };
 
@@ -523,9 +541,9 @@ Shape decode_shape(const ld_paged_cache& c, int64_t q_heads, int64_t width) {
   s.tiles = columns <= 16 ? 1 : columns <= 32 ? 2 : 4;
   s.blocks = static_cast<int>((columns + 16 * s.tiles - 1) / (16 * s.tiles));
   const int64_t tiles = (static_cast<int64_t>(c.table_width) * c.page_size + kTile - 1) / kTile;
-  const double most = static_cast<double>(tiles) * c.num_requests * c.num_kv_heads / kWaves;
+  s.most = static_cast<double>(tiles) * c.num_requests * c.num_kv_heads;
   const int64_t chip = std::max<int64_t>(64, (s.tiles == 4 ? 256 : 512) / s.blocks);
-  s.workers = most >= chip ? chip : static_cast<int64_t>(most) + 1;
+  s.workers = s.most / kWaves >= chip ? chip : static_cast<int64_t>(s.most) / kWaves + 1;
   s.bytes = layout_of(c.num_requests, 16 * s.tiles * s.blocks).piece(s.workers, 0) * 4;
   return s;
 }
@@ -564,6 +582,8 @@ extern "C" int ld_attention_decode(const ld_paged_cache* cache, const ld_attenti
   const int tiles16 = (p.columns + 15) / 16;
   const int64_t joins = static_cast<int64_t>(p.cache.requests) * p.cache.kv_heads * tiles16;
   if (joins > 0x7fffffff) return fail(LD_ERR_INVALID_ARGUMENT, "too many requests and heads");
+  if (s.most > 0x3fffffff)
+    return fail(LD_ERR_INVALID_ARGUMENT, "too many tokens of all tables and heads");
   p.workers = static_cast<int32_t>(s.workers);
   const auto kernel = s.tiles == 1   ? attention_decode_kernel<1>
                       : s.tiles == 2 ? attention_decode_kernel<2>
