@@ -5,14 +5,17 @@
 // whatever the lengths are (they are known on the device alone); runs that begin or end inside a
 // head's tiles leave sums in the workspace, which a second launch joins.
 //
-// A wave takes every fourth tile of its workgroup's run, straight from memory into the operands of
+// Each of four waves takes every fourth tile of its workgroup's run, straight from memory into the operands of
 // v_mfma_f32_16x16x32_bf16: the cache's order of bytes is theirs.  With m = lane % 16 and h = lane / 16,
 //   scores [token, column]: operand A holds the keys of token 16 (m / 4) + 4 t + m % 4 of the tile
 //     in product t (0 .. 3), so that a lane finds the scores of tokens 16 h .. 16 h + 15 of column m;
 //   outputs [element, column]: operand B is these sixteen weights, A sixteen bytes of a page's v,
 //     the same tokens of element 16 b + m.
-// Columns are the request's rows times the q heads of a kv head, CT tiles of 16.  e4m3 times its
-// scale is exact in bf16; weights are rounded to bf16, their sum is not.
+// Columns are the request's rows times the q heads of a kv head.  Where they are more than 16, two or
+// four waves take the same tile for 16 columns each (the second read of a tile is the L2's): a wave of
+// 32 columns does not fit in the registers of two a SIMD, and what it keeps in scratch memory waits
+// for the tiles in flight (31.7 us for the verify of 64 requests, @@).
+// e4m3 times its scale is exact in bf16; weights are rounded to bf16, their sum is not.
 #include <algorithm>
 
 #include "attention_common.h"
@@ -30,7 +33,7 @@ struct DecodeAttention {
 };
 
 // The workspace: the sums of runs, two a workgroup (a run's first piece and, where it is another
-// one, its last), `blocks` x 16 CT columns each: outputs, then the maximum and sum of each column.  Ahead
+// one, its last), of all columns each: outputs, then the maximum and sum of each column.  Ahead
 // of them the run's length and of each request the tiles ahead of it, for the second launch.
 struct Layout {
   int64_t plan;      // floats
@@ -145,24 +148,23 @@ __device__ __forceinline__ void store_out(const Attention& a, int64_t row, int h
   __builtin_memcpy(a.out + (row * a.q_heads + head) * kDim + d, &bits, 16);
 }
 
-template <int CT>
-__global__ __launch_bounds__(kThreads, CT <= 2 ? 2 : 1) void attention_decode_kernel(
-    const DecodeAttention p) {
+// Split: waves a tile, 16 columns each.
+template <int Split>
+__global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const DecodeAttention p) {
   const Cache& c = p.cache;
   const Attention& a = p.a;
-  constexpr int kCols = 16 * CT;
   constexpr int kPad = kDim + 4;
   __shared__ __attribute__((aligned(16))) float sums[kWaves][16][kPad];
-  __shared__ float stats[kWaves][2][kCols];
-  // the columns' queries as operands, where registers hold no more than sixteen columns'
-  __shared__ __attribute__((aligned(16))) u32x4 queries[CT > 1 ? CT : 1][4][CT > 1 ? 64 : 1];
+  __shared__ float stats[kWaves][2][16];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, h = lane >> 4;
-  const int column0 = blockIdx.y * kCols;
+  const int column0 = blockIdx.y * 16 * Split;
+  constexpr int step = kWaves / Split;   // tiles that the workgroup's waves take at a time
+  const int column = column0 + 16 * (wave & (Split - 1)) + m;
 
-  const Layout layout = layout_of(c.requests, static_cast<int64_t>(gridDim.y) * kCols);
+  const Layout layout = layout_of(c.requests, static_cast<int64_t>(gridDim.y) * 16 * Split);
   const bool planner = blockIdx.x == 0 && blockIdx.y == 0 && wave == 0;
   uint32_t* const plan = planner ? reinterpret_cast<uint32_t*>(a.workspace) : nullptr;
   Walk walk;
@@ -195,48 +197,32 @@ __global__ __launch_bounds__(kThreads, CT <= 2 ? 2 : 1) void attention_decode_ke
       const int page = tile < to && token < q.tokens ? table[token >> c.page_log2] : 0;
       return live_page(c, page) ? page : 0;
     };
-    uint32_t tile = from + wave;
+    uint32_t tile = from + wave / Split;
     int k_page = page_of(tile, m >> 2), v_page = page_of(tile, h);
-    int k_next = page_of(tile + kWaves, m >> 2), v_next = page_of(tile + kWaves, h);
+    int k_next = page_of(tile + step, m >> 2), v_next = page_of(tile + step, h);
 
-    // the columns' queries, and how many tokens each sees (a column that there is not: all)
+    // the column's query, and how many tokens it sees (one that there is not: all)
+    const int t_row = column / a.group;
+    const bool real = column < p.columns && t_row < rows;
+    const int limit = real ? static_cast<int>(max(min(q.first + t_row + q.shift + 1,
+                                                      static_cast<int64_t>(q.tokens)), int64_t{0}))
+                           : q.tokens;
+    const uint16_t* const from_q = a.q + (q.first + (real ? t_row : 0)) * a.q_row +
+                                   (head * a.group + (real ? column - t_row * a.group : 0)) * kDim;
     bf16x8 query[4];
-    u32x4 staged[CT];
-    int limit[CT];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      const int column = column0 + 16 * ct + m;
-      const int t = column / a.group;
-      const bool real = column < p.columns && t < rows;
-      limit[ct] = real ? static_cast<int>(max(min(q.first + t + q.shift + 1,
-                                                  static_cast<int64_t>(q.tokens)), int64_t{0}))
-                       : q.tokens;
-      const uint16_t* const from_q = a.q + (q.first + (real ? t : 0)) * a.q_row +
-                                     (head * a.group + (real ? column - t * a.group : 0)) * kDim;
-      auto load_query = [&](int s) {
-        u32x4 x;
-        __builtin_memcpy(&x, from_q + 16 * (4 * (s >> 1) + h) + 8 * (s & 1), 16);
-        return real ? x : u32x4{0, 0, 0, 0};
-      };
-      if constexpr (CT == 1) {
-#pragma unroll
-        for (int s = 0; s < 4; ++s) query[s] = __builtin_bit_cast(bf16x8, load_query(s));
-      } else {
-        staged[ct] = load_query(wave);
-      }
+    for (int s = 0; s < 4; ++s) {
+      u32x4 x;
+      __builtin_memcpy(&x, from_q + 16 * (4 * (s >> 1) + h) + 8 * (s & 1), 16);
+      query[s] = __builtin_bit_cast(bf16x8, real ? x : u32x4{0, 0, 0, 0});
     }
     const int least = static_cast<int>(max(min(q.first + q.shift + 1, static_cast<int64_t>(q.tokens)),
                                            int64_t{0}));   // what the first row sees
 
-    f32x4 o[CT][8];
-    float top[CT], sum[CT];
+    f32x4 o[8];
+    float top = -__builtin_inff(), sum = 0.0f;
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      top[ct] = -__builtin_inff();
-      sum[ct] = 0.0f;
-#pragma unroll
-      for (int b = 0; b < 8; ++b) o[ct][b] = f32x4{0, 0, 0, 0};
-    }
+    for (int b = 0; b < 8; ++b) o[b] = f32x4{0, 0, 0, 0};
 
     u32x4 keys[4][2], values[8];
     float k_scale, v_scale;
@@ -262,80 +248,64 @@ __global__ __launch_bounds__(kThreads, CT <= 2 ? 2 : 1) void attention_decode_ke
       load_keys(tile, k_page);
       load_values(tile, v_page);
     }
-    if constexpr (CT > 1) {   // (the last reads of earlier ones are behind a barrier)
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) queries[ct][wave][lane] = staged[ct];
-      lds_barrier();
-    }
-    for (; tile < to; tile += kWaves) {
+    for (; tile < to; tile += step) {
       const int token0 = static_cast<int>(tile) * kTile;
       const bool live = v_page > 0;
-      f32x4 score[CT][4];
+      f32x4 score[4];
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) score[ct][t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < 4; ++t) {
+        score[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
           const u32x4 x = keys[t][s >> 1];
-          const bf16x8 k = operand8(x[2 * (s & 1)], x[2 * (s & 1) + 1], k_scale);
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
-            score[ct][t] = mfma16(k, CT == 1 ? query[s] : __builtin_bit_cast(bf16x8, queries[ct][s][lane]),
-                                  score[ct][t]);
+          score[t] = mfma16(operand8(x[2 * (s & 1)], x[2 * (s & 1) + 1], k_scale), query[s], score[t]);
         }
-      const bool more = tile + kWaves < to;
-      if (more) load_keys(tile + kWaves, k_next);
+      }
+      const bool more = tile + step < to;
+      if (more) load_keys(tile + step, k_next);
       k_page = k_next;
       const int v_now = v_next;
-      k_next = page_of(tile + 2 * kWaves, m >> 2);
-      v_next = page_of(tile + 2 * kWaves, h);
+      k_next = page_of(tile + 2 * step, m >> 2);
+      v_next = page_of(tile + 2 * step, h);
 
       // a tile that some column does not see whole: scores of -inf, weights of zero
       const bool whole = token0 + kTile <= least && __all(live);
-      bf16x8 weight[CT][2];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        if (!whole) {
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (!live || token0 + 16 * h + 4 * t + i >= limit[ct]) score[ct][t][i] = -__builtin_inff();
-        }
-        float most = kLowest;   // (of a score of -inf that is seen: a weight of zero, not none)
+      float most = kLowest;   // (of a score of -inf that is seen: a weight of zero, not none)
+      if (!whole) {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) most = fmaxf(most, score[ct][t][i]);
-        if (!whole && (!live || token0 + 16 * h >= limit[ct])) most = -__builtin_inff();
-        most = max_over_quarters(most);
-        const float now = fmaxf(top[ct], most);
-        if (__any(now > top[ct])) {
-          const float keep = now == top[ct] ? 1.0f : exp2_fast((top[ct] - now) * a.log2_scale);
-          sum[ct] *= keep;
-#pragma unroll
-          for (int b = 0; b < 8; ++b) o[ct][b] *= keep;
-          top[ct] = now;
-        }
-        const float less = now == -__builtin_inff() ? 0.0f : -now * a.log2_scale;
-        u32x4 bits[2];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          float w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            w[i] = exp2_fast(fmaf(score[ct][t][i], a.log2_scale, less));
-            sum[ct] += w[i];
-          }
-          bits[t >> 1][2 * (t & 1)] = bf16_pair(f32x2{w[0], w[1]});
-          bits[t >> 1][2 * (t & 1) + 1] = bf16_pair(f32x2{w[2], w[3]});
-        }
-        weight[ct][0] = __builtin_bit_cast(bf16x8, bits[0]);
-        weight[ct][1] = __builtin_bit_cast(bf16x8, bits[1]);
+          for (int i = 0; i < 4; ++i)
+            if (!live || token0 + 16 * h + 4 * t + i >= limit) score[t][i] = -__builtin_inff();
+        if (!live || token0 + 16 * h >= limit) most = -__builtin_inff();
       }
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = fmaxf(most, score[t][i]);
+      most = max_over_quarters(most);
+      const float now = fmaxf(top, most);
+      if (__any(now > top)) {
+        const float keep = now == top ? 1.0f : exp2_fast((top - now) * a.log2_scale);
+        sum *= keep;
+#pragma unroll
+        for (int b = 0; b < 8; ++b) o[b] *= keep;
+        top = now;
+      }
+      const float less = now == -__builtin_inff() ? 0.0f : -now * a.log2_scale;
+      u32x4 bits[2];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[i] = exp2_fast(fmaf(score[t][i], a.log2_scale, less));
+          sum += w[i];
+        }
+        bits[t >> 1][2 * (t & 1)] = bf16_pair(f32x2{w[0], w[1]});
+        bits[t >> 1][2 * (t & 1) + 1] = bf16_pair(f32x2{w[2], w[3]});
+      }
+      const bf16x8 weight[2] = {__builtin_bit_cast(bf16x8, bits[0]), __builtin_bit_cast(bf16x8, bits[1])};
 
       if (!whole) {
         // values behind the last token, or without a page, take no part; a value that is not
@@ -350,20 +320,18 @@ __global__ __launch_bounds__(kThreads, CT <= 2 ? 2 : 1) void attention_decode_ke
             strange |= nan_bytes(values[b][w]);
           }
         if (__any(strange != 0)) {
-          bf16x8 seen[CT][2];
+          bf16x8 seen[2];
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
+          for (int u = 0; u < 2; ++u) {
+            u32x4 mask;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              u32x4 bits;
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                const int token = token0 + 16 * h + 8 * u + 2 * w;
-                bits[w] = (live && token < limit[ct] ? 0x3f80u : 0u) |
-                          (live && token + 1 < limit[ct] ? 0x3f800000u : 0u);
-              }
-              seen[ct][u] = __builtin_bit_cast(bf16x8, bits);
+            for (int w = 0; w < 4; ++w) {
+              const int token = token0 + 16 * h + 8 * u + 2 * w;
+              mask[w] = (live && token < limit ? 0x3f80u : 0u) |
+                        (live && token + 1 < limit ? 0x3f800000u : 0u);
             }
+            seen[u] = __builtin_bit_cast(bf16x8, mask);
+          }
 #pragma unroll
           for (int b = 0; b < 8; ++b) {
             u32x4 ones;   // e4m3's 1 where a value is NaN
@@ -373,76 +341,66 @@ __global__ __launch_bounds__(kThreads, CT <= 2 ? 2 : 1) void attention_decode_ke
               ones[w] = at_nan * 0x38u;
               values[b][w] &= ~(at_nan * 0xffu);
             }
+            f32x4 count = {0, 0, 0, 0};
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
-              f32x4 count = {0, 0, 0, 0};
+            for (int u = 0; u < 2; ++u)
+              count = mfma16(operand8(ones[2 * u], ones[2 * u + 1], 1.0f), seen[u], count);
 #pragma unroll
-              for (int u = 0; u < 2; ++u)
-                count = mfma16(operand8(ones[2 * u], ones[2 * u + 1], 1.0f), seen[ct][u], count);
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (count[i] > 0.0f) o[ct][b][i] = __builtin_nanf("");
-            }
+            for (int i = 0; i < 4; ++i)
+              if (count[i] > 0.0f) o[b][i] = __builtin_nanf("");
           }
         }
       }
 #pragma unroll
       for (int b = 0; b < 8; ++b)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const bf16x8 v = operand8(values[b][2 * u], values[b][2 * u + 1], v_scale);
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) o[ct][b] = mfma16(v, weight[ct][u], o[ct][b]);
-        }
+        for (int u = 0; u < 2; ++u)
+          o[b] = mfma16(operand8(values[b][2 * u], values[b][2 * u + 1], v_scale), weight[u], o[b]);
       v_page = v_now;
-      if (more) load_values(tile + kWaves, v_page);
+      if (more) load_values(tile + step, v_page);
     }
 
-    // the waves' sums joined, sixteen columns at a time: thread (column, eight elements)
+    // the waves' sums joined: thread (column, eight elements) of each sixteen columns
     const bool entire = from == 0 && to == tiles;
     float* const piece = a.workspace + layout.piece(blockIdx.x, at == start ? 0 : 1);
+    sum = add_partner<32>(add_partner<16>(sum));
+    if (h == 0) {
+      stats[wave][0][m] = top;
+      stats[wave][1][m] = sum;
+    }
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      float s = sum[ct];
-      s = add_partner<32>(add_partner<16>(s));
-      if (h == 0) {
-        stats[wave][0][16 * ct + m] = top[ct];
-        stats[wave][1][16 * ct + m] = s;
-      }
+    for (int b = 0; b < 8; ++b) *reinterpret_cast<f32x4*>(&sums[wave][m][16 * b + 4 * h]) = o[b];
+    __syncthreads();
+    const int mine = threadIdx.x >> 4, d = 8 * (threadIdx.x & 15);
 #pragma unroll
-      for (int b = 0; b < 8; ++b)
-        *reinterpret_cast<f32x4*>(&sums[wave][m][16 * b + 4 * h]) = o[ct][b];
-      __syncthreads();
-      const int mine = threadIdx.x >> 4, d = 8 * (threadIdx.x & 15);
-      const int column = column0 + 16 * ct + mine;
-      const int t = column / a.group;
-      float best = -__builtin_inff();
+    for (int ct = 0; ct < Split; ++ct) {
+      const int joined = column0 + 16 * ct + mine;
+      const int t = joined / a.group;
+      if (joined >= p.columns || t >= rows) continue;
+      float best = -__builtin_inff(), all = 0.0f, x[8] = {};
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) best = fmaxf(best, stats[w][0][16 * ct + mine]);
-      float all = 0.0f, x[8] = {};
+      for (int w = ct; w < kWaves; w += Split) best = fmaxf(best, stats[w][0][mine]);
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float theirs = stats[w][0][16 * ct + mine];
+      for (int w = ct; w < kWaves; w += Split) {
+        const float theirs = stats[w][0][mine];
         const float keep = theirs == best ? 1.0f : exp2_fast((theirs - best) * a.log2_scale);
         if (theirs > -__builtin_inff()) {
-          all = fmaf(stats[w][1][16 * ct + mine], keep, all);
+          all = fmaf(stats[w][1][mine], keep, all);
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] = fmaf(sums[w][mine][d + i], keep, x[i]);
         }
       }
-      if (column < p.columns && t < rows) {
-        if (entire) {
-          store_out(a, q.first + t, head * a.group + column - t * a.group, d, x, best, all);
-        } else {
-          float* const to_o = piece + static_cast<int64_t>(column) * kDim + d;
-          *reinterpret_cast<f32x4*>(to_o) = f32x4{x[0], x[1], x[2], x[3]};
-          *reinterpret_cast<f32x4*>(to_o + 4) = f32x4{x[4], x[5], x[6], x[7]};
-          if (d == 0)
-            *reinterpret_cast<f32x2*>(piece + layout.columns * kDim + 2 * column) = f32x2{best, all};
-        }
+      if (entire) {
+        store_out(a, q.first + t, head * a.group + joined - t * a.group, d, x, best, all);
+      } else {
+        float* const to_o = piece + static_cast<int64_t>(joined) * kDim + d;
+        *reinterpret_cast<f32x4*>(to_o) = f32x4{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4*>(to_o + 4) = f32x4{x[4], x[5], x[6], x[7]};
+        if (d == 0)
+          *reinterpret_cast<f32x2*>(piece + layout.columns * kDim + 2 * joined) = f32x2{best, all};
       }
-      __syncthreads();
     }
+    __syncthreads();
     at += to - from;
   }
 }
@@ -526,11 +484,11 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Deco
   store_out(a, q.first + t, q_head, d, x, best, all);
 }
 
-// Workgroups of the first launch: two a CU (one with 64 columns), fewer where no table is long
-// enough for a tile a wave each; tiles of 16 columns of each; and the rest of the columns' blocks.
+// Workgroups of the first launch: two a CU, fewer where no table is long enough for a tile a wave
+// each; waves a tile; and how often all of it for 64 columns each.
 struct Shape {
   int64_t workers;
-  int tiles, blocks;
+  int split, blocks;
   double most;       // tiles of 64 tokens, were every table full
   int64_t bytes;
 };
@@ -538,13 +496,13 @@ struct Shape {
 Shape decode_shape(const ld_paged_cache& c, int64_t q_heads, int64_t width) {
   Shape s{};
   const int64_t columns = width * (q_heads / c.num_kv_heads);
-  s.tiles = columns <= 16 ? 1 : columns <= 32 ? 2 : 4;
-  s.blocks = static_cast<int>((columns + 16 * s.tiles - 1) / (16 * s.tiles));
+  s.split = columns <= 16 ? 1 : columns <= 32 ? 2 : 4;
+  s.blocks = static_cast<int>((columns + 16 * s.split - 1) / (16 * s.split));
   const int64_t tiles = (static_cast<int64_t>(c.table_width) * c.page_size + kTile - 1) / kTile;
   s.most = static_cast<double>(tiles) * c.num_requests * c.num_kv_heads;
-  const int64_t chip = std::max<int64_t>(64, (s.tiles == 4 ? 256 : 512) / s.blocks);
+  const int64_t chip = std::max<int64_t>(64, 512 / s.blocks);
   s.workers = s.most / kWaves >= chip ? chip : static_cast<int64_t>(s.most) / kWaves + 1;
-  s.bytes = layout_of(c.num_requests, 16 * s.tiles * s.blocks).piece(s.workers, 0) * 4;
+  s.bytes = layout_of(c.num_requests, 16 * s.split * s.blocks).piece(s.workers, 0) * 4;
   return s;
 }
 
@@ -585,13 +543,14 @@ extern "C" int ld_attention_decode(const ld_paged_cache* cache, const ld_attenti
   if (s.most > 0x3fffffff)
     return fail(LD_ERR_INVALID_ARGUMENT, "too many tokens of all tables and heads");
   p.workers = static_cast<int32_t>(s.workers);
-  const auto kernel = s.tiles == 1   ? attention_decode_kernel<1>
-                      : s.tiles == 2 ? attention_decode_kernel<2>
+  const auto kernel = s.split == 1   ? attention_decode_kernel<1>
+                      : s.split == 2 ? attention_decode_kernel<2>
                                      : attention_decode_kernel<4>;
   const hipStream_t on = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(s.workers), s.blocks), dim3(kThreads), 0, on, p);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(s.workers), s.blocks),
+                     dim3(kThreads), 0, on, p);
   if (const int rc = check_launch("ld_attention_decode")) return rc;
   hipLaunchKernelGGL(attention_join_kernel, dim3(static_cast<uint32_t>(joins)), dim3(kJoinThreads),
-                     0, on, p, layout_of(p.cache.requests, 16 * s.tiles * s.blocks), tiles16);
+                     0, on, p, layout_of(p.cache.requests, 16 * s.split * s.blocks), tiles16);
   return check_launch("ld_attention_decode");
 }
