@@ -1,108 +1,450 @@
-// Attention of prompts over the paged 8-bit cache.
+// Attention of prompts to their tokens in the paged 8-bit cache.
+//
+// Bound by the matrix cores: 4 * 128 operations a query and token, a tile of 64 tokens read once for
+// 128 columns.  A workgroup takes 128 columns of a request and kv head (rows times the q heads that
+// share it), 32 a wave, and walks the tokens that they see, 64 at a time: the tile's codes are loaded
+// ahead, made bf16 (exact: e4m3 times its scale) and laid out in LDS as operands of
+// v_mfma_f32_32x32x16_bf16.  With m = lane % 32 and h = lane / 32,
+//   scores [token, column]: operand A holds, in row m of product t, the key of token 32 t + 16 (m / 4 % 2)
+//     + 4 (m / 8) + m % 4, so that a lane finds tokens 32 t + 16 h + (0 .. 15) of column m in its registers;
+//   outputs [element, column]: operand B is these weights, rounded to bf16, as they lie there.
+// Statistics are a lane's own but for one exchange of halves.  Outputs are scaled anew only where a
+// maximum grew by more than 2^8 in weights.
+//
+// Where there are few columns the tokens are split over workgroups too, whose sums a second launch
+// joins.
+#include <algorithm>
+
 #include "attention_common.h"
 
 namespace ld {
 namespace {
 
-struct AttentionParams {
+constexpr int kTile = 64;        // tokens
+constexpr int kColumns = 128;    // of a workgroup
+constexpr int kPieces16 = 1024;  // 16-byte pieces of a tile's keys, or values, as operands
+
+struct PrefillAttention {
   Cache cache;
   Attention a;
+  int32_t units;    // blocks of columns of all requests, at most
+  int32_t splits;   // workgroups a unit and kv head
 };
 
-// A wave takes one row and q head: 64 tokens at a time, a token's score by a lane, then two
-// elements of the output by a lane, with the running maximum and sum of the softmax.
-__global__ __launch_bounds__(64) void attention_rows_kernel(const AttentionParams p) {
+__device__ __forceinline__ int64_t first_unit(const PrefillAttention& p, int r) {
+  const int64_t row = min(max(static_cast<int64_t>(p.cache.cu[r]), int64_t{0}), p.cache.num_tokens);
+  return row * p.a.group / kColumns + r;
+}
+
+// Unit -> request and block of its columns; false where there is none.  Requests have a run of
+// units each, one more than their columns can fill at the most, so that where it begins follows from
+// cu alone: the last that begins at or before the unit, by a 64-way search.
+__device__ __forceinline__ bool find_unit(const PrefillAttention& p, int64_t unit, int& r,
+                                          int64_t& block) {
+  const int lane = threadIdx.x & 63;
+  int low = 0, count = p.cache.requests;
+  for (;;) {
+    const int step = (count + 63) >> 6;
+    const bool in = lane < (count + step - 1) / step;
+    const int64_t begins = in ? first_unit(p, low + lane * step) : 0;
+    const uint64_t before = __ballot(in && begins <= unit);
+    if (before == 0) return false;
+    const int k = 63 - __clzll(static_cast<long long>(before));
+    low += k * step;
+    if (step == 1) {
+      const int at = __builtin_amdgcn_readlane(static_cast<int>(unit - begins), k);
+      r = low;
+      block = at;
+      return true;
+    }
+    count = min(step, count - k * step);
+  }
+}
+
+__device__ __forceinline__ float* split_at(const PrefillAttention& p, int64_t place) {
+  return p.a.workspace + place * kColumns * (kDim + 2);
+}
+
+// Four elements of an output: divided, gated and rounded.
+__device__ __forceinline__ void store_four(const Attention& a, int64_t row, int head, int d, f32x4 o,
+                                           bool some, float inverse) {
+  if (a.gate != nullptr && some) {
+    uint16_t g[4];
+    __builtin_memcpy(g, a.gate + row * a.gate_row + head * kDim + d, 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] *= sigmoid(bf16_to_f32(g[i]));
+  }
+  uint32_t bits[2] = {0, 0};
+  if (some) {
+    bits[0] = bf16_pair(f32x2{o[0] * inverse, o[1] * inverse});
+    bits[1] = bf16_pair(f32x2{o[2] * inverse, o[3] * inverse});
+  }
+  __builtin_memcpy(a.out + (row * a.q_heads + head) * kDim + d, bits, 8);
+}
+
+__global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const PrefillAttention p) {
   const Cache& c = p.cache;
   const Attention& a = p.a;
-  const int64_t row = blockIdx.x / a.q_heads;
-  const int head = static_cast<int>(blockIdx.x - row * a.q_heads);
-  const int r = request_at(c, row);
-  const Request req = request_of(c, r);
-  if (row < req.first || row >= req.last) return;
-  const int lane = threadIdx.x;
-  const int kv = head / a.group;
-  const int64_t position = row + req.shift;
-  int64_t sees = min(position + 1, static_cast<int64_t>(req.tokens));
-  __shared__ float query[kDim];
-  __shared__ float weight[64];
-  for (int d = lane; d < kDim; d += 64) query[d] = bf16_to_f32(a.q[row * a.q_row + head * kDim + d]);
-  __syncthreads();
-  float top = -3.4028235e38f, total = 0.0f, o0 = 0.0f, o1 = 0.0f;
-  bool any = false;
-  for (int64_t t0 = 0; t0 < sees; t0 += 64) {
-    const int64_t t = t0 + lane;
-    const int page = t < sees ? c.pages[r * c.pages_row + (t >> c.page_log2)] : 0;
-    const bool live = live_page(c, page);
-    float s = -__builtin_inff();
-    if (live) {
-      const int at = static_cast<int>(t) & ((1 << c.page_log2) - 1);
-      const uint32_t* const k = reinterpret_cast<const uint32_t*>(k_tile(c, page, kv));
-      float sum = 0.0f;
-      for (int d = 0; d < kDim; d += 4) {
-        const uint32_t x = k[((d >> 4 << c.page_log2) + at) * 4 + (d >> 2 & 3)];
-        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(x, false);
-        const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(x, true);
-        sum = fmaf(lo[0], query[d], fmaf(lo[1], query[d + 1], sum));
-        sum = fmaf(hi[0], query[d + 2], fmaf(hi[1], query[d + 3], sum));
+  // the tile's keys: [16 elements of a token][half of them][token in the operand's order], and its
+  // values [16 tokens][half of them][element], in pieces of eight
+  __shared__ __attribute__((aligned(16))) u32x4 lds_keys[2][kPieces16];
+  __shared__ __attribute__((aligned(16))) u32x4 lds_values[2][kPieces16];
+  __shared__ int lds_strange[2][kWaves];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m = lane & 31, h = lane >> 5;
+
+  const int head = blockIdx.x % c.kv_heads;
+  const int rest = blockIdx.x / c.kv_heads;
+  const int split = rest % p.splits;
+  const int64_t unit = p.units - 1 - rest / p.splits;   // (the longest walks of a request first)
+  int r;
+  int64_t block;
+  if (!find_unit(p, unit, r, block)) return;
+  const Request q = request_of(c, r);
+  const int64_t columns = (q.last - q.first) * a.group;   // (none: not above zero)
+  if (block * kColumns >= columns) return;
+  const int32_t* const table = c.pages + r * c.pages_row;
+
+  // this lane's column, and how many tokens it, the wave's first and last and the workgroup's last see
+  const int64_t column = block * kColumns + 32 * wave + m;
+  auto sees = [&](int64_t t) {
+    return static_cast<int>(max(min(q.first + t + q.shift + 1, static_cast<int64_t>(q.tokens)), int64_t{0}));
+  };
+  const bool real = column < columns;
+  const int64_t t_row = (real ? column : columns - 1) / a.group;
+  const int g_row = static_cast<int>((real ? column : columns - 1) - t_row * a.group);
+  const int limit = sees(t_row);
+  const int least = __builtin_amdgcn_readlane(limit, 0);
+  const int wave_tiles = (__builtin_amdgcn_readlane(limit, 31) + kTile - 1) / kTile;
+  const int all_tiles = (sees((min(block * kColumns + kColumns, columns) - 1) / a.group) + kTile - 1) / kTile;
+  const int begin = static_cast<int>(static_cast<int64_t>(all_tiles) * split / p.splits);
+  const int end = static_cast<int>(static_cast<int64_t>(all_tiles) * (split + 1) / p.splits);
+  const bool works = block * kColumns + 32 * wave < columns;
+
+  bf16x8 query[8];
+  {
+    const uint16_t* const from = a.q + (q.first + t_row) * a.q_row + (head * a.group + g_row) * kDim;
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      __builtin_memcpy(&query[s], from + 16 * (2 * (s >> 1) + h) + 8 * (s & 1), 16);
+  }
+
+  f32x16 o[4];
+  float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
+
+  // A thread's share of a tile: sixteen elements of token `lane` of chunks `wave` and `wave` + 4 of the keys, and
+  // sixteen tokens (groups wave / 2 and wave / 2 + 2) of one element of the values.
+  const int element = threadIdx.x & 127;
+  const int slot = (lane & 32) + 8 * (lane >> 2 & 3) + 4 * (lane >> 4 & 1) + (lane & 3);
+  auto page_of = [&](int tile) {
+    const int token = tile * kTile + lane;
+    const int page = tile < end && token < q.tokens ? table[token >> c.page_log2] : 0;
+    return live_page(c, page) ? page : 0;
+  };
+  u32x4 keys[2], values[2];
+  float k_scale, v_scale[2];
+  uint64_t live;
+  auto load = [&](int tile, int page) {
+    live = __ballot(page > 0);
+    const int in = (tile * kTile + lane) & ((1 << c.page_log2) - 1);
+    const uint8_t* const at_k = k_tile(c, page, head) + (((wave << c.page_log2) + in) << 4);
+    keys[0] = *reinterpret_cast<const u32x4*>(at_k);
+    keys[1] = *reinterpret_cast<const u32x4*>(at_k + (64 << c.page_log2));
+    k_scale = scale_value(c.k_scale[page * c.k_scale_page + head]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int group = (wave >> 1) + 2 * i;
+      const int theirs = __builtin_amdgcn_readlane(page, 16 * group);
+      const int at = (tile * kTile + 16 * group) & ((1 << c.page_log2) - 1);
+      values[i] = *reinterpret_cast<const u32x4*>(v_tile(c, theirs, head) + (at >> 4) * (kDim * 16) +
+                                                  element * 16);
+      v_scale[i] = scale_value(c.v_scale[theirs * c.v_scale_page + head]);
+    }
+  };
+  auto stage = [&](int tile, int to) {
+    // values behind the last token, or without a page, are zeros
+    bool strange = false;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int group = (wave >> 1) + 2 * i;
+      const int first = tile * kTile + 16 * group;
+      const int kept = live >> (16 * group) & 1 ? q.tokens - first : 0;
+      if (kept < 16) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) values[i][w] &= first_bytes(kept - 4 * w);
       }
-      s = sum * scale_value(c.k_scale[page * c.k_scale_page + kv]);
+      uint32_t any = 0;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) any |= nan_bytes(values[i][w]);
+      strange = strange || any != 0;
+      lds_values[to][(2 * group) * kDim + element] =
+          __builtin_bit_cast(u32x4, operand8(values[i][0], values[i][1], v_scale[i]));
+      lds_values[to][(2 * group + 1) * kDim + element] =
+          __builtin_bit_cast(u32x4, operand8(values[i][2], values[i][3], v_scale[i]));
     }
-    float most = s;
-    for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-    const float now = fmaxf(top, most);
-    const float keep = exp2f((top - now) * a.log2_scale);
-    const float w = live ? exp2f((s - now) * a.log2_scale) : 0.0f;
-    any = any || __any(live);
-    float sum = w;
-    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-    total = total * keep + sum;
-    o0 *= keep;
-    o1 *= keep;
-    top = now;
-    weight[lane] = w;
-    __syncthreads();
-    for (int j = 0; j < 64 && t0 + j < sees; ++j) {
-      const int pg = __shfl(page, j);
-      if (!live_page(c, pg)) continue;
-      const int at = static_cast<int>(t0 + j) & ((1 << c.page_log2) - 1);
-      const uint8_t* const v = v_tile(c, pg, kv) + (at >> 4) * (kDim * 16) + (at & 15);
-      const auto x = __builtin_amdgcn_cvt_pk_f32_fp8(v[lane * 32] | v[lane * 32 + 16] << 8, false);
-      const float vs = scale_value(c.v_scale[pg * c.v_scale_page + kv]);
-      o0 = fmaf(weight[j] * vs, x[0], o0);
-      o1 = fmaf(weight[j] * vs, x[1], o1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int chunk = wave + 4 * i;
+      lds_keys[to][2 * chunk * kTile + slot] =
+          __builtin_bit_cast(u32x4, operand8(keys[i][0], keys[i][1], k_scale));
+      lds_keys[to][(2 * chunk + 1) * kTile + slot] =
+          __builtin_bit_cast(u32x4, operand8(keys[i][2], keys[i][3], k_scale));
     }
-    __syncthreads();
+    const bool some = __any(strange);
+    if (lane == 0) lds_strange[to][wave] = some;
+  };
+
+  int page_next = page_of(begin);
+  uint64_t live_now = 0;
+  if (begin < end) {
+    load(begin, page_next);
+    page_next = page_of(begin + 1);
+    stage(begin, 0);
+    live_now = live;
   }
-  const float inverse = 1.0f / total;
-  o0 = any ? o0 * inverse : 0.0f;
-  o1 = any ? o1 * inverse : 0.0f;
-  if (a.gate != nullptr && any) {
-    const uint16_t* const g = a.gate + row * a.gate_row + head * kDim + 2 * lane;
-    o0 *= sigmoid(bf16_to_f32(g[0]));
-    o1 *= sigmoid(bf16_to_f32(g[1]));
+  __syncthreads();
+  for (int tile = begin; tile < end; ++tile) {
+    const int now_at = (tile - begin) & 1;
+    const bool more = tile + 1 < end;
+    if (more) {
+      load(tile + 1, page_next);
+      page_next = page_of(tile + 2);
+    }
+    if (works && tile < wave_tiles) {
+      const int token0 = tile * kTile;
+      f32x16 score[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) score[t][i] = 0.0f;
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const u32x4 k = lds_keys[now_at][(2 * (2 * (s >> 1) + h) + (s & 1)) * kTile + 32 * t + m];
+          score[t] = mfma32(__builtin_bit_cast(bf16x8, k), query[s], score[t]);
+        }
+      // a tile that some column does not see whole: scores of -inf, weights of zero
+      const bool whole = token0 + kTile <= least && live_now == ~uint64_t{0};
+      float most = kLowest;   // (of a score of -inf that is seen: a weight of zero, not none)
+      if (!whole) {
+        bool any = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const bool lives = live_now >> (32 * t + 16 * h) & 1;
+          any = any || (lives && token0 + 32 * t + 16 * h < limit);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (!lives || token0 + 32 * t + 16 * h + i >= limit) score[t][i] = -__builtin_inff();
+        }
+        if (!any) most = -__builtin_inff();
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, score[t][i]);
+      {
+        const uint32_t u = __float_as_uint(most);
+        const auto x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        most = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+      }
+      if (__any((most - top) * a.log2_scale > 8.0f)) {
+        const float now = fmaxf(top, most);
+        const float keep = now == top ? 1.0f : exp2_fast((top - now) * a.log2_scale);
+        sum *= keep;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) o[b] *= keep;
+        top = now;
+      }
+      const float less = top == -__builtin_inff() ? 0.0f : -top * a.log2_scale;
+      bf16x8 weight[2][2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          u32x4 bits;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float x = exp2_fast(fmaf(score[t][8 * u + 2 * w], a.log2_scale, less));
+            const float y = exp2_fast(fmaf(score[t][8 * u + 2 * w + 1], a.log2_scale, less));
+            sum += x;
+            sum += y;
+            bits[w] = bf16_pair(f32x2{x, y});
+          }
+          weight[t][u] = __builtin_bit_cast(bf16x8, bits);
+        }
+      const bool strange = !whole && (lds_strange[now_at][0] | lds_strange[now_at][1] |
+                                      lds_strange[now_at][2] | lds_strange[now_at][3]) != 0;
+      if (!strange) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              const u32x4 v = lds_values[now_at][(2 * (2 * t + h) + u) * kDim + 32 * b + m];
+              o[b] = mfma32(__builtin_bit_cast(bf16x8, v), weight[t][u], o[b]);
+            }
+      } else {
+        // a value that is not finite reaches the columns that see its token alone
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          f32x16 count;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) count[i] = 0.0f;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              u32x4 v = lds_values[now_at][(2 * (2 * t + h) + u) * kDim + 32 * b + m], ones, seen;
+              const bool lives = live_now >> (32 * t + 16 * h) & 1;
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                const uint32_t lo = (v[w] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u;
+                const uint32_t hi = (v[w] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
+                ones[w] = (lo | hi) & 0x3f803f80u;
+                v[w] &= ~(lo | hi);
+                const int token = token0 + 32 * t + 16 * h + 8 * u + 2 * w;
+                seen[w] = (lives && token < limit ? 0x3f80u : 0u) |
+                          (lives && token + 1 < limit ? 0x3f800000u : 0u);
+              }
+              count = mfma32(__builtin_bit_cast(bf16x8, ones), __builtin_bit_cast(bf16x8, seen), count);
+              o[b] = mfma32(__builtin_bit_cast(bf16x8, v), weight[t][u], o[b]);
+            }
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (count[i] > 0.0f) o[b][i] = __builtin_nanf("");
+        }
+      }
+    }
+    if (more) {
+      stage(tile + 1, now_at ^ 1);
+      live_now = live;
+    }
+    lds_barrier();
   }
-  const uint32_t bits = f32_to_bf16(o0) | static_cast<uint32_t>(f32_to_bf16(o1)) << 16;
-  __builtin_memcpy(a.out + (row * a.q_heads + head) * kDim + 2 * lane, &bits, 4);
+
+  sum = add_partner<32>(sum);
+  if (!real) return;
+  if (p.splits == 1) {
+    const bool some = top > -__builtin_inff();   // the row sees a token
+    const float inverse = 1.0f / sum;
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        store_four(a, q.first + t_row, head * a.group + g_row, 32 * b + 8 * e + 4 * h, quad(o[b], e),
+                   some, inverse);
+  } else {
+    float* const to = split_at(p, (unit * c.kv_heads + head) * p.splits + split);
+    const int at = 32 * wave + m;
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<f32x4*>(to + at * kDim + 32 * b + 8 * e + 4 * h) = quad(o[b], e);
+    if (h == 0) *reinterpret_cast<f32x2*>(to + kColumns * kDim + 2 * at) = f32x2{top, sum};
+  }
+}
+
+// Joins the sums of a unit's splits, in their order: thread (column, four elements), eight columns a
+// workgroup.
+__global__ __launch_bounds__(kThreads) void attention_gather_kernel(const PrefillAttention p) {
+  const Cache& c = p.cache;
+  const Attention& a = p.a;
+  constexpr int kEach = kThreads / 32;
+  const int part = blockIdx.x % (kColumns / kEach);
+  const int rest = blockIdx.x / (kColumns / kEach);
+  const int head = rest % c.kv_heads;
+  const int64_t unit = rest / c.kv_heads;
+  int r;
+  int64_t block;
+  if (!find_unit(p, unit, r, block)) return;
+  const Request q = request_of(c, r);
+  const int within = part * kEach + (threadIdx.x >> 5);
+  const int64_t column = block * kColumns + within;
+  if (column >= (q.last - q.first) * a.group) return;
+  const int d = 4 * (threadIdx.x & 31);
+  const int64_t place = (unit * c.kv_heads + head) * p.splits;
+  float best = -__builtin_inff(), all = 0.0f;
+  f32x4 x = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const float* const from = split_at(p, place + s);
+    const f32x2 stat = *reinterpret_cast<const f32x2*>(from + kColumns * kDim + 2 * within);
+    const f32x4 theirs = *reinterpret_cast<const f32x4*>(from + within * kDim + d);
+    if (stat[0] > -__builtin_inff()) {   // (what saw nothing has sums of zero)
+      const float now = fmaxf(best, stat[0]);
+      const float keep = best == now ? 1.0f : exp2_fast((best - now) * a.log2_scale);
+      const float add = stat[0] == now ? 1.0f : exp2_fast((stat[0] - now) * a.log2_scale);
+      best = now;
+      all = all * keep + stat[1] * add;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = x[i] * keep + theirs[i] * add;
+    }
+  }
+  const int64_t t = column / a.group;
+  store_four(a, q.first + t, head * a.group + static_cast<int>(column - t * a.group), d, x,
+             best > -__builtin_inff(), 1.0f / all);
+}
+
+// Blocks of columns, and over how many workgroups each one's tokens are split: two workgroups a CU
+// between them, each of four tiles at least were its table full.
+struct Shape {
+  int64_t units, splits, bytes;
+};
+
+Shape prefill_shape(const ld_paged_cache& c, int64_t q_heads) {
+  Shape s{};
+  const int64_t group = q_heads / c.num_kv_heads;
+  s.units = c.num_tokens * group / kColumns + c.num_requests;
+  const int64_t tiles = (static_cast<int64_t>(c.table_width) * c.page_size + kTile - 1) / kTile;
+  s.splits = std::max<int64_t>(1, std::min(512 / (s.units * c.num_kv_heads), tiles / 4));
+  s.bytes = s.splits == 1 ? 0 : s.units * c.num_kv_heads * s.splits * kColumns * (kDim + 2) * 4;
+  return s;
 }
 
 }  // namespace
 }  // namespace ld
 
-extern "C" int64_t ld_attention_prefill_workspace_bytes(const ld_paged_cache*,
-                                                        const ld_attention_args*) {
-  return 0;
+extern "C" int64_t ld_attention_prefill_workspace_bytes(const ld_paged_cache* cache,
+                                                        const ld_attention_args* args) {
+  using namespace ld;
+  if (cache == nullptr || args == nullptr || cache->num_requests <= 0 || cache->num_tokens <= 0 ||
+      cache->num_kv_heads <= 0 || args->num_q_heads < cache->num_kv_heads || cache->table_width < 0)
+    return 0;
+  return prefill_shape(*cache, args->num_q_heads).bytes;
 }
 
 extern "C" int ld_attention_prefill(const ld_paged_cache* cache, const ld_attention_args* args,
                                     void* stream) {
   using namespace ld;
-  AttentionParams p{};
+  PrefillAttention p{};
   if (const int rc = cache_params(cache, p.cache)) return rc;
   if (const int rc = attention_params(*cache, args, p.a)) return rc;
   if (p.cache.requests == 0) return LD_OK;
-  const int64_t blocks = p.cache.num_tokens * p.a.q_heads;
+  const Shape s = prefill_shape(*cache, p.a.q_heads);
+  if (s.bytes > 0 && (p.a.workspace == nullptr || !aligned16(p.a.workspace) ||
+                      args->workspace_bytes < s.bytes))
+    return fail(LD_ERR_INVALID_ARGUMENT, "workspace missing or too small");
+  const int64_t blocks = s.units * s.splits * p.cache.kv_heads;
   if (blocks > 0x7fffffff) return fail(LD_ERR_INVALID_ARGUMENT, "too many rows and heads");
-  hipLaunchKernelGGL(attention_rows_kernel, dim3(static_cast<uint32_t>(blocks)), dim3(64), 0,
-                     static_cast<hipStream_t>(stream), p);
+  p.units = static_cast<int32_t>(s.units);
+  p.splits = static_cast<int32_t>(s.splits);
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(attention_prefill_kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kThreads),
+                     0, on, p);
+  if (const int rc = check_launch("ld_attention_prefill")) return rc;
+  if (s.splits == 1) return LD_OK;
+  // (at most 512 units and heads)
+  const int64_t joins = s.units * p.cache.kv_heads * (kColumns / (kThreads / 32));
+  hipLaunchKernelGGL(attention_gather_kernel, dim3(static_cast<uint32_t>(joins)), dim3(kThreads), 0,
+                     on, p);
   return check_launch("ld_attention_prefill");
 }
