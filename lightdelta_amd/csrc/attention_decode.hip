@@ -248,6 +248,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Dec
       load_keys(tile, k_page);
       load_values(tile, v_page);
     }
+    uint32_t strange = 0;
     for (; tile < to; tile += step) {
       const int token0 = static_cast<int>(tile) * kTile;
       const bool live = v_page > 0;
@@ -308,48 +309,18 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Dec
       const bf16x8 weight[2] = {__builtin_bit_cast(bf16x8, bits[0]), __builtin_bit_cast(bf16x8, bits[1])};
 
       if (!whole) {
-        // values behind the last token, or without a page, take no part; a value that is not
-        // finite reaches the columns that see its token alone
+        // values behind the last token, or without a page, are zeros; so are those that are not
+        // finite, and marked below
         const int kept = live ? q.tokens - (token0 + 16 * h) : 0;
-        uint32_t strange = 0;
 #pragma unroll
         for (int b = 0; b < 8; ++b)
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            values[b][w] &= first_bytes(kept - 4 * w);
-            strange |= nan_bytes(values[b][w]);
+            const uint32_t x = values[b][w] & first_bytes(kept - 4 * w);
+            const uint32_t at_nan = nan_bytes(x);
+            strange |= at_nan;
+            values[b][w] = x & ~((at_nan >> 7) * 0xffu);
           }
-        if (__any(strange != 0)) {
-          bf16x8 seen[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            u32x4 mask;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const int token = token0 + 16 * h + 8 * u + 2 * w;
-              mask[w] = (live && token < limit ? 0x3f80u : 0u) |
-                        (live && token + 1 < limit ? 0x3f800000u : 0u);
-            }
-            seen[u] = __builtin_bit_cast(bf16x8, mask);
-          }
-#pragma unroll
-          for (int b = 0; b < 8; ++b) {
-            u32x4 ones;   // e4m3's 1 where a value is NaN
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const uint32_t at_nan = nan_bytes(values[b][w]) >> 7;
-              ones[w] = at_nan * 0x38u;
-              values[b][w] &= ~(at_nan * 0xffu);
-            }
-            f32x4 count = {0, 0, 0, 0};
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-              count = mfma16(operand8(ones[2 * u], ones[2 * u + 1], 1.0f), seen[u], count);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (count[i] > 0.0f) o[b][i] = __builtin_nanf("");
-          }
-        }
       }
 #pragma unroll
       for (int b = 0; b < 8; ++b)
@@ -358,6 +329,40 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Dec
           o[b] = mfma16(operand8(values[b][2 * u], values[b][2 * u + 1], v_scale), weight[u], o[b]);
       v_page = v_now;
       if (more) load_values(tile + step, v_page);
+    }
+
+    if (__any(strange != 0)) {
+      // values that are not finite reach the columns that see their tokens alone: counted from the
+      // codes of those tiles, by products of ones
+      f32x4 count[8];
+#pragma unroll
+      for (int b = 0; b < 8; ++b) count[b] = f32x4{0, 0, 0, 0};
+      for (tile = from + wave / Split; tile < to; tile += step) {
+        const int first = static_cast<int>(tile) * kTile + 16 * h;   // this lane's sixteen tokens
+        const int page = page_of(tile, h);
+        if (static_cast<int>(tile) * kTile + kTile <= least && __all(page > 0)) continue;
+        load_values(tile, page);
+        u32x4 seen[2];
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+          seen[w >> 2][w & 3] = (first + 2 * w < limit ? 0x3f80u : 0u) |
+                                (first + 2 * w + 1 < limit ? 0x3f800000u : 0u);
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          u32x4 ones;   // e4m3's 1 where a value is NaN
+#pragma unroll
+          for (int w = 0; w < 4; ++w) ones[w] = page > 0 ? (nan_bytes(values[b][w]) >> 7) * 0x38u : 0u;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            count[b] = mfma16(operand8(ones[2 * u], ones[2 * u + 1], 1.0f),
+                              __builtin_bit_cast(bf16x8, seen[u]), count[b]);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < 8; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (count[b][i] > 0.0f) o[b][i] = __builtin_nanf("");
     }
 
     // the waves' sums joined: thread (column, eight elements) of each sixteen columns

@@ -89,7 +89,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
   // values [16 tokens][half of them][element], in pieces of eight
   __shared__ __attribute__((aligned(16))) u32x4 lds_keys[2][kPieces16];
   __shared__ __attribute__((aligned(16))) u32x4 lds_values[2][kPieces16];
-  __shared__ int lds_strange[2][kWaves];
+  __shared__ int lds_strange;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -117,6 +117,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
   const int g_row = static_cast<int>((real ? column : columns - 1) - t_row * a.group);
   const int limit = sees(t_row);
   const int least = __builtin_amdgcn_readlane(limit, 0);
+  const int first_limit = sees(block * kColumns / a.group);
   const int wave_tiles = (__builtin_amdgcn_readlane(limit, 31) + kTile - 1) / kTile;
   const int all_tiles = (sees((min(block * kColumns + kColumns, columns) - 1) / a.group) + kTile - 1) / kTile;
   const int begin = static_cast<int>(static_cast<int64_t>(all_tiles) * split / p.splits);
@@ -168,8 +169,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
     }
   };
   auto stage = [&](int tile, int to) {
-    // values behind the last token, or without a page, are zeros
-    bool strange = false;
+    // values behind the last token, or without a page, are zeros; so are those that are not finite,
+    // and marked below, in tiles that some column does not see whole
+    const bool partial = tile * kTile + kTile > first_limit;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int group = (wave >> 1) + 2 * i;
@@ -179,10 +181,16 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
 #pragma unroll
         for (int w = 0; w < 4; ++w) values[i][w] &= first_bytes(kept - 4 * w);
       }
-      uint32_t any = 0;
+      if (partial) {
+        uint32_t any = 0;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) any |= nan_bytes(values[i][w]);
-      strange = strange || any != 0;
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t at_nan = nan_bytes(values[i][w]);
+          any |= at_nan;
+          values[i][w] &= ~((at_nan >> 7) * 0xffu);
+        }
+        if (any != 0) lds_strange = 1;
+      }
       lds_values[to][(2 * group) * kDim + element] =
           __builtin_bit_cast(u32x4, operand8(values[i][0], values[i][1], v_scale[i]));
       lds_values[to][(2 * group + 1) * kDim + element] =
@@ -196,10 +204,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
       lds_keys[to][(2 * chunk + 1) * kTile + slot] =
           __builtin_bit_cast(u32x4, operand8(keys[i][2], keys[i][3], k_scale));
     }
-    const bool some = __any(strange);
-    if (lane == 0) lds_strange[to][wave] = some;
   };
-
+  if (threadIdx.x == 0) lds_strange = 0;
+  __syncthreads();
   int page_next = page_of(begin);
   uint64_t live_now = 0;
   if (begin < end) {
@@ -279,49 +286,15 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
           }
           weight[t][u] = __builtin_bit_cast(bf16x8, bits);
         }
-      const bool strange = !whole && (lds_strange[now_at][0] | lds_strange[now_at][1] |
-                                      lds_strange[now_at][2] | lds_strange[now_at][3]) != 0;
-      if (!strange) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-              const u32x4 v = lds_values[now_at][(2 * (2 * t + h) + u) * kDim + 32 * b + m];
-              o[b] = mfma32(__builtin_bit_cast(bf16x8, v), weight[t][u], o[b]);
-            }
-      } else {
-        // a value that is not finite reaches the columns that see its token alone
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          f32x16 count;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) count[i] = 0.0f;
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              u32x4 v = lds_values[now_at][(2 * (2 * t + h) + u) * kDim + 32 * b + m], ones, seen;
-              const bool lives = live_now >> (32 * t + 16 * h) & 1;
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                const uint32_t lo = (v[w] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u;
-                const uint32_t hi = (v[w] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
-                ones[w] = (lo | hi) & 0x3f803f80u;
-                v[w] &= ~(lo | hi);
-                const int token = token0 + 32 * t + 16 * h + 8 * u + 2 * w;
-                seen[w] = (lives && token < limit ? 0x3f80u : 0u) |
-                          (lives && token + 1 < limit ? 0x3f800000u : 0u);
-              }
-              count = mfma32(__builtin_bit_cast(bf16x8, ones), __builtin_bit_cast(bf16x8, seen), count);
-              o[b] = mfma32(__builtin_bit_cast(bf16x8, v), weight[t][u], o[b]);
-            }
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (count[i] > 0.0f) o[b][i] = __builtin_nanf("");
-        }
-      }
+          for (int b = 0; b < 4; ++b) {
+            const u32x4 v = lds_values[now_at][(2 * (2 * t + h) + u) * kDim + 32 * b + m];
+            o[b] = mfma32(__builtin_bit_cast(bf16x8, v), weight[t][u], o[b]);
+          }
     }
     if (more) {
       stage(tile + 1, now_at ^ 1);
@@ -330,6 +303,45 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
     lds_barrier();
   }
 
+  if (lds_strange) {
+    // values that are not finite reach the columns that see their tokens alone: counted from the
+    // codes of those tiles, by products of ones
+    f32x16 count[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) count[b][i] = 0.0f;
+    for (int tile = max(begin, first_limit / kTile); tile < end; ++tile)
+      for (int t = 0; t < 2; ++t) {
+        const int first = tile * kTile + 32 * t + 16 * h;   // this lane's sixteen tokens
+        const int page = first < q.tokens ? table[first >> c.page_log2] : 0;
+        u32x4 seen[2];
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+          seen[w >> 2][w & 3] = (first + 2 * w < limit ? 0x3f80u : 0u) |
+                                (first + 2 * w + 1 < limit ? 0x3f800000u : 0u);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          u32x4 codes = {0, 0, 0, 0};
+          if (live_page(c, page)) {
+            const int in = first & ((1 << c.page_log2) - 1);
+            codes = *reinterpret_cast<const u32x4*>(v_tile(c, page, head) +
+                                                    ((in >> 4) * kDim + 32 * b + m) * 16);
+          }
+#pragma unroll
+          for (int w = 0; w < 4; ++w) codes[w] = (nan_bytes(codes[w]) >> 7) * 0x38u;   // e4m3's 1
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            count[b] = mfma32(operand8(codes[2 * u], codes[2 * u + 1], 1.0f),
+                              __builtin_bit_cast(bf16x8, seen[u]), count[b]);
+        }
+      }
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (count[b][i] > 0.0f) o[b][i] = __builtin_nanf("");
+  }
   sum = add_partner<32>(sum);
   if (!real) return;
   if (p.splits == 1) {
