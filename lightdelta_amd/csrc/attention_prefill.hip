@@ -237,6 +237,19 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
           const u32x4 k = lds_keys[now_at][(2 * (2 * (s >> 1) + h) + (s & 1)) * kTile + 32 * t + m];
           score[t] = mfma32(__builtin_bit_cast(bf16x8, k), query[s], score[t]);
         }
+      // the first values' operands too, which the weights' arithmetic covers
+      u32x4 early[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) early[b] = lds_values[now_at][2 * h * kDim + 32 * b + m];
+      // (operands read six ahead of the product that takes them)
+      __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+      for (int i = 0; i < 14; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      lds_order();
       // a tile that some column does not see whole: scores of -inf, weights of zero
       const bool whole = token0 + kTile <= least && live_now == ~uint64_t{0};
       float most = kLowest;   // (of a score of -inf that is seen: a weight of zero, not none)
@@ -292,7 +305,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
-            const u32x4 v = lds_values[now_at][(2 * (2 * t + h) + u) * kDim + 32 * b + m];
+            const u32x4 v = t + u == 0 ? early[b]
+                                       : lds_values[now_at][(2 * (2 * t + h) + u) * kDim + 32 * b + m];
             o[b] = mfma32(__builtin_bit_cast(bf16x8, v), weight[t][u], o[b]);
           }
     }
