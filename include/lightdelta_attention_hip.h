@@ -112,7 +112,7 @@ typedef struct ld_attention_args {
  * num_requests * num_kv_heads * (tokens of a table, in 64s) is below 2^30. */
 int ld_attention_decode(const ld_paged_cache* cache, const ld_attention_args* args, void* stream);
 
-/* Requests of any number of rows. */
+/* Requests of any number of rows; num_tokens * num_q_heads / num_kv_heads is at most 2^31 - 256. */
 int ld_attention_prefill(const ld_paged_cache* cache, const ld_attention_args* args, void* stream);
 
 /* Workspace bytes for these sizes, of which only the sizes count; 0 where none is needed.

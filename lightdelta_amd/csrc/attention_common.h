@@ -121,12 +121,25 @@ struct Request {
 __device__ __forceinline__ Request request_of(const Cache& c, int r) {
   Request q;
   const int64_t end = c.cu[r + 1];
-  q.first = max(static_cast<int64_t>(c.cu[r]), int64_t{0});
-  q.last = min(end, c.num_tokens);
+  q.first = min(max(static_cast<int64_t>(c.cu[r]), int64_t{0}), c.num_tokens);
+  q.last = max(min(end, c.num_tokens), int64_t{0});
   const int64_t length = c.lengths[r];
   q.shift = length - end;
   q.tokens = static_cast<int32_t>(
       max(min(length, static_cast<int64_t>(c.table_width) << c.page_log2), int64_t{0}));
+  return q;
+}
+
+// Lane k's, to every lane.  (Rows are below 2^31.)
+__device__ __forceinline__ Request request_from(const Request& x, int k) {
+  Request q;
+  q.first = __builtin_amdgcn_readlane(static_cast<int>(x.first), k);
+  q.last = __builtin_amdgcn_readlane(static_cast<int>(x.last), k);
+  q.shift = static_cast<int64_t>(
+      static_cast<uint64_t>(static_cast<uint32_t>(
+          __builtin_amdgcn_readlane(static_cast<int>(x.shift >> 32), k))) << 32 |
+      static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x.shift), k)));
+  q.tokens = __builtin_amdgcn_readlane(x.tokens, k);
   return q;
 }
 

@@ -107,13 +107,7 @@ struct Walk {
     const uint32_t n = __builtin_amdgcn_readlane(tiles, k);
     first = before + __builtin_amdgcn_readlane(behind, k) - n;
     number = base + k;
-    // (rows are below 2^31)
-    q.first = __builtin_amdgcn_readlane(static_cast<int>(mine.first), k);
-    q.last = __builtin_amdgcn_readlane(static_cast<int>(mine.last), k);
-    q.shift = static_cast<int64_t>(
-        static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine.shift >> 32), k))) << 32 |
-        static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine.shift), k)));
-    q.tokens = __builtin_amdgcn_readlane(mine.tokens, k);
+    q = request_from(mine, k);
     return n;
   }
 };

@@ -31,30 +31,32 @@ struct PrefillAttention {
   int32_t splits;   // workgroups a unit and kv head
 };
 
-__device__ __forceinline__ int64_t first_unit(const PrefillAttention& p, int r) {
-  const int64_t row = min(max(static_cast<int64_t>(p.cache.cu[r]), int64_t{0}), p.cache.num_tokens);
-  return row * p.a.group / kColumns + r;
-}
-
-// Unit -> request and block of its columns; false where there is none.  Requests have a run of
-// units each, one more than their columns can fill at the most, so that where it begins follows from
-// cu alone: the last that begins at or before the unit, by a 64-way search.
-__device__ __forceinline__ bool find_unit(const PrefillAttention& p, int64_t unit, int& r,
-                                          int64_t& block) {
+// Unit -> request, what it has in the call, and block of its columns; false where there is none.
+// Requests have a run of units each, one more than their columns can fill at the most, so that where
+// it begins follows from cu alone: the last that begins at or before the unit, by a 64-way search.
+// (The host has seen to it that columns are below 2^31.)
+__device__ __forceinline__ bool find_unit(const PrefillAttention& p, int unit, int& r, Request& q,
+                                          int& block) {
+  const Cache& c = p.cache;
   const int lane = threadIdx.x & 63;
-  int low = 0, count = p.cache.requests;
+  int low = 0, count = c.requests;
   for (;;) {
     const int step = (count + 63) >> 6;
     const bool in = lane < (count + step - 1) / step;
-    const int64_t begins = in ? first_unit(p, low + lane * step) : 0;
+    const int index = in ? low + lane * step : low;
+    Request mine;
+    if (step == 1) mine = request_of(c, index);   // the last level: all of each candidate at once
+    else mine.first = max(static_cast<int64_t>(c.cu[index]), int64_t{0});
+    const int row = static_cast<int>(min(mine.first, c.num_tokens));
+    const int begins = static_cast<int>(static_cast<uint32_t>(row) * p.a.group / kColumns) + index;
     const uint64_t before = __ballot(in && begins <= unit);
     if (before == 0) return false;
     const int k = 63 - __clzll(static_cast<long long>(before));
     low += k * step;
     if (step == 1) {
-      const int at = __builtin_amdgcn_readlane(static_cast<int>(unit - begins), k);
       r = low;
-      block = at;
+      block = unit - __builtin_amdgcn_readlane(begins, k);
+      q = request_from(mine, k);
       return true;
     }
     count = min(step, count - k * step);
@@ -98,30 +100,29 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
   const int head = blockIdx.x % c.kv_heads;
   const int rest = blockIdx.x / c.kv_heads;
   const int split = rest % p.splits;
-  const int64_t unit = p.units - 1 - rest / p.splits;   // (the longest walks of a request first)
-  int r;
-  int64_t block;
-  if (!find_unit(p, unit, r, block)) return;
-  const Request q = request_of(c, r);
-  const int64_t columns = (q.last - q.first) * a.group;   // (none: not above zero)
+  const int unit = p.units - 1 - rest / p.splits;   // (the longest walks of a request first)
+  int r, block;
+  Request q;
+  if (!find_unit(p, unit, r, q, block)) return;
+  const int columns = static_cast<int>(q.last - q.first) * a.group;   // (none: not above zero)
   if (block * kColumns >= columns) return;
   const int32_t* const table = c.pages + r * c.pages_row;
 
   // this lane's column, and how many tokens it, the wave's first and last and the workgroup's last see
-  const int64_t column = block * kColumns + 32 * wave + m;
-  auto sees = [&](int64_t t) {
+  const int column = block * kColumns + 32 * wave + m;
+  auto sees = [&](uint32_t t) {
     return static_cast<int>(max(min(q.first + t + q.shift + 1, static_cast<int64_t>(q.tokens)), int64_t{0}));
   };
   const bool real = column < columns;
-  const int64_t t_row = (real ? column : columns - 1) / a.group;
-  const int g_row = static_cast<int>((real ? column : columns - 1) - t_row * a.group);
+  const uint32_t group = a.group;
+  const uint32_t t_row = (real ? column : columns - 1) / group;
+  const int g_row = (real ? column : columns - 1) - t_row * group;
   const int limit = sees(t_row);
   const int least = __builtin_amdgcn_readlane(limit, 0);
-  const int first_limit = sees(block * kColumns / a.group);
-  const int wave_tiles = (__builtin_amdgcn_readlane(limit, 31) + kTile - 1) / kTile;
-  const int all_tiles = (sees((min(block * kColumns + kColumns, columns) - 1) / a.group) + kTile - 1) / kTile;
-  const int begin = static_cast<int>(static_cast<int64_t>(all_tiles) * split / p.splits);
-  const int end = static_cast<int>(static_cast<int64_t>(all_tiles) * (split + 1) / p.splits);
+  const int first_limit = sees(block * kColumns / group);
+  const int all_tiles = (sees((min(block * kColumns + kColumns, columns) - 1) / group) + kTile - 1) / kTile;
+  const int each = (all_tiles + p.splits - 1) / p.splits;
+  const int begin = min(split * each, all_tiles), end = min(begin + each, all_tiles);
   const bool works = block * kColumns + 32 * wave < columns;
 
   bf16x8 query[8];
@@ -150,14 +151,14 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
   };
   u32x4 keys[2], values[2];
   float k_scale, v_scale[2];
-  uint64_t live;
-  auto load = [&](int tile, int page) {
-    live = __ballot(page > 0);
+  auto load_keys = [&](int tile, int page) {
     const int in = (tile * kTile + lane) & ((1 << c.page_log2) - 1);
     const uint8_t* const at_k = k_tile(c, page, head) + (((wave << c.page_log2) + in) << 4);
     keys[0] = *reinterpret_cast<const u32x4*>(at_k);
     keys[1] = *reinterpret_cast<const u32x4*>(at_k + (64 << c.page_log2));
     k_scale = scale_value(c.k_scale[page * c.k_scale_page + head]);
+  };
+  auto load_values = [&](int tile, int page) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int group = (wave >> 1) + 2 * i;
@@ -168,34 +169,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
       v_scale[i] = scale_value(c.v_scale[theirs * c.v_scale_page + head]);
     }
   };
-  auto stage = [&](int tile, int to) {
-    // values behind the last token, or without a page, are zeros; so are those that are not finite,
-    // and marked below, in tiles that some column does not see whole
-    const bool partial = tile * kTile + kTile > first_limit;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int group = (wave >> 1) + 2 * i;
-      const int first = tile * kTile + 16 * group;
-      const int kept = live >> (16 * group) & 1 ? q.tokens - first : 0;
-      if (kept < 16) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) values[i][w] &= first_bytes(kept - 4 * w);
-      }
-      if (partial) {
-        uint32_t any = 0;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t at_nan = nan_bytes(values[i][w]);
-          any |= at_nan;
-          values[i][w] &= ~((at_nan >> 7) * 0xffu);
-        }
-        if (any != 0) lds_strange = 1;
-      }
-      lds_values[to][(2 * group) * kDim + element] =
-          __builtin_bit_cast(u32x4, operand8(values[i][0], values[i][1], v_scale[i]));
-      lds_values[to][(2 * group + 1) * kDim + element] =
-          __builtin_bit_cast(u32x4, operand8(values[i][2], values[i][3], v_scale[i]));
-    }
+  auto stage_keys = [&](int to) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int chunk = wave + 4 * i;
@@ -205,84 +179,113 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
           __builtin_bit_cast(u32x4, operand8(keys[i][2], keys[i][3], k_scale));
     }
   };
+  auto stage_values = [&](int tile, uint64_t live, int to) {
+    // values behind the last token, or without a page, are zeros; so are those that are not finite,
+    // and marked below, in tiles that some column does not see whole
+    if (tile * kTile + kTile > first_limit || live != ~uint64_t{0}) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int group = (wave >> 1) + 2 * i;
+        const int kept = live >> (16 * group) & 1 ? q.tokens - (tile * kTile + 16 * group) : 0;
+        uint32_t any = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t x = values[i][w] & first_bytes(kept - 4 * w);
+          const uint32_t at_nan = nan_bytes(x);
+          any |= at_nan;
+          values[i][w] = x & ~((at_nan >> 7) * 0xffu);
+        }
+        if (any != 0) lds_strange = 1;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int group = (wave >> 1) + 2 * i;
+      lds_values[to][(2 * group) * kDim + element] =
+          __builtin_bit_cast(u32x4, operand8(values[i][0], values[i][1], v_scale[i]));
+      lds_values[to][(2 * group + 1) * kDim + element] =
+          __builtin_bit_cast(u32x4, operand8(values[i][2], values[i][3], v_scale[i]));
+    }
+  };
+  auto scores = [&](int at, f32x16 (&x)[2]) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[t][i] = 0.0f;
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const u32x4 k = lds_keys[at][(2 * (2 * (s >> 1) + h) + (s & 1)) * kTile + 32 * t + m];
+        x[t] = mfma32(__builtin_bit_cast(bf16x8, k), query[s], x[t]);
+      }
+  };
+  // Scores of -inf, for weights of zero, where the column does not see a token; and what a new
+  // maximum changes.
+  auto settle = [&](int tile, uint64_t live, f32x16 (&x)[2]) {
+    float most = kLowest;   // (of a score of -inf that is seen: a weight of zero, not none)
+    if (!(tile * kTile + kTile <= least && live == ~uint64_t{0})) {
+      bool any = false;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int token = tile * kTile + 32 * t + 16 * h;
+        const bool lives = live >> (32 * t + 16 * h) & 1;
+        any = any || (lives && token < limit);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (!lives || token + i >= limit) x[t][i] = -__builtin_inff();
+      }
+      if (!any) most = -__builtin_inff();
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) most = fmaxf(most, x[t][i]);
+    const uint32_t u = __float_as_uint(most);
+    const auto y = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    most = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+    if (__any((most - top) * a.log2_scale > 8.0f)) {
+      const float now = fmaxf(top, most);
+      const float keep = now == top ? 1.0f : exp2_fast((top - now) * a.log2_scale);
+      sum *= keep;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) o[b] *= keep;
+      top = now;
+    }
+  };
+
   if (threadIdx.x == 0) lds_strange = 0;
   __syncthreads();
-  int page_next = page_of(begin);
-  uint64_t live_now = 0;
+  // A step finds its tile's scores settled and computes the next tile's beside the weights: keys are
+  // in LDS a tile ahead of values.
+  int page = page_of(begin), page_next = page_of(begin + 1), page_then = page_of(begin + 2);
+  f32x16 score[2];
   if (begin < end) {
-    load(begin, page_next);
-    page_next = page_of(begin + 1);
-    stage(begin, 0);
-    live_now = live;
-  }
-  __syncthreads();
-  for (int tile = begin; tile < end; ++tile) {
-    const int now_at = (tile - begin) & 1;
-    const bool more = tile + 1 < end;
-    if (more) {
-      load(tile + 1, page_next);
-      page_next = page_of(tile + 2);
+    load_keys(begin, page);
+    load_values(begin, page);
+    stage_keys(0);
+    stage_values(begin, __ballot(page > 0), 0);
+    load_keys(begin + 1, page_next);
+    stage_keys(1);
+    lds_barrier();
+    if (works) {
+      scores(0, score);
+      settle(begin, __ballot(page > 0), score);
     }
-    if (works && tile < wave_tiles) {
-      const int token0 = tile * kTile;
-      f32x16 score[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) score[t][i] = 0.0f;
-#pragma unroll
-      for (int s = 0; s < 8; ++s)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const u32x4 k = lds_keys[now_at][(2 * (2 * (s >> 1) + h) + (s & 1)) * kTile + 32 * t + m];
-          score[t] = mfma32(__builtin_bit_cast(bf16x8, k), query[s], score[t]);
-        }
-      // the first values' operands too, which the weights' arithmetic covers
-      u32x4 early[4];
-#pragma unroll
-      for (int b = 0; b < 4; ++b) early[b] = lds_values[now_at][2 * h * kDim + 32 * b + m];
-      // (operands read six ahead of the product that takes them)
-      __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
-#pragma unroll
-      for (int i = 0; i < 14; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-      lds_order();
-      // a tile that some column does not see whole: scores of -inf, weights of zero
-      const bool whole = token0 + kTile <= least && live_now == ~uint64_t{0};
-      float most = kLowest;   // (of a score of -inf that is seen: a weight of zero, not none)
-      if (!whole) {
-        bool any = false;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const bool lives = live_now >> (32 * t + 16 * h) & 1;
-          any = any || (lives && token0 + 32 * t + 16 * h < limit);
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (!lives || token0 + 32 * t + 16 * h + i >= limit) score[t][i] = -__builtin_inff();
-        }
-        if (!any) most = -__builtin_inff();
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) most = fmaxf(most, score[t][i]);
-      {
-        const uint32_t u = __float_as_uint(most);
-        const auto x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-        most = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-      }
-      if (__any((most - top) * a.log2_scale > 8.0f)) {
-        const float now = fmaxf(top, most);
-        const float keep = now == top ? 1.0f : exp2_fast((top - now) * a.log2_scale);
-        sum *= keep;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) o[b] *= keep;
-        top = now;
-      }
+    lds_barrier();
+  }
+  auto step = [&](int tile, int now_at, f32x16 (&mine)[2], f32x16 (&next)[2]) {
+    // (past the last tile pages are 0: bytes that nothing uses)
+    load_values(tile + 1, page_next);
+    load_keys(tile + 2, page_then);
+    page = page_next;
+    page_next = page_then;
+    page_then = page_of(tile + 3);
+    const uint64_t live = __ballot(page > 0);
+    if (works) {
       const float less = top == -__builtin_inff() ? 0.0f : -top * a.log2_scale;
+      __builtin_amdgcn_s_setprio(1);
+      scores(now_at ^ 1, next);
       bf16x8 weight[2][2];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -291,8 +294,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
           u32x4 bits;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const float x = exp2_fast(fmaf(score[t][8 * u + 2 * w], a.log2_scale, less));
-            const float y = exp2_fast(fmaf(score[t][8 * u + 2 * w + 1], a.log2_scale, less));
+            const float x = exp2_fast(fmaf(mine[t][8 * u + 2 * w], a.log2_scale, less));
+            const float y = exp2_fast(fmaf(mine[t][8 * u + 2 * w + 1], a.log2_scale, less));
             sum += x;
             sum += y;
             bits[w] = bf16_pair(f32x2{x, y});
@@ -305,16 +308,33 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
-            const u32x4 v = t + u == 0 ? early[b]
-                                       : lds_values[now_at][(2 * (2 * t + h) + u) * kDim + 32 * b + m];
+            const u32x4 v = lds_values[now_at][(2 * (2 * t + h) + u) * kDim + 32 * b + m];
             o[b] = mfma32(__builtin_bit_cast(bf16x8, v), weight[t][u], o[b]);
           }
+      // (a product of the next scores, an operand read and seven of the weights' instructions at a time)
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 7, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
     }
-    if (more) {
-      stage(tile + 1, now_at ^ 1);
-      live_now = live;
-    }
+    __builtin_amdgcn_s_setprio(0);
+    stage_values(tile + 1, live, now_at ^ 1);
+    stage_keys(now_at);
+    if (works) settle(tile + 1, live, next);
     lds_barrier();
+  };
+  f32x16 other[2];
+  for (int tile = begin; tile < end; tile += 2) {
+    step(tile, 0, score, other);
+    if (tile + 1 < end) step(tile + 1, 1, other, score);
   }
 
   if (lds_strange) {
@@ -368,7 +388,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
         store_four(a, q.first + t_row, head * a.group + g_row, 32 * b + 8 * e + 4 * h, quad(o[b], e),
                    some, inverse);
   } else {
-    float* const to = split_at(p, (unit * c.kv_heads + head) * p.splits + split);
+    float* const to = split_at(p, (static_cast<int64_t>(unit) * c.kv_heads + head) * p.splits + split);
     const int at = 32 * wave + m;
 #pragma unroll
     for (int b = 0; b < 4; ++b)
@@ -388,16 +408,15 @@ __global__ __launch_bounds__(kThreads) void attention_gather_kernel(const Prefil
   const int part = blockIdx.x % (kColumns / kEach);
   const int rest = blockIdx.x / (kColumns / kEach);
   const int head = rest % c.kv_heads;
-  const int64_t unit = rest / c.kv_heads;
-  int r;
-  int64_t block;
-  if (!find_unit(p, unit, r, block)) return;
-  const Request q = request_of(c, r);
+  const int unit = rest / c.kv_heads;
+  int r, block;
+  Request q;
+  if (!find_unit(p, unit, r, q, block)) return;
   const int within = part * kEach + (threadIdx.x >> 5);
-  const int64_t column = block * kColumns + within;
+  const int column = block * kColumns + within;
   if (column >= (q.last - q.first) * a.group) return;
   const int d = 4 * (threadIdx.x & 31);
-  const int64_t place = (unit * c.kv_heads + head) * p.splits;
+  const int64_t place = (static_cast<int64_t>(unit) * c.kv_heads + head) * p.splits;
   float best = -__builtin_inff(), all = 0.0f;
   f32x4 x = {0, 0, 0, 0};
 #pragma unroll 4
@@ -415,8 +434,8 @@ __global__ __launch_bounds__(kThreads) void attention_gather_kernel(const Prefil
       for (int i = 0; i < 4; ++i) x[i] = x[i] * keep + theirs[i] * add;
     }
   }
-  const int64_t t = column / a.group;
-  store_four(a, q.first + t, head * a.group + static_cast<int>(column - t * a.group), d, x,
+  const int t = column / a.group;
+  store_four(a, q.first + t, head * a.group + column - t * a.group, d, x,
              best > -__builtin_inff(), 1.0f / all);
 }
 
@@ -460,7 +479,7 @@ extern "C" int ld_attention_prefill(const ld_paged_cache* cache, const ld_attent
                       args->workspace_bytes < s.bytes))
     return fail(LD_ERR_INVALID_ARGUMENT, "workspace missing or too small");
   const int64_t blocks = s.units * s.splits * p.cache.kv_heads;
-  if (blocks > 0x7fffffff) return fail(LD_ERR_INVALID_ARGUMENT, "too many rows and heads");
+  if (blocks > 0x7fffffff || p.cache.num_tokens * p.a.group > 0x7fffff00) return fail(LD_ERR_INVALID_ARGUMENT, "too many rows and heads");
   p.units = static_cast<int32_t>(s.units);
   p.splits = static_cast<int32_t>(s.splits);
   const hipStream_t on = static_cast<hipStream_t>(stream);
