@@ -166,6 +166,25 @@ __device__ __forceinline__ const uint8_t* v_tile(const Cache& c, int page, int h
   return c.v + page * c.v_page + (static_cast<int64_t>(head) << (7 + c.page_log2));
 }
 
+// The value of the lane that Ctrl names, in the rows of RowMask; 0 where there is none.
+template <int Ctrl, int RowMask>
+__device__ __forceinline__ uint32_t shifted(uint32_t x) {
+  return static_cast<uint32_t>(
+      __builtin_amdgcn_update_dpp(0, static_cast<int>(x), Ctrl, RowMask, 0xF, false));
+}
+
+// The sum of x over the lanes up to and with this one: within rows of 16 lanes, then from each row's
+// last lane to the next row, then to the upper half.
+__device__ __forceinline__ uint32_t sum_up_to(uint32_t x) {
+  x += shifted<0x111, 0xf>(x);
+  x += shifted<0x112, 0xf>(x);
+  x += shifted<0x114, 0xf>(x);
+  x += shifted<0x118, 0xf>(x);
+  x += shifted<0x142, 0xa>(x);
+  x += shifted<0x143, 0xc>(x);
+  return x;
+}
+
 // Codes 4 w .. 4 w + 3 of each word as operands: e4m3 times a power of two is exact in bf16.
 __device__ __forceinline__ bf16x8 operand8(uint32_t lo, uint32_t hi, float scale) {
   u32x4 r;

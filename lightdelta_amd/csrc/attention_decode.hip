@@ -46,13 +46,6 @@ __device__ __host__ inline Layout layout_of(int64_t requests, int64_t columns) {
   return Layout{(requests + 2 + 3) & ~int64_t{3}, columns};
 }
 
-// The value of the lane that Ctrl names, in the rows of RowMask; 0 where there is none.
-template <int Ctrl, int RowMask>
-__device__ __forceinline__ uint32_t shifted(uint32_t x) {
-  return static_cast<uint32_t>(
-      __builtin_amdgcn_update_dpp(0, static_cast<int>(x), Ctrl, RowMask, 0xF, false));
-}
-
 // Requests and their tiles, 64 requests at a time, one a lane; every lane of a wave calls it.
 struct Walk {
   int base = 0;            // the first of the 64
@@ -71,13 +64,7 @@ struct Walk {
     tiles = real && rows > 0 && rows <= p.a.width
                 ? (static_cast<uint32_t>(mine.tokens) + kTile - 1) / kTile : 0;
     behind = tiles;
-    // (within rows of 16 lanes, then from each row's last lane to the next row, then to the upper half)
-    behind += shifted<0x111, 0xf>(behind);
-    behind += shifted<0x112, 0xf>(behind);
-    behind += shifted<0x114, 0xf>(behind);
-    behind += shifted<0x118, 0xf>(behind);
-    behind += shifted<0x142, 0xa>(behind);
-    behind += shifted<0x143, 0xc>(behind);
+    behind = sum_up_to(behind);
     all = __builtin_amdgcn_readlane(behind, 63);
   }
   // Tiles of all requests; ends at the first 64 again.  `plan`: where those ahead of each request

@@ -28,8 +28,90 @@ struct PrefillAttention {
   Cache cache;
   Attention a;
   int32_t units;    // blocks of columns of all requests, at most
-  int32_t splits;   // workgroups a unit and kv head
+  uint32_t room;    // sums that the workspace holds
 };
+
+// Where blocks of columns are few, a request's tokens are split over as many workgroups as make
+// shares of about equal length: the plan, worked out by every workgroup from the lengths, and left in
+// the workspace for the launch that joins.
+constexpr int kShares = 512;      // two a CU
+constexpr int kLeastShare = 4;    // tiles
+
+struct Share {
+  uint32_t first;    // share of the request's first block, per kv head
+  uint32_t splits;   // shares a block
+};
+
+struct Shares {
+  Request mine;         // of this lane's request of the 64 at hand
+  uint32_t splits, blocks, behind, all, before = 0;
+  int base = 0;
+
+  __device__ __forceinline__ uint32_t load(const PrefillAttention& p, int first) {
+    const int r = first + (threadIdx.x & 63);
+    base = first;
+    mine = request_of(p.cache, min(r, p.cache.requests - 1));
+    const int64_t rows = r < p.cache.requests ? max(mine.last - mine.first, int64_t{0}) : 0;
+    blocks = (static_cast<uint32_t>(rows) * p.a.group + kColumns - 1) / kColumns;
+    return (static_cast<uint32_t>(mine.tokens) + kTile - 1) / kTile;   // tiles of its last block
+  }
+  __device__ __forceinline__ void split(uint32_t tiles, uint32_t share) {
+    splits = max((tiles + share - 1) / share, 1u);
+    behind = sum_up_to(blocks * splits);
+    all = __builtin_amdgcn_readlane(behind, 63);
+  }
+  // The share's length: all tiles over the shares, a little more for what 32 bits round off, so that
+  // shares are at most kShares and a block and kv head's one more.
+  __device__ __forceinline__ uint32_t length(const PrefillAttention& p, uint32_t& tiles) {
+    float total = 0.0f;
+    for (int first = 0;; first += 64) {
+      tiles = load(p, first);
+      total += wave_sum(static_cast<float>(blocks) * tiles);
+      if (first + 64 >= p.cache.requests) break;
+    }
+    if (p.cache.requests > 64) tiles = load(p, 0);
+    const float each = total * p.cache.kv_heads * (1.0001f / kShares);
+    return max(static_cast<uint32_t>(min(each, 1e9f)) + 1, static_cast<uint32_t>(kLeastShare));
+  }
+};
+
+// Share -> request, block of its columns and which of its splits; false where there is none.
+__device__ __forceinline__ bool find_share(const PrefillAttention& p, uint32_t share, Share* plan,
+                                           int& r, Request& q, int& block, int& split, int& splits) {
+  Shares s;
+  uint32_t tiles;
+  const uint32_t length = s.length(p, tiles);
+  s.split(tiles, length);
+  if (plan != nullptr) {
+    for (;;) {
+      const int mine = s.base + (threadIdx.x & 63);
+      if (mine < p.cache.requests)
+        plan[mine] = Share{s.before + s.behind - s.blocks * s.splits, s.splits};
+      if (s.base + 64 >= p.cache.requests) break;
+      s.before += s.all;
+      tiles = s.load(p, s.base + 64);
+      s.split(tiles, length);
+    }
+    s.before = 0;
+    if (p.cache.requests > 64) s.split(s.load(p, 0), length);
+  }
+  while (share >= s.before + s.all) {
+    if (s.base + 64 >= p.cache.requests) return false;
+    s.before += s.all;
+    tiles = s.load(p, s.base + 64);
+    s.split(tiles, length);
+  }
+  const uint32_t local = share - s.before;
+  const int k = __popcll(__ballot(s.behind <= local));
+  splits = __builtin_amdgcn_readlane(s.splits, k);
+  const uint32_t first = __builtin_amdgcn_readlane(s.behind, k) -
+                         __builtin_amdgcn_readlane(s.blocks, k) * splits;
+  r = s.base + k;
+  q = request_from(s.mine, k);
+  block = (local - first) / splits;
+  split = (local - first) % splits;
+  return true;
+}
 
 // Unit -> request, what it has in the call, and block of its columns; false where there is none.
 // Requests have a run of units each, one more than their columns can fill at the most, so that where
@@ -63,8 +145,9 @@ __device__ __forceinline__ bool find_unit(const PrefillAttention& p, int unit, i
   }
 }
 
+__device__ __host__ inline int64_t plan_floats(int64_t requests) { return (2 * requests + 3) & ~int64_t{3}; }
 __device__ __forceinline__ float* split_at(const PrefillAttention& p, int64_t place) {
-  return p.a.workspace + place * kColumns * (kDim + 2);
+  return p.a.workspace + plan_floats(p.cache.requests) + place * kColumns * (kDim + 2);
 }
 
 // Four elements of an output: divided, gated and rounded.
@@ -84,6 +167,8 @@ __device__ __forceinline__ void store_four(const Attention& a, int64_t row, int 
   __builtin_memcpy(a.out + (row * a.q_heads + head) * kDim + d, bits, 8);
 }
 
+// Split: workgroups are shares, else units.
+template <bool Split>
 __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const PrefillAttention p) {
   const Cache& c = p.cache;
   const Attention& a = p.a;
@@ -99,11 +184,14 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
 
   const int head = blockIdx.x % c.kv_heads;
   const int rest = blockIdx.x / c.kv_heads;
-  const int split = rest % p.splits;
-  const int unit = p.units - 1 - rest / p.splits;   // (the longest walks of a request first)
-  int r, block;
+  int r, block, split = 0, splits = 1;
   Request q;
-  if (!find_unit(p, unit, r, q, block)) return;
+  if constexpr (Split) {
+    Share* const plan = blockIdx.x == 0 && wave == 0 ? reinterpret_cast<Share*>(a.workspace) : nullptr;
+    if (!find_share(p, rest, plan, r, q, block, split, splits)) return;
+  } else {
+    if (!find_unit(p, p.units - 1 - rest, r, q, block)) return;   // (a request's longest walks first)
+  }
   const int columns = static_cast<int>(q.last - q.first) * a.group;   // (none: not above zero)
   if (block * kColumns >= columns) return;
   const int32_t* const table = c.pages + r * c.pages_row;
@@ -121,7 +209,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
   const int least = __builtin_amdgcn_readlane(limit, 0);
   const int first_limit = sees(block * kColumns / group);
   const int all_tiles = (sees((min(block * kColumns + kColumns, columns) - 1) / group) + kTile - 1) / kTile;
-  const int each = (all_tiles + p.splits - 1) / p.splits;
+  const int each = (all_tiles + splits - 1) / splits;
   const int begin = min(split * each, all_tiles), end = min(begin + each, all_tiles);
   const bool works = block * kColumns + 32 * wave < columns;
 
@@ -378,7 +466,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
   }
   sum = add_partner<32>(sum);
   if (!real) return;
-  if (p.splits == 1) {
+  if (splits == 1) {
     const bool some = top > -__builtin_inff();   // the row sees a token
     const float inverse = 1.0f / sum;
 #pragma unroll
@@ -388,7 +476,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
         store_four(a, q.first + t_row, head * a.group + g_row, 32 * b + 8 * e + 4 * h, quad(o[b], e),
                    some, inverse);
   } else {
-    float* const to = split_at(p, (static_cast<int64_t>(unit) * c.kv_heads + head) * p.splits + split);
+    float* const to = split_at(p, blockIdx.x);
     const int at = 32 * wave + m;
 #pragma unroll
     for (int b = 0; b < 4; ++b)
@@ -399,59 +487,83 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
   }
 }
 
-// Joins the sums of a unit's splits, in their order: thread (column, four elements), eight columns a
-// workgroup.
-__global__ __launch_bounds__(kThreads) void attention_gather_kernel(const PrefillAttention p) {
+// Joins the sums of a unit's shares: thread (column, four elements), eight columns a workgroup, four
+// groups of threads that take every fourth share.
+constexpr int kGatherThreads = 1024;
+constexpr int kGatherColumns = 8;
+__global__ __launch_bounds__(kGatherThreads) void attention_gather_kernel(const PrefillAttention p) {
   const Cache& c = p.cache;
   const Attention& a = p.a;
-  constexpr int kEach = kThreads / 32;
-  const int part = blockIdx.x % (kColumns / kEach);
-  const int rest = blockIdx.x / (kColumns / kEach);
+  const int part = blockIdx.x % (kColumns / kGatherColumns);
+  const int rest = blockIdx.x / (kColumns / kGatherColumns);
   const int head = rest % c.kv_heads;
-  const int unit = rest / c.kv_heads;
   int r, block;
   Request q;
-  if (!find_unit(p, unit, r, q, block)) return;
-  const int within = part * kEach + (threadIdx.x >> 5);
+  if (!find_unit(p, rest / c.kv_heads, r, q, block)) return;
+  const int columns = static_cast<int>(q.last - q.first) * a.group;
+  if (block * kColumns + part * kGatherColumns >= columns) return;
+  const Share plan = reinterpret_cast<const Share*>(a.workspace)[r];
+  const uint32_t first = plan.first + block * plan.splits;
+  // (rows that two requests claim make a plan that the workspace has no room for)
+  if (plan.splits == 1 || static_cast<uint64_t>(first + plan.splits) * c.kv_heads > p.room) return;
+  const int group = threadIdx.x >> 8;
+  const int mine = threadIdx.x >> 5 & 7;
+  const int within = part * kGatherColumns + mine;
   const int column = block * kColumns + within;
-  if (column >= (q.last - q.first) * a.group) return;
   const int d = 4 * (threadIdx.x & 31);
-  const int64_t place = (static_cast<int64_t>(unit) * c.kv_heads + head) * p.splits;
   float best = -__builtin_inff(), all = 0.0f;
   f32x4 x = {0, 0, 0, 0};
-#pragma unroll 4
-  for (int s = 0; s < p.splits; ++s) {
-    const float* const from = split_at(p, place + s);
-    const f32x2 stat = *reinterpret_cast<const f32x2*>(from + kColumns * kDim + 2 * within);
-    const f32x4 theirs = *reinterpret_cast<const f32x4*>(from + within * kDim + d);
-    if (stat[0] > -__builtin_inff()) {   // (what saw nothing has sums of zero)
-      const float now = fmaxf(best, stat[0]);
+  auto add = [&](float top, float total, f32x4 theirs) {
+    if (top > -__builtin_inff()) {   // (what saw nothing has sums of zero)
+      const float now = fmaxf(best, top);
       const float keep = best == now ? 1.0f : exp2_fast((best - now) * a.log2_scale);
-      const float add = stat[0] == now ? 1.0f : exp2_fast((stat[0] - now) * a.log2_scale);
+      const float by = top == now ? 1.0f : exp2_fast((top - now) * a.log2_scale);
       best = now;
-      all = all * keep + stat[1] * add;
+      all = all * keep + total * by;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = x[i] * keep + theirs[i] * add;
+      for (int i = 0; i < 4; ++i) x[i] = x[i] * keep + theirs[i] * by;
+    }
+  };
+  if (column < columns) {
+#pragma unroll 4
+    for (uint32_t s = group; s < plan.splits; s += 4) {
+      const float* const from = split_at(p, static_cast<int64_t>(first + s) * c.kv_heads + head);
+      const f32x2 stat = *reinterpret_cast<const f32x2*>(from + kColumns * kDim + 2 * within);
+      add(stat[0], stat[1], *reinterpret_cast<const f32x4*>(from + within * kDim + d));
     }
   }
+  __shared__ f32x4 sums[3][kGatherColumns][32];
+  __shared__ f32x2 stats[3][kGatherColumns];
+  if (group > 0) {
+    sums[group - 1][mine][threadIdx.x & 31] = x;
+    if (d == 0) stats[group - 1][mine] = f32x2{best, all};
+  }
+  __syncthreads();
+  if (group > 0 || column >= columns) return;
+#pragma unroll
+  for (int g = 0; g < 3; ++g)
+    add(stats[g][mine][0], stats[g][mine][1], sums[g][mine][threadIdx.x & 31]);
   const int t = column / a.group;
   store_four(a, q.first + t, head * a.group + column - t * a.group, d, x,
              best > -__builtin_inff(), 1.0f / all);
 }
 
-// Blocks of columns, and over how many workgroups each one's tokens are split: two workgroups a CU
-// between them, each of four tiles at least were its table full.
+// Blocks of columns, at most, and workgroups: one a block and kv head, or shares where those would not
+// give each CU two and a table holds tokens for more than one.
 struct Shape {
-  int64_t units, splits, bytes;
+  int64_t units, blocks, bytes;
 };
 
 Shape prefill_shape(const ld_paged_cache& c, int64_t q_heads) {
   Shape s{};
   const int64_t group = q_heads / c.num_kv_heads;
   s.units = c.num_tokens * group / kColumns + c.num_requests;
-  const int64_t tiles = (static_cast<int64_t>(c.table_width) * c.page_size + kTile - 1) / kTile;
-  s.splits = std::max<int64_t>(1, std::min(512 / (s.units * c.num_kv_heads), tiles / 4));
-  s.bytes = s.splits == 1 ? 0 : s.units * c.num_kv_heads * s.splits * kColumns * (kDim + 2) * 4;
+  s.blocks = s.units * c.num_kv_heads;
+  if (s.blocks < kShares &&
+      static_cast<int64_t>(c.table_width) * c.page_size > kTile * kLeastShare) {
+    s.blocks += kShares;
+    s.bytes = (plan_floats(c.num_requests) + s.blocks * kColumns * (kDim + 2)) * 4;
+  }
   return s;
 }
 
@@ -478,18 +590,21 @@ extern "C" int ld_attention_prefill(const ld_paged_cache* cache, const ld_attent
   if (s.bytes > 0 && (p.a.workspace == nullptr || !aligned16(p.a.workspace) ||
                       args->workspace_bytes < s.bytes))
     return fail(LD_ERR_INVALID_ARGUMENT, "workspace missing or too small");
-  const int64_t blocks = s.units * s.splits * p.cache.kv_heads;
-  if (blocks > 0x7fffffff || p.cache.num_tokens * p.a.group > 0x7fffff00) return fail(LD_ERR_INVALID_ARGUMENT, "too many rows and heads");
+  if (s.blocks > 0x7fffffff || p.cache.num_tokens * p.a.group > 0x7fffff00)
+    return fail(LD_ERR_INVALID_ARGUMENT, "too many rows and heads");
   p.units = static_cast<int32_t>(s.units);
-  p.splits = static_cast<int32_t>(s.splits);
+  p.room = static_cast<uint32_t>(s.blocks);
   const hipStream_t on = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(attention_prefill_kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kThreads),
-                     0, on, p);
+  const dim3 grid(static_cast<uint32_t>(s.blocks));
+  if (s.bytes == 0) {
+    hipLaunchKernelGGL(attention_prefill_kernel<false>, grid, dim3(kThreads), 0, on, p);
+    return check_launch("ld_attention_prefill");
+  }
+  hipLaunchKernelGGL(attention_prefill_kernel<true>, grid, dim3(kThreads), 0, on, p);
   if (const int rc = check_launch("ld_attention_prefill")) return rc;
-  if (s.splits == 1) return LD_OK;
-  // (at most 512 units and heads)
-  const int64_t joins = s.units * p.cache.kv_heads * (kColumns / (kThreads / 32));
-  hipLaunchKernelGGL(attention_gather_kernel, dim3(static_cast<uint32_t>(joins)), dim3(kThreads), 0,
-                     on, p);
+  // (fewer than 512 units and heads)
+  const int64_t joins = s.units * p.cache.kv_heads * (kColumns / kGatherColumns);
+  hipLaunchKernelGGL(attention_gather_kernel, dim3(static_cast<uint32_t>(joins)),
+                     dim3(kGatherThreads), 0, on, p);
   return check_launch("ld_attention_prefill");
 }
