@@ -31,11 +31,16 @@ struct PrefillAttention {
   uint32_t room;    // sums that the workspace holds
 };
 
-// Where blocks of columns are few, a request's tokens are split over as many workgroups as make
-// shares of about equal length: the plan, worked out by every workgroup from the lengths, and left in
-// the workspace for the launch that joins.
-constexpr int kShares = 512;      // two a CU
-constexpr int kLeastShare = 4;    // tiles
+// Where blocks of columns are fewer than CUs, a request's tokens are split over as many workgroups as
+// make shares of about equal length: the plan, worked out by every workgroup from the lengths, and
+// left in the workspace for the launch that joins.  Sums of a share are 66 KB, written and read
+// again, so that a request whose first rows see fewer than 16 tiles is left whole (a new prompt of 1,500
+// tokens 41 us, split 53), as is every one where blocks fill the CUs (one of 2,048 tokens 52 and 62);
+// 512 tokens behind 2,800 take 40 us, whole 78.
+constexpr int kCus = 256;
+constexpr int kShares = 2 * kCus;
+constexpr int kLeastShare = 8;    // tiles
+constexpr int kLeastWalk = 16;
 
 struct Share {
   uint32_t first;    // share of the request's first block, per kv head
@@ -56,7 +61,7 @@ struct Shares {
     return (static_cast<uint32_t>(mine.tokens) + kTile - 1) / kTile;   // tiles of its last block
   }
   __device__ __forceinline__ void split(uint32_t tiles, uint32_t share) {
-    splits = max((tiles + share - 1) / share, 1u);
+    splits = mine.first + mine.shift < kLeastWalk * kTile ? 1u : (tiles + share - 1) / share;
     behind = sum_up_to(blocks * splits);
     all = __builtin_amdgcn_readlane(behind, 63);
   }
@@ -487,11 +492,14 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
   }
 }
 
-// Joins the sums of a unit's shares: thread (column, four elements), eight columns a workgroup, four
-// groups of threads that take every fourth share.
-constexpr int kGatherThreads = 1024;
+// Joins the sums of a unit's shares: thread (column, four elements), eight columns a workgroup and
+// Groups of threads that take every Groups-th share.  Few units have many shares each: four groups (three
+// prompts behind up to 30,000 tokens, 30 shares: 10 us, one group 23); with more, whose shares are
+// few, the threads of one group start in less time (one prompt of 1,024 tokens 32 us in all, four 37).
 constexpr int kGatherColumns = 8;
-__global__ __launch_bounds__(kGatherThreads) void attention_gather_kernel(const PrefillAttention p) {
+constexpr int kFewUnits = 64;
+template <int Groups>
+__global__ __launch_bounds__(Groups * 256) void attention_gather_kernel(const PrefillAttention p) {
   const Cache& c = p.cache;
   const Attention& a = p.a;
   const int part = blockIdx.x % (kColumns / kGatherColumns);
@@ -525,31 +533,34 @@ __global__ __launch_bounds__(kGatherThreads) void attention_gather_kernel(const 
     }
   };
   if (column < columns) {
-#pragma unroll 4
-    for (uint32_t s = group; s < plan.splits; s += 4) {
+#pragma unroll 8
+    for (uint32_t s = group; s < plan.splits; s += Groups) {
       const float* const from = split_at(p, static_cast<int64_t>(first + s) * c.kv_heads + head);
       const f32x2 stat = *reinterpret_cast<const f32x2*>(from + kColumns * kDim + 2 * within);
       add(stat[0], stat[1], *reinterpret_cast<const f32x4*>(from + within * kDim + d));
     }
   }
-  __shared__ f32x4 sums[3][kGatherColumns][32];
-  __shared__ f32x2 stats[3][kGatherColumns];
-  if (group > 0) {
-    sums[group - 1][mine][threadIdx.x & 31] = x;
-    if (d == 0) stats[group - 1][mine] = f32x2{best, all};
-  }
-  __syncthreads();
-  if (group > 0 || column >= columns) return;
+  if constexpr (Groups > 1) {
+    __shared__ f32x4 sums[Groups - 1][kGatherColumns][32];
+    __shared__ f32x2 stats[Groups - 1][kGatherColumns];
+    if (group > 0) {
+      sums[group - 1][mine][threadIdx.x & 31] = x;
+      if (d == 0) stats[group - 1][mine] = f32x2{best, all};
+    }
+    __syncthreads();
+    if (group > 0) return;
 #pragma unroll
-  for (int g = 0; g < 3; ++g)
-    add(stats[g][mine][0], stats[g][mine][1], sums[g][mine][threadIdx.x & 31]);
+    for (int g = 0; g < Groups - 1; ++g)
+      add(stats[g][mine][0], stats[g][mine][1], sums[g][mine][threadIdx.x & 31]);
+  }
+  if (column >= columns) return;
   const int t = column / a.group;
   store_four(a, q.first + t, head * a.group + column - t * a.group, d, x,
              best > -__builtin_inff(), 1.0f / all);
 }
 
 // Blocks of columns, at most, and workgroups: one a block and kv head, or shares where those would not
-// give each CU two and a table holds tokens for more than one.
+// give each CU one and a table holds tokens for more than one.
 struct Shape {
   int64_t units, blocks, bytes;
 };
@@ -559,8 +570,8 @@ Shape prefill_shape(const ld_paged_cache& c, int64_t q_heads) {
   const int64_t group = q_heads / c.num_kv_heads;
   s.units = c.num_tokens * group / kColumns + c.num_requests;
   s.blocks = s.units * c.num_kv_heads;
-  if (s.blocks < kShares &&
-      static_cast<int64_t>(c.table_width) * c.page_size > kTile * kLeastShare) {
+  if (s.blocks < kCus &&
+      static_cast<int64_t>(c.table_width) * c.page_size > kTile * kLeastWalk) {
     s.blocks += kShares;
     s.bytes = (plan_floats(c.num_requests) + s.blocks * kColumns * (kDim + 2)) * 4;
   }
@@ -602,9 +613,10 @@ extern "C" int ld_attention_prefill(const ld_paged_cache* cache, const ld_attent
   }
   hipLaunchKernelGGL(attention_prefill_kernel<true>, grid, dim3(kThreads), 0, on, p);
   if (const int rc = check_launch("ld_attention_prefill")) return rc;
-  // (fewer than 512 units and heads)
+  // (fewer than 256 units and heads)
   const int64_t joins = s.units * p.cache.kv_heads * (kColumns / kGatherColumns);
-  hipLaunchKernelGGL(attention_gather_kernel, dim3(static_cast<uint32_t>(joins)),
-                     dim3(kGatherThreads), 0, on, p);
+  const int groups = s.units * p.cache.kv_heads <= kFewUnits ? 4 : 1;
+  hipLaunchKernelGGL(groups == 4 ? attention_gather_kernel<4> : attention_gather_kernel<1>,
+                     dim3(static_cast<uint32_t>(joins)), dim3(groups * 256), 0, on, p);
   return check_launch("ld_attention_prefill");
 }
