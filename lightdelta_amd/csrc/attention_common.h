@@ -143,15 +143,36 @@ __device__ __forceinline__ Request request_from(const Request& x, int k) {
   return q;
 }
 
-// The last request that begins at or before `row` (0 if none does).
-__device__ __forceinline__ int request_at(const Cache& c, int64_t row) {
-  int low = 0, high = c.requests - 1;
-  while (low < high) {
-    const int mid = low + (high - low + 1) / 2;
-    if (c.cu[mid] <= row) low = mid;
-    else high = mid - 1;
+// Where each request has a run of numbers, which begins at begins(its first row, its own number) and
+// never before an earlier request's: the request whose run has `number`, what it has in the call and
+// how far into its run that is; false where no run has begun.  The last run that begins at or before
+// it, by a 64-way search with one wave-wide load a level (one level up to 64 requests, two up to
+// 4,096).  Called by every lane of a wave; the results are uniform.
+template <typename F>
+__device__ __forceinline__ bool find_run(const Cache& c, int number, int& r, Request& q, int& within,
+                                         F begins) {
+  const int lane = threadIdx.x & 63;
+  int low = 0, count = c.requests;
+  for (;;) {
+    const int step = (count + 63) >> 6;
+    const bool in = lane < (count + step - 1) / step;
+    const int index = in ? low + lane * step : low;
+    Request mine;
+    if (step == 1) mine = request_of(c, index);   // the last level: all of each candidate at once
+    else mine.first = min(max(static_cast<int64_t>(c.cu[index]), int64_t{0}), c.num_tokens);
+    const int at = begins(static_cast<int>(mine.first), index);
+    const uint64_t before = __ballot(in && at <= number);
+    if (before == 0) return false;
+    const int k = 63 - __clzll(static_cast<long long>(before));
+    low += k * step;
+    if (step == 1) {
+      r = low;
+      within = number - __builtin_amdgcn_readlane(at, k);
+      q = request_from(mine, k);
+      return true;
+    }
+    count = min(step, count - k * step);
   }
-  return low;
 }
 
 __device__ __forceinline__ bool live_page(const Cache& c, int page) {

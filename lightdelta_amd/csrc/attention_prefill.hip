@@ -119,35 +119,13 @@ __device__ __forceinline__ bool find_share(const PrefillAttention& p, uint32_t s
 }
 
 // Unit -> request, what it has in the call, and block of its columns; false where there is none.
-// Requests have a run of units each, one more than their columns can fill at the most, so that where
-// it begins follows from cu alone: the last that begins at or before the unit, by a 64-way search.
-// (The host has seen to it that columns are below 2^31.)
+// Requests have a run of units each, one more than their columns can fill at the most.  (The host has
+// seen to it that columns are below 2^31.)
 __device__ __forceinline__ bool find_unit(const PrefillAttention& p, int unit, int& r, Request& q,
                                           int& block) {
-  const Cache& c = p.cache;
-  const int lane = threadIdx.x & 63;
-  int low = 0, count = c.requests;
-  for (;;) {
-    const int step = (count + 63) >> 6;
-    const bool in = lane < (count + step - 1) / step;
-    const int index = in ? low + lane * step : low;
-    Request mine;
-    if (step == 1) mine = request_of(c, index);   // the last level: all of each candidate at once
-    else mine.first = max(static_cast<int64_t>(c.cu[index]), int64_t{0});
-    const int row = static_cast<int>(min(mine.first, c.num_tokens));
-    const int begins = static_cast<int>(static_cast<uint32_t>(row) * p.a.group / kColumns) + index;
-    const uint64_t before = __ballot(in && begins <= unit);
-    if (before == 0) return false;
-    const int k = 63 - __clzll(static_cast<long long>(before));
-    low += k * step;
-    if (step == 1) {
-      r = low;
-      block = unit - __builtin_amdgcn_readlane(begins, k);
-      q = request_from(mine, k);
-      return true;
-    }
-    count = min(step, count - k * step);
-  }
+  return find_run(p.cache, unit, r, q, block, [&](int row, int request) {
+    return static_cast<int>(static_cast<uint32_t>(row) * p.a.group / kColumns) + request;
+  });
 }
 
 __device__ __host__ inline int64_t plan_floats(int64_t requests) { return (2 * requests + 3) & ~int64_t{3}; }
