@@ -77,7 +77,7 @@ INDEX = {"k": _k_index, "v": _v_index}
 
 
 def _codes(cache):
-    return cache.cpu().view(torch.uint8).reshape(*cache.shape[:2], -1)
+    return cache.cpu().view(torch.uint8).contiguous().flatten(2)
 
 
 def _scales(scale):
