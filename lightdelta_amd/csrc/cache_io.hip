@@ -9,6 +9,8 @@
 //
 // 32 x 1024 tokens of 8 heads: 51 us, 3.9 TB/s (66 with two-byte loads of
 // values and two passes over the rows); 16,755 tokens read back 29 us, 3.5 TB/s (83 with a token a wave).
+#include <algorithm>
+
 #include "attention_common.h"
 
 namespace ld {
@@ -57,14 +59,14 @@ struct Part {
 };
 
 // Requests have a run of units each, as many as pages that their rows can touch: rows / page + 2 (rows
-// begin anywhere in a page).  False where the unit has no page to do with; q and within are set
+// begin anywhere in a page), or as many as rows where that is less.  False where the unit has no page to do with; q and within are set
 // wherever there is a request (within < 0: not).
 __device__ __forceinline__ bool find_part(const Cache& c, int unit, Part& part, Request& q,
                                           int& within) {
   int r;
   within = -1;
   if (!find_run(c, unit, r, q, within, [&](int row, int request) {
-        return (row >> c.page_log2) + 2 * request;
+        return min(row, (row >> c.page_log2) + 2 * request);
       }))
     return false;
   const int64_t begin = max(q.first + q.shift, int64_t{0});
@@ -95,16 +97,26 @@ __device__ __forceinline__ uint32_t finite(uint32_t pair) {   // zero in the pla
          ((pair & 0x7f800000u) == 0x7f800000u ? 0u : pair & 0xffff0000u);
 }
 
+template <int Ctrl>
+__device__ __forceinline__ uint32_t max_with(uint32_t x) {
+  return max(x, static_cast<uint32_t>(
+                    __builtin_amdgcn_update_dpp(0, static_cast<int>(x), Ctrl, 0xF, 0xF, false)));
+}
+
+// The largest of both waves' (`shared`: not in use).
 __device__ __forceinline__ uint32_t over_workgroup(u16x2 x, uint32_t (&shared)[2]) {
   uint32_t most = max(static_cast<uint32_t>(x[0]), static_cast<uint32_t>(x[1]));
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1)
-    most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
+  most = max_with<kDppQuadXor1>(most);
+  most = max_with<kDppQuadXor2>(most);
+  most = max_with<kDppRowHalfMirror>(most);
+  most = max_with<kDppRowMirror>(most);
+  const auto a = __builtin_amdgcn_permlane16_swap(most, most, false, false);
+  most = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+  most = max(b[0], b[1]);
   if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = most;
   __syncthreads();
-  most = max(shared[0], shared[1]);
-  __syncthreads();
-  return most;
+  return max(shared[0], shared[1]);
 }
 
 // Sixteen new elements of a token.
@@ -149,11 +161,11 @@ __global__ __launch_bounds__(kIoThreads) void cache_write_kernel(const RowsParam
   int within;
   if (!find_part(c, blockIdx.x / kinds, part, q, within) || !live_page(c, part.page)) return;
   const int from = part.from, to = part.to;
-  __shared__ uint32_t shared[2];
+  __shared__ uint32_t shared[2][2];
   u16x2 most = {0, 0};
 
   // new rows into registers: zeros for tokens that are not new; and what values share their pieces with
-  uint32_t x[kValueBlocks * 32 > kKeyPieces * 8 ? kValueBlocks * 32 : kKeyPieces * 8];
+  uint32_t x[kValueBlocks * 32 > kKeyPieces * 8 ? kValueBlocks * 32 : kKeyPieces * 8] = {};
   u32x4 codes[kValueBlocks][4] = {};
   u32x4* const tile = reinterpret_cast<u32x4*>(const_cast<uint8_t*>(
       is_values ? v_tile(c, part.page, head) : k_tile(c, part.page, head)));
@@ -167,11 +179,9 @@ __global__ __launch_bounds__(kIoThreads) void cache_write_kernel(const RowsParam
     for (int i = 0; i < kKeyPieces; ++i) {
       const int token = (threadIdx.x >> 3) + i * (kIoThreads / 8);
       uint32_t (&mine)[8] = reinterpret_cast<uint32_t(&)[8]>(x[8 * i]);
+      if (i * 16 >= to || i * 16 + 16 <= from) continue;   // (all threads)
       if (token >= from && token < to)
         __builtin_memcpy(mine, rows + token * row_stride + (threadIdx.x & 7) * 16, 32);
-      else
-#pragma unroll
-        for (int w = 0; w < 8; ++w) mine[w] = 0;
 #pragma unroll
       for (int w = 0; w < 8; ++w) most = larger(most, mine[w]);
     }
@@ -194,7 +204,7 @@ __global__ __launch_bounds__(kIoThreads) void cache_write_kernel(const RowsParam
         for (int d = 0; d < 4; ++d) codes[i][d] = tile[(block >> 5) * kDim + (block & 31) * 4 + d];
     }
   }
-  uint32_t largest = over_workgroup(most, shared);
+  uint32_t largest = over_workgroup(most, shared[0]);
   const bool strange = largest >= 0x7f80u;   // what is not finite does not count
   if (strange) {
     most = u16x2{0, 0};
@@ -202,7 +212,7 @@ __global__ __launch_bounds__(kIoThreads) void cache_write_kernel(const RowsParam
 #pragma unroll
     for (int w = 0; w < kWords; ++w)
       if (is_values ? w < kValueBlocks * 32 : w < kKeyPieces * 8) most = larger(most, finite(x[w]));
-    largest = over_workgroup(most, shared);
+    largest = over_workgroup(most, shared[1]);
   }
   int e = scale_exponent(largest);
   if (from > 0) e = max(e, old);
@@ -216,6 +226,7 @@ __global__ __launch_bounds__(kIoThreads) void cache_write_kernel(const RowsParam
 #pragma unroll
     for (int i = 0; i < kKeyPieces; ++i) {
       const int token = (threadIdx.x >> 3) + i * (kIoThreads / 8);
+      if (i * 16 >= to || (i * 16 + 16 <= from && !grew)) continue;   // (all threads)
       u32x4* const at = tile + ((threadIdx.x & 7) << PageLog2) + token;
       const uint32_t (&mine)[8] = reinterpret_cast<const uint32_t(&)[8]>(x[8 * i]);
       if (token >= from && token < to) {
@@ -335,7 +346,10 @@ int rows_params(const ld_paged_cache* cache, const ld_cache_rows* rows, RowsPara
   p.v = static_cast<uint16_t*>(rows->v);
   p.k_row = rows->k_row_stride;
   p.v_row = rows->v_row_stride;
-  blocks = ((p.cache.num_tokens >> p.cache.page_log2) + 2ll * p.cache.requests) * 2 * p.cache.kv_heads;
+  const int64_t units = std::min((p.cache.num_tokens >> p.cache.page_log2) +
+                                     2 * static_cast<int64_t>(p.cache.requests),
+                                 p.cache.num_tokens);
+  blocks = units * 2 * p.cache.kv_heads;
   if (blocks > 0x7fffffff) return fail(LD_ERR_INVALID_ARGUMENT, "too many pages and heads");
   return LD_OK;
 }
