@@ -22,7 +22,7 @@ namespace {
 
 constexpr int kTile = 64;        // tokens
 constexpr int kColumns = 128;    // of a workgroup
-constexpr int kPieces16 = 1024;  // 16-byte pieces of a tile's keys, or values, as operands
+constexpr int kPieces = kTile * kDim * 2 / 16;   // 16 bytes each, of a tile's keys or values as operands
 
 struct PrefillAttention {
   Cache cache;
@@ -157,8 +157,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
   const Attention& a = p.a;
   // the tile's keys: [16 elements of a token][half of them][token in the operand's order], and its
   // values [16 tokens][half of them][element], in pieces of eight
-  __shared__ __attribute__((aligned(16))) u32x4 lds_keys[2][kPieces16];
-  __shared__ __attribute__((aligned(16))) u32x4 lds_values[2][kPieces16];
+  __shared__ __attribute__((aligned(16))) u32x4 lds_keys[2][kPieces];
+  __shared__ __attribute__((aligned(16))) u32x4 lds_values[2][kPieces];
   __shared__ int lds_strange;
 
   const int lane = threadIdx.x & 63;
@@ -252,8 +252,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
   };
   auto stage_values = [&](int tile, uint64_t live, int to) {
     // values behind the last token, or without a page, are zeros; so are those that are not finite,
-    // and marked below, in tiles that some column does not see whole
-    if (tile * kTile + kTile > first_limit || live != ~uint64_t{0}) {
+    // and marked below, in tiles that some column does not see to its end
+    const bool partial = tile * kTile + kTile > first_limit;
+    if (partial || live != ~uint64_t{0}) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int group = (wave >> 1) + 2 * i;
@@ -262,7 +263,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const uint32_t x = values[i][w] & first_bytes(kept - 4 * w);
-          const uint32_t at_nan = nan_bytes(x);
+          const uint32_t at_nan = partial ? nan_bytes(x) : 0u;
           any |= at_nan;
           values[i][w] = x & ~((at_nan >> 7) * 0xffu);
         }

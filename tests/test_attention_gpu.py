@@ -238,6 +238,26 @@ def test_values_that_are_not_finite(gpu, what, width):
     assert case["out"].isnan().any() and not case["out"].isnan().all()
 
 
+@pytest.mark.parametrize("width", [None, 2])
+def test_not_finite_beside_a_page_that_there_is_not(gpu, width):
+    """A NaN in a value that every row sees, in a tile with a page of no place."""
+    announce(test="not_finite_beside", width=width)
+    for first in (0, 1):
+        case = case_of([200, 150], [2, 2], 16, (4, 2), seed=14, device=gpu)
+        case["pages"][0, first] = 0
+        codes = case["v_cache"].view(torch.uint8).flatten(2)
+        codes[case["pages"][0, 2], 1, oracle.INDEX["v"](16, 3)[50].to(gpu)] = 0x7F
+        check_attention(case, width)
+        assert int(case["out"].isnan().sum()) == 2 * 2  # the rows, and the kv head's two q heads
+
+
+def test_decode_of_rows_before_the_first_token(gpu):
+    """More rows than tokens: those without a position see nothing."""
+    announce(test="decode_before")
+    check_attention(case_of([2, 0, 1, 70], [4, 2, 3, 4], 16, (6, 2), seed=15, device=gpu, gated=True),
+                    4)
+
+
 def test_one_token_takes_all(gpu):
     """Scores of thousands: weights of one and of zero, the largest first, last and in between."""
     announce(test="attention_peaks")
