@@ -333,11 +333,16 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
   int page = page_of(begin), page_next = page_of(begin + 1), page_then = page_of(begin + 2);
   f32x16 score[2];
   if (begin < end) {
+    load_keys(begin + 1, page_next);
+    const u32x4 second[2] = {keys[0], keys[1]};
+    const float second_scale = k_scale;
     load_keys(begin, page);
     load_values(begin, page);
     stage_keys(0);
     stage_values(begin, __ballot(page > 0), 0);
-    load_keys(begin + 1, page_next);
+    keys[0] = second[0];
+    keys[1] = second[1];
+    k_scale = second_scale;
     stage_keys(1);
     lds_barrier();
     if (works) {
