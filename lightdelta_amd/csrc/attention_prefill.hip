@@ -150,6 +150,21 @@ __device__ __forceinline__ void store_four(const Attention& a, int64_t row, int 
   __builtin_memcpy(a.out + (row * a.q_heads + head) * kDim + d, bits, 8);
 }
 
+// Eight elements of an output that is divided already, gated and rounded.
+__device__ __forceinline__ void store_out(const Attention& a, int64_t row, int head, int d,
+                                          float (&o)[8], bool some) {
+  if (a.gate != nullptr) {
+    uint16_t g[8];
+    __builtin_memcpy(g, a.gate + row * a.gate_row + head * kDim + d, 16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] *= sigmoid(bf16_to_f32(g[i]));
+  }
+  u32x4 bits;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bits[i] = some ? bf16_pair(f32x2{o[2 * i], o[2 * i + 1]}) : 0u;
+  __builtin_memcpy(a.out + (row * a.q_heads + head) * kDim + d, &bits, 16);
+}
+
 // Split: workgroups are shares, else units.
 template <bool Split>
 __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const PrefillAttention p) {
@@ -157,8 +172,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
   const Attention& a = p.a;
   // the tile's keys: [16 elements of a token][half of them][token in the operand's order], and its
   // values [16 tokens][half of them][element], in pieces of eight
-  __shared__ __attribute__((aligned(16))) u32x4 lds_keys[2][kPieces];
-  __shared__ __attribute__((aligned(16))) u32x4 lds_values[2][kPieces];
+  __shared__ __attribute__((aligned(16))) u32x4 lds[4][kPieces];
+  u32x4 (&lds_keys)[2][kPieces] = reinterpret_cast<u32x4(&)[2][kPieces]>(lds[0]);
+  u32x4 (&lds_values)[2][kPieces] = reinterpret_cast<u32x4(&)[2][kPieces]>(lds[2]);
   __shared__ int lds_strange;
 
   const int lane = threadIdx.x & 63;
@@ -454,17 +470,34 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
         if (count[b][i] > 0.0f) o[b][i] = __builtin_nanf("");
   }
   sum = add_partner<32>(sum);
-  if (!real) return;
   if (splits == 1) {
+    // by way of LDS, a wave's 32 columns a quarter of it, so that sixteen lanes store a row's 256 bytes
+    // (a lane's own are sixteen pieces of 8 in as many rows); piece j of column n at j ^ n
+    __syncthreads();   // (the last values read)
+    u32x4* const mine = lds[wave];
     const bool some = top > -__builtin_inff();   // the row sees a token
     const float inverse = 1.0f / sum;
 #pragma unroll
     for (int b = 0; b < 4; ++b)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        store_four(a, q.first + t_row, head * a.group + g_row, 32 * b + 8 * e + 4 * h, quad(o[b], e),
-                   some, inverse);
-  } else {
+      for (int e = 0; e < 4; ++e) {
+        f32x4 x = quad(o[b], e);
+        x *= inverse;
+        mine[32 * m + ((8 * b + 2 * e + h) ^ m)] = __builtin_bit_cast(u32x4, x);
+      }
+    lds_order();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int n = 4 * i + (lane >> 4), j = lane & 15;
+      const int t = __shfl(static_cast<int>(t_row), n), g = __shfl(g_row, n);
+      const bool any = __shfl(some ? 1 : 0, n) != 0;
+      if (block * kColumns + 32 * wave + n >= columns) continue;
+      const f32x4 lo = __builtin_bit_cast(f32x4, mine[32 * n + ((2 * j) ^ n)]);
+      const f32x4 hi = __builtin_bit_cast(f32x4, mine[32 * n + ((2 * j + 1) ^ n)]);
+      float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      store_out(a, q.first + t, head * a.group + g, 8 * j, x, any);
+    }
+  } else if (real) {
     float* const to = split_at(p, blockIdx.x);
     const int at = 32 * wave + m;
 #pragma unroll
