@@ -35,8 +35,8 @@ extern "C" {
  * Request r has the rows cu[r] .. cu[r+1]-1 of the call's activations, which are the last of its
  * lengths[r] tokens: row i is at position lengths[r] - cu[r+1] + i.  The token at position t lies
  * in page pages[r * pages_row_stride + t / page_size].  Positions from table_width * page_size on
- * have no page.  A page outside 1 .. num_pages - 1 is padding: never read, never written, and its
- * tokens are attended to by none.  lengths[r] <= 0 is a request without tokens.
+ * have no page.  A page outside 1 .. num_pages - 1 is padding: never written, and its tokens are
+ * attended to by none, whatever page 0 holds.  lengths[r] <= 0 is a request without tokens.
  */
 typedef struct ld_paged_cache {
   void* k;

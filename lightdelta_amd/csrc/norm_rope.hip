@@ -11,7 +11,8 @@
 //
 // 32,768 tokens of 16 + 16 heads: 101 us, 5.3 TB/s (260 with a round at a time, an angle per element and
 // pairs by shuffles); one token of them 2.5 us.  Few tokens are split over waves by rounds, so that a
-// small launch's latency is one batch's.
+// small launch's latency is one batch's.  With positions of several axes an angle's lane picks its own
+// position; 16,384 tokens of 32 + 8 heads, half of each rotated: 73 us, 4.6 TB/s.
 #include <algorithm>
 #include <type_traits>
 

@@ -23,4 +23,8 @@ Modules and what pins each one (details in each module's header):
             the error that a correct fp32 implementation may have.  Pinned by the sum over
             token pairs, by decode steps against a prefill, and by the rotation's invariants
             (tests/test_linear_cpu.py).
+  attention the paged 8-bit cache, softmax attention over it and norm_rope_axes from their
+            definitions in 64 bits, with the error that a correct fp32 implementation may
+            have.  Codes and rounding pinned by torch's e4m3 type, attention by a dense softmax
+            over the cache read back, writing by closed cases (tests/test_attention_cpu.py).
 """
