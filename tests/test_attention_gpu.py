@@ -193,6 +193,16 @@ def test_decode_long_and_many(gpu, lengths):
     check_attention(case_of(lengths, new, 16, (4, 2), seed=9, device=gpu), 3)
 
 
+@pytest.mark.parametrize("requests", [90, 200, 260])
+@pytest.mark.parametrize("width", [1, 3])
+def test_decode_of_many_short(gpu, requests, width):
+    """About one, two or three tiles of 64 tokens a workgroup, of one head and the next."""
+    announce(test="decode_short", requests=requests, width=width)
+    lengths = [7 * i % 200 for i in range(requests)]
+    new = [min(n, 1 + i % width) if n else 1 for i, n in enumerate(lengths)]
+    check_attention(case_of(lengths, new, 64, (6, 3), seed=11, device=gpu), width)
+
+
 def test_decode_of_more_rows_than_its_width(gpu):
     announce(test="decode_wide")
     check_attention(case_of([40, 50, 9], [2, 3, 9], 32, (4, 2), seed=10, device=gpu), 2)
