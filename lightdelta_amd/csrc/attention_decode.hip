@@ -19,7 +19,7 @@
 //
 // 33 requests of up to 8,000 tokens, 8 kv heads: 46 us and 5 for the join, 221 MB at 4.8 TB/s; of it about
 // 5 until a workgroup's first tile is there (lengths, table and codes wait for one another).  One request
-// of 501 tokens: 7.6 and 2.9 us.
+// of 501 tokens: 5.9 and 3.3 us.  64 requests of up to four rows and 4,000 tokens: 19 and 5.
 #include <algorithm>
 
 #include "attention_common.h"
@@ -102,13 +102,12 @@ struct Walk {
   }
 };
 
-// Tiles of a workgroup's run: a whole number for each of its waves; where there is less than one for
-// each, no more than it takes, since the heads of a run are taken one after another (32 requests of up
-// to 100 tokens 8.6 us, with four tiles a run 16.5; one of 3,000 tokens 11.8 and 11.6).
+// Tiles of a workgroup's run.  (With a whole number for each of its waves, of which there would be
+// fewer runs, 32 requests of up to 100 tokens take 16.5 us and not 8.5, their heads being taken one
+// after another, and 64 of up to 2,000 tokens and 8 kv heads 36 and not 34.)
 __device__ __forceinline__ uint32_t run_length(const DecodeAttention& p, uint32_t total) {
   const uint32_t workers = static_cast<uint32_t>(p.workers);
-  const uint32_t n = max((total * p.cache.kv_heads + workers - 1) / workers, 1u);
-  return n < kWaves ? n : (n + kWaves - 1) / kWaves * kWaves;
+  return max((total * p.cache.kv_heads + workers - 1) / workers, 1u);
 }
 
 __device__ __forceinline__ u32x4 eight_bf16(const float (&x)[8]) {
@@ -176,8 +175,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Dec
     const int rows = static_cast<int>(q.last - q.first);
     const int32_t* const table = c.pages + r * c.pages_row;
 
-    // The tiles' pages first: the keys wait for them.  A tile's pages: that of tokens 16 (m / 4) .. for the keys, 16 h .. for the values (0, whose
-    // bytes are read and not used, where there is none).
+    // The tiles' pages first: the keys wait for them.  A tile's pages: that of tokens 16 (m / 4) .. for
+    // the keys, 16 h .. for the values (0, whose bytes are read and not used, where there is none).
     auto page_of = [&](uint32_t tile, int group) {
       const int token = static_cast<int>(tile) * kTile + 16 * group;
       const int page = tile < to && token < q.tokens ? table[token >> c.page_log2] : 0;
@@ -396,16 +395,23 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Dec
   }
 }
 
-// Sixteen columns of a request and kv head a workgroup: joins the sums of the runs that its tiles
-// were cut into; zeros for a request without tokens or with more rows than the width.  Four groups
-// of threads take every fourth piece, a thread eight elements of a column.
-constexpr int kJoinThreads = 1024;
-__global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const DecodeAttention p,
-                                                                      Layout layout, int tiles16) {
+// Some columns of a request and kv head a workgroup: joins the sums of the runs that its tiles were
+// cut into; zeros for a request without tokens or with more rows than the width.  Groups of threads
+// take every Groups-th piece, a thread eight elements of a column.
+// Four columns and eight groups start sooner than sixteen and four (one request of 501 tokens 8.2 and
+// 8.5 us, 32 up to 1,000 11.1 and 12.5, 64 of up to four rows and 4,000 tokens 23.8 and 23.6).  A head
+// that may be in more than 48 pieces has two columns and 32 groups (one request of 100,000 tokens, 256
+// pieces, 18.8 and 27.0; four up to 20,000, 64 pieces, 16.9 and 19.1; of one tile 9.1 and 8.2).
+constexpr int kJoinColumns = 4, kJoinGroups = 8;
+constexpr int kFewColumns = 2, kFewGroups = 32;
+constexpr int kManyPieces = 48;
+template <int Columns, int Groups>
+__global__ __launch_bounds__(Columns * 16 * Groups) void attention_join_kernel(const DecodeAttention p,
+                                                                               Layout layout, int parts) {
   const Cache& c = p.cache;
   const Attention& a = p.a;
-  const int tile16 = blockIdx.x % tiles16;
-  const int rest = blockIdx.x / tiles16;
+  const int part = blockIdx.x % parts;
+  const int rest = blockIdx.x / parts;
   const int head = rest % c.kv_heads;
   const int r = rest / c.kv_heads;
   const uint32_t* const plan = reinterpret_cast<const uint32_t*>(a.workspace);
@@ -413,9 +419,9 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Deco
   const uint32_t tiles = plan[2 + r] - first;
   const Request q = request_of(c, r);
   const int64_t rows = q.last - q.first;
-  const int group = threadIdx.x >> 8;
-  const int mine = threadIdx.x >> 4 & 15, d = 8 * (threadIdx.x & 15);
-  const int column = 16 * tile16 + mine;
+  const int group = threadIdx.x / (16 * Columns);
+  const int mine = (threadIdx.x >> 4) % Columns, d = 8 * (threadIdx.x & 15);
+  const int column = Columns * part + mine;
   const int t = column / a.group;
   const int q_head = head * a.group + column - t * a.group;
   if (tiles == 0) {
@@ -432,7 +438,7 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Deco
   float best = -__builtin_inff(), all = 0.0f, x[8] = {};
   if (real) {
 #pragma unroll 4
-    for (uint32_t w = w0 + group; w <= w1; w += 4) {
+    for (uint32_t w = w0 + group; w <= w1; w += Groups) {
       const float* const from = a.workspace + layout.piece(w, w == w0 && begin != w * run);
       const f32x2 stat = *reinterpret_cast<const f32x2*>(from + layout.columns * kDim + 2 * column);
       const f32x4 lo = *reinterpret_cast<const f32x4*>(from + static_cast<int64_t>(column) * kDim + d);
@@ -451,20 +457,20 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Deco
       }
     }
   }
-  __shared__ __attribute__((aligned(16))) float sums[4][16][kDim + 4];
-  __shared__ f32x2 stats[4][16];
+  __shared__ __attribute__((aligned(16))) float sums[Groups][Columns][kDim + 4];
+  __shared__ f32x2 stats[Groups][Columns];
   *reinterpret_cast<f32x4*>(&sums[group][mine][d]) = f32x4{x[0], x[1], x[2], x[3]};
   *reinterpret_cast<f32x4*>(&sums[group][mine][d + 4]) = f32x4{x[4], x[5], x[6], x[7]};
   if (d == 0) stats[group][mine] = f32x2{best, all};
   __syncthreads();
   if (group > 0 || !real) return;
 #pragma unroll
-  for (int g = 0; g < 4; ++g) best = fmaxf(best, stats[g][mine][0]);
+  for (int g = 0; g < Groups; ++g) best = fmaxf(best, stats[g][mine][0]);
   all = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = 0.0f;
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
+  for (int g = 0; g < Groups; ++g) {
     const f32x2 stat = stats[g][mine];
     if (stat[0] > -__builtin_inff()) {
       const float add = stat[0] == best ? 1.0f : exp2_fast((stat[0] - best) * a.log2_scale);
@@ -476,7 +482,8 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Deco
   store_out(a, q.first + t, q_head, d, x, best, all);
 }
 
-// Workgroups of the first launch: two a CU, fewer where tables have not a tile for each; waves a tile; and how often all of it for 64 columns each.
+// Workgroups of the first launch: two a CU, fewer where tables have not a tile for each; waves a tile;
+// and how often all of it for 64 columns each.
 struct Shape {
   int64_t workers;
   int split, blocks;
@@ -528,8 +535,10 @@ extern "C" int ld_attention_decode(const ld_paged_cache* cache, const ld_attenti
   if (p.a.workspace == nullptr || !aligned16(p.a.workspace) || args->workspace_bytes < s.bytes)
     return fail(LD_ERR_INVALID_ARGUMENT, "workspace missing or too small");
   p.columns = p.a.width * p.a.group;
-  const int tiles16 = (p.columns + 15) / 16;
-  const int64_t joins = static_cast<int64_t>(p.cache.requests) * p.cache.kv_heads * tiles16;
+  const bool few = s.workers > static_cast<int64_t>(kManyPieces) * p.cache.requests * p.cache.kv_heads;
+  const int each = few ? kFewColumns : kJoinColumns;
+  const int parts = (p.columns + each - 1) / each;
+  const int64_t joins = static_cast<int64_t>(p.cache.requests) * p.cache.kv_heads * parts;
   if (joins > 0x7fffffff) return fail(LD_ERR_INVALID_ARGUMENT, "too many requests and heads");
   if (s.most > 0x3fffffff)
     return fail(LD_ERR_INVALID_ARGUMENT, "too many tokens of all tables and heads");
@@ -541,7 +550,10 @@ extern "C" int ld_attention_decode(const ld_paged_cache* cache, const ld_attenti
   hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(s.workers), s.blocks),
                      dim3(kThreads), 0, on, p);
   if (const int rc = check_launch("ld_attention_decode")) return rc;
-  hipLaunchKernelGGL(attention_join_kernel, dim3(static_cast<uint32_t>(joins)), dim3(kJoinThreads),
-                     0, on, p, layout_of(p.cache.requests, 16 * s.split * s.blocks), tiles16);
+  hipLaunchKernelGGL((few ? attention_join_kernel<kFewColumns, kFewGroups>
+                          : attention_join_kernel<kJoinColumns, kJoinGroups>),
+                     dim3(static_cast<uint32_t>(joins)),
+                     dim3(few ? kFewColumns * 16 * kFewGroups : kJoinColumns * 16 * kJoinGroups), 0, on, p,
+                     layout_of(p.cache.requests, 16 * s.split * s.blocks), parts);
   return check_launch("ld_attention_decode");
 }
