@@ -240,6 +240,15 @@ __device__ __forceinline__ float max_over_quarters(float x) {
 
 constexpr float kLowest = -3.4028234663852886e38f;
 
+// Weights are exp2(score * log2_scale - top * log2_scale) by one fused operation a score, whose second
+// product is rounded: off by up to 2^-24 of it in the exponent, 2^-14 where it is up to this.  Past it
+// (2^31, say, where that is a factor of 2^128) a wave subtracts the maximum itself ahead, exactly
+// where the weight counts.
+constexpr float kFar = 1024.0f;
+__device__ __forceinline__ bool far_scores(float top, float log2_scale) {   // (no score: top = 0)
+  return __any(fabsf(top) * log2_scale > kFar);
+}
+
 // 2^e for -126 <= e <= 127.
 __device__ __forceinline__ float power_of_two(int e) {
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);

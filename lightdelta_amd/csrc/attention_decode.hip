@@ -278,7 +278,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Dec
         for (int b = 0; b < 8; ++b) o[b] *= keep;
         top = now;
       }
-      const float less = now == -__builtin_inff() ? 0.0f : -now * a.log2_scale;
+      const float some = now == -__builtin_inff() ? 0.0f : now;
+      float less = -some * a.log2_scale;
+      if (far_scores(some, a.log2_scale)) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) score[t] -= some;
+        less = 0.0f;
+      }
       u32x4 bits[2];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {

@@ -312,8 +312,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
         x[t] = mfma32(__builtin_bit_cast(bf16x8, k), query[s], x[t]);
       }
   };
-  // Scores of -inf, for weights of zero, where the column does not see a token; and what a new
-  // maximum changes.
+  // Scores of -inf, for weights of zero, where the column does not see a token; what a new maximum
+  // changes; and what scores are less by in the exponent.
+  float less = 0.0f;
   auto settle = [&](int tile, uint64_t live, f32x16 (&x)[2]) {
     float most = kLowest;   // (of a score of -inf that is seen: a weight of zero, not none)
     if (!(tile * kTile + kTile <= least && live == ~uint64_t{0})) {
@@ -343,6 +344,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
 #pragma unroll
       for (int b = 0; b < 4; ++b) o[b] *= keep;
       top = now;
+    }
+    const float some = top == -__builtin_inff() ? 0.0f : top;
+    less = -some * a.log2_scale;
+    if (far_scores(some, a.log2_scale)) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) x[t] -= some;
+      less = 0.0f;
     }
   };
 
@@ -380,7 +388,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
     page_then = page_of(tile + 3);
     const uint64_t live = __ballot(page > 0);
     if (works) {
-      const float less = top == -__builtin_inff() ? 0.0f : -top * a.log2_scale;
       __builtin_amdgcn_s_setprio(1);   // (ahead of a wave that stages: 8,192 tokens 287 us, without 317)
       scores(now_at ^ 1, next);
       bf16x8 weight[2][2];
