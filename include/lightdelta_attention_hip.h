@@ -103,7 +103,7 @@ typedef struct ld_attention_args {
   void* out;
   int32_t num_q_heads;
   int32_t width; /* decode only: 1 .. LD_MAX_TOKENS */
-  float scale;   /* positive */
+  float scale;   /* positive, log2(e) * scale finite */
   void* workspace; /* 16-byte aligned device memory, ..._workspace_bytes of it */
   int64_t workspace_bytes;
 } ld_attention_args;

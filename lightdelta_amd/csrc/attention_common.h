@@ -91,8 +91,9 @@ inline int attention_params(const ld_paged_cache& c, const ld_attention_args* fr
   if (a.num_q_heads <= 0 || a.num_q_heads > 1 << 16 || a.num_q_heads % c.num_kv_heads != 0)
     return fail(LD_ERR_INVALID_ARGUMENT,
                 "num_q_heads must be a positive multiple of num_kv_heads, at most 2^16");
-  if (!(a.scale > 0.0f && a.scale <= 3.4028235e38f))
-    return fail(LD_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+  const float log2_scale = a.scale * 1.44269504088896340736f;
+  if (!(a.scale > 0.0f && log2_scale <= 3.4028235e38f))
+    return fail(LD_ERR_INVALID_ARGUMENT, "scale must be positive, log2(e) times it finite");
   p = Attention{};
   if (c.num_requests == 0 || c.num_tokens == 0) return LD_OK;
   if (!a.q || !a.out) return fail(LD_ERR_INVALID_ARGUMENT, "attention: NULL tensor pointer");
@@ -105,7 +106,7 @@ inline int attention_params(const ld_paged_cache& c, const ld_attention_args* fr
   p.q_heads = a.num_q_heads;
   p.group = a.num_q_heads / c.num_kv_heads;
   p.width = a.width;
-  p.log2_scale = a.scale * 1.44269504088896340736f;
+  p.log2_scale = log2_scale;
   return LD_OK;
 }
 

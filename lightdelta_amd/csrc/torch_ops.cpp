@@ -731,8 +731,8 @@ void attend(const at::Tensor& q, const at::Tensor& pages, const at::Tensor& cu,
   TORCH_CHECK(out.device() == q.device() && out.scalar_type() == at::kBFloat16 &&
                   out.sizes() == q.sizes() && out.is_contiguous(),
               "out must be contiguous CUDA BF16 [tokens,q_heads,128]");
-  TORCH_CHECK(scale > 0 && scale <= std::numeric_limits<float>::max(),
-              "scale must be positive and finite");
+  TORCH_CHECK(scale > 0 && scale * 1.44269504088896340736 <= std::numeric_limits<float>::max(),
+              "scale must be positive, log2(e) times it finite");
   TORCH_CHECK(q.size(0) <= INT32_MAX, "too many tokens");
   if (nothing(cache)) return;
   ld_attention_args args{};

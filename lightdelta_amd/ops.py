@@ -83,6 +83,7 @@ can run without a GPU.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 from pathlib import Path
 
@@ -811,7 +812,8 @@ def check_attention_prefill(q, pages, cu, lengths, k_cache, v_cache, k_scale, v_
     _require(out.device == q.device and out.dtype == torch.bfloat16
              and tuple(out.shape) == tuple(q.shape) and out.is_contiguous(),
              "out must be contiguous CUDA BF16 [tokens,q_heads,128]")
-    _require(0 < scale <= torch.finfo(torch.float32).max, "scale must be positive and finite")
+    _require(scale > 0 and scale * math.log2(math.e) <= torch.finfo(torch.float32).max,
+             "scale must be positive, log2(e) times it finite")
     _require(q.shape[0] <= _INT32_MAX, "too many tokens")
     return q_heads, heads
 

@@ -92,3 +92,17 @@ def test_largest_score_takes_all(gpu, power, scale, width):
         case["q"][:, 1::2, 5] *= -1
         set_keys(case, 5, lambda n: (torch.randint(-14, 15, (n,), generator=gen) * 32.0))
         check_exact_scores(case, width, scale, f"scores of 2^{power}")
+
+
+@pytest.mark.parametrize("width", [None, 4])
+def test_largest_scale(gpu, width):
+    """Scales up to 2.3e38: equal scores give the mean of the values, others the largest's."""
+    announce(test="score_scale", width=width)
+    gen = torch.Generator().manual_seed(4)
+    for case in cases(gpu, width):
+        for power in (None, -8, -60):
+            case["q"] = torch.zeros_like(case["q"])
+            if power is not None:
+                case["q"][..., 5] = 2.0**power
+            set_keys(case, 5, lambda n: torch.randint(-14, 15, (n,), generator=gen) * 32.0)
+            check_exact_scores(case, width, 2.3e38, f"scores of 2^{power}")
