@@ -76,6 +76,9 @@ typedef struct ld_cache_rows {
  * 448 as 448; what is not finite as NaN); where a scale grew, values of earlier tokens of the page
  * are rounded anew to the larger one.  Bytes of later tokens of a page are left as they were.  A
  * page is written for one request of a call only.
+ *
+ * Here and in ld_cache_read num_kv_heads * (num_tokens / page_size + 2 * num_requests), or num_kv_heads *
+ * num_tokens where that is less, is below 2^24.
  */
 int ld_cache_write(const ld_paged_cache* cache, const ld_cache_rows* rows, void* stream);
 
@@ -109,10 +112,12 @@ typedef struct ld_attention_args {
 } ld_attention_args;
 
 /* Decode and speculative verify: requests of at most `width` rows (one with more gets zeros).
- * num_requests * num_kv_heads * (tokens of a table, in 64s) is below 2^30. */
+ * num_requests * num_kv_heads * (tokens of a table, in 64s) is below 2^30, and num_requests *
+ * num_kv_heads * (columns of a kv head, num_q_heads / num_kv_heads * width, in 4s) below 2^23. */
 int ld_attention_decode(const ld_paged_cache* cache, const ld_attention_args* args, void* stream);
 
-/* Requests of any number of rows; num_tokens * num_q_heads / num_kv_heads is at most 2^31 - 256. */
+/* Requests of any number of rows; num_tokens * num_q_heads / num_kv_heads is at most 2^31 - 256, and
+ * num_tokens * num_q_heads / 128 + num_requests * num_kv_heads below 2^24. */
 int ld_attention_prefill(const ld_paged_cache* cache, const ld_attention_args* args, void* stream);
 
 /* Workspace bytes for these sizes, of which only the sizes count; 0 where none is needed.

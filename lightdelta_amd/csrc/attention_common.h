@@ -110,6 +110,9 @@ inline int attention_params(const ld_paged_cache& c, const ld_attention_args* fr
   return LD_OK;
 }
 
+// A launch has fewer than 2^32 threads in a dimension.
+inline bool launches(int64_t blocks, int threads) { return blocks <= 0xffffffffLL / threads; }
+
 namespace {
 
 // What a request has in this call: rows first .. last - 1 of the activations, of which row i is at

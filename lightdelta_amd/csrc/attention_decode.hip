@@ -545,7 +545,9 @@ extern "C" int ld_attention_decode(const ld_paged_cache* cache, const ld_attenti
   const int each = few ? kFewColumns : kJoinColumns;
   const int parts = (p.columns + each - 1) / each;
   const int64_t joins = static_cast<int64_t>(p.cache.requests) * p.cache.kv_heads * parts;
-  if (joins > 0x7fffffff) return fail(LD_ERR_INVALID_ARGUMENT, "too many requests and heads");
+  const int join_threads = few ? kFewColumns * 16 * kFewGroups : kJoinColumns * 16 * kJoinGroups;
+  if (!launches(joins, join_threads))
+    return fail(LD_ERR_INVALID_ARGUMENT, "too many requests and heads");
   if (s.most > 0x3fffffff)
     return fail(LD_ERR_INVALID_ARGUMENT, "too many tokens of all tables and heads");
   p.workers = static_cast<int32_t>(s.workers);
@@ -558,8 +560,7 @@ extern "C" int ld_attention_decode(const ld_paged_cache* cache, const ld_attenti
   if (const int rc = check_launch("ld_attention_decode")) return rc;
   hipLaunchKernelGGL((few ? attention_join_kernel<kFewColumns, kFewGroups>
                           : attention_join_kernel<kJoinColumns, kJoinGroups>),
-                     dim3(static_cast<uint32_t>(joins)),
-                     dim3(few ? kFewColumns * 16 * kFewGroups : kJoinColumns * 16 * kJoinGroups), 0, on, p,
+                     dim3(static_cast<uint32_t>(joins)), dim3(join_threads), 0, on, p,
                      layout_of(p.cache.requests, 16 * s.split * s.blocks), parts);
   return check_launch("ld_attention_decode");
 }

@@ -630,7 +630,7 @@ extern "C" int ld_attention_prefill(const ld_paged_cache* cache, const ld_attent
   if (s.bytes > 0 && (p.a.workspace == nullptr || !aligned16(p.a.workspace) ||
                       args->workspace_bytes < s.bytes))
     return fail(LD_ERR_INVALID_ARGUMENT, "workspace missing or too small");
-  if (s.blocks > 0x7fffffff || p.cache.num_tokens * p.a.group > 0x7fffff00)
+  if (!launches(s.blocks, kThreads) || p.cache.num_tokens * p.a.group > 0x7fffff00)
     return fail(LD_ERR_INVALID_ARGUMENT, "too many rows and heads");
   p.units = static_cast<int32_t>(s.units);
   p.room = static_cast<uint32_t>(s.blocks);

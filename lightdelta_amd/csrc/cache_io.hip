@@ -389,7 +389,7 @@ int rows_params(const ld_paged_cache* cache, const ld_cache_rows* rows, RowsPara
                                      2 * static_cast<int64_t>(p.cache.requests),
                                  p.cache.num_tokens);
   blocks = units * 2 * p.cache.kv_heads;
-  if (blocks > 0x7fffffff) return fail(LD_ERR_INVALID_ARGUMENT, "too many pages and heads");
+  if (!launches(blocks, kIoThreads)) return fail(LD_ERR_INVALID_ARGUMENT, "too many pages and heads");
   return LD_OK;
 }
 
