@@ -78,7 +78,8 @@ typedef struct ld_cache_rows {
  * page is written for one request of a call only.
  *
  * Here and in ld_cache_read num_kv_heads * (num_tokens / page_size + 2 * num_requests), or num_kv_heads *
- * num_tokens where that is less, is below 2^24.
+ * num_tokens where that is less, is below 2^24, and num_tokens / page_size + 2 * num_requests below
+ * 2^31.
  */
 int ld_cache_write(const ld_paged_cache* cache, const ld_cache_rows* rows, void* stream);
 

@@ -385,9 +385,10 @@ int rows_params(const ld_paged_cache* cache, const ld_cache_rows* rows, RowsPara
   p.v = static_cast<uint16_t*>(rows->v);
   p.k_row = rows->k_row_stride;
   p.v_row = rows->v_row_stride;
-  const int64_t units = std::min((p.cache.num_tokens >> p.cache.page_log2) +
-                                     2 * static_cast<int64_t>(p.cache.requests),
-                                 p.cache.num_tokens);
+  const int64_t counted = (p.cache.num_tokens >> p.cache.page_log2) +
+                          2 * static_cast<int64_t>(p.cache.requests);
+  if (counted > 0x7fffffff) return fail(LD_ERR_INVALID_ARGUMENT, "too many requests");
+  const int64_t units = std::min(counted, p.cache.num_tokens);
   blocks = units * 2 * p.cache.kv_heads;
   if (!launches(blocks, kIoThreads)) return fail(LD_ERR_INVALID_ARGUMENT, "too many pages and heads");
   return LD_OK;

@@ -38,3 +38,12 @@ def test_launches_of_too_many_threads():
     # (a join of four columns a workgroup of 512 threads: 2 kv heads of two each)
     refused("too many requests and heads", lib.ld_attention_decode,
             _lib.PagedCache(**dict(GOOD, num_tokens=2**21, num_requests=2**21)), args)
+
+
+def test_more_requests_than_their_units_are_counted_for():
+    """The cache's pages are found by a count of rows / page + 2 * requests, which is held in 32 bits."""
+    lib = _lib.load()
+    rows = _lib.CacheRows(k=16, v=16, k_row_stride=256, v_row_stride=256)
+    many = _lib.PagedCache(**dict(GOOD, num_tokens=1000, num_requests=2**30))
+    for call in (lib.ld_cache_write, lib.ld_cache_read):
+        refused("too many requests", call, many, rows)
