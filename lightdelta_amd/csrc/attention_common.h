@@ -253,6 +253,11 @@ __device__ __forceinline__ bool far_scores(float top, float log2_scale) {   // (
   return __any(fabsf(top) * log2_scale > kFar);
 }
 
+// Every weight is 2^-24 of that, the sums with them: so that a sum of products passes fp32's range
+// with 2^24 of the cache's largest values (2^16 where a maximum may be behind by 2^8), not with two,
+// and products with its smallest keep 16 bits.
+constexpr float kHeadroom = -24.0f;
+
 // 2^e for -126 <= e <= 127.
 __device__ __forceinline__ float power_of_two(int e) {
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);

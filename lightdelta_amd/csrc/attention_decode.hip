@@ -279,11 +279,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Dec
         top = now;
       }
       const float some = now == -__builtin_inff() ? 0.0f : now;
-      float less = -some * a.log2_scale;
+      float less = fmaf(-some, a.log2_scale, kHeadroom);
       if (far_scores(some, a.log2_scale)) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) score[t] -= some;
-        less = 0.0f;
+        less = kHeadroom;
       }
       u32x4 bits[2];
 #pragma unroll

@@ -346,11 +346,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
       top = now;
     }
     const float some = top == -__builtin_inff() ? 0.0f : top;
-    less = -some * a.log2_scale;
+    less = fmaf(-some, a.log2_scale, kHeadroom);
     if (far_scores(some, a.log2_scale)) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) x[t] -= some;
-      less = 0.0f;
+      less = kHeadroom;
     }
   };
 

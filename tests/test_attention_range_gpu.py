@@ -106,3 +106,24 @@ def test_largest_scale(gpu, width):
                 case["q"][..., 5] = 2.0**power
             set_keys(case, 5, lambda n: torch.randint(-14, 15, (n,), generator=gen) * 32.0)
             check_exact_scores(case, width, 2.3e38, f"scores of 2^{power}")
+
+
+@pytest.mark.parametrize("width", [None, 4])
+@pytest.mark.parametrize("exponent", [119, 100, 0, -60, -100])
+@pytest.mark.parametrize("power", [None, 0, 20])
+def test_values_of_any_size(gpu, power, exponent, width):
+    """Values up to the largest that the cache holds, whose mean is finite and whose sum is not, and
+    down to the smallest; queries of zero, scores a few units apart, and the largest last."""
+    announce(test="value_range", power=power, exponent=exponent, width=width)
+    gen = torch.Generator().manual_seed(5)
+    for case in cases(gpu, width):
+        case["v_scale"].view(torch.uint8).fill_(127 + exponent)
+        values = case["v_cache"].view(torch.uint8)
+        values[:, :, :, 40:60] = 0x7E
+        values[:, :, :, 60:80] = 0xFE
+        case["q"] = torch.zeros_like(case["q"])
+        if power is not None:
+            case["q"][..., 0], case["q"][..., 17] = 2.0**power, 1.0
+        set_keys(case, 0, torch.ones)
+        set_keys(case, 17, lambda n: torch.randint(-8, 9, (n,), generator=gen) / 2)
+        check_exact_scores(case, width, 1.0, f"values of 2^{exponent}")
