@@ -92,7 +92,8 @@ int ld_cache_read(const ld_paged_cache* cache, const ld_cache_rows* rows, void* 
  * reads kv head h / (num_q_heads / num_kv_heads):
  *   p_j = exp(scale * q . k_j) / sum_j exp(scale * q . k_j)      o = sum_j p_j v_j
  *   out = bf16(o), or with a gate bf16(o * sigmoid(gate))
- * with scores, statistics and sums in fp32 and p in bf16.  A row that sees no token gets zeros.
+ * with scores, statistics and sums in fp32 and p, ahead of its product with v, in bf16 (prefill) or as a
+ * sum of two bf16 (decode).  A row that sees no token gets zeros.
  * Rows outside every request are left as they were.  What is not finite in a key or value
  * reaches the rows that see it, nothing else.
  *   q, gate  bf16 [num_tokens, num_q_heads, 128], rows q_row_stride and gate_row_stride elements

@@ -14,8 +14,9 @@
 // Columns are the request's rows times the q heads of a kv head.  Where they are more than 16, two or
 // four waves take the same tile for 16 columns each (the second read of a tile is the L2's): a wave of
 // 32 columns does not fit in the registers of two a SIMD, and what it keeps in scratch memory waits
-// for the tiles in flight (31.7 us for a verify of 64 requests of up to 4,000 tokens, 23.4 so).
-// e4m3 times its scale is exact in bf16; weights are rounded to bf16, their sum is not.
+// for the tiles in flight (31.7 us for a verify of 64 requests of up to 4,000 tokens, 23.4 without).
+// e4m3 times its scale is exact in bf16; weights are two bf16 each (2^-17 of one is lost), in a product
+// each with the same operand of values: 33 requests 42.1 us (41.5 with one bf16), a verify 24.4 (23.3).
 //
 // 33 requests of up to 8,000 tokens, 8 kv heads: 46 us and 5 for the join, 221 MB at 4.8 TB/s; of it about
 // 5 until a workgroup's first tile is there (lengths, table and codes wait for one another).  One request
@@ -285,7 +286,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Dec
         for (int t = 0; t < 4; ++t) score[t] -= some;
         less = kHeadroom;
       }
-      u32x4 bits[2];
+      u32x4 bits[2], rest[2];   // weights as two bf16 each
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         float w[4];
@@ -294,10 +295,15 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Dec
           w[i] = exp2_fast(fmaf(score[t][i], a.log2_scale, less));
           sum += w[i];
         }
-        bits[t >> 1][2 * (t & 1)] = bf16_pair(f32x2{w[0], w[1]});
-        bits[t >> 1][2 * (t & 1) + 1] = bf16_pair(f32x2{w[2], w[3]});
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t pair = bf16_pair(f32x2{w[2 * i], w[2 * i + 1]});
+          bits[t >> 1][2 * (t & 1) + i] = pair;
+          rest[t >> 1][2 * (t & 1) + i] =
+              bf16_pair(f32x2{w[2 * i] - __uint_as_float(pair << 16),
+                              w[2 * i + 1] - __uint_as_float(pair & 0xffff0000u)});
+        }
       }
-      const bf16x8 weight[2] = {__builtin_bit_cast(bf16x8, bits[0]), __builtin_bit_cast(bf16x8, bits[1])};
 
       if (!whole) {
         // values behind the last token, or without a page, are zeros; so are those that are not
@@ -316,8 +322,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Dec
 #pragma unroll
       for (int b = 0; b < 8; ++b)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          o[b] = mfma16(operand8(values[b][2 * u], values[b][2 * u + 1], v_scale), weight[u], o[b]);
+        for (int u = 0; u < 2; ++u) {
+          const bf16x8 v = operand8(values[b][2 * u], values[b][2 * u + 1], v_scale);
+          o[b] = mfma16(v, __builtin_bit_cast(bf16x8, rest[u]), o[b]);
+          o[b] = mfma16(v, __builtin_bit_cast(bf16x8, bits[u]), o[b]);
+        }
       v_page = v_now;
       if (more) load_values(tile + step, v_page);
     }

@@ -127,3 +127,24 @@ def test_values_of_any_size(gpu, power, exponent, width):
         set_keys(case, 0, torch.ones)
         set_keys(case, 17, lambda n: torch.randint(-8, 9, (n,), generator=gen) / 2)
         check_exact_scores(case, width, 1.0, f"values of 2^{exponent}")
+
+
+def test_weights_of_decode(gpu):
+    """Decode's weights are two bf16 each: about equal ones times 1 and -1, whose sum is small beside
+    them.  A weight is off by 2^-17 as it is held, by 2^-18 from its exponent (near 24, rounded twice
+    at 2^-20) and by 2^-21 from exp2; two sums of 129 at the most by 2^-16: together below 2^-15 of
+    the sum of weights."""
+    announce(test="decode_weights")
+    gen = torch.Generator().manual_seed(6)
+    case = case_of([2, 18, 70, 129], [1, 2, 2, 2], PAGE, (4, 2), seed=23, device=gpu)
+    for x in ("k_scale", "v_scale"):
+        case[x].view(torch.uint8).fill_(127)
+    values = case["v_cache"].view(torch.uint8)
+    values[..., 0::2], values[..., 1::2] = 0x38, 0xB8
+    case["q"] = torch.zeros_like(case["q"])
+    case["q"][..., 17] = 2.0**-6
+    set_keys(case, 17, lambda n: torch.randint(-8, 9, (n,), generator=gen) / 2)
+    want, _ = oracle.expected_attention(case["q"], *(case[x] for x in CACHE), None, case["out"], 1.0, 2)
+    attend(case, 2, 1.0)
+    torch.cuda.synchronize()
+    within(case["out"], want, 2.0**-15 + 2.0**-8 * (want.abs() + 2.0**-15), "out")
