@@ -7,7 +7,11 @@
 // v_mfma_f32_32x32x16_bf16.  With m = lane % 32 and h = lane / 32,
 //   scores [token, column]: operand A holds, in row m of product t, the key of token 32 t + 16 (m / 4 % 2)
 //     + 4 (m / 8) + m % 4, so that a lane finds tokens 32 t + 16 h + (0 .. 15) of column m in its registers;
-//   outputs [element, column]: operand B is these weights, rounded to bf16, as they lie there.
+//   outputs [element, column]: operand B is these weights, rounded to bf16, as they lie there (their sum
+//     is of the unrounded ones).
+// With a second bf16 for what the first rounds off, products are 3 for 2: 1 x 8,192 tokens 408 us and not 284,
+// 13 prompts 88 and not 66, 3 behind long contexts 52 and not 43, for an error of 0.0016 of the outputs' size
+// and not 0.0018, 0.0016 of it the outputs' own rounding.
 // Statistics are a lane's own but for one exchange of halves.  Outputs are scaled anew only where a
 // maximum grew by more than 2^8 in weights.
 //
