@@ -75,7 +75,7 @@ typedef struct ld_cache_rows {
  * that it has.  A value x is held as the e4m3 nearest to x * 2^-e (ties to even; magnitudes over
  * 448 as 448; what is not finite as NaN); where a scale grew, values of earlier tokens of the page
  * are rounded anew to the larger one.  Bytes of later tokens of a page are left as they were.  A
- * page is written for one request of a call only.
+ * page is written for one request of a call only, and at one place of its table.
  *
  * Here and in ld_cache_read num_kv_heads * (num_tokens / page_size + 2 * num_requests), or num_kv_heads *
  * num_tokens where that is less, is below 2^24, and num_tokens / page_size + 2 * num_requests below
@@ -83,7 +83,8 @@ typedef struct ld_cache_rows {
  */
 int ld_cache_write(const ld_paged_cache* cache, const ld_cache_rows* rows, void* stream);
 
-/* The values at the rows' places, in bf16 (exactly); zeros where a row has no page.  Rows outside every request are left as they were. */
+/* The values at the rows' places, in bf16 (exactly); zeros where a row has no page.  Rows outside every
+ * request are left as they were. */
 int ld_cache_read(const ld_paged_cache* cache, const ld_cache_rows* rows, void* stream);
 
 /*
@@ -95,7 +96,7 @@ int ld_cache_read(const ld_paged_cache* cache, const ld_cache_rows* rows, void* 
  * with scores, statistics and sums in fp32 and p, ahead of its product with v, in bf16 (prefill) or as a
  * sum of two bf16 (decode).  A row that sees no token gets zeros.
  * Rows outside every request are left as they were.  What is not finite in a key or value
- * reaches the rows that see it, nothing else.
+ * reaches the rows that see it, nothing else; a q . k past fp32's range is not finite.
  *   q, gate  bf16 [num_tokens, num_q_heads, 128], rows q_row_stride and gate_row_stride elements
  *            apart (gate NULL: none)
  *   out      bf16 [num_tokens, num_q_heads, 128] contiguous, overlaps no other argument

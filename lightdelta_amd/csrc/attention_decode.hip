@@ -16,11 +16,13 @@
 // 32 columns does not fit in the registers of two a SIMD, and what it keeps in scratch memory waits
 // for the tiles in flight (31.7 us for a verify of 64 requests of up to 4,000 tokens, 23.4 without).
 // e4m3 times its scale is exact in bf16; weights are two bf16 each (2^-17 of one is lost), in a product
-// each with the same operand of values: 33 requests 42.1 us (41.5 with one bf16), a verify 24.4 (23.3).
+// each with the same operand of values: the 33 requests below 51.4 us (50.5 with one bf16), the verify 24.5
+// (23.3).
 //
-// 33 requests of up to 8,000 tokens, 8 kv heads: 46 us and 5 for the join, 221 MB at 4.8 TB/s; of it about
+// 33 requests of up to 8,000 tokens, 8 kv heads: 47 us and 5 for the join, 221 MB at 4.7 TB/s; of it about
 // 5 until a workgroup's first tile is there (lengths, table and codes wait for one another).  One request
-// of 501 tokens: 5.9 and 3.3 us.  64 requests of up to four rows and 4,000 tokens: 19 and 5.
+// of 177 tokens: 6.0 and 3.4 us.  64 requests of up to four rows and 4,000 tokens: 21 and 5.  512 requests
+// of one row and 250 to 2,000 tokens, 2 kv heads: 54 in all, 221 MB at 4.1 TB/s.
 #include <algorithm>
 
 #include "attention_common.h"
@@ -104,8 +106,8 @@ struct Walk {
 };
 
 // Tiles of a workgroup's run.  (With a whole number for each of its waves, of which there would be
-// fewer runs, 32 requests of up to 100 tokens take 16.5 us and not 8.5, their heads being taken one
-// after another, and 64 of up to 2,000 tokens and 8 kv heads 36 and not 34.)
+// fewer runs, 32 requests of 13 to 96 tokens take 17.1 us in a graph and not 8.9, their heads being taken
+// one after another, and 64 of 250 to 2,000 tokens and 8 kv heads 30.3 and not 27.9.)
 __device__ __forceinline__ uint32_t run_length(const DecodeAttention& p, uint32_t total) {
   const uint32_t workers = static_cast<uint32_t>(p.workers);
   return max((total * p.cache.kv_heads + workers - 1) / workers, 1u);
@@ -413,10 +415,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Dec
 // Some columns of a request and kv head a workgroup: joins the sums of the runs that its tiles were
 // cut into; zeros for a request without tokens or with more rows than the width.  Groups of threads
 // take every Groups-th piece, a thread eight elements of a column.
-// Four columns and eight groups start sooner than sixteen and four (one request of 501 tokens 8.2 and
-// 8.5 us, 32 up to 1,000 11.1 and 12.5, 64 of up to four rows and 4,000 tokens 23.8 and 23.6).  A head
-// that may be in more than 48 pieces has two columns and 32 groups (one request of 100,000 tokens, 256
-// pieces, 18.8 and 27.0; four up to 20,000, 64 pieces, 16.9 and 19.1; of one tile 9.1 and 8.2).
+// Four columns and eight groups start sooner than sixteen and four (both launches in a graph, 8 q heads on
+// each of 2: one request of 177 tokens 8.4 and 8.7 us, of 7,000 17.7 and 26.2, 32 of 125 to 1,000 10.9 and
+// 11.9, 64 of four rows and 500 to 4,000 25.9 and 25.7).  A head that may be in more than 48 pieces has two
+// columns and 32 groups (one request of 7,000 tokens 13.4 and 17.7, of 35,000 18.0 and 27.1, of 100,000, 223
+// pieces, 23.8 and 34.4; four of 20,000, 63 pieces, 19.7 and 20.8; of 177 in a table for 100,000s 9.4 and
+// 8.6).
 constexpr int kJoinColumns = 4, kJoinGroups = 8;
 constexpr int kFewColumns = 2, kFewGroups = 32;
 constexpr int kManyPieces = 48;

@@ -19,8 +19,8 @@
 // joins.
 //
 // One prompt of 8,192 tokens, 16 q heads on 2: 284 us, 970 TFLOP/s, the matrix cores busy 46% of the cycles
-// (at the 2.0 GHz that the card holds) and vector issue 43%.  13 prompts up to 1,500 tokens behind up
-// to 1,000, 32 q heads on 8: 66 us; three of 20 to 90 behind up to 30,000: 43, of it 11 for the join.
+// (at the 2.0 GHz that the card holds) and vector issue 43%.  13 prompts of 1 to 1,132 tokens behind up
+// to 1,000, 32 q heads on 8: 66 us; three of 32 to 78 behind 5,300 to 21,200: 42, of it 11 for the join.
 #include <algorithm>
 
 #include "attention_common.h"
@@ -527,7 +527,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_prefill_kernel(const Pr
 
 // Joins the sums of a unit's shares: thread (column, four elements), eight columns a workgroup and
 // Groups of threads that take every Groups-th share.  Few units have many shares each: four groups (three
-// prompts behind up to 30,000 tokens, 30 shares: 10 us, one group 23); with more, whose shares are
+// prompts behind up to 21,200 tokens, 30 shares: 10 us, one group 23); with more, whose shares are
 // few, the threads of one group start in less time (one prompt of 1,024 tokens 32 us in all, four 37).
 constexpr int kGatherColumns = 8;
 constexpr int kFewUnits = 64;

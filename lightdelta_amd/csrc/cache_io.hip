@@ -7,8 +7,10 @@
 // sixteen tokens, transposed in registers, and 32 threads a row of each token.  A page's new rows
 // stay in registers between the search for their largest magnitude and their rounding.
 //
-// 32 x 1024 tokens of 8 heads: 46 us, 4.35 TB/s (66 with two-byte loads of
-// values and two passes over the rows); 16,755 tokens read back 29 us, 3.5 TB/s (83 with a token a wave).
+// 32 x 1024 tokens of 8 heads: 46 us, 4.4 TB/s (66 with two-byte loads of
+// values and two passes over the rows); 16,755 tokens read back 30 us, 3.4 TB/s (83 with a token a wave):
+// no byte more than those of codes and rows, but every workgroup's one page waits for lengths, table, scale
+// and codes in turn.
 #include <algorithm>
 
 #include "attention_common.h"
@@ -21,8 +23,8 @@ constexpr int kIoThreads = 128;
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-// Two fp32 as e4m3 in the low 16 bits: to the nearest, ties to even.  The instruction gives NaN
-// past 448, so that callers limit what is finite.
+// Four fp32 as e4m3, the first in the lowest byte: to the nearest, ties to even.  The instruction gives
+// NaN past 448, so that callers limit what is finite.
 __device__ __forceinline__ uint32_t four_fp8(float a, float b, float c, float d) {
   const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true));
@@ -59,8 +61,8 @@ struct Part {
 };
 
 // Requests have a run of units each, as many as pages that their rows can touch: rows / page + 2 (rows
-// begin anywhere in a page), or as many as rows where that is less.  False where the unit has no page to do with; q and within are set
-// wherever there is a request (within < 0: not).
+// begin anywhere in a page), or as many as rows where that is less.  False where the unit has no page to do
+// with; q and within are set wherever there is a request (within < 0: not).
 __device__ __forceinline__ bool find_part(const Cache& c, int unit, Part& part, Request& q,
                                           int& within) {
   int r;
