@@ -5,7 +5,13 @@ from __future__ import annotations
 
 import pytest
 
-from tests.test_attention_gpu import announce, case_of, check_attention
+from tests.test_attention_gpu import (
+    announce,
+    case_of,
+    check_attention,
+    check_read,
+    check_write,
+)
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +38,16 @@ def test_shares_of_many_requests(gpu, requests, heads):
     for i, (length, rows) in split.items():
         lengths[i], new[i] = length, rows
     check_attention(case_of(lengths, new, 64, heads, seed=32, device=gpu))
+
+
+def test_thousands_of_requests(gpu):
+    """Requests are found by a search of three levels past 4,096 of them."""
+    announce(test="thousands")
+    lengths = [i % 23 if i % 3 else 0 for i in range(4400)]
+    new = [min(n, 1 + i % 2) for i, n in enumerate(lengths)]
+    lengths[4200], new[4200] = 70, 40
+    case = case_of(lengths, new, 16, (2, 1), seed=33, device=gpu, front=1, behind=3)
+    check_write(case)
+    check_read(case)
+    check_attention(case)
+    check_attention(case, width=2)
